@@ -80,6 +80,19 @@ SIGNATURES = {
                                                   _i32, _i32, _vp, _vp, _vp, _vp, _vp]),
     "hmoe_grouped_down_fp8_mx": (_i32, [_vp, _vp, _vp, _i32, _i64, _i32, _i32, _vp, _vp, _vp,
                                         _vp]),
+    "hmoe_quantize_rows_mxfp4": (_i32, [_vp, _i32, _i64, _i32, _vp, _vp, _vp]),
+    "hmoe_dequantize_rows_mxfp4": (_i32, [_vp, _vp, _i64, _i32, _vp, _i32, _vp]),
+    "hmoe_packed_mxfp4_gate_up_bytes": (_sz, [_i32, _i32, _i32]),
+    "hmoe_pack_mxfp4_gate_up": (_i32, [_vp, _vp, _i32, _i32, _i32, _i32, _vp, _vp, _vp]),
+    "hmoe_packed_mxfp4_down_bytes": (_sz, [_i32, _i32, _i32]),
+    "hmoe_pack_mxfp4_down": (_i32, [_vp, _i32, _i32, _i32, _i32, _vp, _vp, _vp]),
+    "hmoe_unpack_mxfp4": (_i32, [_vp, _vp, _i32, _i32, _i32, _vp, _i32, _vp]),
+    "hmoe_grouped_gate_up_mxfp4": (_i32, [_vp, _vp, _vp, _i32, _i64, _i32, _i32, _vp, _vp, _vp,
+                                          _vp, _vp]),
+    "hmoe_grouped_gate_up_mxfp4_gather": (_i32, [_vp, _vp, _i64, _i32, _vp, _vp, _i32, _i64, _i32,
+                                                 _i32, _vp, _vp, _vp, _vp, _vp]),
+    "hmoe_grouped_down_mxfp4": (_i32, [_vp, _vp, _vp, _i32, _i64, _i32, _i32, _vp, _vp, _vp,
+                                       _vp]),
     "hmoe_aux_workspace_bytes": (_sz, [_i32, _i32, _i32]),
     "hmoe_router_aux": (_i32, [_vp, _vp, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _sz, _vp]),
     "hmoe_combine_bwd": (_i32, [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _f32, _vp]),

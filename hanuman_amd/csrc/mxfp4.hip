@@ -1,0 +1,285 @@
+// MXFP4 rows and operands: quantising, reading back, and packing the expert
+// masters for the grouped products (quant_mxfp4.h has the format).  All of it is
+// bound by memory: no value is looked at twice.
+#include "quant_mxfp4.h"
+#include "quant_e4m3.h"
+
+namespace hmoe {
+namespace {
+
+__device__ __forceinline__ uint32_t umax32(uint32_t a, uint32_t b) { return a > b ? a : b; }
+
+// Rows are whole blocks, so a matrix is one run of them.  A lane takes eight
+// values and four neighbours a block.
+template <typename TI>
+__global__ __launch_bounds__(256) void quantize_rows_mxfp4_kernel(const TI* __restrict__ a,
+                                                                  int64_t chunks,
+                                                                  uint8_t* __restrict__ q,
+                                                                  uint8_t* __restrict__ exps) {
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * 256;
+  for (int64_t c = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; c < chunks; c += stride) {
+    Chunk8<TI> x;
+    x.load_nt(a + c * 8);
+    float v[8];
+    uint32_t amax = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      v[i] = x.get(i);
+      amax = umax32(amax, __float_as_uint(v[i]) & 0x7fffffffu);
+    }
+    // chunks is a multiple of 4: a block's four lanes are here together
+    amax = umax32(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), 1)));
+    amax = umax32(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), 2)));
+    const uint32_t e = mxfp4_exponent(amax);
+    reinterpret_cast<uint32_t*>(q)[c] = mxfp4_codes8(v, mxfp4_inverse(e));
+    if ((c & 3) == 0) exps[c >> 2] = static_cast<uint8_t>(e);
+  }
+}
+
+__device__ __forceinline__ void store8(float* o, const float (&v)[8]) {
+  *reinterpret_cast<f32x4*>(o) = f32x4{v[0], v[1], v[2], v[3]};
+  *reinterpret_cast<f32x4*>(o + 4) = f32x4{v[4], v[5], v[6], v[7]};
+}
+// (the values are exact in bf16, a sum of no more than two bits' weight: the
+// upper half of the float32 is all of it)
+__device__ __forceinline__ void store8(uint16_t* o, const float (&v)[8]) {
+  u32x4 w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    w[i] = (__float_as_uint(v[2 * i]) >> 16) | (__float_as_uint(v[2 * i + 1]) & 0xffff0000u);
+  *reinterpret_cast<u32x4*>(o) = w;
+}
+
+// OPERAND: codes and exponents lie as the packed operands keep them (rows of
+// `cols` values, `rows` of them an expert); the values come out row by row.
+template <typename TO, bool OPERAND>
+__global__ __launch_bounds__(256) void dequantize_mxfp4_kernel(const uint8_t* __restrict__ q,
+                                                               const uint8_t* __restrict__ exps,
+                                                               int64_t chunks, int rows, int cols,
+                                                               TO* __restrict__ out) {
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * 256;
+  for (int64_t c = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; c < chunks; c += stride) {
+    int64_t word = c, block = c >> 2;
+    if constexpr (OPERAND) {
+      const int per_row = cols / 8;
+      const int64_t row_all = c / per_row;
+      const int k8 = static_cast<int>(c - row_all * per_row);  // columns 8 k8 .. + 8
+      const int64_t n = row_all / rows;
+      const int p = static_cast<int>(row_all - n * rows);
+      const int64_t frag = (n * (rows / 32) + p / 32) * (cols / 64) + k8 / 8;
+      word = (frag * 64 + ((k8 >> 2) & 1) * 32 + (p & 31)) * 4 + (k8 & 3);
+      block = ((n * (cols / 128) + k8 / 16) * rows + p) * 4 + ((k8 >> 2) & 3);
+    }
+    float v[8];
+    mxfp4_values8(reinterpret_cast<const uint32_t*>(q)[word], mxfp4_scale(exps[block]), v);
+    store8(out + c * 8, v);
+  }
+}
+
+// Two neighbouring columns of a master.
+__device__ __forceinline__ void load2(const float* p, float& a, float& b) {
+  const float2 v = *reinterpret_cast<const float2*>(p);
+  a = v.x;
+  b = v.y;
+}
+__device__ __forceinline__ void load2(const uint16_t* p, float& a, float& b) {
+  const uint32_t v = *reinterpret_cast<const uint32_t*>(p);
+  a = __uint_as_float(v << 16);
+  b = __uint_as_float(v & 0xffff0000u);
+}
+
+// One wave: 64 columns x 128 rows of a master src[e][K][C], which are 64 operand
+// rows x 128 of the reduction.  Lane 32 h + i takes columns 2 i, 2 i + 1 of
+// blocks h and 2 + h: its 32 values of a column are a block and, packed, the 16
+// bytes that the matrix instruction's lane holds, so nothing moves between lanes
+// but the exponents.  GATE_UP: grid.z counts gate, then up, of each expert.
+template <typename TW, bool GATE_UP>
+__global__ __launch_bounds__(256) void pack_mxfp4_kernel(const TW* __restrict__ src0,
+                                                         const TW* __restrict__ src1, int kdim,
+                                                         int cols, uint8_t* __restrict__ dst,
+                                                         uint8_t* __restrict__ exps) {
+  const int lane = threadIdx.x & 63;
+  const int half = lane >> 5, i2 = (lane & 31) * 2;
+  const int c0 = blockIdx.x * 64;
+  const int kb = blockIdx.y * 4 + (threadIdx.x >> 6);  // 128 rows of the reduction
+  if (kb * 128 >= kdim) return;
+  const int e = GATE_UP ? blockIdx.z >> 1 : blockIdx.z;
+  const int which = GATE_UP ? blockIdx.z & 1 : 0;
+  const int rows = GATE_UP ? 2 * cols : cols;
+  const TW* src = (which ? src1 : src0) + static_cast<int64_t>(e) * kdim * cols + c0 + i2;
+  uint32_t ex[2] = {0, 0};  // this lane's columns' exponent words
+#pragma unroll
+  for (int b = 0; b < 2; ++b) {
+    const int k0 = kb * 128 + b * 64 + half * 32;
+    float v[2][32];
+    uint32_t amax[2] = {0, 0};
+#pragma unroll
+    for (int r = 0; r < 32; ++r) {
+      load2(src + static_cast<int64_t>(k0 + r) * cols, v[0][r], v[1][r]);
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int r = 0; r < 32; ++r) amax[j] = umax32(amax[j], __float_as_uint(v[j][r]) & 0x7fffffffu);
+      const uint32_t ee = mxfp4_exponent(amax[j]);
+      const float inv = mxfp4_inverse(ee);
+      u32x4 w;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        float t[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) t[r] = v[j][g * 8 + r];
+        w[g] = mxfp4_codes8(t, inv);
+      }
+      // column c of the master is operand row p
+      const int c = c0 + i2 + j;
+      const int p = GATE_UP ? (c >> 5) * 64 + which * 32 + (c & 31) : c;
+      const int64_t frag = (static_cast<int64_t>(e) * (rows / 32) + p / 32) * (kdim / 64) + kb * 2 + b;
+      *reinterpret_cast<u32x4*>(dst + (frag * 64 + half * 32 + (p & 31)) * 16) = w;
+      ex[j] |= ee << (16 * b + 8 * half);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const uint32_t word = ex[j] | static_cast<uint32_t>(__shfl_xor(static_cast<int>(ex[j]), 32));
+    const int c = c0 + i2 + j;
+    const int p = GATE_UP ? (c >> 5) * 64 + which * 32 + (c & 31) : c;
+    if (half == 0)
+      *reinterpret_cast<uint32_t*>(exps + ((static_cast<int64_t>(e) * (kdim / 128) + kb) * rows + p) * 4) = word;
+  }
+}
+
+unsigned chunk_grid(int64_t chunks) {
+  const int64_t blocks = ceil_div(chunks, 256);
+  return static_cast<unsigned>(blocks < 65536 ? blocks : 65536);
+}
+
+int pack_mxfp4(const char* what, const void* w0, const void* w1, int w_dtype, int n_experts, int kdim,
+               int cols, uint8_t* packed, uint8_t* exps, hipStream_t s) {
+  const bool gate_up = w1 != nullptr;
+  const int z = gate_up ? 2 * n_experts : n_experts;
+  const dim3 grid(cols / 64, static_cast<unsigned>(ceil_div(kdim / 128, 4)), z);
+#define HMOE_LAUNCH_PACK4(TW, GU)                                                              \
+  hipLaunchKernelGGL((pack_mxfp4_kernel<TW, GU>), grid, dim3(256), 0, s,                       \
+                     static_cast<const TW*>(w0), static_cast<const TW*>(w1), kdim, cols, packed, exps)
+  if (w_dtype == HMOE_F32 && gate_up) HMOE_LAUNCH_PACK4(float, true);
+  else if (w_dtype == HMOE_F32) HMOE_LAUNCH_PACK4(float, false);
+  else if (gate_up) HMOE_LAUNCH_PACK4(uint16_t, true);
+  else HMOE_LAUNCH_PACK4(uint16_t, false);
+#undef HMOE_LAUNCH_PACK4
+  return check_launch(what);
+}
+
+// The sizes that every packed MXFP4 operand has: whole 128-value groups of the
+// reduction, rows in blocks of 32 (gate/up: 64).
+int check_operand(const char* what, int n_experts, int d_model, int d_ff) {
+  HMOE_REQUIRE(n_experts >= 1 && n_experts <= 1024, "%s: n_experts must be in [1, 1024] (got %d)", what,
+               n_experts);
+  HMOE_REQUIRE_CODE(d_model >= 128 && d_model % 128 == 0, HMOE_ERR_UNSUPPORTED,
+                    "%s: d_model must be a multiple of 128 (got %d)", what, d_model);
+  HMOE_REQUIRE_CODE(d_ff >= 128 && d_ff % 128 == 0, HMOE_ERR_UNSUPPORTED,
+                    "%s: d_ff must be a multiple of 128 (got %d)", what, d_ff);
+  return HMOE_OK;
+}
+
+template <bool OPERAND>
+int dequantize(const char* what, const uint8_t* q, const uint8_t* exps, int64_t chunks, int rows, int cols,
+               void* out, int out_dtype, hipStream_t s) {
+  if (out_dtype == HMOE_F32)
+    hipLaunchKernelGGL((dequantize_mxfp4_kernel<float, OPERAND>), dim3(chunk_grid(chunks)), dim3(256), 0, s,
+                       q, exps, chunks, rows, cols, static_cast<float*>(out));
+  else
+    hipLaunchKernelGGL((dequantize_mxfp4_kernel<uint16_t, OPERAND>), dim3(chunk_grid(chunks)), dim3(256), 0,
+                       s, q, exps, chunks, rows, cols, static_cast<uint16_t*>(out));
+  return check_launch(what);
+}
+
+}  // namespace
+}  // namespace hmoe
+
+extern "C" int hmoe_quantize_rows_mxfp4(const void* a, int a_dtype, int64_t rows, int cols, uint8_t* q,
+                                        uint8_t* exps, hmoe_stream_t stream) {
+  using namespace hmoe;
+  HMOE_REQUIRE(rows >= 0, "quantize_rows_mxfp4: rows must be >= 0");
+  HMOE_REQUIRE_CODE(cols >= kMxBlock && cols % kMxBlock == 0, HMOE_ERR_UNSUPPORTED,
+                    "quantize_rows_mxfp4: cols must be a multiple of 32 (got %d)", cols);
+  HMOE_REQUIRE(a_dtype == HMOE_F32 || a_dtype == HMOE_BF16,
+               "quantize_rows_mxfp4: a dtype must be F32 or BF16");
+  if (rows == 0) return HMOE_OK;
+  HMOE_REQUIRE(a && q && exps, "quantize_rows_mxfp4: null pointer argument");
+  HMOE_REQUIRE_ALIGNED("quantize_rows_mxfp4", a, q, exps);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const int64_t chunks = rows * (cols / 8);
+  if (a_dtype == HMOE_BF16)
+    hipLaunchKernelGGL(quantize_rows_mxfp4_kernel<uint16_t>, dim3(chunk_grid(chunks)), dim3(256), 0, s,
+                       static_cast<const uint16_t*>(a), chunks, q, exps);
+  else
+    hipLaunchKernelGGL(quantize_rows_mxfp4_kernel<float>, dim3(chunk_grid(chunks)), dim3(256), 0, s,
+                       static_cast<const float*>(a), chunks, q, exps);
+  return check_launch("hmoe_quantize_rows_mxfp4");
+}
+
+extern "C" int hmoe_dequantize_rows_mxfp4(const uint8_t* q, const uint8_t* exps, int64_t rows, int cols,
+                                          void* out, int out_dtype, hmoe_stream_t stream) {
+  using namespace hmoe;
+  HMOE_REQUIRE(rows >= 0, "dequantize_rows_mxfp4: rows must be >= 0");
+  HMOE_REQUIRE_CODE(cols >= kMxBlock && cols % kMxBlock == 0, HMOE_ERR_UNSUPPORTED,
+                    "dequantize_rows_mxfp4: cols must be a multiple of 32 (got %d)", cols);
+  HMOE_REQUIRE(out_dtype == HMOE_F32 || out_dtype == HMOE_BF16,
+               "dequantize_rows_mxfp4: out dtype must be F32 or BF16");
+  if (rows == 0) return HMOE_OK;
+  HMOE_REQUIRE(q && exps && out, "dequantize_rows_mxfp4: null pointer argument");
+  HMOE_REQUIRE_ALIGNED("dequantize_rows_mxfp4", q, exps, out);
+  return dequantize<false>("hmoe_dequantize_rows_mxfp4", q, exps, rows * (cols / 8), 0, cols, out, out_dtype,
+                           static_cast<hipStream_t>(stream));
+}
+
+extern "C" size_t hmoe_packed_mxfp4_gate_up_bytes(int n_experts, int d_model, int d_ff) {
+  if (n_experts <= 0 || d_model <= 0 || d_ff <= 0) return 0;
+  return static_cast<size_t>(n_experts) * d_ff * d_model;
+}
+
+extern "C" size_t hmoe_packed_mxfp4_down_bytes(int n_experts, int d_ff, int d_model) {
+  if (n_experts <= 0 || d_model <= 0 || d_ff <= 0) return 0;
+  return static_cast<size_t>(n_experts) * d_model * (d_ff / 2);
+}
+
+extern "C" int hmoe_pack_mxfp4_gate_up(const void* w_gate, const void* w_up, int w_dtype, int n_experts,
+                                       int d_model, int d_ff, uint8_t* packed, uint8_t* exps,
+                                       hmoe_stream_t stream) {
+  using namespace hmoe;
+  if (int rc = check_operand("pack_mxfp4_gate_up", n_experts, d_model, d_ff)) return rc;
+  HMOE_REQUIRE(w_dtype == HMOE_F32 || w_dtype == HMOE_BF16,
+               "pack_mxfp4_gate_up: weight dtype must be F32 or BF16");
+  HMOE_REQUIRE(w_gate && w_up && packed && exps, "pack_mxfp4_gate_up: null pointer argument");
+  HMOE_REQUIRE_ALIGNED("pack_mxfp4_gate_up", w_gate, w_up, packed, exps);
+  return pack_mxfp4("hmoe_pack_mxfp4_gate_up", w_gate, w_up, w_dtype, n_experts, d_model, d_ff, packed, exps,
+                    static_cast<hipStream_t>(stream));
+}
+
+extern "C" int hmoe_pack_mxfp4_down(const void* w_down, int w_dtype, int n_experts, int d_ff, int d_model,
+                                    uint8_t* packed, uint8_t* exps, hmoe_stream_t stream) {
+  using namespace hmoe;
+  if (int rc = check_operand("pack_mxfp4_down", n_experts, d_model, d_ff)) return rc;
+  HMOE_REQUIRE(w_dtype == HMOE_F32 || w_dtype == HMOE_BF16, "pack_mxfp4_down: weight dtype must be F32 or BF16");
+  HMOE_REQUIRE(w_down && packed && exps, "pack_mxfp4_down: null pointer argument");
+  HMOE_REQUIRE_ALIGNED("pack_mxfp4_down", w_down, packed, exps);
+  return pack_mxfp4("hmoe_pack_mxfp4_down", w_down, nullptr, w_dtype, n_experts, d_ff, d_model, packed, exps,
+                    static_cast<hipStream_t>(stream));
+}
+
+extern "C" int hmoe_unpack_mxfp4(const uint8_t* packed, const uint8_t* exps, int n_experts, int rows, int cols,
+                                 void* out, int out_dtype, hmoe_stream_t stream) {
+  using namespace hmoe;
+  HMOE_REQUIRE(n_experts >= 1 && n_experts <= 1024, "unpack_mxfp4: n_experts must be in [1, 1024] (got %d)",
+               n_experts);
+  HMOE_REQUIRE_CODE(rows >= 32 && rows % 32 == 0, HMOE_ERR_UNSUPPORTED,
+                    "unpack_mxfp4: rows must be a multiple of 32 (got %d)", rows);
+  HMOE_REQUIRE_CODE(cols >= 128 && cols % 128 == 0, HMOE_ERR_UNSUPPORTED,
+                    "unpack_mxfp4: cols must be a multiple of 128 (got %d)", cols);
+  HMOE_REQUIRE(out_dtype == HMOE_F32 || out_dtype == HMOE_BF16, "unpack_mxfp4: out dtype must be F32 or BF16");
+  HMOE_REQUIRE(packed && exps && out, "unpack_mxfp4: null pointer argument");
+  HMOE_REQUIRE_ALIGNED("unpack_mxfp4", packed, exps, out);
+  return dequantize<true>("hmoe_unpack_mxfp4", packed, exps, static_cast<int64_t>(n_experts) * rows * (cols / 8),
+                          rows, cols, out, out_dtype, static_cast<hipStream_t>(stream));
+}

@@ -688,6 +688,179 @@ def grouped_down_fp8_mx(h_q: torch.Tensor, h_exp: torch.Tensor, offsets: torch.T
     return ys
 
 
+# ---------------------------------------------------------- MXFP4 experts --
+# 32 values of a row share a power-of-two scale (an E8M0 byte), each is a 4-bit
+# e2m1 code; ``hmoe_quantize_rows_mxfp4`` has the rule.  Served weights only: there
+# is no backward, as for the e4m3 experts.
+
+def _u8(name: str, dev, *shapes):
+    """Checks ``(tensor, shape)`` pairs of an MXFP4 call: uint8, on one device (the
+    current one, whose stream the call takes), of those sizes."""
+    for t, shape in shapes:
+        _check(t, name)
+        if t.dtype != torch.uint8 or tuple(t.shape) != tuple(shape):
+            raise ValueError(f"{name}: expected uint8 {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+        _same_device(name, t, dev)
+
+
+def _same_device(name: str, t: torch.Tensor, dev):
+    if t.device != dev:
+        raise ValueError(f"{name}: tensors on {t.device} and {dev}")
+
+
+def _current_device(name: str, t: torch.Tensor):
+    _check(t, name)
+    if t.device.index != torch.cuda.current_device():
+        raise ValueError(f"{name}: tensors on {t.device}, but the current device is "
+                         f"cuda:{torch.cuda.current_device()}")
+    return t.device
+
+
+def quantize_rows_mxfp4(a: torch.Tensor):
+    """MXFP4 rows of a float32 or bf16 matrix ``[rows, cols]``: codes uint8 ``[rows,
+    cols / 2]`` (the even column in a byte's low half) and biased exponents uint8
+    ``[rows, cols / 32]``."""
+    dev = _current_device("quantize_rows_mxfp4", a)
+    _check(a, "a", 2)
+    rows, cols = a.shape
+    q = torch.empty((rows, cols // 2), dtype=torch.uint8, device=dev)
+    exps = torch.empty((rows, cols // 32), dtype=torch.uint8, device=dev)
+    call("hmoe_quantize_rows_mxfp4", _ptr(a), _dtype_code(a), rows, cols, _ptr(q), _ptr(exps),
+         _stream())
+    return q, exps
+
+
+def dequantize_rows_mxfp4(q: torch.Tensor, exps: torch.Tensor,
+                          out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values ``[rows, cols]`` of MXFP4 rows (exact in both types)."""
+    dev = _current_device("dequantize_rows_mxfp4", q)
+    _check(q, "q", 2)
+    rows, cols = q.shape[0], q.shape[1] * 2
+    _u8("dequantize_rows_mxfp4", dev, (q, q.shape), (exps, (rows, cols // 32)))
+    if out_dtype not in _DT:
+        raise TypeError(f"unsupported dtype {out_dtype}; expected float32 or bfloat16")
+    out = torch.empty((rows, cols), dtype=out_dtype, device=dev)
+    call("hmoe_dequantize_rows_mxfp4", _ptr(q), _ptr(exps), rows, cols, _ptr(out), _DT[out_dtype],
+         _stream())
+    return out
+
+
+def _mxfp4_operand(N: int, rows: int, k: int, dev):
+    """Empty codes and exponents of a packed operand (see ``hmoe_pack_mxfp4_gate_up``)."""
+    return (torch.empty((N, rows // 32, k // 64, 64, 16), dtype=torch.uint8, device=dev),
+            torch.empty((N, k // 128, rows, 4), dtype=torch.uint8, device=dev))
+
+
+def pack_mxfp4_gate_up(w_gate: torch.Tensor, w_up: torch.Tensor):
+    """MXFP4 gate/up operand of ``[N,D,F]`` masters, quantised along ``D``: codes
+    ``[N, 2F/32, D/64, 64, 16]`` and exponents ``[N, D/128, 2F, 4]``."""
+    dev = _current_device("pack_mxfp4_gate_up", w_gate)
+    _check(w_gate, "w_gate", 3)
+    _check(w_up, "w_up", 3)
+    _same_device("pack_mxfp4_gate_up", w_up, dev)
+    if w_gate.shape != w_up.shape or w_gate.dtype != w_up.dtype:
+        raise ValueError("w_gate and w_up must have the same shape and dtype")
+    N, D, F = w_gate.shape
+    out, exps = _mxfp4_operand(N, 2 * F, D, dev)
+    call("hmoe_pack_mxfp4_gate_up", _ptr(w_gate), _ptr(w_up), _dtype_code(w_gate), N, D, F,
+         _ptr(out), _ptr(exps), _stream())
+    return out, exps
+
+
+def pack_mxfp4_down(w_down: torch.Tensor):
+    """MXFP4 down operand of the ``[N,F,D]`` master, quantised along ``F``: codes
+    ``[N, D/32, F/64, 64, 16]`` and exponents ``[N, F/128, D, 4]``."""
+    dev = _current_device("pack_mxfp4_down", w_down)
+    _check(w_down, "w_down", 3)
+    N, F, D = w_down.shape
+    out, exps = _mxfp4_operand(N, D, F, dev)
+    call("hmoe_pack_mxfp4_down", _ptr(w_down), _dtype_code(w_down), N, F, D, _ptr(out),
+         _ptr(exps), _stream())
+    return out, exps
+
+
+def _mxfp4_sizes(name: str, packed: torch.Tensor, exps: torch.Tensor, dev):
+    """``(N, rows, K)`` of a packed operand, its tensors checked."""
+    _check(packed, name, 5)
+    N, rows, k = packed.shape[0], packed.shape[1] * 32, packed.shape[2] * 64
+    _u8(name, dev, (packed, (N, rows // 32, k // 64, 64, 16)), (exps, (N, k // 128, rows, 4)))
+    return N, rows, k
+
+
+def unpack_mxfp4(packed: torch.Tensor, exps: torch.Tensor,
+                 out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The weights ``[N, rows, K]`` of a packed MXFP4 operand: in bf16 the operand that
+    the bf16 products take (:func:`pack_gate_up`, :func:`pack_down`)."""
+    dev = _current_device("unpack_mxfp4", packed)
+    N, rows, k = _mxfp4_sizes("unpack_mxfp4", packed, exps, dev)
+    if out_dtype not in _DT:
+        raise TypeError(f"unsupported dtype {out_dtype}; expected float32 or bfloat16")
+    out = torch.empty((N, rows, k), dtype=out_dtype, device=dev)
+    call("hmoe_unpack_mxfp4", _ptr(packed), _ptr(exps), N, rows, k, _ptr(out), _DT[out_dtype],
+         _stream())
+    return out
+
+
+def _check_offsets(name: str, offsets: torch.Tensor, N: int, dev):
+    _check(offsets, "offsets", 1)
+    _same_device(name, offsets, dev)
+    if offsets.numel() != N + 1 or offsets.dtype != torch.int32:
+        raise ValueError(f"{name}: offsets must be int32 [{N + 1}]")
+
+
+def grouped_gate_up_mxfp4(xs_q: torch.Tensor, xs_exp: torch.Tensor, offsets: torch.Tensor,
+                          w_packed: torch.Tensor, w_exp: torch.Tensor):
+    """MXFP4 ``h = silu(g) * u`` of MXFP4 rows in the experts' order: codes ``[rows,
+    F/2]`` and exponents ``[rows, F/32]``.  Rows past ``offsets[-1]`` are not written."""
+    name = "grouped_gate_up_mxfp4"
+    dev = _current_device(name, xs_q)
+    N, F2, D = _mxfp4_sizes(name, w_packed, w_exp, dev)
+    rows, F = xs_q.shape[0], F2 // 2
+    _u8(name, dev, (xs_q, (rows, D // 2)), (xs_exp, (rows, D // 32)))
+    _check_offsets(name, offsets, N, dev)
+    h_q = torch.empty((rows, F // 2), dtype=torch.uint8, device=dev)
+    h_exp = torch.empty((rows, F // 32), dtype=torch.uint8, device=dev)
+    call("hmoe_grouped_gate_up_mxfp4", _ptr(xs_q), _ptr(xs_exp), _ptr(offsets), N, rows, D, F,
+         _ptr(w_packed), _ptr(w_exp), _ptr(h_q), _ptr(h_exp), _stream())
+    return h_q, h_exp
+
+
+def grouped_gate_up_mxfp4_gather(x_q: torch.Tensor, x_exp: torch.Tensor, plan: Plan,
+                                 w_packed: torch.Tensor, w_exp: torch.Tensor):
+    """:func:`grouped_gate_up_mxfp4` gathering its rows from the quantised tokens
+    through ``perm_src``."""
+    name = "grouped_gate_up_mxfp4_gather"
+    dev = _current_device(name, x_q)
+    N, F2, D = _mxfp4_sizes(name, w_packed, w_exp, dev)
+    T, F = x_q.shape[0], F2 // 2
+    _u8(name, dev, (x_q, (T, D // 2)), (x_exp, (T, D // 32)))
+    if plan.n_experts != N or plan.slot_pos.numel() != T * plan.top_k:
+        raise ValueError(f"{name}: the plan is of other tokens or experts")
+    _check_offsets(name, plan.offsets, N, dev)
+    h_q = torch.empty((plan.rows_cap, F // 2), dtype=torch.uint8, device=dev)
+    h_exp = torch.empty((plan.rows_cap, F // 32), dtype=torch.uint8, device=dev)
+    call("hmoe_grouped_gate_up_mxfp4_gather", _ptr(x_q), _ptr(x_exp), T, plan.top_k,
+         _ptr(plan.perm_src), _ptr(plan.offsets), N, plan.rows_cap, D, F, _ptr(w_packed),
+         _ptr(w_exp), _ptr(h_q), _ptr(h_exp), _stream())
+    return h_q, h_exp
+
+
+def grouped_down_mxfp4(h_q: torch.Tensor, h_exp: torch.Tensor, offsets: torch.Tensor,
+                       w_packed: torch.Tensor, w_exp: torch.Tensor) -> torch.Tensor:
+    """bf16 ``ys`` of MXFP4 rows times the MXFP4 down operand.  Rows past
+    ``offsets[-1]`` are not written."""
+    name = "grouped_down_mxfp4"
+    dev = _current_device(name, h_q)
+    N, D, F = _mxfp4_sizes(name, w_packed, w_exp, dev)
+    rows = h_q.shape[0]
+    _u8(name, dev, (h_q, (rows, F // 2)), (h_exp, (rows, F // 32)))
+    _check_offsets(name, offsets, N, dev)
+    ys = torch.empty((rows, D), dtype=torch.bfloat16, device=dev)
+    call("hmoe_grouped_down_mxfp4", _ptr(h_q), _ptr(h_exp), _ptr(offsets), N, rows, F, D,
+         _ptr(w_packed), _ptr(w_exp), _ptr(ys), _stream())
+    return ys
+
+
 # ---------------------------------------------------------------- combine --
 
 def combine(ys: torch.Tensor, plan: Plan, gates: torch.Tensor,

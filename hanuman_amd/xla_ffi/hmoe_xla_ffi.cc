@@ -555,6 +555,209 @@ XLA_FFI_DEFINE_HANDLER_SYMBOL(HmoeGroupedDownFp8Mx, GroupedDownFp8MxImpl,
                                   .Arg<ffi::Buffer<ffi::F32>>()
                                   .Ret<ffi::Buffer<ffi::BF16>>());
 
+// ---- MXFP4 experts: 4-bit rows times 4-bit weights ---------------------------
+// The products take their sizes from the operands: a packed operand's codes are [N,
+// rows / 32, K / 64, 64, 16], its exponents [N, K / 128, rows, 4].
+namespace {
+
+ffi::Error BadMxfp4(const char* what) {
+  return ffi::Error(ffi::ErrorCode::kInvalidArgument, std::string(what) + ": operand shapes do not agree");
+}
+
+// Rows of `rows` x `cols` values in codes and exponents, and a packed operand.
+template <typename Q, typename E>
+bool Mxfp4Rows(const Q& q, const E& e, int64_t rows, int64_t cols) {
+  return q.dimensions().size() == 2 && e.dimensions().size() == 2 && Rows(q) == rows && Rows(e) == rows &&
+         Cols(q) * 2 == cols && Cols(e) * 32 == cols;
+}
+template <typename Q, typename E>
+bool Mxfp4Operand(const Q& q, const E& e) {
+  auto d = q.dimensions(), x = e.dimensions();
+  return d.size() == 5 && x.size() == 4 && d[3] == 64 && d[4] == 16 && x[0] == d[0] && x[1] * 2 == d[2] &&
+         x[2] == d[1] * 32 && x[3] == 4;
+}
+
+}  // namespace
+
+// a [R, C] (f32/bf16) -> q [R, C / 2], exps [R, C / 32].
+static ffi::Error QuantizeRowsMxfp4Impl(hipStream_t stream, ffi::AnyBuffer a, ffi::ResultBuffer<ffi::U8> q,
+                                        ffi::ResultBuffer<ffi::U8> exps) {
+  const int d = DtypeCode(a.element_type());
+  if (d < 0) return BadDtype("hmoe_quantize_rows_mxfp4");
+  if (!Mxfp4Rows(*q, *exps, Rows(a), Cols(a))) return BadMxfp4("hmoe_quantize_rows_mxfp4");
+  return Status(hmoe_quantize_rows_mxfp4(a.untyped_data(), d, Rows(a), static_cast<int>(Cols(a)),
+                                         q->typed_data(), exps->typed_data(), S(stream)));
+}
+XLA_FFI_DEFINE_HANDLER_SYMBOL(HmoeQuantizeRowsMxfp4, QuantizeRowsMxfp4Impl,
+                              ffi::Ffi::Bind()
+                                  .Ctx<ffi::PlatformStream<hipStream_t>>()
+                                  .Arg<ffi::AnyBuffer>()
+                                  .Ret<ffi::Buffer<ffi::U8>>()
+                                  .Ret<ffi::Buffer<ffi::U8>>());
+
+// q [R, C / 2], exps [R, C / 32] -> out [R, C] (f32/bf16).
+static ffi::Error DequantizeRowsMxfp4Impl(hipStream_t stream, ffi::Buffer<ffi::U8> q,
+                                          ffi::Buffer<ffi::U8> exps, ffi::Result<ffi::AnyBuffer> out) {
+  const int d = DtypeCode(out->element_type());
+  if (d < 0) return BadDtype("hmoe_dequantize_rows_mxfp4");
+  if (!Mxfp4Rows(q, exps, Rows(*out), Cols(*out))) return BadMxfp4("hmoe_dequantize_rows_mxfp4");
+  return Status(hmoe_dequantize_rows_mxfp4(q.typed_data(), exps.typed_data(), Rows(q),
+                                           static_cast<int>(Cols(*out)), out->untyped_data(), d, S(stream)));
+}
+XLA_FFI_DEFINE_HANDLER_SYMBOL(HmoeDequantizeRowsMxfp4, DequantizeRowsMxfp4Impl,
+                              ffi::Ffi::Bind()
+                                  .Ctx<ffi::PlatformStream<hipStream_t>>()
+                                  .Arg<ffi::Buffer<ffi::U8>>()
+                                  .Arg<ffi::Buffer<ffi::U8>>()
+                                  .Ret<ffi::AnyBuffer>());
+
+// w_gate, w_up [N, D, F] (f32/bf16) -> codes, exponents of the gate/up operand.
+static ffi::Error PackMxfp4GateUpImpl(hipStream_t stream, ffi::AnyBuffer wg, ffi::AnyBuffer wu,
+                                      ffi::ResultBuffer<ffi::U8> packed, ffi::ResultBuffer<ffi::U8> exps) {
+  const int d = DtypeCode(wg.element_type());
+  if (d < 0 || DtypeCode(wu.element_type()) != d) return BadDtype("hmoe_pack_mxfp4_gate_up");
+  auto dims = wg.dimensions();
+  auto out = packed->dimensions();
+  if (!Mxfp4Operand(*packed, *exps) || out[0] != dims[0] || out[1] * 16 != dims[2] || out[2] * 64 != dims[1])
+    return BadMxfp4("hmoe_pack_mxfp4_gate_up");
+  return Status(hmoe_pack_mxfp4_gate_up(wg.untyped_data(), wu.untyped_data(), d, static_cast<int>(dims[0]),
+                                        static_cast<int>(dims[1]), static_cast<int>(dims[2]),
+                                        packed->typed_data(), exps->typed_data(), S(stream)));
+}
+XLA_FFI_DEFINE_HANDLER_SYMBOL(HmoePackMxfp4GateUp, PackMxfp4GateUpImpl,
+                              ffi::Ffi::Bind()
+                                  .Ctx<ffi::PlatformStream<hipStream_t>>()
+                                  .Arg<ffi::AnyBuffer>()
+                                  .Arg<ffi::AnyBuffer>()
+                                  .Ret<ffi::Buffer<ffi::U8>>()
+                                  .Ret<ffi::Buffer<ffi::U8>>());
+
+// w_down [N, F, D] (f32/bf16) -> codes, exponents of the down operand.
+static ffi::Error PackMxfp4DownImpl(hipStream_t stream, ffi::AnyBuffer wd, ffi::ResultBuffer<ffi::U8> packed,
+                                    ffi::ResultBuffer<ffi::U8> exps) {
+  const int d = DtypeCode(wd.element_type());
+  if (d < 0) return BadDtype("hmoe_pack_mxfp4_down");
+  auto dims = wd.dimensions();
+  auto out = packed->dimensions();
+  if (!Mxfp4Operand(*packed, *exps) || out[0] != dims[0] || out[1] * 32 != dims[2] || out[2] * 64 != dims[1])
+    return BadMxfp4("hmoe_pack_mxfp4_down");
+  return Status(hmoe_pack_mxfp4_down(wd.untyped_data(), d, static_cast<int>(dims[0]),
+                                     static_cast<int>(dims[1]), static_cast<int>(dims[2]),
+                                     packed->typed_data(), exps->typed_data(), S(stream)));
+}
+XLA_FFI_DEFINE_HANDLER_SYMBOL(HmoePackMxfp4Down, PackMxfp4DownImpl,
+                              ffi::Ffi::Bind()
+                                  .Ctx<ffi::PlatformStream<hipStream_t>>()
+                                  .Arg<ffi::AnyBuffer>()
+                                  .Ret<ffi::Buffer<ffi::U8>>()
+                                  .Ret<ffi::Buffer<ffi::U8>>());
+
+// codes, exponents of an operand -> out [N, rows, K] (f32/bf16).
+static ffi::Error UnpackMxfp4Impl(hipStream_t stream, ffi::Buffer<ffi::U8> packed, ffi::Buffer<ffi::U8> exps,
+                                  ffi::Result<ffi::AnyBuffer> out) {
+  const int d = DtypeCode(out->element_type());
+  if (d < 0) return BadDtype("hmoe_unpack_mxfp4");
+  auto in = packed.dimensions();
+  auto dims = out->dimensions();
+  if (!Mxfp4Operand(packed, exps) || dims.size() != 3 || dims[0] != in[0] || dims[1] != in[1] * 32 ||
+      dims[2] != in[2] * 64)
+    return BadMxfp4("hmoe_unpack_mxfp4");
+  return Status(hmoe_unpack_mxfp4(packed.typed_data(), exps.typed_data(), static_cast<int>(dims[0]),
+                                  static_cast<int>(dims[1]), static_cast<int>(dims[2]), out->untyped_data(), d,
+                                  S(stream)));
+}
+XLA_FFI_DEFINE_HANDLER_SYMBOL(HmoeUnpackMxfp4, UnpackMxfp4Impl,
+                              ffi::Ffi::Bind()
+                                  .Ctx<ffi::PlatformStream<hipStream_t>>()
+                                  .Arg<ffi::Buffer<ffi::U8>>()
+                                  .Arg<ffi::Buffer<ffi::U8>>()
+                                  .Ret<ffi::AnyBuffer>());
+
+// xs_q, xs_exp (rows in the experts' order), offsets [N+1], gate/up operand ->
+// h_q [rows, F / 2], h_exp [rows, F / 32].
+static ffi::Error GroupedGateUpMxfp4Impl(hipStream_t stream, ffi::Buffer<ffi::U8> xs_q,
+                                         ffi::Buffer<ffi::U8> xs_exp, ffi::Buffer<ffi::S32> offsets,
+                                         ffi::Buffer<ffi::U8> w, ffi::Buffer<ffi::U8> w_exp,
+                                         ffi::ResultBuffer<ffi::U8> h_q, ffi::ResultBuffer<ffi::U8> h_exp) {
+  auto d = w.dimensions();
+  const int64_t n = static_cast<int64_t>(offsets.element_count()) - 1;
+  if (!Mxfp4Operand(w, w_exp) || d[0] != n || !Mxfp4Rows(xs_q, xs_exp, Rows(xs_q), d[2] * 64) ||
+      !Mxfp4Rows(*h_q, *h_exp, Rows(xs_q), d[1] * 16))
+    return BadMxfp4("hmoe_grouped_gate_up_mxfp4");
+  return Status(hmoe_grouped_gate_up_mxfp4(xs_q.typed_data(), xs_exp.typed_data(), offsets.typed_data(),
+                                           static_cast<int>(n), Rows(xs_q), static_cast<int>(d[2] * 64),
+                                           static_cast<int>(d[1] * 16), w.typed_data(), w_exp.typed_data(),
+                                           h_q->typed_data(), h_exp->typed_data(), S(stream)));
+}
+XLA_FFI_DEFINE_HANDLER_SYMBOL(HmoeGroupedGateUpMxfp4, GroupedGateUpMxfp4Impl,
+                              ffi::Ffi::Bind()
+                                  .Ctx<ffi::PlatformStream<hipStream_t>>()
+                                  .Arg<ffi::Buffer<ffi::U8>>()
+                                  .Arg<ffi::Buffer<ffi::U8>>()
+                                  .Arg<ffi::Buffer<ffi::S32>>()
+                                  .Arg<ffi::Buffer<ffi::U8>>()
+                                  .Arg<ffi::Buffer<ffi::U8>>()
+                                  .Ret<ffi::Buffer<ffi::U8>>()
+                                  .Ret<ffi::Buffer<ffi::U8>>());
+
+// x_q, x_exp (tokens), perm_src [rows_cap], offsets [N+1], gate/up operand ->
+// h_q [rows_cap, F / 2], h_exp [rows_cap, F / 32].
+static ffi::Error GroupedGateUpMxfp4GatherImpl(hipStream_t stream, ffi::Buffer<ffi::U8> x_q,
+                                               ffi::Buffer<ffi::U8> x_exp, ffi::Buffer<ffi::S32> perm_src,
+                                               ffi::Buffer<ffi::S32> offsets, ffi::Buffer<ffi::U8> w,
+                                               ffi::Buffer<ffi::U8> w_exp, int64_t top_k,
+                                               ffi::ResultBuffer<ffi::U8> h_q,
+                                               ffi::ResultBuffer<ffi::U8> h_exp) {
+  auto d = w.dimensions();
+  const int64_t n = static_cast<int64_t>(offsets.element_count()) - 1;
+  const int64_t rows = static_cast<int64_t>(perm_src.element_count());
+  if (!Mxfp4Operand(w, w_exp) || d[0] != n || !Mxfp4Rows(x_q, x_exp, Rows(x_q), d[2] * 64) ||
+      !Mxfp4Rows(*h_q, *h_exp, rows, d[1] * 16))
+    return BadMxfp4("hmoe_grouped_gate_up_mxfp4_gather");
+  return Status(hmoe_grouped_gate_up_mxfp4_gather(
+      x_q.typed_data(), x_exp.typed_data(), Rows(x_q), static_cast<int>(top_k), perm_src.typed_data(),
+      offsets.typed_data(), static_cast<int>(n), rows, static_cast<int>(d[2] * 64),
+      static_cast<int>(d[1] * 16), w.typed_data(), w_exp.typed_data(), h_q->typed_data(),
+      h_exp->typed_data(), S(stream)));
+}
+XLA_FFI_DEFINE_HANDLER_SYMBOL(HmoeGroupedGateUpMxfp4Gather, GroupedGateUpMxfp4GatherImpl,
+                              ffi::Ffi::Bind()
+                                  .Ctx<ffi::PlatformStream<hipStream_t>>()
+                                  .Arg<ffi::Buffer<ffi::U8>>()
+                                  .Arg<ffi::Buffer<ffi::U8>>()
+                                  .Arg<ffi::Buffer<ffi::S32>>()
+                                  .Arg<ffi::Buffer<ffi::S32>>()
+                                  .Arg<ffi::Buffer<ffi::U8>>()
+                                  .Arg<ffi::Buffer<ffi::U8>>()
+                                  .Attr<int64_t>("top_k")
+                                  .Ret<ffi::Buffer<ffi::U8>>()
+                                  .Ret<ffi::Buffer<ffi::U8>>());
+
+// h_q, h_exp, offsets [N+1], down operand -> ys [rows, D] bf16.
+static ffi::Error GroupedDownMxfp4Impl(hipStream_t stream, ffi::Buffer<ffi::U8> h_q,
+                                       ffi::Buffer<ffi::U8> h_exp, ffi::Buffer<ffi::S32> offsets,
+                                       ffi::Buffer<ffi::U8> w, ffi::Buffer<ffi::U8> w_exp,
+                                       ffi::ResultBuffer<ffi::BF16> ys) {
+  auto d = w.dimensions();
+  const int64_t n = static_cast<int64_t>(offsets.element_count()) - 1;
+  if (!Mxfp4Operand(w, w_exp) || d[0] != n || !Mxfp4Rows(h_q, h_exp, Rows(h_q), d[2] * 64) ||
+      Rows(*ys) != Rows(h_q) || Cols(*ys) != d[1] * 32)
+    return BadMxfp4("hmoe_grouped_down_mxfp4");
+  return Status(hmoe_grouped_down_mxfp4(h_q.typed_data(), h_exp.typed_data(), offsets.typed_data(),
+                                        static_cast<int>(n), Rows(h_q), static_cast<int>(d[2] * 64),
+                                        static_cast<int>(d[1] * 32), w.typed_data(), w_exp.typed_data(),
+                                        ys->untyped_data(), S(stream)));
+}
+XLA_FFI_DEFINE_HANDLER_SYMBOL(HmoeGroupedDownMxfp4, GroupedDownMxfp4Impl,
+                              ffi::Ffi::Bind()
+                                  .Ctx<ffi::PlatformStream<hipStream_t>>()
+                                  .Arg<ffi::Buffer<ffi::U8>>()
+                                  .Arg<ffi::Buffer<ffi::U8>>()
+                                  .Arg<ffi::Buffer<ffi::S32>>()
+                                  .Arg<ffi::Buffer<ffi::U8>>()
+                                  .Arg<ffi::Buffer<ffi::U8>>()
+                                  .Ret<ffi::Buffer<ffi::BF16>>());
+
 // float32 compute dtype: masters as they are.
 static ffi::Error GroupedGateUpF32Impl(hipStream_t stream, ffi::Buffer<ffi::F32> xs,
                                        ffi::Buffer<ffi::S32> offsets,

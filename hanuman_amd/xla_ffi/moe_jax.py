@@ -74,6 +74,14 @@ TARGETS = {
     "hmoe_grouped_gate_up_fp8_qh": "HmoeGroupedGateUpFp8Qh",
     "hmoe_grouped_gate_up_fp8_gather_qh": "HmoeGroupedGateUpFp8GatherQh",
     "hmoe_grouped_down_fp8_mx": "HmoeGroupedDownFp8Mx",
+    "hmoe_quantize_rows_mxfp4": "HmoeQuantizeRowsMxfp4",
+    "hmoe_dequantize_rows_mxfp4": "HmoeDequantizeRowsMxfp4",
+    "hmoe_pack_mxfp4_gate_up": "HmoePackMxfp4GateUp",
+    "hmoe_pack_mxfp4_down": "HmoePackMxfp4Down",
+    "hmoe_unpack_mxfp4": "HmoeUnpackMxfp4",
+    "hmoe_grouped_gate_up_mxfp4": "HmoeGroupedGateUpMxfp4",
+    "hmoe_grouped_gate_up_mxfp4_gather": "HmoeGroupedGateUpMxfp4Gather",
+    "hmoe_grouped_down_mxfp4": "HmoeGroupedDownMxfp4",
     "hmoe_grouped_gate_up_f32": "HmoeGroupedGateUpF32",
     "hmoe_grouped_down_f32": "HmoeGroupedDownF32",
     "hmoe_combine": "HmoeCombine",

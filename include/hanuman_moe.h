@@ -381,6 +381,72 @@ int hmoe_grouped_wgrad_down_f32(const float* h, const float* d_ys, const int32_t
                                 int n_experts, int d_ff, int d_model, float* dw_down,
                                 hmoe_stream_t stream);
 
+/* ---- MXFP4 experts (no reference code): 4-bit rows times 4-bit weights -------
+ *
+ * MXFP4: every 32 consecutive values of a row share a power-of-two scale, an
+ * E8M0 byte E for 2^(E - 127), and each value is an e2m1 code (0, 0.5, 1, 1.5, 2,
+ * 3, 4, 6 and their negatives).  The scale is the smallest power of two at which
+ * the block's largest value rounds to 6 or less (E >= 0), a code is the value over
+ * the scale rounded to nearest, ties to the even code.  A block with a value that
+ * is not finite has E = 255 and zero codes and stands for NaN; a product with it is
+ * NaN.  A value past the format's range (a block whose largest is 1.75 * 2^127 or
+ * more) reads back as infinity.  Every pointer of an operand is 16-byte aligned. */
+
+/* a [rows, cols] (F32/BF16) -> q [rows, cols / 2] uint8 (the even column in a
+ * byte's low half), exps [rows, cols / 32] uint8.  cols % 32 == 0. */
+int hmoe_quantize_rows_mxfp4(const void* a, int a_dtype, int64_t rows, int cols, uint8_t* q,
+                             uint8_t* exps, hmoe_stream_t stream);
+/* The values of such rows, out [rows, cols] (F32/BF16; exact in both). */
+int hmoe_dequantize_rows_mxfp4(const uint8_t* q, const uint8_t* exps, int64_t rows, int cols,
+                               void* out, int out_dtype, hmoe_stream_t stream);
+
+/* Expert masters (F32/BF16) quantised along the reduction, blocks of 32 of its
+ * values, into the products' operands.  Operand rows are those of
+ * hmoe_pack_gate_up (2F an expert, 32 gate and 32 up columns alternating) and
+ * hmoe_pack_down (D an expert).  With K the reduction (D, F):
+ *   codes [N][rows / 32][K / 64][64][16]: bytes of lane 32 h + r hold the 32 codes
+ *         of row r (of the 32) from column 32 h (of the 64) on
+ *   exps  [N][K / 128][rows][4]
+ * of hmoe_packed_mxfp4_*_bytes and a sixteenth of that.  D % 128 == 0, F % 128 ==
+ * 0, N <= 1024. */
+size_t hmoe_packed_mxfp4_gate_up_bytes(int n_experts, int d_model, int d_ff);
+int hmoe_pack_mxfp4_gate_up(const void* w_gate, const void* w_up, int w_dtype, int n_experts,
+                            int d_model, int d_ff, uint8_t* packed, uint8_t* exps,
+                            hmoe_stream_t stream);
+size_t hmoe_packed_mxfp4_down_bytes(int n_experts, int d_ff, int d_model);
+int hmoe_pack_mxfp4_down(const void* w_down, int w_dtype, int n_experts, int d_ff, int d_model,
+                         uint8_t* packed, uint8_t* exps, hmoe_stream_t stream);
+/* The values of a packed operand, out [N, rows, cols] (F32/BF16): in BF16 the
+ * operand of the bf16 products (hmoe_pack_gate_up, hmoe_pack_down) with the same
+ * weights.  rows % 32 == 0, cols % 128 == 0. */
+int hmoe_unpack_mxfp4(const uint8_t* packed, const uint8_t* exps, int n_experts, int rows, int cols,
+                      void* out, int out_dtype, hmoe_stream_t stream);
+
+/* h of rows r of expert e's segment [offsets[e], offsets[e+1]) as MXFP4 rows: with
+ * g and u the float32 sums xs[r]·Wg[e] and xs[r]·Wu[e], h = silu(g) * u in float32
+ * and quantised from there (h is rounded once, to its codes).  xs_q [rows_cap, D/2],
+ * xs_exp [rows_cap, D/32], h_q [rows_cap, F/2], h_exp [rows_cap, F/32].  Rows past
+ * offsets[N] are not written.  D % 128 == 0, F % 128 == 0, N <= 1024. */
+int hmoe_grouped_gate_up_mxfp4(const uint8_t* xs_q, const uint8_t* xs_exp, const int32_t* offsets,
+                               int n_experts, int64_t rows_cap, int d_model, int d_ff,
+                               const uint8_t* w_packed, const uint8_t* w_exp, uint8_t* h_q,
+                               uint8_t* h_exp, hmoe_stream_t stream);
+/* The same h with the rows gathered by the product's loads, as
+ * hmoe_grouped_gate_up_gather does: x_q [tokens, D/2] and x_exp [tokens, D/32] are
+ * the quantised tokens and row r is token perm_src[r] / top_k (token 0 where
+ * perm_src[r] is -1).  tokens * D / 2 < 2^31. */
+int hmoe_grouped_gate_up_mxfp4_gather(const uint8_t* x_q, const uint8_t* x_exp, int64_t tokens,
+                                      int top_k, const int32_t* perm_src, const int32_t* offsets,
+                                      int n_experts, int64_t rows_cap, int d_model, int d_ff,
+                                      const uint8_t* w_packed, const uint8_t* w_exp, uint8_t* h_q,
+                                      uint8_t* h_exp, hmoe_stream_t stream);
+/* ys[r, :] = bf16( h[r]·Wd[e] ) per expert segment (float32 sums), ys [rows_cap, D]
+ * bf16.  Rows past offsets[N] are not written. */
+int hmoe_grouped_down_mxfp4(const uint8_t* h_q, const uint8_t* h_exp, const int32_t* offsets,
+                            int n_experts, int64_t rows_cap, int d_ff, int d_model,
+                            const uint8_t* w_packed, const uint8_t* w_exp, void* ys,
+                            hmoe_stream_t stream);
+
 /* ---- combine: moe.py:80-85 (replaces `ys[inv]` and the weighted einsum) - */
 
 /* out[t] = sum_k g'[t,k] * ys[slot_pos[t*K+k]] (+ residual[t]), g' the gates
