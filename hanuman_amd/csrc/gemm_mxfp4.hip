@@ -14,6 +14,9 @@
 // block (p / 32, k / 64) has the 32 codes of row r from column 32 h on, so a
 // fragment is one 1 KB run of memory, and its exponents [K / 128][rows][4] give
 // the lanes of a fragment one run of 128 bytes per 128 columns.
+#include <atomic>
+#include <type_traits>
+
 #include "quant_mxfp4.h"
 
 namespace hmoe {
@@ -208,6 +211,422 @@ __global__ __launch_bounds__(256) void grouped_mxfp4_rows(
   }
 }
 
+// ---- tiles for experts with many rows ------------------------------------------
+// One workgroup of eight waves a CU loops over BM x 256 tiles.  A K step is 128
+// values = 64 bytes of every row; the operands go from global memory into a ring of
+// four LDS stages (buffer_load ... lds), three steps ahead and on into the next
+// tile.  A's part of a stage has 64-byte rows whose 16-byte chunk c sits at c ^
+// swz64(r), so that 16 lanes of a fragment read cover all banks; B's is the
+// operand's own blocks of 1 KB, read lane by lane.  A step is two sub-steps of one
+// MFMA per pair of fragments; the fragments of the next sub-step are read during
+// each, so one barrier a step suffices: it is passed with the step after next in
+// LDS.  The exponents of four steps come together (16 bytes of every row of A, 1 KB
+// of B a step) into one of three regions, by one instruction of each wave.  (A tile's
+// last group may be one step: the steps being loaded then span three groups.)
+constexpr int kTileThreads = 512;
+constexpr int kStages = 4;
+constexpr int kRegions = 3;
+constexpr int kNumXcd = 8;
+constexpr int kTileN = 256;
+constexpr int kTileGroup = 8;
+
+template <int BM>
+struct TileCfg {
+  static constexpr int kA = BM * 64, kB = kTileN * 64;
+  static constexpr int kStage = kA + kB;
+  static constexpr int kExA = BM * 16, kExB = kTileN * 16;
+  static constexpr int kEx = kExA + kExB;
+  static constexpr int kLds = kStages * kStage + kRegions * kEx;
+  static constexpr int kNA = BM / 128, kNB = kTileN / 128;  // DMA instructions a wave and step
+  static constexpr int kFR = BM / 64;                       // row fragments a wave
+};
+
+typedef __attribute__((address_space(3))) void* lds_ptr_t;
+
+__device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, uint8_t* dst, uint32_t voff, int soff) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr_t)dst, 16, voff, soff, 0, 0);
+}
+
+// A use that later code is not moved before.  (A function of its own, like dma16:
+// where the operand's type depends on a template the host pass drops the kernel.)
+__device__ __forceinline__ void use_here(const f32x16& v) { asm volatile("" ::"v"(v)); }
+
+__device__ __forceinline__ int swz64(int r) { return (r >> 2) & 3; }
+
+// s_waitcnt vmcnt(N) lgkmcnt(0)
+template <int N>
+__device__ __forceinline__ void wait_vm_lgkm0() {
+  static_assert(N >= 0 && N < 64, "vmcnt is a 6-bit count");
+  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x0070);
+}
+
+// Exclusive scan of the experts' counts of BM-row tiles into tstart[0 .. n_experts].
+template <int BM>
+__device__ __forceinline__ int scan_tiles(const int32_t* __restrict__ offsets, int n_experts, int32_t* tstart,
+                                          int32_t* tmp) {
+  constexpr int kPer = kMaxExperts / kTileThreads;
+  const int tid = threadIdx.x;
+  int local[kPer], sum = 0;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    const int e = tid * kPer + j;
+    local[j] = e < n_experts ? (offsets[e + 1] - offsets[e] + BM - 1) / BM : 0;
+    sum += local[j];
+  }
+  tmp[tid] = sum;
+  __syncthreads();
+  for (int off = 1; off < kTileThreads; off <<= 1) {
+    const int v = tid >= off ? tmp[tid - off] : 0;
+    __syncthreads();
+    tmp[tid] += v;
+    __syncthreads();
+  }
+  int run = tmp[tid] - sum;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    const int e = tid * kPer + j;
+    if (e < n_experts) tstart[e] = run;
+    run += local[j];
+  }
+  if (tid == kTileThreads - 1) tstart[n_experts] = tmp[kTileThreads - 1];
+  __syncthreads();
+  return tstart[n_experts];
+}
+
+struct Tile {
+  int e, row0, rows, n0;
+};
+
+template <int BM, bool GATE_UP, bool GATHER>
+__global__ __launch_bounds__(kTileThreads) void grouped_mxfp4_tiles(
+    const uint8_t* __restrict__ A, const uint8_t* __restrict__ a_exp, const uint8_t* __restrict__ B,
+    const uint8_t* __restrict__ b_exp, const int32_t* __restrict__ offsets, int n_experts, int kdim, int ncols,
+    uint8_t* __restrict__ C, uint8_t* __restrict__ c_exp, const int32_t* __restrict__ gather_src, int gather_k,
+    int gather_rows) {
+  typedef TileCfg<BM> Cfg;
+  constexpr int kNA = Cfg::kNA, kNB = Cfg::kNB, kFR = Cfg::kFR;
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  __shared__ int32_t tstart[kMaxExperts + 1];
+  __shared__ int32_t scan_tmp[kTileThreads];
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n_tiles_n = ncols / kTileN;
+  const int total = __builtin_amdgcn_readfirstlane(scan_tiles<BM>(offsets, n_experts, tstart, scan_tmp)) * n_tiles_n;
+  // the tiles are split evenly over the XCDs (workgroup i runs on XCD i % 8)
+  const int xcd = blockIdx.x % kNumXcd;
+  const int per_xcd = gridDim.x / kNumXcd;
+  const int lo = static_cast<int>((static_cast<int64_t>(total) * xcd) / kNumXcd);
+  const int hi = static_cast<int>((static_cast<int64_t>(total) * (xcd + 1)) / kNumXcd);
+  const int first = lo + static_cast<int>(blockIdx.x) / kNumXcd;
+  if (first >= hi) return;  // uniform per workgroup
+  const int ks = kdim / 128;
+  const int row_bytes = kdim / 2, ex_bytes = kdim / 32;
+  const int iters = (hi - first + per_xcd - 1) / per_xcd * ks;
+
+  // An expert's tiles in groups of kTileGroup row tiles, each swept column by
+  // column (row tile fastest): an XCD's workgroups share few blocks of A and B.
+  auto decode = [&](int t) __attribute__((always_inline)) {
+    const int m_any = t / n_tiles_n;
+    int l = 0, h = n_experts;  // largest e with tstart[e] <= m_any (it has a tile)
+    while (h - l > 1) {
+      const int mid = (l + h) >> 1;
+      if (tstart[mid] <= m_any) l = mid; else h = mid;
+    }
+    const int e = __builtin_amdgcn_readfirstlane(l);
+    const int ts = __builtin_amdgcn_readfirstlane(tstart[e]);
+    const int me = __builtin_amdgcn_readfirstlane(tstart[e + 1]) - ts;
+    const int u = t - ts * n_tiles_n;
+    const int g = u / (kTileGroup * n_tiles_n);
+    const int gm = me - g * kTileGroup < kTileGroup ? me - g * kTileGroup : kTileGroup;
+    const int v = u - g * kTileGroup * n_tiles_n;
+    const int n_tile = v / gm;
+    Tile r;
+    r.e = e;
+    r.row0 = __builtin_amdgcn_readfirstlane(offsets[e]) + (g * kTileGroup + (v - n_tile * gm)) * BM;
+    r.rows = __builtin_amdgcn_readfirstlane(offsets[e + 1]) - r.row0;
+    r.rows = r.rows < BM ? r.rows : BM;
+    r.n0 = n_tile * kTileN;
+    return r;
+  };
+
+  // ---- load side -----------------------------------------------------------------
+  // A: instruction j of wave w fills rows 16 (w kNA + j) + lane / 4, chunk (lane & 3)
+  // ^ swz64(row).  B: blocks of 1 KB, block b = 2 (column / 32) + (64 values of the
+  // step), instruction j of wave w block w kNB + j.
+  const int a_row = 16 * wave * kNA + (lane >> 2);
+  const int a_byte = ((lane & 3) ^ ((lane >> 4) & 3)) * 16;
+  __amdgpu_buffer_rsrc_t a_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(A), 0,
+                                                                    GATHER ? gather_rows * row_bytes : 0, kBufferWord3);
+  __amdgpu_buffer_rsrc_t ae_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(a_exp), 0,
+                                                                     GATHER ? gather_rows * ex_bytes : 0, kBufferWord3);
+  __amdgpu_buffer_rsrc_t b_rsrc = a_rsrc, be_rsrc = a_rsrc;
+  uint32_t a_voff[kNA], ae_voff = 0, b_voff[kNB];
+#pragma unroll
+  for (int j = 0; j < kNB; ++j) {
+    const int blk = wave * kNB + j;
+    b_voff[j] = static_cast<uint32_t>((blk >> 1) * (kdim / 64) * 1024 + (blk & 1) * 1024 + lane * 16);
+  }
+  // waves 0 .. BM / 64 - 1 bring A's exponents, the next four B's (a step each)
+  constexpr int kExWavesA = BM / 64;
+  const bool ex_a = wave < kExWavesA, ex_b = wave >= kExWavesA && wave < kExWavesA + 4;
+  int ld_kb = 0, ld_g = 0, ld_t = first, ld_region = 0;
+  int32_t pf_src[kNA], pf_ex = 0;  // GATHER: sources of this lane's rows in the next tile
+  auto fetch_src = [&](int t) __attribute__((always_inline)) {
+    const Tile q = decode(t);
+#pragma unroll
+    for (int j = 0; j < kNA; ++j) {
+      const int r = a_row + 16 * j;
+      pf_src[j] = gather_src[q.row0 + (r < q.rows ? r : q.rows - 1)];
+    }
+    const int r = 64 * wave + lane;
+    if (ex_a) pf_ex = gather_src[q.row0 + (r < q.rows ? r : q.rows - 1)];
+  };
+  auto token = [&](int32_t slot) __attribute__((always_inline)) {
+    const int tk = slot >= 0 ? slot / gather_k : 0;  // a row without a source reads token 0
+    return static_cast<uint32_t>(tk < gather_rows ? tk : gather_rows - 1);
+  };
+  auto set_load_tile = [&](int t) __attribute__((always_inline)) {
+    const Tile q = decode(t);
+    const int64_t block = static_cast<int64_t>(q.e) * (ncols / 32) + q.n0 / 32;
+    b_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(B + block * (kdim / 64) * 1024), 0,
+                                               kTileN * row_bytes, kBufferWord3);
+    be_rsrc = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t*>(b_exp + (static_cast<int64_t>(q.e) * ks * ncols + q.n0) * 4), 0,
+        ((ks - 1) * ncols + kTileN) * 4, kBufferWord3);
+    if (GATHER) {
+#pragma unroll
+      for (int j = 0; j < kNA; ++j) a_voff[j] = token(pf_src[j]) * static_cast<uint32_t>(row_bytes) + a_byte;
+      ae_voff = token(pf_ex) * static_cast<uint32_t>(ex_bytes);
+      if (t + per_xcd < hi) fetch_src(t + per_xcd);
+    } else {
+      // rows past the segment repeat its last one; their results are not stored
+      a_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(A + static_cast<int64_t>(q.row0) * row_bytes), 0,
+                                                 q.rows * row_bytes, kBufferWord3);
+      ae_rsrc = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<uint8_t*>(a_exp + static_cast<int64_t>(q.row0) * ex_bytes), 0, q.rows * ex_bytes, kBufferWord3);
+#pragma unroll
+      for (int j = 0; j < kNA; ++j) {
+        const int r = a_row + 16 * j;
+        a_voff[j] = static_cast<uint32_t>((r < q.rows ? r : q.rows - 1) * row_bytes + a_byte);
+      }
+      const int r = 64 * wave + lane;
+      ae_voff = static_cast<uint32_t>((r < q.rows ? r : q.rows - 1) * ex_bytes);
+    }
+  };
+  // The exponents of steps ld_kb .. ld_kb + 3 (what a short last group reads past a
+  // row's end is not used; past the buffer it is not read).
+  auto issue_ex = [&]() __attribute__((always_inline)) {
+    uint8_t* ex = smem + kStages * Cfg::kStage + ld_region * Cfg::kEx;
+    if (ex_a) dma16(ae_rsrc, ex + wave * 1024, ae_voff + static_cast<uint32_t>(ld_kb * 4), 0);
+    if (ex_b) {
+      const int step = wave - kExWavesA;
+      if (ld_kb + step < ks)
+        dma16(be_rsrc, ex + Cfg::kExA + step * 1024, static_cast<uint32_t>(lane * 16), (ld_kb + step) * ncols * 4);
+    }
+  };
+  auto issue_a = [&](int stage, int j) __attribute__((always_inline)) {
+    dma16(a_rsrc, smem + stage * Cfg::kStage + (wave * kNA + j) * 1024, a_voff[j], ld_kb * 64);
+  };
+  auto issue_b = [&](int stage, int j) __attribute__((always_inline)) {
+    dma16(b_rsrc, smem + stage * Cfg::kStage + Cfg::kA + (wave * kNB + j) * 1024, b_voff[j], ld_kb * 2048);
+  };
+  // (every step loaded: the last one again, into a stage that nothing reads, so
+  // that a step always issues as many)
+  bool ld_more = true;
+  auto advance = [&]() __attribute__((always_inline)) {
+    if (ld_g + 1 < iters) {
+      ++ld_g;
+      if (++ld_kb == ks) {
+        ld_kb = 0;
+        ld_t += per_xcd;
+        set_load_tile(ld_t);
+      }
+      if ((ld_kb & 3) == 0) ld_region = ld_region + 1 == kRegions ? 0 : ld_region + 1;
+    } else {
+      ld_more = false;
+    }
+  };
+
+  // ---- compute side ----------------------------------------------------------------
+  // Wave w: rows (BM / 2) (w & 1) .. and columns 64 (w >> 1) .. of the tile.
+  const int wm = wave & 1, wn = wave >> 1;
+  const int frow = lane & 31, half = lane >> 5;
+  const int fsw = swz64(frow);
+  const int a_off = (wm * (BM / 2) + frow) * 64;
+  const int b_off = Cfg::kA + wn * 4096 + lane * 16;
+  u32x4 fa[2][kFR], fb[2][2];
+  int exa[2][kFR], exb[2][2];
+  auto read_frags = [&](auto Qc, int stage) __attribute__((always_inline)) {
+    constexpr int q = decltype(Qc)::value;
+    const uint8_t* st = smem + stage * Cfg::kStage;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) fb[q][j] = *reinterpret_cast<const u32x4*>(st + b_off + j * 2048 + q * 1024);
+#pragma unroll
+    for (int i = 0; i < kFR; ++i)
+      fa[q][i] = *reinterpret_cast<const u32x4*>(st + a_off + i * 2048 + (((2 * q + half) ^ fsw) * 16));
+  };
+  // Exponent words of a step, shifted so that byte 0 (2) is this lane's block of the
+  // first (second) sub-step.
+  auto read_ex = [&](auto Bc, int region, int kb) __attribute__((always_inline)) {
+    constexpr int b = decltype(Bc)::value;
+    const uint8_t* ex = smem + kStages * Cfg::kStage + region * Cfg::kEx;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      exb[b][j] = static_cast<int>(*reinterpret_cast<const uint32_t*>(
+                                       ex + Cfg::kExA + (kb & 3) * 1024 + (wn * 64 + j * 32 + frow) * 4) >>
+                                   (8 * half));
+#pragma unroll
+    for (int i = 0; i < kFR; ++i)
+      exa[b][i] = static_cast<int>(*reinterpret_cast<const uint32_t*>(
+                                       ex + (wm * (BM / 2) + i * 32 + frow) * 16 + (kb & 3) * 4) >>
+                                   (8 * half));
+  };
+  f32x16 acc[kFR][2];
+
+  int rd_kb = 0, rd_region = 0;  // the step whose fragments are read next
+  auto rd_advance = [&]() __attribute__((always_inline)) {
+    if (++rd_kb == ks) rd_kb = 0;
+    if ((rd_kb & 3) == 0) rd_region = rd_region + 1 == kRegions ? 0 : rd_region + 1;
+  };
+
+  // Step g on exponent words b = g & 1.
+  auto step = [&](auto Bc, int g) __attribute__((always_inline)) {
+    constexpr int b = decltype(Bc)::value;
+    const int stage = g & 3, next = (g + 1) & 3, fill = (g + 3) & 3;
+    if (ld_more && (ld_kb & 3) == 0) issue_ex();
+#pragma unroll
+    for (int j = 0; j < kNA; ++j) issue_a(fill, j);
+#pragma unroll
+    for (int j = 0; j < kNB; ++j) issue_b(fill, j);
+    advance();
+    read_frags(std::integral_constant<int, 1>{}, stage);
+#pragma unroll
+    for (int i = 0; i < kFR; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) acc[i][j] = mfma_fp4<0>(fb[0][j], fa[0][i], acc[i][j], exb[b][j], exa[b][i]);
+    read_frags(std::integral_constant<int, 0>{}, next);
+    read_ex(std::integral_constant<int, b ^ 1>{}, rd_region, rd_kb);
+    rd_advance();
+#pragma unroll
+    for (int i = 0; i < kFR; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) acc[i][j] = mfma_fp4<2>(fb[1][j], fa[1][i], acc[i][j], exb[b][j], exa[b][i]);
+    // used here, before the barrier, so that the products are not moved past it
+#pragma unroll
+    for (int i = 0; i < kFR; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) use_here(acc[i][j]);
+    // this wave's loads of step g + 2 have landed (step g + 3's may fly); after the
+    // barrier every wave's have
+    wait_vm_lgkm0<kNA + kNB>();
+    __builtin_amdgcn_s_barrier();
+  };
+
+  if (GATHER) fetch_src(first);
+  set_load_tile(first);
+#pragma unroll
+  for (int st = 0; st < 3; ++st) {
+    if (ld_more && (ld_kb & 3) == 0) issue_ex();
+#pragma unroll
+    for (int j = 0; j < kNA; ++j) issue_a(st, j);
+#pragma unroll
+    for (int j = 0; j < kNB; ++j) issue_b(st, j);
+    advance();
+  }
+  wait_vm_lgkm0<kNA + kNB>();
+  __builtin_amdgcn_s_barrier();
+  read_frags(std::integral_constant<int, 0>{}, 0);
+  read_ex(std::integral_constant<int, 0>{}, 0, 0);
+  rd_advance();
+
+  int g = 0;
+  for (int t = first; t < hi; t += per_xcd) {
+#pragma unroll
+    for (int i = 0; i < kFR; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+    for (int kb = 0; kb < ks; ++kb, ++g) {
+      step(std::integral_constant<int, 0>{}, g);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) exb[0][j] = exb[1][j];
+#pragma unroll
+      for (int i = 0; i < kFR; ++i) exa[0][i] = exa[1][i];
+    }
+    const Tile q = decode(t);
+    const int64_t r0 = q.row0;
+    const int row = wm * (BM / 2) + frow;
+    if constexpr (GATE_UP) {
+      const int d_ff = ncols / 2;
+      const __amdgpu_buffer_rsrc_t q_out =
+          __builtin_amdgcn_make_buffer_rsrc(C + r0 * (d_ff / 2), 0, q.rows * (d_ff / 2), kBufferWord3);
+      const __amdgpu_buffer_rsrc_t e_out =
+          __builtin_amdgcn_make_buffer_rsrc(c_exp + r0 * (d_ff / 32), 0, q.rows * (d_ff / 32), kBufferWord3);
+#pragma unroll
+      for (int i = 0; i < kFR; ++i)
+        store_h_block(acc[i][0], acc[i][1], q_out, e_out, row + 32 * i, q.n0 / 2 + wn * 32, d_ff, half);
+    } else {
+      const __amdgpu_buffer_rsrc_t out =
+          __builtin_amdgcn_make_buffer_rsrc(C + r0 * ncols * 2, 0, q.rows * ncols * 2, kBufferWord3);
+#pragma unroll
+      for (int i = 0; i < kFR; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) store_y_block(acc[i][j], out, row + 32 * i, q.n0 + wn * 64 + 32 * j, ncols, half);
+    }
+  }
+  // nothing may still be writing into LDS when the workgroup ends
+  __builtin_amdgcn_s_waitcnt(0);
+}
+
+// Workgroups of a persistent launch: one a CU, a multiple of the XCDs.
+int persistent_grid(const char* what, hipStream_t s, int* grid, int* dev_out) {
+  int dev = 0;
+  if (hipStreamGetDevice(s, &dev) != hipSuccess && hipGetDevice(&dev) != hipSuccess) {
+    set_error("%s: cannot query the stream's device", what);
+    return HMOE_ERR_HIP;
+  }
+  static std::atomic<int> cached[64];
+  int cus = dev >= 0 && dev < 64 ? cached[dev].load(std::memory_order_relaxed) : 0;
+  if (cus == 0) {
+    if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0) {
+      set_error("%s: cannot query the CU count of device %d", what, dev);
+      return HMOE_ERR_HIP;
+    }
+    if (dev >= 0 && dev < 64) cached[dev].store(cus, std::memory_order_relaxed);
+  }
+  const int g = cus / kNumXcd * kNumXcd;
+  *grid = g > 0 ? g : kNumXcd;
+  *dev_out = dev;
+  return HMOE_OK;
+}
+
+// Allows a kernel its dynamic LDS, once per device.
+template <typename Kernel>
+int allow_lds(const char* what, Kernel kernel, int bytes, int dev, std::atomic<uint64_t>* done) {
+  const uint64_t bit = dev >= 0 && dev < 64 ? uint64_t(1) << dev : 0;
+  if (bit != 0 && (done->load(std::memory_order_acquire) & bit) != 0) return HMOE_OK;
+  if (hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) !=
+      hipSuccess) {
+    set_error("%s: cannot allow %d bytes of dynamic LDS on device %d", what, bytes, dev);
+    return HMOE_ERR_HIP;
+  }
+  done->fetch_or(bit, std::memory_order_release);
+  return HMOE_OK;
+}
+
+template <int BM, bool GATE_UP, bool GATHER, typename... Args>
+int launch_tiles(const char* what, hipStream_t s, Args... args) {
+  int dev = 0, grid = 0;
+  if (int rc = persistent_grid(what, s, &grid, &dev)) return rc;
+  static std::atomic<uint64_t> done{0};
+  if (int rc = allow_lds(what, grouped_mxfp4_tiles<BM, GATE_UP, GATHER>, TileCfg<BM>::kLds, dev, &done)) return rc;
+  hipLaunchKernelGGL((grouped_mxfp4_tiles<BM, GATE_UP, GATHER>), dim3(grid), dim3(kTileThreads), TileCfg<BM>::kLds, s,
+                     args...);
+  return check_launch(what);
+}
+
 // The checks that the products share.
 int check_product(const char* what, int n_experts, int64_t rows_cap, int d_model, int d_ff) {
   HMOE_REQUIRE(n_experts >= 1 && n_experts <= kMaxExperts, "%s: n_experts must be in [1, %d] (got %d)", what,
@@ -225,6 +644,16 @@ int launch_product(const char* what, const uint8_t* a, const uint8_t* a_exp, con
                    const uint8_t* b_exp, const int32_t* offsets, int n_experts, int64_t rows_cap, int kdim,
                    int ncols, uint8_t* c, uint8_t* c_exp, const int32_t* gather_src, int gather_k,
                    int gather_rows, hipStream_t s) {
+  const double mean = static_cast<double>(rows_cap) / n_experts;
+  if (mean >= 64 && ncols % kTileN == 0) {
+    HMOE_REQUIRE(static_cast<int64_t>(kdim / 128) * ncols * 4 < (int64_t(1) << 31), "%s: operand too large", what);
+    HMOE_REQUIRE((ceil_div(rows_cap, 128) + n_experts) * (ncols / kTileN) < (int64_t(1) << 31), "%s: too many tiles", what);
+    if (mean >= 160)
+      return launch_tiles<256, GATE_UP, GATHER>(what, s, a, a_exp, b, b_exp, offsets, n_experts, kdim, ncols, c, c_exp,
+                                                gather_src, gather_k, gather_rows);
+    return launch_tiles<128, GATE_UP, GATHER>(what, s, a, a_exp, b, b_exp, offsets, n_experts, kdim, ncols, c, c_exp,
+                                              gather_src, gather_k, gather_rows);
+  }
   // an expert's last tile may hold one row
   const int64_t full = ceil_div(rows_cap, 32) + n_experts;
   const int64_t m_tiles = full < rows_cap ? full : rows_cap;
