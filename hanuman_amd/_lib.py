@@ -87,6 +87,7 @@ SIGNATURES = {
     "hmoe_packed_mxfp4_down_bytes": (_sz, [_i32, _i32, _i32]),
     "hmoe_pack_mxfp4_down": (_i32, [_vp, _i32, _i32, _i32, _i32, _vp, _vp, _vp]),
     "hmoe_unpack_mxfp4": (_i32, [_vp, _vp, _i32, _i32, _i32, _vp, _i32, _vp]),
+    "hmoe_grouped_mxfp4_form": (_i64, [_i64, _i32, _i32, _i32, _i32]),
     "hmoe_grouped_gate_up_mxfp4": (_i32, [_vp, _vp, _vp, _i32, _i64, _i32, _i32, _vp, _vp, _vp,
                                           _vp, _vp]),
     "hmoe_grouped_gate_up_mxfp4_gather": (_i32, [_vp, _vp, _i64, _i32, _vp, _vp, _i32, _i64, _i32,

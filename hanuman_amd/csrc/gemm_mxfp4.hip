@@ -14,7 +14,9 @@
 // block (p / 32, k / 64) has the 32 codes of row r from column 32 h on, so a
 // fragment is one 1 KB run of memory, and its exponents [K / 128][rows][4] give
 // the lanes of a fragment one run of 128 bytes per 128 columns.
+#include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <type_traits>
 
 #include "quant_mxfp4.h"
@@ -24,6 +26,7 @@ namespace {
 
 constexpr int kMaxExperts = 1024;
 constexpr int kBufferWord3 = 0x00020000;
+constexpr int kNonTemporal = 2;  // cache policy of a buffer access
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
@@ -89,14 +92,14 @@ __device__ __forceinline__ bool find_row_tile(const int32_t* __restrict__ offset
   return false;
 }
 
-// Epilogues.  Lane L of an accumulator holds row L % 32 of A's fragment and
-// columns 8 q + 4 (L / 32) + 0..3 (q = 0..3) of B's.  Stores go through a buffer
-// whose range ends at the segment's last row.
+// Epilogues.  Lane L of an accumulator holds row L % 32 of A's fragment and columns 8 q
+// + 4 (L / 32) + 0..3 (q = 0..3) of B's.  Stores go through a buffer whose range ends
+// at the segment's last row.
 //
-// h of 32 columns: gate in g, up in u; one scale block of the row.
-__device__ __forceinline__ void store_h_block(const f32x16& g, const f32x16& u, __amdgpu_buffer_rsrc_t q_out,
-                                              __amdgpu_buffer_rsrc_t e_out, int row, int hcol, int d_ff,
-                                              int half) {
+// h of 32 columns (gate in g, up in u), one scale block of the row: its exponent, and in
+// w[0] this lane's halves of dwords 0 and 1 of the row's 16 bytes of codes, in w[1] of
+// dwords 2 and 3.
+__device__ __forceinline__ uint32_t quantise_h(const f32x16& g, const f32x16& u, uint32_t (&w)[2]) {
   float h[16];
   uint32_t amax = 0;
 #pragma unroll
@@ -109,7 +112,6 @@ __device__ __forceinline__ void store_h_block(const f32x16& g, const f32x16& u, 
   const auto sw = __builtin_amdgcn_permlane32_swap(amax, amax, false, false);
   const uint32_t e = mxfp4_exponent(sw[0] > sw[1] ? sw[0] : sw[1]);
   const float inv = mxfp4_inverse(e);
-  uint32_t w[2];
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     float v[8];
@@ -117,19 +119,47 @@ __device__ __forceinline__ void store_h_block(const f32x16& g, const f32x16& u, 
     for (int k = 0; k < 8; ++k) v[k] = h[8 * j + k];
     w[j] = mxfp4_codes8(v, inv);
   }
-  // w[0] has this lane's halves of dwords 0 and 1 of the row's 16 bytes, w[1] of 2
-  // and 3; lanes 0..31 take dwords 0 and 1, lanes 32..63 the others
+  return e;
+}
+// The halves of lanes L (lo) and L + 32 (hi) put together.
+__device__ __forceinline__ u32x2_t join_codes(uint32_t lo, uint32_t hi) {
+  return u32x2_t{(lo & 0xffffu) | (hi << 16), (lo >> 16) | (hi & 0xffff0000u)};
+}
+
+// One block: lanes 0..31 store dwords 0 and 1 of their row, lanes 32..63 the others.
+__device__ __forceinline__ void store_h_block(const f32x16& g, const f32x16& u, __amdgpu_buffer_rsrc_t q_out,
+                                              __amdgpu_buffer_rsrc_t e_out, int row, int hcol, int d_ff,
+                                              int half) {
+  uint32_t w[2];
+  const uint32_t e = quantise_h(g, u, w);
   const auto t = __builtin_amdgcn_permlane32_swap(w[0], w[1], false, false);
-  const u32x2_t d = {(t[0] & 0xffffu) | (t[1] << 16), (t[0] >> 16) | (t[1] & 0xffff0000u)};
-  __builtin_amdgcn_raw_buffer_store_b64(d, q_out, (row * d_ff + hcol) / 2 + 8 * half, 0, 0);
+  __builtin_amdgcn_raw_buffer_store_b64(join_codes(t[0], t[1]), q_out, (row * d_ff + hcol) / 2 + 8 * half, 0, 0);
   if (half == 0)
     __builtin_amdgcn_raw_buffer_store_b8(static_cast<uint8_t>(e), e_out, row * (d_ff / 32) + hcol / 32, 0, 0);
 }
 
-// 32 bf16 columns of a row: lanes L and L + 32 trade groups, so that each stores
-// two runs of 16 bytes.
-__device__ __forceinline__ void store_y_block(const f32x16& y, __amdgpu_buffer_rsrc_t out, int row, int col,
-                                              int ldc, int half) {
+// Two blocks side by side: lanes 0..31 store the first's 16 bytes of their row and both
+// exponents, lanes 32..63 the second's.
+__device__ __forceinline__ void store_h_blocks(const f32x16 (&acc)[4], __amdgpu_buffer_rsrc_t q_out,
+                                               __amdgpu_buffer_rsrc_t e_out, int row, int hcol, int d_ff,
+                                               int half) {
+  uint32_t w0[2], w1[2];
+  const uint32_t e0 = quantise_h(acc[0], acc[1], w0);
+  const uint32_t e1 = quantise_h(acc[2], acc[3], w1);
+  // (lanes 0..31 give their halves of block 1 for the others' of block 0)
+  const auto a = __builtin_amdgcn_permlane32_swap(w0[0], w1[0], false, false);
+  const auto b = __builtin_amdgcn_permlane32_swap(w0[1], w1[1], false, false);
+  const u32x2_t lo = join_codes(a[0], a[1]), hi = join_codes(b[0], b[1]);
+  const u32x4 codes = {lo[0], lo[1], hi[0], hi[1]};
+  __builtin_amdgcn_raw_buffer_store_b128(codes, q_out, (row * d_ff + hcol) / 2 + 16 * half, 0, 0);
+  if (half == 0)
+    __builtin_amdgcn_raw_buffer_store_b16(static_cast<uint16_t>(e0 | (e1 << 8)), e_out,
+                                          row * (d_ff / 32) + hcol / 32, 0, 0);
+}
+
+// 32 bf16 columns of a row: lanes L and L + 32 trade groups, after which lane L < 32
+// holds columns 0..7 and 16..23 of its row, lane L + 32 columns 8..15 and 24..31.
+__device__ __forceinline__ void pack_y_block(const f32x16& y, u32x4& lo, u32x4& hi) {
   uint32_t d[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) d[k] = pack_bf16x2_rne(y[2 * k], y[2 * k + 1]);
@@ -142,27 +172,63 @@ __device__ __forceinline__ void store_y_block(const f32x16& y, __amdgpu_buffer_r
     d[4 + w] = p23[0];
     d[6 + w] = p23[1];
   }
+  lo = u32x4{d[0], d[1], d[2], d[3]};
+  hi = u32x4{d[4], d[5], d[6], d[7]};
+}
+__device__ __forceinline__ void store_y_block(const f32x16& y, __amdgpu_buffer_rsrc_t out, int row, int col,
+                                              int ldc, int half) {
+  u32x4 lo, hi;
+  pack_y_block(y, lo, hi);
   const int off = (row * ldc + col + half * 8) * 2;
-  const u32x4 lo = {d[0], d[1], d[2], d[3]};
-  const u32x4 hi = {d[4], d[5], d[6], d[7]};
   __builtin_amdgcn_raw_buffer_store_b128(lo, out, off, 0, 0);
   __builtin_amdgcn_raw_buffer_store_b128(hi, out, off + 32, 0, 0);
 }
 
-// A wave: 32 rows x 64 columns, operands straight from memory into registers.
-// Four waves side by side.
-template <bool GATE_UP, bool GATHER>
+// Two blocks side by side (64 columns, 32 rows), through 4 KB of LDS that only this
+// wave uses, so that a store instruction writes whole 128-byte lines: chunk c of row r
+// sits at c ^ (r & 7).  ys is far larger than the caches where tiles are taken, and kept
+// out of them: at 131072 x 2048 outputs of 1024 values the product takes 287 us with
+// 32-byte stores from the accumulators, 245 us with whole lines, 187 us with whole lines
+// that are not cached.
+__device__ __forceinline__ void store_y_blocks(const f32x16& y0, const f32x16& y1, uint8_t* lds,
+                                               __amdgpu_buffer_rsrc_t out, int row0, int col, int ldc, int lane) {
+  const int r = lane & 31, half = lane >> 5;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    u32x4 lo, hi;
+    pack_y_block(j == 0 ? y0 : y1, lo, hi);
+    uint8_t* p = lds + r * 128;
+    *reinterpret_cast<u32x4*>(p + (((4 * j + half) ^ (r & 7)) * 16)) = lo;
+    *reinterpret_cast<u32x4*>(p + (((4 * j + 2 + half) ^ (r & 7)) * 16)) = hi;
+  }
+#pragma unroll
+  for (int m = 0; m < 4; ++m) {
+    const int rr = 8 * m + (lane >> 3);
+    const u32x4 v = *reinterpret_cast<const u32x4*>(lds + rr * 128 + (((lane & 7) ^ (rr & 7)) * 16));
+    __builtin_amdgcn_raw_buffer_store_b128(v, out, ((row0 + rr) * ldc + col + (lane & 7) * 8) * 2, 0, kNonTemporal);
+  }
+}
+
+// ---- few rows ---------------------------------------------------------------------
+// 32 rows x 64 columns a wave, operands straight from memory into registers: with few
+// rows an expert every weight is used once or twice, and a fragment is one run of 1 KB.
+// Four groups of 128 values are loaded together, so that a wave has 20 KB on the way.
+// A workgroup is four waves: side by side (SPLIT 1), or on a quarter of the reduction
+// each, joined in LDS in their order (SPLIT 4).  The split shortens the one chain of
+// loads that a call of few tiles consists of.
+template <bool GATE_UP, bool GATHER, int SPLIT>
 __global__ __launch_bounds__(256) void grouped_mxfp4_rows(
     const uint8_t* __restrict__ A, const uint8_t* __restrict__ a_exp, const uint8_t* __restrict__ B,
     const uint8_t* __restrict__ b_exp, const int32_t* __restrict__ offsets, int n_experts, int kdim, int ncols,
     uint8_t* __restrict__ C, uint8_t* __restrict__ c_exp, const int32_t* __restrict__ gather_src, int gather_k,
     int gather_rows) {
   const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int frow = lane & 31, half = lane >> 5;
   RowTile t;
   if (!find_row_tile(offsets, n_experts, 32, blockIdx.y, t)) return;
-  const int n0 = (blockIdx.x * 4 + (threadIdx.x >> 6)) * 64;
-  if (n0 >= ncols) return;
+  const int n0 = SPLIT == 1 ? (blockIdx.x * 4 + wave) * 64 : blockIdx.x * 64;
+  if (n0 >= ncols) return;  // (SPLIT 1 only: no barrier follows there)
   int src = t.row0 + (frow < t.rows ? frow : t.rows - 1);  // rows past the segment repeat its last one
   if (GATHER) {
     const int slot = gather_src[src];
@@ -177,23 +243,69 @@ __global__ __launch_bounds__(256) void grouped_mxfp4_rows(
   const uint8_t* b1 = b0 + static_cast<int64_t>(kdim / 64) * 1024;
   const uint8_t* be = b_exp + (static_cast<int64_t>(t.e) * groups * ncols + n0 + frow) * 4;
   f32x16 acc0 = {}, acc1 = {};
-  for (int k = 0; k < groups; ++k) {
+  struct Group {
     u32x4 fa[2], f0[2], f1[2];
+    uint32_t ea, e0, e1;
+  };
+  auto load = [&](Group& p, int k) __attribute__((always_inline)) {
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
-      fa[q] = *reinterpret_cast<const u32x4*>(a + k * 64 + q * 32);
-      f0[q] = *reinterpret_cast<const u32x4*>(b0 + k * 2048 + q * 1024);
-      f1[q] = *reinterpret_cast<const u32x4*>(b1 + k * 2048 + q * 1024);
+      p.fa[q] = *reinterpret_cast<const u32x4*>(a + k * 64 + q * 32);
+      p.f0[q] = *reinterpret_cast<const u32x4*>(b0 + static_cast<int64_t>(k) * 2048 + q * 1024);
+      p.f1[q] = *reinterpret_cast<const u32x4*>(b1 + static_cast<int64_t>(k) * 2048 + q * 1024);
     }
-    // byte 0 (2) of the shifted words: this lane's block of the first (second) 64
-    const int ea = static_cast<int>(*reinterpret_cast<const uint32_t*>(ae + k * 4) >> (8 * half));
     const uint8_t* bk = be + static_cast<int64_t>(k) * ncols * 4;
-    const int e0 = static_cast<int>(*reinterpret_cast<const uint32_t*>(bk) >> (8 * half));
-    const int e1 = static_cast<int>(*reinterpret_cast<const uint32_t*>(bk + 128) >> (8 * half));
-    acc0 = mfma_fp4<0>(f0[0], fa[0], acc0, e0, ea);
-    acc1 = mfma_fp4<0>(f1[0], fa[0], acc1, e1, ea);
-    acc0 = mfma_fp4<2>(f0[1], fa[1], acc0, e0, ea);
-    acc1 = mfma_fp4<2>(f1[1], fa[1], acc1, e1, ea);
+    p.ea = *reinterpret_cast<const uint32_t*>(ae + k * 4);
+    p.e0 = *reinterpret_cast<const uint32_t*>(bk);
+    p.e1 = *reinterpret_cast<const uint32_t*>(bk + 128);
+  };
+  auto use = [&](const Group& p) __attribute__((always_inline)) {
+    // byte 0 (2) of the shifted words: this lane's block of the first (second) 64
+    const int ea = static_cast<int>(p.ea >> (8 * half));
+    const int e0 = static_cast<int>(p.e0 >> (8 * half));
+    const int e1 = static_cast<int>(p.e1 >> (8 * half));
+    acc0 = mfma_fp4<0>(p.f0[0], p.fa[0], acc0, e0, ea);
+    acc1 = mfma_fp4<0>(p.f1[0], p.fa[0], acc1, e1, ea);
+    acc0 = mfma_fp4<2>(p.f0[1], p.fa[1], acc0, e0, ea);
+    acc1 = mfma_fp4<2>(p.f1[1], p.fa[1], acc1, e1, ea);
+  };
+  int k = SPLIT == 1 ? 0 : groups * wave / SPLIT;
+  const int end = SPLIT == 1 ? groups : groups * (wave + 1) / SPLIT;
+  for (; k + 4 <= end; k += 4) {
+    Group p[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) load(p[j], k + j);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) use(p[j]);
+  }
+  for (; k < end; ++k) {
+    Group p;
+    load(p, k);
+    use(p);
+  }
+  if constexpr (SPLIT > 1) {
+    // wave 0 adds the others' sums, in their order
+    __shared__ f32x4 part[SPLIT - 1][8][64];
+    if (wave > 0) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        part[wave - 1][r][lane] = f32x4{acc0[4 * r], acc0[4 * r + 1], acc0[4 * r + 2], acc0[4 * r + 3]};
+        part[wave - 1][4 + r][lane] = f32x4{acc1[4 * r], acc1[4 * r + 1], acc1[4 * r + 2], acc1[4 * r + 3]};
+      }
+    }
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int w = 0; w < SPLIT - 1; ++w)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const f32x4 p0 = part[w][r][lane], p1 = part[w][4 + r][lane];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          acc0[4 * r + i] += p0[i];
+          acc1[4 * r + i] += p1[i];
+        }
+      }
   }
   const int64_t r0 = t.row0;
   if constexpr (GATE_UP) {
@@ -212,39 +324,43 @@ __global__ __launch_bounds__(256) void grouped_mxfp4_rows(
 }
 
 // ---- tiles for experts with many rows ------------------------------------------
-// One workgroup of eight waves a CU loops over BM x 256 tiles.  A K step is 128
-// values = 64 bytes of every row; the operands go from global memory into a ring of
-// four LDS stages (buffer_load ... lds), three steps ahead and on into the next
-// tile.  A's part of a stage has 64-byte rows whose 16-byte chunk c sits at c ^
-// swz64(r), so that 16 lanes of a fragment read cover all banks; B's is the
-// operand's own blocks of 1 KB, read lane by lane.  A step is two sub-steps of one
-// MFMA per pair of fragments; the fragments of the next sub-step are read during
-// each, so one barrier a step suffices: it is passed with the step after next in
-// LDS.  The exponents of four steps come together (16 bytes of every row of A, 1 KB
-// of B a step) into one of three regions, by one instruction of each wave.  (A tile's
-// last group may be one step: the steps being loaded then span three groups.)
-constexpr int kTileThreads = 512;
-constexpr int kStages = 4;
-constexpr int kRegions = 3;
+// Two workgroups of four waves share a CU, each looping over BM x 256 tiles: while one
+// is in its epilogue (the SwiGLU's exponentials and reciprocals alone take a quarter of
+// the products' time), switches tiles or waits at its barrier, the other's products run.
+// A K step is 128 values = 64 bytes of every row; the operands go from global memory
+// into a ring of three LDS stages (buffer_load ... lds), two steps ahead and on into
+// the next tile, one barrier a step.  A's part of a stage has 64-byte rows whose 16-byte
+// chunk c sits at c ^ swz64(r), so that 16 lanes of a fragment read cover all banks;
+// B's is the operand's own blocks of 1 KB, read lane by lane, and its exponents are a
+// run of 1 KB.  A's exponents, 16 bytes of every row, come for up to four steps at once
+// into one of two regions (three with 64 rows, where a tile may be a single step).  The
+// last column tile may be 128 columns wide: the waves of the other half load and compute
+// the first half's again and store nothing.
+constexpr int kTileThreads = 256;
+constexpr int kStages = 3;
 constexpr int kNumXcd = 8;
 constexpr int kTileN = 256;
 constexpr int kTileGroup = 8;
 
 template <int BM>
 struct TileCfg {
-  static constexpr int kA = BM * 64, kB = kTileN * 64;
-  static constexpr int kStage = kA + kB;
-  static constexpr int kExA = BM * 16, kExB = kTileN * 16;
-  static constexpr int kEx = kExA + kExB;
-  static constexpr int kLds = kStages * kStage + kRegions * kEx;
-  static constexpr int kNA = BM / 128, kNB = kTileN / 128;  // DMA instructions a wave and step
-  static constexpr int kFR = BM / 64;                       // row fragments a wave
+  static constexpr int kA = BM * 64, kB = kTileN * 64, kExB = kTileN * 4;
+  static constexpr int kStage = kA + kB + kExB;
+  static constexpr int kExA = BM * 16;
+  static constexpr int kRegions = BM == 64 ? 3 : 2;
+  static constexpr int kLds = kStages * kStage + kRegions * kExA;
+  static constexpr int kNA = BM / 64, kNB = kTileN / 64;  // DMA instructions a wave and step
+  static constexpr int kFR = BM / 64;                      // row fragments a wave
+  static_assert(2 * kLds <= 160 * 1024, "two workgroups a CU");
 };
 
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
 
 __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, uint8_t* dst, uint32_t voff, int soff) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr_t)dst, 16, voff, soff, 0, 0);
+}
+__device__ __forceinline__ void dma4(__amdgpu_buffer_rsrc_t r, uint8_t* dst, uint32_t voff, int soff) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr_t)dst, 4, voff, soff, 0, 0);
 }
 
 // A use that later code is not moved before.  (A function of its own, like dma16:
@@ -260,45 +376,80 @@ __device__ __forceinline__ void wait_vm_lgkm0() {
   __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x0070);
 }
 
-// Exclusive scan of the experts' counts of BM-row tiles into tstart[0 .. n_experts].
-template <int BM>
-__device__ __forceinline__ int scan_tiles(const int32_t* __restrict__ offsets, int n_experts, int32_t* tstart,
-                                          int32_t* tmp) {
-  constexpr int kPer = kMaxExperts / kTileThreads;
-  const int tid = threadIdx.x;
-  int local[kPer], sum = 0;
+// Row tiles of all experts.
+__device__ __forceinline__ int count_row_tiles(const int32_t* __restrict__ offsets, int n_experts, int bm) {
+  const int lane = threadIdx.x & 63;
+  int sum = 0;
+  for (int e = lane; e < n_experts; e += 64) sum += (offsets[e + 1] - offsets[e] + bm - 1) / bm;
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    const int e = tid * kPer + j;
-    local[j] = e < n_experts ? (offsets[e + 1] - offsets[e] + BM - 1) / BM : 0;
-    sum += local[j];
-  }
-  tmp[tid] = sum;
-  __syncthreads();
-  for (int off = 1; off < kTileThreads; off <<= 1) {
-    const int v = tid >= off ? tmp[tid - off] : 0;
-    __syncthreads();
-    tmp[tid] += v;
-    __syncthreads();
-  }
-  int run = tmp[tid] - sum;
-#pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    const int e = tid * kPer + j;
-    if (e < n_experts) tstart[e] = run;
-    run += local[j];
-  }
-  if (tid == kTileThreads - 1) tstart[n_experts] = tmp[kTileThreads - 1];
-  __syncthreads();
-  return tstart[n_experts];
+  for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
+  return __builtin_amdgcn_readfirstlane(sum);
 }
 
-struct Tile {
-  int e, row0, rows, n0;
+// Where a workgroup is in the experts' tiles.  An expert's tiles are taken in groups of
+// kTileGroup row tiles, each swept column by column (row tile fastest), so that an XCD's
+// workgroups share few blocks of A and B.
+template <int BM>
+struct TileCursor {
+  int e, before, tiles;  // expert, row tiles before its first, its row tiles
+  int seg0, seg1;        // its rows
+  int row0, rows, n0;    // the tile
+
+  __device__ __forceinline__ void expert(const int32_t* __restrict__ offsets, int n) {
+    e = n;
+    seg0 = __builtin_amdgcn_readfirstlane(offsets[n]);
+    seg1 = __builtin_amdgcn_readfirstlane(offsets[n + 1]);
+    tiles = (seg1 - seg0 + BM - 1) / BM;
+  }
+  // The expert of row tile m, 64 experts at a time (m is below their row tiles).
+  __device__ __forceinline__ void find(const int32_t* __restrict__ offsets, int n_experts, int m) {
+    const int lane = threadIdx.x & 63;
+    before = 0;
+    for (int base = 0;; base += 64) {
+      const int ee = base + lane;
+      const int mine = ee < n_experts ? (offsets[ee + 1] - offsets[ee] + BM - 1) / BM : 0;
+      int sum = mine;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int up = __shfl_up(sum, d);
+        sum += lane >= d ? up : 0;
+      }
+      const int total = lane_bcast(sum, 63);
+      if (m < before + total || base + 64 >= n_experts) {
+        const uint64_t past = __ballot(before + sum > m);
+        const int src = past != 0 ? __builtin_ctzll(past) : 63;
+        before += lane_bcast(sum - mine, src);
+        expert(offsets, base + src);
+        return;
+      }
+      before += total;
+    }
+  }
+  // On to tile t (t grows from call to call).
+  __device__ __forceinline__ void move(const int32_t* __restrict__ offsets, int t, int n_tiles_n) {
+    const int m_any = t / n_tiles_n;
+    while (m_any >= before + tiles) {
+      before += tiles;
+      expert(offsets, e + 1);
+    }
+    const int u = t - before * n_tiles_n;
+    const int g = u / (kTileGroup * n_tiles_n);
+    const int left = tiles - g * kTileGroup;
+    const int gm = left < kTileGroup ? left : kTileGroup;
+    const int v = u - g * kTileGroup * n_tiles_n;
+    const int n_tile = v / gm;
+    row0 = seg0 + (g * kTileGroup + (v - n_tile * gm)) * BM;
+    rows = seg1 - row0 < BM ? seg1 - row0 : BM;
+    n0 = n_tile * kTileN;
+  }
 };
 
+// Steps of the group that starts with `left` steps to go: four, but no group of one
+// after another (the steps in the ring then span two groups at most).
+__device__ __forceinline__ int group_steps(int left) { return left == 5 ? 3 : left < 4 ? left : 4; }
+
 template <int BM, bool GATE_UP, bool GATHER>
-__global__ __launch_bounds__(kTileThreads) void grouped_mxfp4_tiles(
+__global__ __launch_bounds__(kTileThreads, 2) void grouped_mxfp4_tiles(
     const uint8_t* __restrict__ A, const uint8_t* __restrict__ a_exp, const uint8_t* __restrict__ B,
     const uint8_t* __restrict__ b_exp, const int32_t* __restrict__ offsets, int n_experts, int kdim, int ncols,
     uint8_t* __restrict__ C, uint8_t* __restrict__ c_exp, const int32_t* __restrict__ gather_src, int gather_k,
@@ -306,13 +457,11 @@ __global__ __launch_bounds__(kTileThreads) void grouped_mxfp4_tiles(
   typedef TileCfg<BM> Cfg;
   constexpr int kNA = Cfg::kNA, kNB = Cfg::kNB, kFR = Cfg::kFR;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-  __shared__ int32_t tstart[kMaxExperts + 1];
-  __shared__ int32_t scan_tmp[kTileThreads];
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int n_tiles_n = ncols / kTileN;
-  const int total = __builtin_amdgcn_readfirstlane(scan_tiles<BM>(offsets, n_experts, tstart, scan_tmp)) * n_tiles_n;
+  const int n_tiles_n = (ncols + kTileN - 1) / kTileN;
+  const int total = count_row_tiles(offsets, n_experts, BM) * n_tiles_n;
   // the tiles are split evenly over the XCDs (workgroup i runs on XCD i % 8)
   const int xcd = blockIdx.x % kNumXcd;
   const int per_xcd = gridDim.x / kNumXcd;
@@ -324,36 +473,14 @@ __global__ __launch_bounds__(kTileThreads) void grouped_mxfp4_tiles(
   const int row_bytes = kdim / 2, ex_bytes = kdim / 32;
   const int iters = (hi - first + per_xcd - 1) / per_xcd * ks;
 
-  // An expert's tiles in groups of kTileGroup row tiles, each swept column by
-  // column (row tile fastest): an XCD's workgroups share few blocks of A and B.
-  auto decode = [&](int t) __attribute__((always_inline)) {
-    const int m_any = t / n_tiles_n;
-    int l = 0, h = n_experts;  // largest e with tstart[e] <= m_any (it has a tile)
-    while (h - l > 1) {
-      const int mid = (l + h) >> 1;
-      if (tstart[mid] <= m_any) l = mid; else h = mid;
-    }
-    const int e = __builtin_amdgcn_readfirstlane(l);
-    const int ts = __builtin_amdgcn_readfirstlane(tstart[e]);
-    const int me = __builtin_amdgcn_readfirstlane(tstart[e + 1]) - ts;
-    const int u = t - ts * n_tiles_n;
-    const int g = u / (kTileGroup * n_tiles_n);
-    const int gm = me - g * kTileGroup < kTileGroup ? me - g * kTileGroup : kTileGroup;
-    const int v = u - g * kTileGroup * n_tiles_n;
-    const int n_tile = v / gm;
-    Tile r;
-    r.e = e;
-    r.row0 = __builtin_amdgcn_readfirstlane(offsets[e]) + (g * kTileGroup + (v - n_tile * gm)) * BM;
-    r.rows = __builtin_amdgcn_readfirstlane(offsets[e + 1]) - r.row0;
-    r.rows = r.rows < BM ? r.rows : BM;
-    r.n0 = n_tile * kTileN;
-    return r;
-  };
-
   // ---- load side -----------------------------------------------------------------
   // A: instruction j of wave w fills rows 16 (w kNA + j) + lane / 4, chunk (lane & 3)
   // ^ swz64(row).  B: blocks of 1 KB, block b = 2 (column / 32) + (64 values of the
-  // step), instruction j of wave w block w kNB + j.
+  // step), instruction j of wave w block w kNB + j; its exponents 256 bytes a wave.
+  static_assert(kNB == 4, "two blocks of columns a wave");
+  TileCursor<BM> ld;
+  ld.find(offsets, n_experts, first / n_tiles_n);
+  TileCursor<BM> cur = ld;
   const int a_row = 16 * wave * kNA + (lane >> 2);
   const int a_byte = ((lane & 3) ^ ((lane >> 4) & 3)) * 16;
   __amdgpu_buffer_rsrc_t a_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(A), 0,
@@ -361,219 +488,193 @@ __global__ __launch_bounds__(kTileThreads) void grouped_mxfp4_tiles(
   __amdgpu_buffer_rsrc_t ae_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(a_exp), 0,
                                                                      GATHER ? gather_rows * ex_bytes : 0, kBufferWord3);
   __amdgpu_buffer_rsrc_t b_rsrc = a_rsrc, be_rsrc = a_rsrc;
-  uint32_t a_voff[kNA], ae_voff = 0, b_voff[kNB];
-#pragma unroll
-  for (int j = 0; j < kNB; ++j) {
-    const int blk = wave * kNB + j;
-    b_voff[j] = static_cast<uint32_t>((blk >> 1) * (kdim / 64) * 1024 + (blk & 1) * 1024 + lane * 16);
-  }
-  // waves 0 .. BM / 64 - 1 bring A's exponents, the next four B's (a step each)
-  constexpr int kExWavesA = BM / 64;
-  const bool ex_a = wave < kExWavesA, ex_b = wave >= kExWavesA && wave < kExWavesA + 4;
-  int ld_kb = 0, ld_g = 0, ld_t = first, ld_region = 0;
-  int32_t pf_src[kNA], pf_ex = 0;  // GATHER: sources of this lane's rows in the next tile
-  auto fetch_src = [&](int t) __attribute__((always_inline)) {
-    const Tile q = decode(t);
+  uint32_t a_voff[kNA], ae_voff = 0;
+  const int b_col = (kdim / 64) * 1024;  // bytes of 32 columns
+  int b_wave = 0, be_wave = 0;           // where this wave's part of B's tile begins
+  const bool ex_a = wave < BM / 64;  // the waves that bring A's exponents
+  int ld_kb = 0, ld_left = 0, ld_g = 0, ld_t = first, ld_region = Cfg::kRegions - 1, ld_stage = 0;
+  int32_t pf_src[kNA], pf_ex = 0;  // GATHER: sources of this lane's rows
+  auto fetch_src = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int j = 0; j < kNA; ++j) {
       const int r = a_row + 16 * j;
-      pf_src[j] = gather_src[q.row0 + (r < q.rows ? r : q.rows - 1)];
+      pf_src[j] = gather_src[ld.row0 + (r < ld.rows ? r : ld.rows - 1)];
     }
     const int r = 64 * wave + lane;
-    if (ex_a) pf_ex = gather_src[q.row0 + (r < q.rows ? r : q.rows - 1)];
+    if (ex_a) pf_ex = gather_src[ld.row0 + (r < ld.rows ? r : ld.rows - 1)];
   };
   auto token = [&](int32_t slot) __attribute__((always_inline)) {
     const int tk = slot >= 0 ? slot / gather_k : 0;  // a row without a source reads token 0
     return static_cast<uint32_t>(tk < gather_rows ? tk : gather_rows - 1);
   };
-  auto set_load_tile = [&](int t) __attribute__((always_inline)) {
-    const Tile q = decode(t);
-    const int64_t block = static_cast<int64_t>(q.e) * (ncols / 32) + q.n0 / 32;
-    b_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(B + block * (kdim / 64) * 1024), 0,
-                                               kTileN * row_bytes, kBufferWord3);
+  auto set_load_tile = [&]() __attribute__((always_inline)) {
+    ld.move(offsets, ld_t, n_tiles_n);
+    if (GATHER) fetch_src();
+    const int64_t block = static_cast<int64_t>(ld.e) * (ncols / 32) + ld.n0 / 32;
+    const int width = ncols - ld.n0 < kTileN ? ncols - ld.n0 : kTileN;
+    const int part = 64 * wave < width ? wave : wave - 2;  // (a tile of 128 columns: waves 0 and 1 again)
+    b_wave = part * 2 * b_col;
+    be_wave = part * 256;
+    b_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(B + block * b_col), 0, width * row_bytes,
+                                               kBufferWord3);
     be_rsrc = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<uint8_t*>(b_exp + (static_cast<int64_t>(q.e) * ks * ncols + q.n0) * 4), 0,
-        ((ks - 1) * ncols + kTileN) * 4, kBufferWord3);
+        const_cast<uint8_t*>(b_exp + (static_cast<int64_t>(ld.e) * ks * ncols + ld.n0) * 4), 0,
+        ((ks - 1) * ncols + width) * 4, kBufferWord3);
     if (GATHER) {
 #pragma unroll
       for (int j = 0; j < kNA; ++j) a_voff[j] = token(pf_src[j]) * static_cast<uint32_t>(row_bytes) + a_byte;
       ae_voff = token(pf_ex) * static_cast<uint32_t>(ex_bytes);
-      if (t + per_xcd < hi) fetch_src(t + per_xcd);
     } else {
       // rows past the segment repeat its last one; their results are not stored
-      a_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(A + static_cast<int64_t>(q.row0) * row_bytes), 0,
-                                                 q.rows * row_bytes, kBufferWord3);
+      a_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(A + static_cast<int64_t>(ld.row0) * row_bytes),
+                                                 0, ld.rows * row_bytes, kBufferWord3);
       ae_rsrc = __builtin_amdgcn_make_buffer_rsrc(
-          const_cast<uint8_t*>(a_exp + static_cast<int64_t>(q.row0) * ex_bytes), 0, q.rows * ex_bytes, kBufferWord3);
+          const_cast<uint8_t*>(a_exp + static_cast<int64_t>(ld.row0) * ex_bytes), 0, ld.rows * ex_bytes, kBufferWord3);
 #pragma unroll
       for (int j = 0; j < kNA; ++j) {
         const int r = a_row + 16 * j;
-        a_voff[j] = static_cast<uint32_t>((r < q.rows ? r : q.rows - 1) * row_bytes + a_byte);
+        a_voff[j] = static_cast<uint32_t>((r < ld.rows ? r : ld.rows - 1) * row_bytes + a_byte);
       }
       const int r = 64 * wave + lane;
-      ae_voff = static_cast<uint32_t>((r < q.rows ? r : q.rows - 1) * ex_bytes);
+      ae_voff = static_cast<uint32_t>((r < ld.rows ? r : ld.rows - 1) * ex_bytes);
     }
+    ld_kb = 0;
   };
-  // The exponents of steps ld_kb .. ld_kb + 3 (what a short last group reads past a
-  // row's end is not used; past the buffer it is not read).
-  auto issue_ex = [&]() __attribute__((always_inline)) {
-    uint8_t* ex = smem + kStages * Cfg::kStage + ld_region * Cfg::kEx;
-    if (ex_a) dma16(ae_rsrc, ex + wave * 1024, ae_voff + static_cast<uint32_t>(ld_kb * 4), 0);
-    if (ex_b) {
-      const int step = wave - kExWavesA;
-      if (ld_kb + step < ks)
-        dma16(be_rsrc, ex + Cfg::kExA + step * 1024, static_cast<uint32_t>(lane * 16), (ld_kb + step) * ncols * 4);
-    }
-  };
-  auto issue_a = [&](int stage, int j) __attribute__((always_inline)) {
-    dma16(a_rsrc, smem + stage * Cfg::kStage + (wave * kNA + j) * 1024, a_voff[j], ld_kb * 64);
-  };
-  auto issue_b = [&](int stage, int j) __attribute__((always_inline)) {
-    dma16(b_rsrc, smem + stage * Cfg::kStage + Cfg::kA + (wave * kNB + j) * 1024, b_voff[j], ld_kb * 2048);
-  };
-  // (every step loaded: the last one again, into a stage that nothing reads, so
-  // that a step always issues as many)
-  bool ld_more = true;
-  auto advance = [&]() __attribute__((always_inline)) {
-    if (ld_g + 1 < iters) {
-      ++ld_g;
-      if (++ld_kb == ks) {
-        ld_kb = 0;
+  // One step into the ring.  (Every step loaded: the last one again, into a stage that
+  // nothing reads, so that a step always issues as many.)
+  auto issue = [&]() __attribute__((always_inline)) {
+    if (ld_g < iters && ld_left == 0) {
+      if (ld_kb == ks) {
         ld_t += per_xcd;
-        set_load_tile(ld_t);
+        set_load_tile();
       }
-      if ((ld_kb & 3) == 0) ld_region = ld_region + 1 == kRegions ? 0 : ld_region + 1;
-    } else {
-      ld_more = false;
+      ld_left = group_steps(ks - ld_kb);
+      ld_region = ld_region + 1 == Cfg::kRegions ? 0 : ld_region + 1;
+      // (what a short group reads past a row's end is not used; past the buffer it is
+      // not read)
+      if (ex_a)
+        dma16(ae_rsrc, smem + kStages * Cfg::kStage + ld_region * Cfg::kExA + wave * 1024,
+              ae_voff + static_cast<uint32_t>(ld_kb * 4), 0);
     }
+    const int kb = ld_g < iters ? ld_kb : ld_kb - 1;
+    uint8_t* st = smem + ld_stage * Cfg::kStage;
+#pragma unroll
+    for (int j = 0; j < kNA; ++j) dma16(a_rsrc, st + (wave * kNA + j) * 1024, a_voff[j], kb * 64);
+#pragma unroll
+    for (int j = 0; j < kNB; ++j)
+      dma16(b_rsrc, st + Cfg::kA + (wave * kNB + j) * 1024, static_cast<uint32_t>(lane * 16),
+            b_wave + (j >> 1) * b_col + kb * 2048 + (j & 1) * 1024);
+    dma4(be_rsrc, st + Cfg::kA + Cfg::kB + wave * 256, static_cast<uint32_t>(lane * 4), be_wave + kb * ncols * 4);
+    if (ld_g < iters) {
+      ++ld_g;
+      ++ld_kb;
+      --ld_left;
+    }
+    ld_stage = ld_stage + 1 == kStages ? 0 : ld_stage + 1;
   };
 
   // ---- compute side ----------------------------------------------------------------
-  // Wave w: rows (BM / 2) (w & 1) .. and columns 64 (w >> 1) .. of the tile.
+  // Wave w: rows (BM / 2) (w & 1) .. and columns 128 (w >> 1) .. of the tile.
   const int wm = wave & 1, wn = wave >> 1;
   const int frow = lane & 31, half = lane >> 5;
   const int fsw = swz64(frow);
   const int a_off = (wm * (BM / 2) + frow) * 64;
-  const int b_off = Cfg::kA + wn * 4096 + lane * 16;
-  u32x4 fa[2][kFR], fb[2][2];
-  int exa[2][kFR], exb[2][2];
-  auto read_frags = [&](auto Qc, int stage) __attribute__((always_inline)) {
-    constexpr int q = decltype(Qc)::value;
+  const int b_off = Cfg::kA + wn * 8192 + lane * 16;
+  const int be_off = Cfg::kA + Cfg::kB + (wn * 128 + frow) * 4;
+  const int ae_off = kStages * Cfg::kStage + (wm * (BM / 2) + frow) * 16;
+  f32x16 acc[kFR][4];
+  int stage = 0, region = Cfg::kRegions - 1, left = 0, in_group = 0;
+  auto step = [&]() __attribute__((always_inline)) {
     const uint8_t* st = smem + stage * Cfg::kStage;
+    u32x4 fa[2][kFR], fb[2][4];
+    int exa[kFR], exb[4];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) fb[q][j] = *reinterpret_cast<const u32x4*>(st + b_off + j * 2048 + q * 1024);
-#pragma unroll
-    for (int i = 0; i < kFR; ++i)
-      fa[q][i] = *reinterpret_cast<const u32x4*>(st + a_off + i * 2048 + (((2 * q + half) ^ fsw) * 16));
-  };
-  // Exponent words of a step, shifted so that byte 0 (2) is this lane's block of the
-  // first (second) sub-step.
-  auto read_ex = [&](auto Bc, int region, int kb) __attribute__((always_inline)) {
-    constexpr int b = decltype(Bc)::value;
-    const uint8_t* ex = smem + kStages * Cfg::kStage + region * Cfg::kEx;
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-      exb[b][j] = static_cast<int>(*reinterpret_cast<const uint32_t*>(
-                                       ex + Cfg::kExA + (kb & 3) * 1024 + (wn * 64 + j * 32 + frow) * 4) >>
-                                   (8 * half));
+    for (int j = 0; j < 4; ++j)
+      exb[j] = static_cast<int>(*reinterpret_cast<const uint32_t*>(st + be_off + j * 128) >> (8 * half));
 #pragma unroll
     for (int i = 0; i < kFR; ++i)
-      exa[b][i] = static_cast<int>(*reinterpret_cast<const uint32_t*>(
-                                       ex + (wm * (BM / 2) + i * 32 + frow) * 16 + (kb & 3) * 4) >>
-                                   (8 * half));
-  };
-  f32x16 acc[kFR][2];
-
-  int rd_kb = 0, rd_region = 0;  // the step whose fragments are read next
-  auto rd_advance = [&]() __attribute__((always_inline)) {
-    if (++rd_kb == ks) rd_kb = 0;
-    if ((rd_kb & 3) == 0) rd_region = rd_region + 1 == kRegions ? 0 : rd_region + 1;
-  };
-
-  // Step g on exponent words b = g & 1.
-  auto step = [&](auto Bc, int g) __attribute__((always_inline)) {
-    constexpr int b = decltype(Bc)::value;
-    const int stage = g & 3, next = (g + 1) & 3, fill = (g + 3) & 3;
-    if (ld_more && (ld_kb & 3) == 0) issue_ex();
+      exa[i] = static_cast<int>(*reinterpret_cast<const uint32_t*>(smem + ae_off + region * Cfg::kExA + i * 512 +
+                                                                   in_group * 4) >>
+                                (8 * half));
 #pragma unroll
-    for (int j = 0; j < kNA; ++j) issue_a(fill, j);
+    for (int q = 0; q < 2; ++q) {
 #pragma unroll
-    for (int j = 0; j < kNB; ++j) issue_b(fill, j);
-    advance();
-    read_frags(std::integral_constant<int, 1>{}, stage);
+      for (int j = 0; j < 4; ++j) fb[q][j] = *reinterpret_cast<const u32x4*>(st + b_off + j * 2048 + q * 1024);
+#pragma unroll
+      for (int i = 0; i < kFR; ++i)
+        fa[q][i] = *reinterpret_cast<const u32x4*>(st + a_off + i * 2048 + (((2 * q + half) ^ fsw) * 16));
+    }
 #pragma unroll
     for (int i = 0; i < kFR; ++i)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) acc[i][j] = mfma_fp4<0>(fb[0][j], fa[0][i], acc[i][j], exb[b][j], exa[b][i]);
-    read_frags(std::integral_constant<int, 0>{}, next);
-    read_ex(std::integral_constant<int, b ^ 1>{}, rd_region, rd_kb);
-    rd_advance();
+      for (int j = 0; j < 4; ++j) acc[i][j] = mfma_fp4<0>(fb[0][j], fa[0][i], acc[i][j], exb[j], exa[i]);
 #pragma unroll
     for (int i = 0; i < kFR; ++i)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) acc[i][j] = mfma_fp4<2>(fb[1][j], fa[1][i], acc[i][j], exb[b][j], exa[b][i]);
+      for (int j = 0; j < 4; ++j) acc[i][j] = mfma_fp4<2>(fb[1][j], fa[1][i], acc[i][j], exb[j], exa[i]);
     // used here, before the barrier, so that the products are not moved past it
 #pragma unroll
     for (int i = 0; i < kFR; ++i)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) use_here(acc[i][j]);
-    // this wave's loads of step g + 2 have landed (step g + 3's may fly); after the
-    // barrier every wave's have
-    wait_vm_lgkm0<kNA + kNB>();
-    __builtin_amdgcn_s_barrier();
+      for (int j = 0; j < 4; ++j) use_here(acc[i][j]);
   };
 
-  if (GATHER) fetch_src(first);
-  set_load_tile(first);
-#pragma unroll
-  for (int st = 0; st < 3; ++st) {
-    if (ld_more && (ld_kb & 3) == 0) issue_ex();
-#pragma unroll
-    for (int j = 0; j < kNA; ++j) issue_a(st, j);
-#pragma unroll
-    for (int j = 0; j < kNB; ++j) issue_b(st, j);
-    advance();
-  }
-  wait_vm_lgkm0<kNA + kNB>();
-  __builtin_amdgcn_s_barrier();
-  read_frags(std::integral_constant<int, 0>{}, 0);
-  read_ex(std::integral_constant<int, 0>{}, 0, 0);
-  rd_advance();
-
+  ld.move(offsets, first, n_tiles_n);
+  set_load_tile();
+  issue();
+  issue();
   int g = 0;
   for (int t = first; t < hi; t += per_xcd) {
 #pragma unroll
     for (int i = 0; i < kFR; ++i)
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
     for (int kb = 0; kb < ks; ++kb, ++g) {
-      step(std::integral_constant<int, 0>{}, g);
-#pragma unroll
-      for (int j = 0; j < 2; ++j) exb[0][j] = exb[1][j];
-#pragma unroll
-      for (int i = 0; i < kFR; ++i) exa[0][i] = exa[1][i];
+      // this wave's loads of step g have landed (step g + 1's may fly); after the
+      // barrier every wave's have, and every wave is done with step g - 1, whose stage
+      // the next loads take
+      wait_vm_lgkm0<kNA + kNB + 1>();
+      __builtin_amdgcn_s_barrier();
+      issue();
+      if (left == 0) {
+        left = group_steps(ks - kb);
+        region = region + 1 == Cfg::kRegions ? 0 : region + 1;
+        in_group = 0;
+      }
+      step();
+      --left;
+      ++in_group;
+      stage = stage + 1 == kStages ? 0 : stage + 1;
     }
-    const Tile q = decode(t);
-    const int64_t r0 = q.row0;
+    cur.move(offsets, t, n_tiles_n);
+    const int64_t r0 = cur.row0;
     const int row = wm * (BM / 2) + frow;
+    const bool mine = cur.n0 + wn * 128 < ncols;  // uniform per wave
     if constexpr (GATE_UP) {
       const int d_ff = ncols / 2;
       const __amdgpu_buffer_rsrc_t q_out =
-          __builtin_amdgcn_make_buffer_rsrc(C + r0 * (d_ff / 2), 0, q.rows * (d_ff / 2), kBufferWord3);
+          __builtin_amdgcn_make_buffer_rsrc(C + r0 * (d_ff / 2), 0, cur.rows * (d_ff / 2), kBufferWord3);
       const __amdgpu_buffer_rsrc_t e_out =
-          __builtin_amdgcn_make_buffer_rsrc(c_exp + r0 * (d_ff / 32), 0, q.rows * (d_ff / 32), kBufferWord3);
+          __builtin_amdgcn_make_buffer_rsrc(c_exp + r0 * (d_ff / 32), 0, cur.rows * (d_ff / 32), kBufferWord3);
 #pragma unroll
       for (int i = 0; i < kFR; ++i)
-        store_h_block(acc[i][0], acc[i][1], q_out, e_out, row + 32 * i, q.n0 / 2 + wn * 32, d_ff, half);
+        if (mine) store_h_blocks(acc[i], q_out, e_out, row + 32 * i, cur.n0 / 2 + wn * 64, d_ff, half);
     } else {
       const __amdgpu_buffer_rsrc_t out =
-          __builtin_amdgcn_make_buffer_rsrc(C + r0 * ncols * 2, 0, q.rows * ncols * 2, kBufferWord3);
+          __builtin_amdgcn_make_buffer_rsrc(C + r0 * ncols * 2, 0, cur.rows * ncols * 2, kBufferWord3);
+      // through the stage of the last step, which every wave has read once all are here
+      // and which the next step's loads take after their barrier
+      uint8_t* const lds = smem + (stage == 0 ? kStages - 1 : stage - 1) * Cfg::kStage + wave * 4096;
+      __builtin_amdgcn_s_barrier();
 #pragma unroll
       for (int i = 0; i < kFR; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) store_y_block(acc[i][j], out, row + 32 * i, q.n0 + wn * 64 + 32 * j, ncols, half);
+        for (int j = 0; j < 4; j += 2)
+          if (mine)
+            store_y_blocks(acc[i][j], acc[i][j + 1], lds, out, wm * (BM / 2) + 32 * i, cur.n0 + wn * 128 + 32 * j, ncols,
+                         lane);
     }
   }
   // nothing may still be writing into LDS when the workgroup ends
@@ -616,15 +717,10 @@ int allow_lds(const char* what, Kernel kernel, int bytes, int dev, std::atomic<u
   return HMOE_OK;
 }
 
-template <int BM, bool GATE_UP, bool GATHER, typename... Args>
-int launch_tiles(const char* what, hipStream_t s, Args... args) {
-  int dev = 0, grid = 0;
-  if (int rc = persistent_grid(what, s, &grid, &dev)) return rc;
-  static std::atomic<uint64_t> done{0};
-  if (int rc = allow_lds(what, grouped_mxfp4_tiles<BM, GATE_UP, GATHER>, TileCfg<BM>::kLds, dev, &done)) return rc;
-  hipLaunchKernelGGL((grouped_mxfp4_tiles<BM, GATE_UP, GATHER>), dim3(grid), dim3(kTileThreads), TileCfg<BM>::kLds, s,
-                     args...);
-  return check_launch(what);
+// Tiles of 32 rows at most: an expert's last one may hold a single row.
+int64_t max_row_tiles(int64_t rows, int n_experts) {
+  const int64_t full = ceil_div(rows, 32) + n_experts;
+  return full < rows ? full : rows;
 }
 
 // The checks that the products share.
@@ -639,34 +735,102 @@ int check_product(const char* what, int n_experts, int64_t rows_cap, int d_model
   return HMOE_OK;
 }
 
+// Which kernel a product takes: the one with the least estimated time, from three
+// measured rates (MI355X, us, `steps` = K / 128):
+//   rows split four ways: 3.5, and 0.55 ns for every 32 rows x 64 columns x 128 values;
+//   64-row tiles:  4.2 + 0.5 a step while there is one a CU, 0.8 when there are two, and
+//     for every further two;
+//   128-row tiles: 5.0 + 0.7 and 1.23 alike.
+// None is faster than reading the experts' weights at 5.9 TB/s, which the first comes
+// nearest to.  Measured against each other (rows, 64, 128), us:
+//   gate/up 64 experts, D 2048, F 1024, top-8: 1 token 4.8, 11.6, 15.4; 48 tokens 24.0,
+//     25.0, 27.6; 512 tokens 39.9, 33.3, 35.9; 1000 tokens 68.7, 36.9, 35.9;
+//   32 experts, D 4096, F 2048, top-4: 300 tokens 68.2, 51.7, 64.1;
+//   24 experts, D 1152, F 640, top-3: 333 tokens 7.9, 8.9, 11.4; 800 tokens 13.2, 9.0,
+//     11.4; 2000 tokens 22.7, 16.6, 14.4;
+//   one segment, D 2048, F 1024: 64 rows 5.6, 11.9, 15.4; 2000 rows 19.4, 12.2, 15.7; 8000
+//     rows 64.7, 28.1, 23.7.
+// Below four steps the split has nothing to split: 2000 tokens on 8 experts, D 256, 8.7
+// against 5.5 with the waves side by side.
+enum Form { kRows1, kRows4, kTiles64, kTiles128 };
+
+// The experts that have rows, and the row tiles of all.  The counts are known only to
+// the device: an expert is taken to have none as often as chance has it, and past three
+// quarters of a tile some need another.
+double live_experts(int64_t rows, int n_experts) {
+  return n_experts * -std::expm1(-static_cast<double>(rows) / n_experts);
+}
+double row_tiles(int64_t rows, int n_experts, int bm) {
+  if (n_experts == 1) return static_cast<double>(ceil_div(rows, bm));
+  const double n = live_experts(rows, n_experts), mean = rows / n;
+  return n * (mean <= 0.75 * bm ? 1.0 : mean / bm + 0.5);
+}
+
+Form choose_form(int64_t rows, int n_experts, int kdim, int ncols, int cus) {
+  const double steps = kdim / 128;
+  const double n = live_experts(rows, n_experts);
+  const double weights = n * ncols * kdim * (17.0 / 32.0) / 5.9e6;
+  const double tiles32 = row_tiles(rows, n_experts, 32);
+  const double by_rows = std::max(3.5 + tiles32 * (ncols / 64) * steps * 0.55e-3, weights * (0.9 + 0.1 * tiles32 / n));
+  const auto by_tiles = [&](int bm, double start, double alone, double paired) {
+    const double tiles = row_tiles(rows, n_experts, bm) * static_cast<double>(ceil_div(ncols, kTileN));
+    const double step = tiles <= cus ? alone : paired * std::ceil(tiles / (2.0 * cus) - 0.02);
+    return std::max(start + steps * step, 1.1 * weights);
+  };
+  const double by_64 = by_tiles(64, 4.2, 0.5, 0.8);
+  const double by_128 = steps > 1 ? by_tiles(128, 5.0, 0.7, 1.23) : by_64 + 1.0;
+  // (a grid holds 65535 tiles along y)
+  if (by_rows <= std::min(by_64, by_128) && max_row_tiles(rows, n_experts) <= 65535)
+    return steps < 4 ? kRows1 : kRows4;
+  return by_64 <= by_128 ? kTiles64 : kTiles128;
+}
+
 template <bool GATE_UP, bool GATHER>
 int launch_product(const char* what, const uint8_t* a, const uint8_t* a_exp, const uint8_t* b,
                    const uint8_t* b_exp, const int32_t* offsets, int n_experts, int64_t rows_cap, int kdim,
                    int ncols, uint8_t* c, uint8_t* c_exp, const int32_t* gather_src, int gather_k,
                    int gather_rows, hipStream_t s) {
-  const double mean = static_cast<double>(rows_cap) / n_experts;
-  if (mean >= 64 && ncols % kTileN == 0) {
-    HMOE_REQUIRE(static_cast<int64_t>(kdim / 128) * ncols * 4 < (int64_t(1) << 31), "%s: operand too large", what);
-    HMOE_REQUIRE((ceil_div(rows_cap, 128) + n_experts) * (ncols / kTileN) < (int64_t(1) << 31), "%s: too many tiles", what);
-    if (mean >= 160)
-      return launch_tiles<256, GATE_UP, GATHER>(what, s, a, a_exp, b, b_exp, offsets, n_experts, kdim, ncols, c, c_exp,
-                                                gather_src, gather_k, gather_rows);
-    return launch_tiles<128, GATE_UP, GATHER>(what, s, a, a_exp, b, b_exp, offsets, n_experts, kdim, ncols, c, c_exp,
-                                              gather_src, gather_k, gather_rows);
+  HMOE_REQUIRE(static_cast<int64_t>(kdim / 128) * ncols * 4 < (int64_t(1) << 31), "%s: operand too large", what);
+  HMOE_REQUIRE((ceil_div(rows_cap, 64) + n_experts) * ceil_div(ncols, kTileN) < (int64_t(1) << 31),
+               "%s: too many tiles", what);
+  int dev = 0, cus = 0;
+  if (int rc = persistent_grid(what, s, &cus, &dev)) return rc;
+  const Form form = choose_form(rows_cap, n_experts, kdim, ncols, cus);
+  if (form == kTiles64 || form == kTiles128) {
+    const auto launch = [&](auto BM) {
+      constexpr int bm = decltype(BM)::value;
+      static std::atomic<uint64_t> done{0};
+      if (int rc = allow_lds(what, grouped_mxfp4_tiles<bm, GATE_UP, GATHER>, TileCfg<bm>::kLds, dev, &done)) return rc;
+      hipLaunchKernelGGL((grouped_mxfp4_tiles<bm, GATE_UP, GATHER>), dim3(2 * cus), dim3(kTileThreads),
+                         TileCfg<bm>::kLds, s, a, a_exp, b, b_exp, offsets, n_experts, kdim, ncols, c, c_exp,
+                         gather_src, gather_k, gather_rows);
+      return check_launch(what);
+    };
+    return form == kTiles64 ? launch(std::integral_constant<int, 64>{}) : launch(std::integral_constant<int, 128>{});
   }
-  // an expert's last tile may hold one row
-  const int64_t full = ceil_div(rows_cap, 32) + n_experts;
-  const int64_t m_tiles = full < rows_cap ? full : rows_cap;
-  HMOE_REQUIRE(m_tiles <= 65535, "%s: too many row tiles", what);
-  hipLaunchKernelGGL((grouped_mxfp4_rows<GATE_UP, GATHER>),
-                     dim3(static_cast<unsigned>(ceil_div(ncols, 256)), static_cast<unsigned>(m_tiles)), dim3(256),
-                     0, s, a, a_exp, b, b_exp, offsets, n_experts, kdim, ncols, c, c_exp, gather_src, gather_k,
-                     gather_rows);
+  const unsigned m_tiles = static_cast<unsigned>(max_row_tiles(rows_cap, n_experts));
+  if (form == kRows4)
+    hipLaunchKernelGGL((grouped_mxfp4_rows<GATE_UP, GATHER, 4>), dim3(ncols / 64, m_tiles), dim3(256), 0, s, a, a_exp,
+                       b, b_exp, offsets, n_experts, kdim, ncols, c, c_exp, gather_src, gather_k, gather_rows);
+  else
+    hipLaunchKernelGGL((grouped_mxfp4_rows<GATE_UP, GATHER, 1>),
+                       dim3(static_cast<unsigned>(ceil_div(ncols, 256)), m_tiles), dim3(256), 0, s, a, a_exp, b, b_exp,
+                       offsets, n_experts, kdim, ncols, c, c_exp, gather_src, gather_k, gather_rows);
   return check_launch(what);
 }
 
 }  // namespace
 }  // namespace hmoe
+
+extern "C" int64_t hmoe_grouped_mxfp4_form(int64_t rows_cap, int n_experts, int kdim, int ncols, int cus) {
+  using namespace hmoe;
+  if (rows_cap < 1 || n_experts < 1 || n_experts > kMaxExperts || cus < 1 || kdim < 128 || kdim % 128 != 0 ||
+      ncols < 128 || ncols % 128 != 0) {
+    set_error("grouped_mxfp4_form: sizes that the products refuse");
+    return -1;
+  }
+  return choose_form(rows_cap, n_experts, kdim, ncols, cus);
+}
 
 extern "C" int hmoe_grouped_gate_up_mxfp4(const uint8_t* xs_q, const uint8_t* xs_exp, const int32_t* offsets,
                                           int n_experts, int64_t rows_cap, int d_model, int d_ff,

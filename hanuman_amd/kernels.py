@@ -30,7 +30,9 @@ def _ptr(t):
 
 
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    # torch.cuda.current_stream().cuda_stream without the Stream object, which takes
+    # 2.7 us to make: as long as a launch
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def _check(t: torch.Tensor, name: str, ndim: int | None = None):
@@ -693,12 +695,14 @@ def grouped_down_fp8_mx(h_q: torch.Tensor, h_exp: torch.Tensor, offsets: torch.T
 # e2m1 code; ``hmoe_quantize_rows_mxfp4`` has the rule.  Served weights only: there
 # is no backward, as for the e4m3 experts.
 
-def _u8(name: str, dev, *shapes):
-    """Checks ``(tensor, shape)`` pairs of an MXFP4 call: uint8, on one device (the
-    current one, whose stream the call takes), of those sizes."""
-    for t, shape in shapes:
+def _u8(name: str, dev, t: torch.Tensor, shape: tuple):
+    """Checks a code or exponent tensor of an MXFP4 call: uint8, contiguous, on the
+    call's device, of that size.  (One expression for what is right: the smallest calls
+    are as long as their checks.)"""
+    if not (t.__class__ is torch.Tensor and t.dtype is torch.uint8 and t.shape == shape
+            and t.device == dev and t.is_contiguous()):
         _check(t, name)
-        if t.dtype != torch.uint8 or tuple(t.shape) != tuple(shape):
+        if t.dtype != torch.uint8 or t.shape != shape:
             raise ValueError(f"{name}: expected uint8 {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
         _same_device(name, t, dev)
 
@@ -709,11 +713,14 @@ def _same_device(name: str, t: torch.Tensor, dev):
 
 
 def _current_device(name: str, t: torch.Tensor):
+    """The device of a call's first tensor, which has to be the current one: the call
+    goes to that one's current stream."""
     _check(t, name)
-    if t.device.index != torch.cuda.current_device():
-        raise ValueError(f"{name}: tensors on {t.device}, but the current device is "
+    dev = t.device
+    if dev.index != torch._C._cuda_getDevice():
+        raise ValueError(f"{name}: tensors on {dev}, but the current device is "
                          f"cuda:{torch.cuda.current_device()}")
-    return t.device
+    return dev
 
 
 def quantize_rows_mxfp4(a: torch.Tensor):
@@ -736,7 +743,8 @@ def dequantize_rows_mxfp4(q: torch.Tensor, exps: torch.Tensor,
     dev = _current_device("dequantize_rows_mxfp4", q)
     _check(q, "q", 2)
     rows, cols = q.shape[0], q.shape[1] * 2
-    _u8("dequantize_rows_mxfp4", dev, (q, q.shape), (exps, (rows, cols // 32)))
+    _u8("dequantize_rows_mxfp4", dev, q, q.shape)
+    _u8("dequantize_rows_mxfp4", dev, exps, (rows, cols // 32))
     if out_dtype not in _DT:
         raise TypeError(f"unsupported dtype {out_dtype}; expected float32 or bfloat16")
     out = torch.empty((rows, cols), dtype=out_dtype, device=dev)
@@ -782,8 +790,10 @@ def pack_mxfp4_down(w_down: torch.Tensor):
 def _mxfp4_sizes(name: str, packed: torch.Tensor, exps: torch.Tensor, dev):
     """``(N, rows, K)`` of a packed operand, its tensors checked."""
     _check(packed, name, 5)
-    N, rows, k = packed.shape[0], packed.shape[1] * 32, packed.shape[2] * 64
-    _u8(name, dev, (packed, (N, rows // 32, k // 64, 64, 16)), (exps, (N, k // 128, rows, 4)))
+    N, blocks, chunks = packed.shape[:3]
+    rows, k = blocks * 32, chunks * 64
+    _u8(name, dev, packed, (N, rows // 32, k // 64, 64, 16))
+    _u8(name, dev, exps, (N, k // 128, rows, 4))
     return N, rows, k
 
 
@@ -816,7 +826,8 @@ def grouped_gate_up_mxfp4(xs_q: torch.Tensor, xs_exp: torch.Tensor, offsets: tor
     dev = _current_device(name, xs_q)
     N, F2, D = _mxfp4_sizes(name, w_packed, w_exp, dev)
     rows, F = xs_q.shape[0], F2 // 2
-    _u8(name, dev, (xs_q, (rows, D // 2)), (xs_exp, (rows, D // 32)))
+    _u8(name, dev, xs_q, (rows, D // 2))
+    _u8(name, dev, xs_exp, (rows, D // 32))
     _check_offsets(name, offsets, N, dev)
     h_q = torch.empty((rows, F // 2), dtype=torch.uint8, device=dev)
     h_exp = torch.empty((rows, F // 32), dtype=torch.uint8, device=dev)
@@ -833,7 +844,8 @@ def grouped_gate_up_mxfp4_gather(x_q: torch.Tensor, x_exp: torch.Tensor, plan: P
     dev = _current_device(name, x_q)
     N, F2, D = _mxfp4_sizes(name, w_packed, w_exp, dev)
     T, F = x_q.shape[0], F2 // 2
-    _u8(name, dev, (x_q, (T, D // 2)), (x_exp, (T, D // 32)))
+    _u8(name, dev, x_q, (T, D // 2))
+    _u8(name, dev, x_exp, (T, D // 32))
     if plan.n_experts != N or plan.slot_pos.numel() != T * plan.top_k:
         raise ValueError(f"{name}: the plan is of other tokens or experts")
     _check_offsets(name, plan.offsets, N, dev)
@@ -853,7 +865,8 @@ def grouped_down_mxfp4(h_q: torch.Tensor, h_exp: torch.Tensor, offsets: torch.Te
     dev = _current_device(name, h_q)
     N, D, F = _mxfp4_sizes(name, w_packed, w_exp, dev)
     rows = h_q.shape[0]
-    _u8(name, dev, (h_q, (rows, F // 2)), (h_exp, (rows, F // 32)))
+    _u8(name, dev, h_q, (rows, F // 2))
+    _u8(name, dev, h_exp, (rows, F // 32))
     _check_offsets(name, offsets, N, dev)
     ys = torch.empty((rows, D), dtype=torch.bfloat16, device=dev)
     call("hmoe_grouped_down_mxfp4", _ptr(h_q), _ptr(h_exp), _ptr(offsets), N, rows, F, D,

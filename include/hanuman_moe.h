@@ -422,6 +422,13 @@ int hmoe_pack_mxfp4_down(const void* w_down, int w_dtype, int n_experts, int d_f
 int hmoe_unpack_mxfp4(const uint8_t* packed, const uint8_t* exps, int n_experts, int rows, int cols,
                       void* out, int out_dtype, hmoe_stream_t stream);
 
+/* The form in which the products below run `kdim` values of the reduction and `ncols`
+ * columns (gate/up: 2 d_ff) on a device of `cus` CUs: 0 and 1, 32 rows from memory into
+ * registers, the reduction split over four waves in 1; 2 and 3, tiles of 64 and 128 rows
+ * through LDS.  -1 for sizes that they refuse.  A host-side query.  Forms 0, 2 and 3 sum
+ * in the same order and give the same bits; 1 adds four parts. */
+int64_t hmoe_grouped_mxfp4_form(int64_t rows_cap, int n_experts, int kdim, int ncols, int cus);
+
 /* h of rows r of expert e's segment [offsets[e], offsets[e+1]) as MXFP4 rows: with
  * g and u the float32 sums xs[r]·Wg[e] and xs[r]·Wu[e], h = silu(g) * u in float32
  * and quantised from there (h is rounded once, to its codes).  xs_q [rows_cap, D/2],

@@ -212,6 +212,43 @@ def test_products(gpu, shape):
     assert torch.equal(K.grouped_down_mxfp4(h_q, h_e, plan.offsets, *dn), ys)
 
 
+FORMS = [
+    # the shape, and the form that its gate/up and down products take
+    ((6000, 3, 1, 128, 1280), 2, 1),    # one step a tile
+    ((8000, 2, 1, 256, 384), 2, 0),     # two
+    ((3000, 4, 2, 640, 384), 2, 2),     # five (groups of three and two), three
+    ((4000, 2, 1, 1152, 1152), 3, 3),   # nine; a last column tile of 128
+    ((2600, 2, 2, 512, 1152), 3, 2),    # a whole group of four
+    ((1500, 20, 2, 640, 1152), 2, 1),   # segments that end inside tiles
+]
+
+
+@pytest.mark.parametrize("shape,gate_up,down", FORMS, ids=lambda s: "x".join(map(str, s)) if isinstance(s, tuple) else str(s))
+def test_forms(gpu, shape, gate_up, down):
+    tokens, experts, active, d_model, d_ff = shape
+    cus = torch.cuda.get_device_properties(gpu).multi_processor_count // 8 * 8
+    form = _lib.lib().hmoe_grouped_mxfp4_form
+    if cus == 256:
+        assert form(tokens * active, experts, d_model, 2 * d_ff, cus) == gate_up
+        assert form(tokens * active, experts, d_ff, d_model, cus) == down
+    test_products(gpu, shape)
+
+
+def test_forms_agree(gpu):
+    """The first expert's rows alone, in registers, and among many, through LDS: the same
+    sums in the same order."""
+    D, F, rows = 384, 640, 6000
+    rng = np.random.default_rng(12)
+    x_q, x_e = K.quantize_rows_mxfp4(torch.randn((rows, D), device=gpu))
+    gu = [_to(np.stack(t), gpu) for t in zip(*(R.packed_operand(*R.quantise(rng.standard_normal((2 * F, D)))) for _ in range(2)))]
+    off = torch.tensor([0, 70, rows], dtype=torch.int32, device=gpu)
+    form = _lib.lib().hmoe_grouped_mxfp4_form
+    assert form(rows, 2, D, 2 * F, 256) >= 2 and form(70, 2, D, 2 * F, 256) == 0
+    many = K.grouped_gate_up_mxfp4(x_q, x_e, off, *gu)
+    few = K.grouped_gate_up_mxfp4(x_q[:70].contiguous(), x_e[:70].contiguous(), off.clamp(max=70), *gu)
+    assert torch.equal(many[0][:70], few[0]) and torch.equal(many[1][:70], few[1])
+
+
 @pytest.mark.parametrize("shape,skew", [((300, 6, 1, 256, 128), 3.0), ((90, 20, 2, 128, 256), 1.0)])
 def test_skewed_products(gpu, shape, skew):
     """Nearly all rows on the first experts, the last ones empty."""

@@ -91,6 +91,14 @@ def test_sizes():
     assert lib.hmoe_packed_mxfp4_gate_up_bytes(0, 256, 128) == 0
 
 
+def test_form():
+    form = _lib.lib().hmoe_grouped_mxfp4_form
+    assert form(8, 64, 2048, 2048, 256) == 1 and form(131072, 64, 2048, 2048, 256) == 3
+    for bad in ((0, 64, 2048, 2048, 256), (8, 0, 2048, 2048, 256), (8, 2000, 2048, 2048, 256),
+                (8, 64, 100, 2048, 256), (8, 64, 2048, 64, 256), (8, 64, 2048, 2048, 0)):
+        assert form(*bad) == -1
+
+
 def test_python_layer():
     """Tensors that are not on a GPU are refused before anything is looked at."""
     x = torch.zeros((4, 64))
