@@ -695,16 +695,20 @@ def grouped_down_fp8_mx(h_q: torch.Tensor, h_exp: torch.Tensor, offsets: torch.T
 # e2m1 code; ``hmoe_quantize_rows_mxfp4`` has the rule.  Served weights only: there
 # is no backward, as for the e4m3 experts.
 
+_U8, _TENSOR = torch.uint8, torch.Tensor
+
+
 def _u8(name: str, dev, t: torch.Tensor, shape: tuple):
     """Checks a code or exponent tensor of an MXFP4 call: uint8, contiguous, on the
     call's device, of that size.  (One expression for what is right: the smallest calls
     are as long as their checks.)"""
-    if not (t.__class__ is torch.Tensor and t.dtype is torch.uint8 and t.shape == shape
-            and t.device == dev and t.is_contiguous()):
-        _check(t, name)
-        if t.dtype != torch.uint8 or t.shape != shape:
-            raise ValueError(f"{name}: expected uint8 {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
-        _same_device(name, t, dev)
+    if (t.__class__ is _TENSOR and t.dtype is _U8 and t.shape == shape and t.is_contiguous()
+            and t.device == dev):
+        return
+    _check(t, name)
+    if t.dtype != _U8 or t.shape != shape:
+        raise ValueError(f"{name}: expected uint8 {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+    _same_device(name, t, dev)
 
 
 def _same_device(name: str, t: torch.Tensor, dev):
@@ -712,10 +716,10 @@ def _same_device(name: str, t: torch.Tensor, dev):
         raise ValueError(f"{name}: tensors on {t.device} and {dev}")
 
 
-def _current_device(name: str, t: torch.Tensor):
+def _current_device(name: str, t: torch.Tensor, ndim: int):
     """The device of a call's first tensor, which has to be the current one: the call
     goes to that one's current stream."""
-    _check(t, name)
+    _check(t, name, ndim)
     dev = t.device
     if dev.index != torch._C._cuda_getDevice():
         raise ValueError(f"{name}: tensors on {dev}, but the current device is "
@@ -727,8 +731,7 @@ def quantize_rows_mxfp4(a: torch.Tensor):
     """MXFP4 rows of a float32 or bf16 matrix ``[rows, cols]``: codes uint8 ``[rows,
     cols / 2]`` (the even column in a byte's low half) and biased exponents uint8
     ``[rows, cols / 32]``."""
-    dev = _current_device("quantize_rows_mxfp4", a)
-    _check(a, "a", 2)
+    dev = _current_device("quantize_rows_mxfp4", a, 2)
     rows, cols = a.shape
     q = torch.empty((rows, cols // 2), dtype=torch.uint8, device=dev)
     exps = torch.empty((rows, cols // 32), dtype=torch.uint8, device=dev)
@@ -740,9 +743,9 @@ def quantize_rows_mxfp4(a: torch.Tensor):
 def dequantize_rows_mxfp4(q: torch.Tensor, exps: torch.Tensor,
                           out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values ``[rows, cols]`` of MXFP4 rows (exact in both types)."""
-    dev = _current_device("dequantize_rows_mxfp4", q)
-    _check(q, "q", 2)
-    rows, cols = q.shape[0], q.shape[1] * 2
+    dev = _current_device("dequantize_rows_mxfp4", q, 2)
+    rows, half = q.shape
+    cols = half * 2
     _u8("dequantize_rows_mxfp4", dev, q, q.shape)
     _u8("dequantize_rows_mxfp4", dev, exps, (rows, cols // 32))
     if out_dtype not in _DT:
@@ -762,8 +765,7 @@ def _mxfp4_operand(N: int, rows: int, k: int, dev):
 def pack_mxfp4_gate_up(w_gate: torch.Tensor, w_up: torch.Tensor):
     """MXFP4 gate/up operand of ``[N,D,F]`` masters, quantised along ``D``: codes
     ``[N, 2F/32, D/64, 64, 16]`` and exponents ``[N, D/128, 2F, 4]``."""
-    dev = _current_device("pack_mxfp4_gate_up", w_gate)
-    _check(w_gate, "w_gate", 3)
+    dev = _current_device("pack_mxfp4_gate_up", w_gate, 3)
     _check(w_up, "w_up", 3)
     _same_device("pack_mxfp4_gate_up", w_up, dev)
     if w_gate.shape != w_up.shape or w_gate.dtype != w_up.dtype:
@@ -778,8 +780,7 @@ def pack_mxfp4_gate_up(w_gate: torch.Tensor, w_up: torch.Tensor):
 def pack_mxfp4_down(w_down: torch.Tensor):
     """MXFP4 down operand of the ``[N,F,D]`` master, quantised along ``F``: codes
     ``[N, D/32, F/64, 64, 16]`` and exponents ``[N, F/128, D, 4]``."""
-    dev = _current_device("pack_mxfp4_down", w_down)
-    _check(w_down, "w_down", 3)
+    dev = _current_device("pack_mxfp4_down", w_down, 3)
     N, F, D = w_down.shape
     out, exps = _mxfp4_operand(N, D, F, dev)
     call("hmoe_pack_mxfp4_down", _ptr(w_down), _dtype_code(w_down), N, F, D, _ptr(out),
@@ -789,19 +790,20 @@ def pack_mxfp4_down(w_down: torch.Tensor):
 
 def _mxfp4_sizes(name: str, packed: torch.Tensor, exps: torch.Tensor, dev):
     """``(N, rows, K)`` of a packed operand, its tensors checked."""
-    _check(packed, name, 5)
-    N, blocks, chunks = packed.shape[:3]
-    rows, k = blocks * 32, chunks * 64
-    _u8(name, dev, packed, (N, rows // 32, k // 64, 64, 16))
-    _u8(name, dev, exps, (N, k // 128, rows, 4))
-    return N, rows, k
+    if packed.dim() != 5:
+        _check(packed, name, 5)
+    N, blocks, chunks, _, _ = packed.shape
+    rows = blocks * 32
+    _u8(name, dev, packed, (N, blocks, chunks, 64, 16))
+    _u8(name, dev, exps, (N, chunks // 2, rows, 4))
+    return N, rows, chunks * 64
 
 
 def unpack_mxfp4(packed: torch.Tensor, exps: torch.Tensor,
                  out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The weights ``[N, rows, K]`` of a packed MXFP4 operand: in bf16 the operand that
     the bf16 products take (:func:`pack_gate_up`, :func:`pack_down`)."""
-    dev = _current_device("unpack_mxfp4", packed)
+    dev = _current_device("unpack_mxfp4", packed, 5)
     N, rows, k = _mxfp4_sizes("unpack_mxfp4", packed, exps, dev)
     if out_dtype not in _DT:
         raise TypeError(f"unsupported dtype {out_dtype}; expected float32 or bfloat16")
@@ -811,11 +813,13 @@ def unpack_mxfp4(packed: torch.Tensor, exps: torch.Tensor,
     return out
 
 
-def _check_offsets(name: str, offsets: torch.Tensor, N: int, dev):
-    _check(offsets, "offsets", 1)
-    _same_device(name, offsets, dev)
-    if offsets.numel() != N + 1 or offsets.dtype != torch.int32:
-        raise ValueError(f"{name}: offsets must be int32 [{N + 1}]")
+def _check_i32(name: str, what: str, t: torch.Tensor, numel: int, dev):
+    if (t.__class__ is _TENSOR and t.dtype is torch.int32 and t.numel() == numel and t.is_contiguous()
+            and t.device == dev):
+        return
+    _check(t, what)
+    _same_device(name, t, dev)
+    raise ValueError(f"{name}: {what} must be int32 [{numel}]")
 
 
 def grouped_gate_up_mxfp4(xs_q: torch.Tensor, xs_exp: torch.Tensor, offsets: torch.Tensor,
@@ -823,12 +827,12 @@ def grouped_gate_up_mxfp4(xs_q: torch.Tensor, xs_exp: torch.Tensor, offsets: tor
     """MXFP4 ``h = silu(g) * u`` of MXFP4 rows in the experts' order: codes ``[rows,
     F/2]`` and exponents ``[rows, F/32]``.  Rows past ``offsets[-1]`` are not written."""
     name = "grouped_gate_up_mxfp4"
-    dev = _current_device(name, xs_q)
+    dev = _current_device(name, xs_q, 2)
     N, F2, D = _mxfp4_sizes(name, w_packed, w_exp, dev)
     rows, F = xs_q.shape[0], F2 // 2
     _u8(name, dev, xs_q, (rows, D // 2))
     _u8(name, dev, xs_exp, (rows, D // 32))
-    _check_offsets(name, offsets, N, dev)
+    _check_i32(name, "offsets", offsets, N + 1, dev)
     h_q = torch.empty((rows, F // 2), dtype=torch.uint8, device=dev)
     h_exp = torch.empty((rows, F // 32), dtype=torch.uint8, device=dev)
     call("hmoe_grouped_gate_up_mxfp4", _ptr(xs_q), _ptr(xs_exp), _ptr(offsets), N, rows, D, F,
@@ -841,14 +845,15 @@ def grouped_gate_up_mxfp4_gather(x_q: torch.Tensor, x_exp: torch.Tensor, plan: P
     """:func:`grouped_gate_up_mxfp4` gathering its rows from the quantised tokens
     through ``perm_src``."""
     name = "grouped_gate_up_mxfp4_gather"
-    dev = _current_device(name, x_q)
+    dev = _current_device(name, x_q, 2)
     N, F2, D = _mxfp4_sizes(name, w_packed, w_exp, dev)
     T, F = x_q.shape[0], F2 // 2
     _u8(name, dev, x_q, (T, D // 2))
     _u8(name, dev, x_exp, (T, D // 32))
     if plan.n_experts != N or plan.slot_pos.numel() != T * plan.top_k:
         raise ValueError(f"{name}: the plan is of other tokens or experts")
-    _check_offsets(name, plan.offsets, N, dev)
+    _check_i32(name, "offsets", plan.offsets, N + 1, dev)
+    _check_i32(name, "perm_src", plan.perm_src, plan.rows_cap, dev)
     h_q = torch.empty((plan.rows_cap, F // 2), dtype=torch.uint8, device=dev)
     h_exp = torch.empty((plan.rows_cap, F // 32), dtype=torch.uint8, device=dev)
     call("hmoe_grouped_gate_up_mxfp4_gather", _ptr(x_q), _ptr(x_exp), T, plan.top_k,
@@ -862,12 +867,12 @@ def grouped_down_mxfp4(h_q: torch.Tensor, h_exp: torch.Tensor, offsets: torch.Te
     """bf16 ``ys`` of MXFP4 rows times the MXFP4 down operand.  Rows past
     ``offsets[-1]`` are not written."""
     name = "grouped_down_mxfp4"
-    dev = _current_device(name, h_q)
+    dev = _current_device(name, h_q, 2)
     N, D, F = _mxfp4_sizes(name, w_packed, w_exp, dev)
     rows = h_q.shape[0]
     _u8(name, dev, h_q, (rows, F // 2))
     _u8(name, dev, h_exp, (rows, F // 32))
-    _check_offsets(name, offsets, N, dev)
+    _check_i32(name, "offsets", offsets, N + 1, dev)
     ys = torch.empty((rows, D), dtype=torch.bfloat16, device=dev)
     call("hmoe_grouped_down_mxfp4", _ptr(h_q), _ptr(h_exp), _ptr(offsets), N, rows, F, D,
          _ptr(w_packed), _ptr(w_exp), _ptr(ys), _stream())
