@@ -841,7 +841,8 @@ extern "C" int hmoe_grouped_gate_up_mxfp4(const uint8_t* xs_q, const uint8_t* xs
   if (int rc = check_product(what, n_experts, rows_cap, d_model, d_ff)) return rc;
   if (rows_cap == 0) return HMOE_OK;
   HMOE_REQUIRE(xs_q && xs_exp && offsets && w_packed && w_exp && h_q && h_exp, "%s: null pointer argument", what);
-  HMOE_REQUIRE_ALIGNED(what, xs_q, xs_exp, w_packed, w_exp, h_q);
+  HMOE_REQUIRE_ALIGNED(what, 16, xs_q, w_packed, h_q);
+  HMOE_REQUIRE_ALIGNED(what, 4, xs_exp, w_exp, h_exp);
   return launch_product<true, false>(what, xs_q, xs_exp, w_packed, w_exp, offsets, n_experts, rows_cap, d_model,
                                      2 * d_ff, h_q, h_exp, nullptr, 1, 1, static_cast<hipStream_t>(stream));
 }
@@ -861,7 +862,8 @@ extern "C" int hmoe_grouped_gate_up_mxfp4_gather(const uint8_t* x_q, const uint8
   if (rows_cap == 0) return HMOE_OK;
   HMOE_REQUIRE(x_q && x_exp && perm_src && offsets && w_packed && w_exp && h_q && h_exp,
                "%s: null pointer argument", what);
-  HMOE_REQUIRE_ALIGNED(what, x_q, x_exp, w_packed, w_exp, h_q);
+  HMOE_REQUIRE_ALIGNED(what, 16, x_q, w_packed, h_q);
+  HMOE_REQUIRE_ALIGNED(what, 4, x_exp, w_exp, h_exp);
   return launch_product<true, true>(what, x_q, x_exp, w_packed, w_exp, offsets, n_experts, rows_cap, d_model,
                                     2 * d_ff, h_q, h_exp, perm_src, top_k, static_cast<int>(tokens),
                                     static_cast<hipStream_t>(stream));
@@ -876,7 +878,8 @@ extern "C" int hmoe_grouped_down_mxfp4(const uint8_t* h_q, const uint8_t* h_exp,
   if (int rc = check_product(what, n_experts, rows_cap, d_model, d_ff)) return rc;
   if (rows_cap == 0) return HMOE_OK;
   HMOE_REQUIRE(h_q && h_exp && offsets && w_packed && w_exp && ys, "%s: null pointer argument", what);
-  HMOE_REQUIRE_ALIGNED(what, h_q, h_exp, w_packed, w_exp, ys);
+  HMOE_REQUIRE_ALIGNED(what, 16, h_q, w_packed, ys);
+  HMOE_REQUIRE_ALIGNED(what, 4, h_exp, w_exp);
   return launch_product<false, false>(what, h_q, h_exp, w_packed, w_exp, offsets, n_experts, rows_cap, d_ff,
                                       d_model, static_cast<uint8_t*>(ys), nullptr, nullptr, 1, 1,
                                       static_cast<hipStream_t>(stream));

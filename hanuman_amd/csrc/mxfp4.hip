@@ -221,7 +221,7 @@ extern "C" int hmoe_quantize_rows_mxfp4(const void* a, int a_dtype, int64_t rows
                "quantize_rows_mxfp4: a dtype must be F32 or BF16");
   if (rows == 0) return HMOE_OK;
   HMOE_REQUIRE(a && q && exps, "quantize_rows_mxfp4: null pointer argument");
-  HMOE_REQUIRE_ALIGNED("quantize_rows_mxfp4", a, q, exps);
+  HMOE_REQUIRE_ALIGNED("quantize_rows_mxfp4", 16, a, q);
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int64_t chunks = rows * (cols / 8);
   if (a_dtype == HMOE_BF16)
@@ -243,7 +243,7 @@ extern "C" int hmoe_dequantize_rows_mxfp4(const uint8_t* q, const uint8_t* exps,
                "dequantize_rows_mxfp4: out dtype must be F32 or BF16");
   if (rows == 0) return HMOE_OK;
   HMOE_REQUIRE(q && exps && out, "dequantize_rows_mxfp4: null pointer argument");
-  HMOE_REQUIRE_ALIGNED("dequantize_rows_mxfp4", q, exps, out);
+  HMOE_REQUIRE_ALIGNED("dequantize_rows_mxfp4", 16, q, out);
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int64_t chunks = rows * (cols / 8);
   if (out_dtype == HMOE_F32)
@@ -273,7 +273,8 @@ extern "C" int hmoe_pack_mxfp4_gate_up(const void* w_gate, const void* w_up, int
   HMOE_REQUIRE(w_dtype == HMOE_F32 || w_dtype == HMOE_BF16,
                "pack_mxfp4_gate_up: weight dtype must be F32 or BF16");
   HMOE_REQUIRE(w_gate && w_up && packed && exps, "pack_mxfp4_gate_up: null pointer argument");
-  HMOE_REQUIRE_ALIGNED("pack_mxfp4_gate_up", w_gate, w_up, packed, exps);
+  HMOE_REQUIRE_ALIGNED("pack_mxfp4_gate_up", 16, w_gate, w_up, packed);
+  HMOE_REQUIRE_ALIGNED("pack_mxfp4_gate_up", 4, exps);
   return pack_mxfp4("hmoe_pack_mxfp4_gate_up", w_gate, w_up, w_dtype, n_experts, d_model, d_ff, packed, exps,
                     static_cast<hipStream_t>(stream));
 }
@@ -284,7 +285,8 @@ extern "C" int hmoe_pack_mxfp4_down(const void* w_down, int w_dtype, int n_exper
   if (int rc = check_operand("pack_mxfp4_down", n_experts, d_model, d_ff)) return rc;
   HMOE_REQUIRE(w_dtype == HMOE_F32 || w_dtype == HMOE_BF16, "pack_mxfp4_down: weight dtype must be F32 or BF16");
   HMOE_REQUIRE(w_down && packed && exps, "pack_mxfp4_down: null pointer argument");
-  HMOE_REQUIRE_ALIGNED("pack_mxfp4_down", w_down, packed, exps);
+  HMOE_REQUIRE_ALIGNED("pack_mxfp4_down", 16, w_down, packed);
+  HMOE_REQUIRE_ALIGNED("pack_mxfp4_down", 4, exps);
   return pack_mxfp4("hmoe_pack_mxfp4_down", w_down, nullptr, w_dtype, n_experts, d_ff, d_model, packed, exps,
                     static_cast<hipStream_t>(stream));
 }
@@ -300,7 +302,7 @@ extern "C" int hmoe_unpack_mxfp4(const uint8_t* packed, const uint8_t* exps, int
                     "unpack_mxfp4: cols must be a multiple of 128 (got %d)", cols);
   HMOE_REQUIRE(out_dtype == HMOE_F32 || out_dtype == HMOE_BF16, "unpack_mxfp4: out dtype must be F32 or BF16");
   HMOE_REQUIRE(packed && exps && out, "unpack_mxfp4: null pointer argument");
-  HMOE_REQUIRE_ALIGNED("unpack_mxfp4", packed, exps, out);
+  HMOE_REQUIRE_ALIGNED("unpack_mxfp4", 16, packed, out);
   const int64_t row_blocks = static_cast<int64_t>(n_experts) * (rows / 32);
   const int64_t col_blocks = ceil_div(cols / 64, kUnpackBlocks);
   HMOE_REQUIRE(row_blocks < (int64_t(1) << 31) && col_blocks <= 65535, "unpack_mxfp4: operand too large");

@@ -20,12 +20,12 @@ namespace hmoe {
 
 constexpr int kMxBlock = 32;
 
-// Operands are read and written 16 bytes at a time.
-inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-#define HMOE_REQUIRE_ALIGNED(what, ...)                                                    \
-  do {                                                                                     \
-    for (const void* p_ : std::initializer_list<const void*>{__VA_ARGS__})                 \
-      HMOE_REQUIRE(::hmoe::aligned16(p_), "%s: operands must be 16-byte aligned", (what)); \
+// Codes and values are read and written 16 bytes at a time, exponents by words.
+inline bool aligned_to(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+#define HMOE_REQUIRE_ALIGNED(what, bytes, ...)                                                \
+  do {                                                                                        \
+    for (const void* p_ : std::initializer_list<const void*>{__VA_ARGS__})                    \
+      HMOE_REQUIRE(::hmoe::aligned_to(p_, bytes), "%s: an operand is not %d-byte aligned", (what), (bytes)); \
   } while (0)
 
 // E from the largest of the block's |v| as float32 bits (as integers they order

@@ -5,7 +5,8 @@ and runs the layer (router -> plan -> permute -> grouped SwiGLU -> combine)
 entirely through ``libhanuman_moe.so``; ``forward`` is the step ``bench.py``
 times and the GPU tests check.  With bf16 tokens and SwiGLU experts the
 permutation is fused into the gate/up GEMM (``xs`` is then ``None``); with
-fp8 experts on bf16 tokens the gate/up GEMM gathers from the per-token codes.
+fp8 experts on bf16 tokens the gate/up GEMM gathers from the per-token codes,
+with mxfp4 experts from the tokens' 4-bit rows.
 """
 from __future__ import annotations
 
@@ -22,11 +23,12 @@ class DeviceLayer:
     def __init__(self, inp: Inputs, device: str | torch.device = "cuda",
                  fused_ffn: bool | None = None):
         wl: Workload = inp.wl
-        if wl.expert_dtype not in ("bf16", "fp8", "f32"):
+        if wl.expert_dtype not in ("bf16", "fp8", "f32", "mxfp4"):
             raise NotImplementedError(f"{wl.name}: expert dtype {wl.expert_dtype} is not built")
         self.wl = wl
         self.fp8 = wl.expert_dtype == "fp8"
         self.f32 = wl.expert_dtype == "f32"
+        self.mxfp4 = wl.expert_dtype == "mxfp4"
         dev = torch.device(device)
         self.device = dev
         self.x = torch.from_numpy(inp.x).to(dev, _TORCH_DT[wl.x_dtype]).contiguous()
@@ -42,6 +44,7 @@ class DeviceLayer:
         self.w_down = None
         self.w_gate_up_scale = None
         self.w_down_scale = None
+        self.w_gate_up_exp = self.w_down_exp = None
         self.w_gate = self.w_up = self.w_down_f32 = None
         if wl.expert == "swiglu" and self.f32:
             # float32 compute: the masters as they are
@@ -53,18 +56,22 @@ class DeviceLayer:
             wu = torch.from_numpy(inp.w_up).to(dev)
             if self.fp8:
                 self.w_gate_up, self.w_gate_up_scale = K.pack_fp8_gate_up(wg, wu)
+            elif self.mxfp4:
+                self.w_gate_up, self.w_gate_up_exp = K.pack_mxfp4_gate_up(wg, wu)
             else:
                 self.w_gate_up = K.pack_gate_up(wg, wu)
             del wg, wu
             wd = torch.from_numpy(inp.w_down).to(dev)
             if self.fp8:
                 self.w_down, self.w_down_scale = K.pack_fp8_down(wd)
+            elif self.mxfp4:
+                self.w_down, self.w_down_exp = K.pack_mxfp4_down(wd)
             else:
                 self.w_down = K.pack_down(wd)
             del wd
         # bf16 SwiGLU experts on bf16 tokens: the gate/up GEMM gathers its rows
         # from x itself (hmoe_grouped_gate_up_gather), no dispatched copy.
-        self.fused_dispatch = (wl.expert == "swiglu" and not self.fp8
+        self.fused_dispatch = (wl.expert == "swiglu" and not self.fp8 and not self.mxfp4
                                and self.x.dtype == torch.bfloat16)
         # fp8 experts on bf16 tokens: x is quantised per token and the gate/up
         # GEMM gathers from its codes (hmoe_grouped_gate_up_fp8_gather).
@@ -127,6 +134,14 @@ class DeviceLayer:
         ys = K.grouped_down_fp8_mx(h_q, h_e, plan.offsets, self.w_down, self.w_down_scale)
         return xs_q, xs_s, h_q, h_e, ys
 
+    def experts_mxfp4(self, plan):
+        """MXFP4 tokens and expert GEMMs: (x_q, x_exp, h_q, h_exp, ys), codes and biased
+        exponents of the tokens and of h."""
+        x_q, x_e = K.quantize_rows_mxfp4(self.x)
+        h_q, h_e = K.grouped_gate_up_mxfp4_gather(x_q, x_e, plan, self.w_gate_up, self.w_gate_up_exp)
+        ys = K.grouped_down_mxfp4(h_q, h_e, plan.offsets, self.w_down, self.w_down_exp)
+        return x_q, x_e, h_q, h_e, ys
+
     def forward(self) -> dict:
         wl = self.wl
         logits, top_idx, gates, xq = self.route_quant()
@@ -137,6 +152,10 @@ class DeviceLayer:
             xs, xs_s, h_q, h_e, ys = self.experts_fp8(plan, xq)
             extra = {"xs_scale": xs_s, "h_q": h_q, "h_exp": h_e,
                      "xs_per_token": self.fp8_gather}
+        elif self.mxfp4 and wl.expert == "swiglu":
+            x_q, x_e, h_q, h_e, ys = self.experts_mxfp4(plan)
+            xs = None
+            extra = {"x_q": x_q, "x_exp": x_e, "h_q": h_q, "h_exp": h_e}
         elif self.f32:
             xs = K.permute_rows(self.x, plan, torch.float32)
             h = K.grouped_gate_up_f32(xs, plan.offsets, self.w_gate, self.w_up)

@@ -171,21 +171,33 @@ class MoE:
 
     Reference behaviour by default.  Keyword-only extensions (not in the
     reference): ``routing="softmax"`` (top-k of softmax, renormalised gates,
-    no bias, no scaling) and ``capacity_factor`` (per-expert capacity
-    ``ceil(CF*T*K/N)`` with token-order priority; ``None`` = dropless).
+    no bias, no scaling), ``capacity_factor`` (per-expert capacity
+    ``ceil(CF*T*K/N)`` with token-order priority; ``None`` = dropless) and
+    ``expert_dtype="mxfp4"`` (the routed experts on 4-bit operands quantised from
+    the masters, tokens and ``h`` quantised on the way; bfloat16 compute otherwise.
+    For inference: a call that autograd would record is refused).
     """
 
     def __init__(self, d_model: int, d_ff: int, n_experts: int, n_active: int,
                  n_shared_experts: int, router_init_std: float, routed_scaling_factor: float,
                  dtype, rngs, mesh=None, d_ff_shared: int | None = None, *,
                  routing: str = "sigmoid", capacity_factor: float | None = None,
-                 device: str | torch.device | None = None):
+                 expert_dtype: str | None = None, device: str | torch.device | None = None):
         if mesh is not None:
             size = getattr(getattr(mesh, "devices", None), "size", 1)
             if size > 1:
                 raise NotImplementedError("one GPU holds every expert; a multi-device mesh is not built")
         if routing not in ("sigmoid", "softmax"):
             raise ValueError(f"routing must be 'sigmoid' or 'softmax' (got {routing!r})")
+        if expert_dtype not in (None, "mxfp4"):
+            raise ValueError(f"expert_dtype must be None or 'mxfp4' (got {expert_dtype!r})")
+        if expert_dtype == "mxfp4":
+            if _torch_dtype(dtype) != torch.bfloat16:
+                raise ValueError("mxfp4 experts belong to the bfloat16 compute dtype")
+            # (256: the shared experts stay on the bf16 products)
+            if d_model % 256 or d_ff % 128:
+                raise ValueError("a layer with mxfp4 experts needs d_model that is a multiple of 256 "
+                                 f"and d_ff of 128 (got {d_model}, {d_ff})")
         dev = torch.device(device) if device is not None else torch.device("cuda")
         self.mesh = mesh
         self.expert_axis_name = None
@@ -196,6 +208,7 @@ class MoE:
         self.dtype = _torch_dtype(dtype)
         self.routing = routing
         self.capacity_factor = capacity_factor
+        self.expert_dtype = expert_dtype
         g = _generator(rngs, dev)
 
         def normal(shape, std):
@@ -218,6 +231,7 @@ class MoE:
             self.shared_w_down = Param(normal((n_shared_experts, dfs, d_model), std))
         self._routed_pack = _PackCache()
         self._shared_pack = _PackCache()
+        self._mxfp4_pack = _PackCache()
         self._routed_bwd_pack = _PackCache()
         self._shared_bwd_pack = _PackCache()
         self._backward_expected = True   # there was one since the last joint pack
@@ -290,6 +304,12 @@ class MoE:
                                       BackwardOperands.from_packed(gate_up_dgrad, down_dgrad))
             return gate_up, down
         return self._routed_pack.get((wg, wu, wd), build)
+
+    def _packed_mxfp4(self):
+        """The routed experts' MXFP4 operands (codes and exponents of gate/up, of down)."""
+        wg, wu, wd = self.expert_w_gate.value, self.expert_w_up.value, self.expert_w_down.value
+        return self._mxfp4_pack.get((wg, wu, wd), lambda: (
+            *K.pack_mxfp4_gate_up(wg.detach(), wu.detach()), *K.pack_mxfp4_down(wd.detach())))
 
     def _packed_shared(self, masters=None):
         """One ``(gate_up, down)`` of packed operands per shared expert."""
@@ -372,6 +392,9 @@ class MoE:
         are differentiable, ``expert_counts`` is not (``train.py:191-200``
         differentiates the same outputs)."""
         if torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in self._params())):
+            if self.expert_dtype is not None:
+                raise NotImplementedError("mxfp4 experts have no backward: call under torch.no_grad(), "
+                                          "or train the layer without expert_dtype")
             out, z, bal, ent, counts = _MoEFunction.apply(self, x, *self._params())
             return out, {"router_z_loss": z, "balance_loss": bal, "mean_entropy": ent,
                          "expert_counts": counts}
@@ -417,6 +440,18 @@ class MoE:
                          "plan": plan, "xs": xs, "h": h, "ys": ys, "h_shared": hs, "mode": mode,
                          "rsf": rsf, "batch": B, "seq": S}
             return out.reshape(B, S, D), losses, counts, saved
+        if self.expert_dtype == "mxfp4":
+            gate_up, gate_up_exp, down, down_exp = self._packed_mxfp4()
+            h_q, h_exp = K.grouped_gate_up_mxfp4_gather(*K.quantize_rows_mxfp4(x2), plan, gate_up,
+                                                        gate_up_exp)
+            ys = K.grouped_down_mxfp4(h_q, h_exp, plan.offsets, down, down_exp)
+            if x2.dtype == torch.float32 and self.n_shared_experts > 0:
+                shared = self._shared_ffn_promoted(x2)
+            else:
+                shared = self._shared_ffn(x2)
+            out = K.combine(ys, plan, gates, shared, torch.float32)
+            losses, counts = K.router_aux(logits, top_idx, B, S)
+            return out.reshape(B, S, D), losses, counts, None
         wgu, wd = self._packed_routed(train=save)
         if x2.dtype == torch.bfloat16 and not save and self.n_shared_experts > 0:
             # few rows an expert: the shared experts' tiles in the routed launches

@@ -390,7 +390,8 @@ int hmoe_grouped_wgrad_down_f32(const float* h, const float* d_ys, const int32_t
  * the scale rounded to nearest, ties to the even code.  A block with a value that
  * is not finite has E = 255 and zero codes and stands for NaN; a product with it is
  * NaN.  A value past the format's range (a block whose largest is 1.75 * 2^127 or
- * more) reads back as infinity.  Every pointer of an operand is 16-byte aligned. */
+ * more) reads back as infinity.  Codes and values are 16-byte aligned, exponents 4-byte
+ * (rows of either kind may start anywhere a row starts). */
 
 /* a [rows, cols] (F32/BF16) -> q [rows, cols / 2] uint8 (the even column in a
  * byte's low half), exps [rows, cols / 32] uint8.  cols % 32 == 0. */

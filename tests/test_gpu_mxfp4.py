@@ -283,6 +283,25 @@ def test_rows_past_the_segments_stay(gpu, rows_cap):
     assert torch.equal(h_q[:33], want_q) and torch.equal(h_e[:33], want_e)
 
 
+def test_rows_inside_a_buffer(gpu):
+    """Operands that start at a later row of their buffers: exponents then lie on words only."""
+    D, F = 384, 128
+    rng = np.random.default_rng(14)
+    x_q, x_e = K.quantize_rows_mxfp4(torch.randn((2003, D), device=gpu))
+    gu = [_to(t[None], gpu) for t in R.packed_operand(*R.quantise(rng.standard_normal((2 * F, D))))]
+    dn = [_to(t[None], gpu) for t in R.packed_operand(*R.quantise(rng.standard_normal((D, F))))]
+    for start, rows in ((1, 33), (3, 2000)):
+        off = torch.tensor([0, rows], dtype=torch.int32, device=gpu)
+        a_q, a_e = x_q[start:start + rows], x_e[start:start + rows]
+        assert a_e.data_ptr() % 16 != 0
+        h = K.grouped_gate_up_mxfp4(a_q, a_e, off, *gu)
+        want = K.grouped_gate_up_mxfp4(a_q.clone(), a_e.clone(), off, *gu)
+        assert torch.equal(h[0], want[0]) and torch.equal(h[1], want[1])
+        h_q, h_e = (torch.cat((t[:1], t)) for t in h)
+        assert torch.equal(K.grouped_down_mxfp4(h_q[1:], h_e[1:], off, *dn), K.grouped_down_mxfp4(*h, off, *dn))
+    assert torch.equal(K.dequantize_rows_mxfp4(x_q[1:], x_e[1:]), K.dequantize_rows_mxfp4(x_q, x_e)[1:])
+
+
 def test_dropped_slots(gpu):
     """A capacity that drops slots: the kept rows are right, and combine leaves out the others."""
     shape = (64, 4, 2, 256, 128)

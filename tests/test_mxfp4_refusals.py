@@ -115,3 +115,14 @@ def test_python_layer():
             call()
     with pytest.raises(TypeError):
         K.quantize_rows_mxfp4([1.0])
+
+
+def test_module_arguments():
+    from hanuman_amd import MoE
+    with pytest.raises(ValueError, match="expert_dtype"):
+        MoE(256, 128, 4, 2, 1, 0.02, 1.0, "bfloat16", rngs=0, expert_dtype="fp4", device="cpu")
+    with pytest.raises(ValueError, match="bfloat16"):
+        MoE(256, 128, 4, 2, 1, 0.02, 1.0, "float32", rngs=0, expert_dtype="mxfp4", device="cpu")
+    for d, f in ((128, 128), (384, 128), (192, 128), (256, 64)):
+        with pytest.raises(ValueError, match="128"):
+            MoE(d, f, 4, 2, 1, 0.02, 1.0, "bfloat16", rngs=0, expert_dtype="mxfp4", device="cpu")
