@@ -332,10 +332,18 @@ __global__ __launch_bounds__(256) void grouped_mxfp4_rows(
 // the next tile, one barrier a step.  A's part of a stage has 64-byte rows whose 16-byte
 // chunk c sits at c ^ swz64(r), so that 16 lanes of a fragment read cover all banks;
 // B's is the operand's own blocks of 1 KB, read lane by lane, and its exponents are a
-// run of 1 KB.  A's exponents, 16 bytes of every row, come for up to four steps at once
+// run of 1 KB, put down in the order in which a lane reads four words.  A's exponents, 16 bytes of every row, come for up to four steps at once
 // into one of two regions (three with 64 rows, where a tile may be a single step).  The
 // last column tile may be 128 columns wide: the waves of the other half load and compute
 // the first half's again and store nothing.
+//
+// What bounds the large products is power: with these operands the matrix cores alone,
+// fed from registers, run at 1.65 GHz and 6.5 PFLOP/s.  Gate/up of 131072 rows, D 2048, F
+// 1024 (1.1 TFLOP) takes 333 us, 300 of them in the loop at 1.6 to 1.8 GHz, 1580 cycles for
+// two workgroups' steps (1024 of MFMA).  One workgroup of eight waves on 256 x 256 tiles (a
+// third less from L2) took 336 us at 1.8 GHz and 1750 cycles, four waves of 128 x 128
+// (a third less from LDS too) 400 us, the 16 x 16 x 128 MFMA 1900 cycles at 1.95 GHz, all
+// about 300 us in the loop.
 constexpr int kTileThreads = 256;
 constexpr int kStages = 3;
 constexpr int kNumXcd = 8;
@@ -490,7 +498,10 @@ __global__ __launch_bounds__(kTileThreads, 2) void grouped_mxfp4_tiles(
   __amdgpu_buffer_rsrc_t b_rsrc = a_rsrc, be_rsrc = a_rsrc;
   uint32_t a_voff[kNA], ae_voff = 0;
   const int b_col = (kdim / 64) * 1024;  // bytes of 32 columns
-  int b_wave = 0, be_wave = 0;           // where this wave's part of B's tile begins
+  // (words of a half's columns c, c + 32, c + 64, c + 96 together, as a lane reads them)
+  const int ex_word = (wave & 1) * 64 + lane;
+  const uint32_t be_voff = static_cast<uint32_t>(((ex_word & 3) * 32 + (ex_word >> 2)) * 4);
+  int b_wave = 0, be_wave = 0;       // where this wave's part of B's tile begins
   const bool ex_a = wave < BM / 64;  // the waves that bring A's exponents
   int ld_kb = 0, ld_left = 0, ld_g = 0, ld_t = first, ld_region = Cfg::kRegions - 1, ld_stage = 0;
   int32_t pf_src[kNA], pf_ex = 0;  // GATHER: sources of this lane's rows
@@ -514,7 +525,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void grouped_mxfp4_tiles(
     const int width = ncols - ld.n0 < kTileN ? ncols - ld.n0 : kTileN;
     const int part = 64 * wave < width ? wave : wave - 2;  // (a tile of 128 columns: waves 0 and 1 again)
     b_wave = part * 2 * b_col;
-    be_wave = part * 256;
+    be_wave = (part >> 1) * 512;
     b_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(B + block * b_col), 0, width * row_bytes,
                                                kBufferWord3);
     be_rsrc = __builtin_amdgcn_make_buffer_rsrc(
@@ -564,7 +575,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void grouped_mxfp4_tiles(
     for (int j = 0; j < kNB; ++j)
       dma16(b_rsrc, st + Cfg::kA + (wave * kNB + j) * 1024, static_cast<uint32_t>(lane * 16),
             b_wave + (j >> 1) * b_col + kb * 2048 + (j & 1) * 1024);
-    dma4(be_rsrc, st + Cfg::kA + Cfg::kB + wave * 256, static_cast<uint32_t>(lane * 4), be_wave + kb * ncols * 4);
+    dma4(be_rsrc, st + Cfg::kA + Cfg::kB + wave * 256, be_voff, be_wave + kb * ncols * 4);
     if (ld_g < iters) {
       ++ld_g;
       ++ld_kb;
@@ -580,7 +591,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void grouped_mxfp4_tiles(
   const int fsw = swz64(frow);
   const int a_off = (wm * (BM / 2) + frow) * 64;
   const int b_off = Cfg::kA + wn * 8192 + lane * 16;
-  const int be_off = Cfg::kA + Cfg::kB + (wn * 128 + frow) * 4;
+  const int be_off = Cfg::kA + Cfg::kB + wn * 512 + frow * 16;
   const int ae_off = kStages * Cfg::kStage + (wm * (BM / 2) + frow) * 16;
   f32x16 acc[kFR][4];
   int stage = 0, region = Cfg::kRegions - 1, left = 0, in_group = 0;
@@ -588,9 +599,9 @@ __global__ __launch_bounds__(kTileThreads, 2) void grouped_mxfp4_tiles(
     const uint8_t* st = smem + stage * Cfg::kStage;
     u32x4 fa[2][kFR], fb[2][4];
     int exa[kFR], exb[4];
+    const u32x4 exw = *reinterpret_cast<const u32x4*>(st + be_off);
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      exb[j] = static_cast<int>(*reinterpret_cast<const uint32_t*>(st + be_off + j * 128) >> (8 * half));
+    for (int j = 0; j < 4; ++j) exb[j] = static_cast<int>(exw[j] >> (8 * half));
 #pragma unroll
     for (int i = 0; i < kFR; ++i)
       exa[i] = static_cast<int>(*reinterpret_cast<const uint32_t*>(smem + ae_off + region * Cfg::kExA + i * 512 +
