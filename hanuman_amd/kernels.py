@@ -731,11 +731,11 @@ def quantize_rows_mxfp4(a: torch.Tensor):
     """MXFP4 rows of a float32 or bf16 matrix ``[rows, cols]``: codes uint8 ``[rows,
     cols / 2]`` (the even column in a byte's low half) and biased exponents uint8
     ``[rows, cols / 32]``."""
-    dev = _current_device("quantize_rows_mxfp4", a, 2)
+    _current_device("quantize_rows_mxfp4", a, 2)
     rows, cols = a.shape
-    q = torch.empty((rows, cols // 2), dtype=torch.uint8, device=dev)
-    exps = torch.empty((rows, cols // 32), dtype=torch.uint8, device=dev)
-    call("hmoe_quantize_rows_mxfp4", _ptr(a), _dtype_code(a), rows, cols, _ptr(q), _ptr(exps),
+    q = a.new_empty((rows, cols // 2), dtype=_U8)
+    exps = q.new_empty((rows, cols // 32))
+    call("hmoe_quantize_rows_mxfp4", a.data_ptr(), _dtype_code(a), rows, cols, q.data_ptr(), exps.data_ptr(),
          _stream())
     return q, exps
 
@@ -750,16 +750,16 @@ def dequantize_rows_mxfp4(q: torch.Tensor, exps: torch.Tensor,
     _u8("dequantize_rows_mxfp4", dev, exps, (rows, cols // 32))
     if out_dtype not in _DT:
         raise TypeError(f"unsupported dtype {out_dtype}; expected float32 or bfloat16")
-    out = torch.empty((rows, cols), dtype=out_dtype, device=dev)
-    call("hmoe_dequantize_rows_mxfp4", _ptr(q), _ptr(exps), rows, cols, _ptr(out), _DT[out_dtype],
-         _stream())
+    out = q.new_empty((rows, cols), dtype=out_dtype)
+    call("hmoe_dequantize_rows_mxfp4", q.data_ptr(), exps.data_ptr(), rows, cols, out.data_ptr(),
+         _DT[out_dtype], _stream())
     return out
 
 
 def _mxfp4_operand(N: int, rows: int, k: int, dev):
     """Empty codes and exponents of a packed operand (see ``hmoe_pack_mxfp4_gate_up``)."""
-    return (torch.empty((N, rows // 32, k // 64, 64, 16), dtype=torch.uint8, device=dev),
-            torch.empty((N, k // 128, rows, 4), dtype=torch.uint8, device=dev))
+    codes = torch.empty((N, rows // 32, k // 64, 64, 16), dtype=_U8, device=dev)
+    return codes, codes.new_empty((N, k // 128, rows, 4))
 
 
 def pack_mxfp4_gate_up(w_gate: torch.Tensor, w_up: torch.Tensor):
@@ -772,8 +772,8 @@ def pack_mxfp4_gate_up(w_gate: torch.Tensor, w_up: torch.Tensor):
         raise ValueError("w_gate and w_up must have the same shape and dtype")
     N, D, F = w_gate.shape
     out, exps = _mxfp4_operand(N, 2 * F, D, dev)
-    call("hmoe_pack_mxfp4_gate_up", _ptr(w_gate), _ptr(w_up), _dtype_code(w_gate), N, D, F,
-         _ptr(out), _ptr(exps), _stream())
+    call("hmoe_pack_mxfp4_gate_up", w_gate.data_ptr(), w_up.data_ptr(), _dtype_code(w_gate), N, D, F,
+         out.data_ptr(), exps.data_ptr(), _stream())
     return out, exps
 
 
@@ -783,8 +783,8 @@ def pack_mxfp4_down(w_down: torch.Tensor):
     dev = _current_device("pack_mxfp4_down", w_down, 3)
     N, F, D = w_down.shape
     out, exps = _mxfp4_operand(N, D, F, dev)
-    call("hmoe_pack_mxfp4_down", _ptr(w_down), _dtype_code(w_down), N, F, D, _ptr(out),
-         _ptr(exps), _stream())
+    call("hmoe_pack_mxfp4_down", w_down.data_ptr(), _dtype_code(w_down), N, F, D, out.data_ptr(),
+         exps.data_ptr(), _stream())
     return out, exps
 
 
@@ -808,7 +808,7 @@ def unpack_mxfp4(packed: torch.Tensor, exps: torch.Tensor,
     if out_dtype not in _DT:
         raise TypeError(f"unsupported dtype {out_dtype}; expected float32 or bfloat16")
     out = torch.empty((N, rows, k), dtype=out_dtype, device=dev)
-    call("hmoe_unpack_mxfp4", _ptr(packed), _ptr(exps), N, rows, k, _ptr(out), _DT[out_dtype],
+    call("hmoe_unpack_mxfp4", packed.data_ptr(), exps.data_ptr(), N, rows, k, out.data_ptr(), _DT[out_dtype],
          _stream())
     return out
 
@@ -833,10 +833,10 @@ def grouped_gate_up_mxfp4(xs_q: torch.Tensor, xs_exp: torch.Tensor, offsets: tor
     _u8(name, dev, xs_q, (rows, D // 2))
     _u8(name, dev, xs_exp, (rows, D // 32))
     _check_i32(name, "offsets", offsets, N + 1, dev)
-    h_q = torch.empty((rows, F // 2), dtype=torch.uint8, device=dev)
-    h_exp = torch.empty((rows, F // 32), dtype=torch.uint8, device=dev)
-    call("hmoe_grouped_gate_up_mxfp4", _ptr(xs_q), _ptr(xs_exp), _ptr(offsets), N, rows, D, F,
-         _ptr(w_packed), _ptr(w_exp), _ptr(h_q), _ptr(h_exp), _stream())
+    h_q = xs_q.new_empty((rows, F // 2))
+    h_exp = xs_q.new_empty((rows, F // 32))
+    call("hmoe_grouped_gate_up_mxfp4", xs_q.data_ptr(), xs_exp.data_ptr(), offsets.data_ptr(), N, rows, D, F,
+         w_packed.data_ptr(), w_exp.data_ptr(), h_q.data_ptr(), h_exp.data_ptr(), _stream())
     return h_q, h_exp
 
 
@@ -854,11 +854,11 @@ def grouped_gate_up_mxfp4_gather(x_q: torch.Tensor, x_exp: torch.Tensor, plan: P
         raise ValueError(f"{name}: the plan is of other tokens or experts")
     _check_i32(name, "offsets", plan.offsets, N + 1, dev)
     _check_i32(name, "perm_src", plan.perm_src, plan.rows_cap, dev)
-    h_q = torch.empty((plan.rows_cap, F // 2), dtype=torch.uint8, device=dev)
-    h_exp = torch.empty((plan.rows_cap, F // 32), dtype=torch.uint8, device=dev)
-    call("hmoe_grouped_gate_up_mxfp4_gather", _ptr(x_q), _ptr(x_exp), T, plan.top_k,
-         _ptr(plan.perm_src), _ptr(plan.offsets), N, plan.rows_cap, D, F, _ptr(w_packed),
-         _ptr(w_exp), _ptr(h_q), _ptr(h_exp), _stream())
+    h_q = x_q.new_empty((plan.rows_cap, F // 2))
+    h_exp = x_q.new_empty((plan.rows_cap, F // 32))
+    call("hmoe_grouped_gate_up_mxfp4_gather", x_q.data_ptr(), x_exp.data_ptr(), T, plan.top_k,
+         plan.perm_src.data_ptr(), plan.offsets.data_ptr(), N, plan.rows_cap, D, F, w_packed.data_ptr(),
+         w_exp.data_ptr(), h_q.data_ptr(), h_exp.data_ptr(), _stream())
     return h_q, h_exp
 
 
@@ -873,9 +873,9 @@ def grouped_down_mxfp4(h_q: torch.Tensor, h_exp: torch.Tensor, offsets: torch.Te
     _u8(name, dev, h_q, (rows, F // 2))
     _u8(name, dev, h_exp, (rows, F // 32))
     _check_i32(name, "offsets", offsets, N + 1, dev)
-    ys = torch.empty((rows, D), dtype=torch.bfloat16, device=dev)
-    call("hmoe_grouped_down_mxfp4", _ptr(h_q), _ptr(h_exp), _ptr(offsets), N, rows, F, D,
-         _ptr(w_packed), _ptr(w_exp), _ptr(ys), _stream())
+    ys = h_q.new_empty((rows, D), dtype=torch.bfloat16)
+    call("hmoe_grouped_down_mxfp4", h_q.data_ptr(), h_exp.data_ptr(), offsets.data_ptr(), N, rows, F, D,
+         w_packed.data_ptr(), w_exp.data_ptr(), ys.data_ptr(), _stream())
     return ys
 
 
