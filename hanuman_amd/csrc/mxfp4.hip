@@ -36,21 +36,33 @@ __global__ __launch_bounds__(256) void quantize_rows_mxfp4_kernel(const TI* __re
   }
 }
 
-__device__ __forceinline__ void store8(float* o, const float (&v)[8]) {
-  *reinterpret_cast<f32x4*>(o) = f32x4{v[0], v[1], v[2], v[3]};
-  *reinterpret_cast<f32x4*>(o + 4) = f32x4{v[4], v[5], v[6], v[7]};
+// Eight values of a row.  PAST: past the caches, for matrices that they cannot hold.
+template <bool PAST, typename V>
+__device__ __forceinline__ void store16(V* o, V v) {
+  if (PAST) __builtin_nontemporal_store(v, o);
+  else *o = v;
 }
-// (the values are exact in bf16, a sum of no more than two bits' weight: the
-// upper half of the float32 is all of it)
+template <bool PAST>
+__device__ __forceinline__ void store8(float* o, const float (&v)[8]) {
+  store16<PAST>(reinterpret_cast<f32x4*>(o), f32x4{v[0], v[1], v[2], v[3]});
+  store16<PAST>(reinterpret_cast<f32x4*>(o + 4), f32x4{v[4], v[5], v[6], v[7]});
+}
+// (the values have two significant bits: the upper half of the float32 is all of them)
+template <bool PAST>
 __device__ __forceinline__ void store8(uint16_t* o, const float (&v)[8]) {
   u32x4 w;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     w[i] = (__float_as_uint(v[2 * i]) >> 16) | (__float_as_uint(v[2 * i + 1]) & 0xffff0000u);
-  *reinterpret_cast<u32x4*>(o) = w;
+  store16<PAST>(reinterpret_cast<u32x4*>(o), w);
 }
 
-template <typename TO>
+// Written values that are more than the L2s (8 x 4 MB) go past them: 134 M values to
+// bf16 (268 MB) take 65 us through them and 47 past them, 33 M 13.6 and 11.2.  Fewer are
+// left to the caches, from which what follows reads them.
+constexpr int64_t kCachedBytes = int64_t(32) << 20;
+
+template <typename TO, bool PAST>
 __global__ __launch_bounds__(256) void dequantize_rows_mxfp4_kernel(const uint8_t* __restrict__ q,
                                                                     const uint8_t* __restrict__ exps,
                                                                     int64_t chunks, TO* __restrict__ out) {
@@ -58,16 +70,16 @@ __global__ __launch_bounds__(256) void dequantize_rows_mxfp4_kernel(const uint8_
   for (int64_t c = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; c < chunks; c += stride) {
     float v[8];
     mxfp4_values8(reinterpret_cast<const uint32_t*>(q)[c], mxfp4_scale(exps[c >> 2]), v);
-    store8(out + c * 8, v);
+    store8<PAST>(out + c * 8, v);
   }
 }
 
 // A packed operand's values row by row.  A workgroup takes 32 rows x 64 kUnpackBlocks
 // columns, eight values a thread and block of 1 KB, so that eight threads write a run of
 // 128 (bf16) or 256 bytes.  Bound by memory: 268 M values to bf16 (0.68 GB moved) in
-// 130-150 us; found by dividing a flat index it took 232 us, most of it the divisions.
+// 145 us; found by dividing a flat index it took 232 us, most of it the divisions.
 constexpr int kUnpackBlocks = 4;
-template <typename TO>
+template <typename TO, bool PAST>
 __global__ __launch_bounds__(256) void unpack_mxfp4_kernel(const uint8_t* __restrict__ packed,
                                                            const uint8_t* __restrict__ exps, int rows, int cols,
                                                            TO* __restrict__ out) {
@@ -96,19 +108,21 @@ __global__ __launch_bounds__(256) void unpack_mxfp4_kernel(const uint8_t* __rest
     if (b < blocks) {
       float v[8];
       mxfp4_values8(w[j], mxfp4_scale(e[j]), v);
-      store8(o + b * 64, v);
+      store8<PAST>(o + b * 64, v);
     }
   }
 }
 
-// Two neighbouring columns of a master.
+// Two neighbouring columns of a master, which is read once (past the caches: 268 M
+// float32 masters packed in 213 us, through them in 237).
 __device__ __forceinline__ void load2(const float* p, float& a, float& b) {
-  const float2 v = *reinterpret_cast<const float2*>(p);
-  a = v.x;
-  b = v.y;
+  typedef float f32x2_t __attribute__((ext_vector_type(2)));
+  const f32x2_t v = __builtin_nontemporal_load(reinterpret_cast<const f32x2_t*>(p));
+  a = v[0];
+  b = v[1];
 }
 __device__ __forceinline__ void load2(const uint16_t* p, float& a, float& b) {
-  const uint32_t v = *reinterpret_cast<const uint32_t*>(p);
+  const uint32_t v = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p));
   a = __uint_as_float(v << 16);
   b = __uint_as_float(v & 0xffff0000u);
 }
@@ -246,12 +260,15 @@ extern "C" int hmoe_dequantize_rows_mxfp4(const uint8_t* q, const uint8_t* exps,
   HMOE_REQUIRE_ALIGNED("dequantize_rows_mxfp4", 16, q, out);
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int64_t chunks = rows * (cols / 8);
-  if (out_dtype == HMOE_F32)
-    hipLaunchKernelGGL(dequantize_rows_mxfp4_kernel<float>, dim3(chunk_grid(chunks)), dim3(256), 0, s, q, exps,
-                       chunks, static_cast<float*>(out));
-  else
-    hipLaunchKernelGGL(dequantize_rows_mxfp4_kernel<uint16_t>, dim3(chunk_grid(chunks)), dim3(256), 0, s, q, exps,
-                       chunks, static_cast<uint16_t*>(out));
+  const bool past = rows * cols * (out_dtype == HMOE_F32 ? 4 : 2) > kCachedBytes;
+#define HMOE_LAUNCH_DEQUANT4(TO, PAST)                                                                        \
+  hipLaunchKernelGGL((dequantize_rows_mxfp4_kernel<TO, PAST>), dim3(chunk_grid(chunks)), dim3(256), 0, s, q, \
+                     exps, chunks, static_cast<TO*>(out))
+  if (out_dtype == HMOE_F32 && past) HMOE_LAUNCH_DEQUANT4(float, true);
+  else if (out_dtype == HMOE_F32) HMOE_LAUNCH_DEQUANT4(float, false);
+  else if (past) HMOE_LAUNCH_DEQUANT4(uint16_t, true);
+  else HMOE_LAUNCH_DEQUANT4(uint16_t, false);
+#undef HMOE_LAUNCH_DEQUANT4
   return check_launch("hmoe_dequantize_rows_mxfp4");
 }
 
@@ -308,11 +325,14 @@ extern "C" int hmoe_unpack_mxfp4(const uint8_t* packed, const uint8_t* exps, int
   HMOE_REQUIRE(row_blocks < (int64_t(1) << 31) && col_blocks <= 65535, "unpack_mxfp4: operand too large");
   hipStream_t s = static_cast<hipStream_t>(stream);
   const dim3 grid(static_cast<unsigned>(row_blocks), static_cast<unsigned>(col_blocks));
-  if (out_dtype == HMOE_F32)
-    hipLaunchKernelGGL(unpack_mxfp4_kernel<float>, grid, dim3(256), 0, s, packed, exps, rows, cols,
-                       static_cast<float*>(out));
-  else
-    hipLaunchKernelGGL(unpack_mxfp4_kernel<uint16_t>, grid, dim3(256), 0, s, packed, exps, rows, cols,
-                       static_cast<uint16_t*>(out));
+  const bool past = row_blocks * 32 * cols * (out_dtype == HMOE_F32 ? 4 : 2) > kCachedBytes;
+#define HMOE_LAUNCH_UNPACK4(TO, PAST)                                                                      \
+  hipLaunchKernelGGL((unpack_mxfp4_kernel<TO, PAST>), grid, dim3(256), 0, s, packed, exps, rows, cols, \
+                     static_cast<TO*>(out))
+  if (out_dtype == HMOE_F32 && past) HMOE_LAUNCH_UNPACK4(float, true);
+  else if (out_dtype == HMOE_F32) HMOE_LAUNCH_UNPACK4(float, false);
+  else if (past) HMOE_LAUNCH_UNPACK4(uint16_t, true);
+  else HMOE_LAUNCH_UNPACK4(uint16_t, false);
+#undef HMOE_LAUNCH_UNPACK4
   return check_launch("hmoe_unpack_mxfp4");
 }
