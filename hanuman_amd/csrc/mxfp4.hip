@@ -211,14 +211,14 @@ int pack_mxfp4(const char* what, const void* w0, const void* w1, int w_dtype, in
 }
 
 // The sizes that every packed MXFP4 operand has: whole 128-value groups of the
-// reduction, rows in blocks of 32 (gate/up: 64).
+// reduction, rows in blocks of 32 (gate/up: 64), and the products' limits.
 int check_operand(const char* what, int n_experts, int d_model, int d_ff) {
   HMOE_REQUIRE(n_experts >= 1 && n_experts <= 1024, "%s: n_experts must be in [1, 1024] (got %d)", what,
                n_experts);
-  HMOE_REQUIRE_CODE(d_model >= 128 && d_model % 128 == 0, HMOE_ERR_UNSUPPORTED,
-                    "%s: d_model must be a multiple of 128 (got %d)", what, d_model);
-  HMOE_REQUIRE_CODE(d_ff >= 128 && d_ff % 128 == 0, HMOE_ERR_UNSUPPORTED,
-                    "%s: d_ff must be a multiple of 128 (got %d)", what, d_ff);
+  HMOE_REQUIRE_CODE(d_model >= 128 && d_model % 128 == 0 && d_model <= (1 << 20), HMOE_ERR_UNSUPPORTED,
+                    "%s: d_model must be a multiple of 128 up to 2^20 (got %d)", what, d_model);
+  HMOE_REQUIRE_CODE(d_ff >= 128 && d_ff % 128 == 0 && d_ff <= (1 << 20), HMOE_ERR_UNSUPPORTED,
+                    "%s: d_ff must be a multiple of 128 up to 2^20 (got %d)", what, d_ff);
   return HMOE_OK;
 }
 
@@ -322,7 +322,8 @@ extern "C" int hmoe_unpack_mxfp4(const uint8_t* packed, const uint8_t* exps, int
   HMOE_REQUIRE_ALIGNED("unpack_mxfp4", 16, packed, out);
   const int64_t row_blocks = static_cast<int64_t>(n_experts) * (rows / 32);
   const int64_t col_blocks = ceil_div(cols / 64, kUnpackBlocks);
-  HMOE_REQUIRE(row_blocks < (int64_t(1) << 31) && col_blocks <= 65535, "unpack_mxfp4: operand too large");
+  // (a launch has fewer than 2^32 threads along x)
+  HMOE_REQUIRE(row_blocks * 256 < (int64_t(1) << 32) && col_blocks <= 65535, "unpack_mxfp4: operand too large");
   hipStream_t s = static_cast<hipStream_t>(stream);
   const dim3 grid(static_cast<unsigned>(row_blocks), static_cast<unsigned>(col_blocks));
   const bool past = row_blocks * 32 * cols * (out_dtype == HMOE_F32 ? 4 : 2) > kCachedBytes;

@@ -584,7 +584,7 @@ static ffi::Error QuantizeRowsMxfp4Impl(hipStream_t stream, ffi::AnyBuffer a, ff
                                         ffi::ResultBuffer<ffi::U8> exps) {
   const int d = DtypeCode(a.element_type());
   if (d < 0) return BadDtype("hmoe_quantize_rows_mxfp4");
-  if (!Mxfp4Rows(*q, *exps, Rows(a), Cols(a))) return BadMxfp4("hmoe_quantize_rows_mxfp4");
+  if (a.dimensions().size() != 2 || !Mxfp4Rows(*q, *exps, Rows(a), Cols(a))) return BadMxfp4("hmoe_quantize_rows_mxfp4");
   return Status(hmoe_quantize_rows_mxfp4(a.untyped_data(), d, Rows(a), static_cast<int>(Cols(a)),
                                          q->typed_data(), exps->typed_data(), S(stream)));
 }
@@ -600,7 +600,7 @@ static ffi::Error DequantizeRowsMxfp4Impl(hipStream_t stream, ffi::Buffer<ffi::U
                                           ffi::Buffer<ffi::U8> exps, ffi::Result<ffi::AnyBuffer> out) {
   const int d = DtypeCode(out->element_type());
   if (d < 0) return BadDtype("hmoe_dequantize_rows_mxfp4");
-  if (!Mxfp4Rows(q, exps, Rows(*out), Cols(*out))) return BadMxfp4("hmoe_dequantize_rows_mxfp4");
+  if (out->dimensions().size() != 2 || !Mxfp4Rows(q, exps, Rows(*out), Cols(*out))) return BadMxfp4("hmoe_dequantize_rows_mxfp4");
   return Status(hmoe_dequantize_rows_mxfp4(q.typed_data(), exps.typed_data(), Rows(q),
                                            static_cast<int>(Cols(*out)), out->untyped_data(), d, S(stream)));
 }
@@ -618,7 +618,9 @@ static ffi::Error PackMxfp4GateUpImpl(hipStream_t stream, ffi::AnyBuffer wg, ffi
   if (d < 0 || DtypeCode(wu.element_type()) != d) return BadDtype("hmoe_pack_mxfp4_gate_up");
   auto dims = wg.dimensions();
   auto out = packed->dimensions();
-  if (!Mxfp4Operand(*packed, *exps) || out[0] != dims[0] || out[1] * 16 != dims[2] || out[2] * 64 != dims[1])
+  auto up = wu.dimensions();
+  if (dims.size() != 3 || up.size() != 3 || up[0] != dims[0] || up[1] != dims[1] || up[2] != dims[2] ||
+      !Mxfp4Operand(*packed, *exps) || out[0] != dims[0] || out[1] * 16 != dims[2] || out[2] * 64 != dims[1])
     return BadMxfp4("hmoe_pack_mxfp4_gate_up");
   return Status(hmoe_pack_mxfp4_gate_up(wg.untyped_data(), wu.untyped_data(), d, static_cast<int>(dims[0]),
                                         static_cast<int>(dims[1]), static_cast<int>(dims[2]),
@@ -639,7 +641,8 @@ static ffi::Error PackMxfp4DownImpl(hipStream_t stream, ffi::AnyBuffer wd, ffi::
   if (d < 0) return BadDtype("hmoe_pack_mxfp4_down");
   auto dims = wd.dimensions();
   auto out = packed->dimensions();
-  if (!Mxfp4Operand(*packed, *exps) || out[0] != dims[0] || out[1] * 32 != dims[2] || out[2] * 64 != dims[1])
+  if (dims.size() != 3 || !Mxfp4Operand(*packed, *exps) || out[0] != dims[0] || out[1] * 32 != dims[2] ||
+      out[2] * 64 != dims[1])
     return BadMxfp4("hmoe_pack_mxfp4_down");
   return Status(hmoe_pack_mxfp4_down(wd.untyped_data(), d, static_cast<int>(dims[0]),
                                      static_cast<int>(dims[1]), static_cast<int>(dims[2]),
@@ -741,7 +744,7 @@ static ffi::Error GroupedDownMxfp4Impl(hipStream_t stream, ffi::Buffer<ffi::U8> 
   auto d = w.dimensions();
   const int64_t n = static_cast<int64_t>(offsets.element_count()) - 1;
   if (!Mxfp4Operand(w, w_exp) || d[0] != n || !Mxfp4Rows(h_q, h_exp, Rows(h_q), d[2] * 64) ||
-      Rows(*ys) != Rows(h_q) || Cols(*ys) != d[1] * 32)
+      ys->dimensions().size() != 2 || Rows(*ys) != Rows(h_q) || Cols(*ys) != d[1] * 32)
     return BadMxfp4("hmoe_grouped_down_mxfp4");
   return Status(hmoe_grouped_down_mxfp4(h_q.typed_data(), h_exp.typed_data(), offsets.typed_data(),
                                         static_cast<int>(n), Rows(h_q), static_cast<int>(d[2] * 64),

@@ -409,7 +409,7 @@ int hmoe_dequantize_rows_mxfp4(const uint8_t* q, const uint8_t* exps, int64_t ro
  *         of row r (of the 32) from column 32 h (of the 64) on
  *   exps  [N][K / 128][rows][4]
  * of hmoe_packed_mxfp4_*_bytes and a sixteenth of that.  D % 128 == 0, F % 128 ==
- * 0, N <= 1024. */
+ * 0, both up to 2^20, N <= 1024. */
 size_t hmoe_packed_mxfp4_gate_up_bytes(int n_experts, int d_model, int d_ff);
 int hmoe_pack_mxfp4_gate_up(const void* w_gate, const void* w_up, int w_dtype, int n_experts,
                             int d_model, int d_ff, uint8_t* packed, uint8_t* exps,
@@ -434,7 +434,8 @@ int64_t hmoe_grouped_mxfp4_form(int64_t rows_cap, int n_experts, int kdim, int n
  * g and u the float32 sums xs[r]·Wg[e] and xs[r]·Wu[e], h = silu(g) * u in float32
  * and quantised from there (h is rounded once, to its codes).  xs_q [rows_cap, D/2],
  * xs_exp [rows_cap, D/32], h_q [rows_cap, F/2], h_exp [rows_cap, F/32].  Rows past
- * offsets[N] are not written.  D % 128 == 0, F % 128 == 0, N <= 1024. */
+ * offsets[N] are not written.  D % 128 == 0, F % 128 == 0, both up to 2^20, N <= 1024,
+ * rows_cap <= 2^30. */
 int hmoe_grouped_gate_up_mxfp4(const uint8_t* xs_q, const uint8_t* xs_exp, const int32_t* offsets,
                                int n_experts, int64_t rows_cap, int d_model, int d_ff,
                                const uint8_t* w_packed, const uint8_t* w_exp, uint8_t* h_q,

@@ -126,3 +126,18 @@ def test_module_arguments():
     for d, f in ((128, 128), (384, 128), (192, 128), (256, 64)):
         with pytest.raises(ValueError, match="128"):
             MoE(d, f, 4, 2, 1, 0.02, 1.0, "bfloat16", rngs=0, expert_dtype="mxfp4", device="cpu")
+
+
+def test_limits():
+    """Sizes whose rows, tiles or threads would not be counted in 32 bits."""
+    for name, args in PRODUCTS:
+        expect(INVALID, "rows_cap", name, *args(4, (1 << 30) + 1, 256, 128, P))
+        expect(INVALID, "rows_cap", name, *args(1, (1 << 31) - 1, 128, 128, P))
+        expect(UNSUPPORTED, "d_model", name, *args(4, 10, 1 << 21, 128, P))
+        expect(UNSUPPORTED, "d_ff", name, *args(4, 10, 256, 1 << 21, P))
+    for name, args in (("hmoe_pack_mxfp4_gate_up", lambda d, f: (P, P, F32, 1, d, f, P, P, S)),
+                       ("hmoe_pack_mxfp4_down", lambda d, f: (P, F32, 1, f, d, P, P, S))):
+        expect(UNSUPPORTED, "d_model", name, *args(1 << 21, 128))
+        expect(UNSUPPORTED, "d_ff", name, *args(128, 1 << 30))
+    expect(INVALID, "too large", "hmoe_unpack_mxfp4", P, P, 1024, 1 << 19, 128, P, BF16, S)
+    assert _lib.lib().hmoe_grouped_mxfp4_form((1 << 30) + 1, 4, 256, 256, 256) == -1
