@@ -175,7 +175,10 @@ class MoE:
     ``ceil(CF*T*K/N)`` with token-order priority; ``None`` = dropless) and
     ``expert_dtype="mxfp4"`` (the routed experts on 4-bit operands quantised from
     the masters, tokens and ``h`` quantised on the way; bfloat16 compute otherwise.
-    For inference: a call that autograd would record is refused).
+    For inference: a call that autograd would record is refused).  As everywhere
+    in this module, operands are packed on the calling stream by the first call and
+    by the first one after a master changed: other streams wait for that call, and a
+    graph is captured after it and again after a change.
     """
 
     def __init__(self, d_model: int, d_ff: int, n_experts: int, n_active: int,
