@@ -39,6 +39,8 @@ SIGNATURES = {
                            _vp, _vp, _vp, _vp]),
     "hmoe_router_quant_fp8": (_i32, [_vp, _i32, _vp, _i32, _vp, _i64, _i32, _i32, _i32, _i32,
                                      _f32, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "hmoe_router_quant_mxfp4": (_i32, [_vp, _i32, _vp, _i32, _vp, _i64, _i32, _i32, _i32, _i32,
+                                     _f32, _vp, _vp, _vp, _vp, _vp, _vp]),
     "hmoe_router_from_logits": (_i32, [_vp, _vp, _i64, _i32, _i32, _i32, _f32, _vp, _vp, _vp]),
     "hmoe_dispatch_plan": (_i32, [_vp, _i64, _i32, _i32, _i64, _vp, _vp, _vp, _vp, _vp, _vp,
                                   _sz, _vp]),

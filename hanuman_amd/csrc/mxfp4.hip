@@ -7,8 +7,6 @@
 namespace hmoe {
 namespace {
 
-__device__ __forceinline__ uint32_t umax32(uint32_t a, uint32_t b) { return a > b ? a : b; }
-
 // Rows are whole blocks, so a matrix is one run of them.  A lane takes eight
 // values and four neighbours a block.
 template <typename TI>
@@ -20,19 +18,7 @@ __global__ __launch_bounds__(256) void quantize_rows_mxfp4_kernel(const TI* __re
   for (int64_t c = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; c < chunks; c += stride) {
     Chunk8<TI> x;
     x.load_nt(a + c * 8);
-    float v[8];
-    uint32_t amax = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      v[i] = x.get(i);
-      amax = umax32(amax, __float_as_uint(v[i]) & 0x7fffffffu);
-    }
-    // chunks is a multiple of 4: a block's four lanes are here together
-    amax = umax32(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), 1)));
-    amax = umax32(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), 2)));
-    const uint32_t e = mxfp4_exponent(amax);
-    reinterpret_cast<uint32_t*>(q)[c] = mxfp4_codes8(v, mxfp4_inverse(e));
-    if ((c & 3) == 0) exps[c >> 2] = static_cast<uint8_t>(e);
+    quant_chunk_mxfp4(x, c, q, exps);  // (chunks is a multiple of 4: a block's lanes are here together)
   }
 }
 

@@ -57,6 +57,26 @@ __device__ __forceinline__ uint32_t mxfp4_codes8(const float (&v)[8], float inv)
   return inv != 0.0f ? w : 0u;
 }
 
+__device__ __forceinline__ uint32_t umax32(uint32_t a, uint32_t b) { return a > b ? a : b; }
+
+// Eight values of a row (chunk c of it) to a word of codes, and the block's exponent.  Four
+// neighbouring lanes hold a block.
+template <typename Values>
+__device__ __forceinline__ void quant_chunk_mxfp4(const Values& x, int64_t c, uint8_t* q, uint8_t* exps) {
+  float v[8];
+  uint32_t amax = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    v[i] = x.get(i);
+    amax = umax32(amax, __float_as_uint(v[i]) & 0x7fffffffu);
+  }
+  amax = umax32(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), 1)));
+  amax = umax32(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), 2)));
+  const uint32_t e = mxfp4_exponent(amax);
+  reinterpret_cast<uint32_t*>(q)[c] = mxfp4_codes8(v, mxfp4_inverse(e));
+  if ((c & 3) == 0) exps[c >> 2] = static_cast<uint8_t>(e);
+}
+
 // The eight values of a word of codes.
 __device__ __forceinline__ void mxfp4_values8(uint32_t w, float scale, float (&v)[8]) {
   typedef float f32x2_t __attribute__((ext_vector_type(2)));

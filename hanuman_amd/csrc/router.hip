@@ -11,6 +11,7 @@
 
 #include "hmoe_common.h"
 #include "quant_e4m3.h"
+#include "quant_mxfp4.h"
 
 namespace hmoe {
 namespace {
@@ -303,16 +304,30 @@ struct X8<uint16_t> {
     return __uint_as_float((i & 1) ? (u & 0xffff0000u) : (u << 16));
   }
 };
-// Rows n_waves block .. + n_waves of x to e4m3, one per wave.
-template <typename XT>
+// What a router's launch quantises x to beside the routing.
+enum QuantX { kQuantNone, kQuantE4m3, kQuantMxfp4 };
+
+// Rows n_waves block .. + n_waves of x to e4m3 (x_scale: float per row) or MXFP4 (x_scale:
+// an exponent byte per 32 values), one per wave.
+template <int QX, typename XT>
 __device__ __forceinline__ void router_quant_rows(const XT* __restrict__ x, int block, int n_waves,
                                                   int64_t tokens, int d_model,
                                                   uint8_t* __restrict__ x_q,
-                                                  float* __restrict__ x_scale) {
+                                                  void* __restrict__ x_scales) {
   static_assert(sizeof(XT) == 2, "x is quantised from bf16");
   const int64_t r = static_cast<int64_t>(block) * n_waves + (threadIdx.x >> 6);
   if (r >= tokens) return;
   const uint16_t* xr = reinterpret_cast<const uint16_t*>(x) + r * d_model;
+  if constexpr (QX == kQuantMxfp4) {
+    uint8_t* exps = static_cast<uint8_t*>(x_scales) + r * (d_model / kMxBlock);
+    for (int c = threadIdx.x & 63; c < d_model / 8; c += 64) {
+      X8<uint16_t> v;
+      v.load(xr + c * 8);
+      quant_chunk_mxfp4(v, c, x_q + r * (d_model / 2), exps);
+    }
+    return;
+  }
+  float* x_scale = static_cast<float*>(x_scales);
   if (d_model <= 64 * kRowRegs * 8)
     quant_row_e4m3<true>(xr, d_model, x_q + r * d_model, x_scale + r);
   else
@@ -415,24 +430,24 @@ __device__ __forceinline__ double widen_w(uint32_t bits) {
 // 16), more than MT / 2, and router_groups waves for each.  TOK tokens in a
 // chain: 16, or 4 on the 4x4x4 form.
 //
-// QX: the launch also quantises x to e4m3 per token (the rule and code of
-// hmoe_quantize_rows_fp8): workgroups past the first router_blocks take one
+// QX: the launch also quantises x, to e4m3 per token or to MXFP4 (the rules and code of
+// hmoe_quantize_rows_fp8 and hmoe_quantize_rows_mxfp4): workgroups past the first router_blocks take one
 // row of x per wave.  They start once the router's workgroups are placed and
 // run beside them, whose float64 MFMA chains leave the memory system and most
 // of the VALU issue idle.
-template <int MT, int TOK, bool TAIL, typename XT, typename WT, bool QX>
+template <int MT, int TOK, bool TAIL, typename XT, typename WT, int QX>
 __global__ __launch_bounds__(64 * MT * router_groups(MT), MT > 8 || TOK == 16 ? 4 : 2) void router_kernel(
     const XT* __restrict__ x, const WT* __restrict__ w, const float* __restrict__ bias,
     int64_t tokens, int d_model, int n_experts, int top_k, int mode, float rsf,
     float* __restrict__ logits, int32_t* __restrict__ top_idx, float* __restrict__ gates,
-    uint8_t* __restrict__ x_q, float* __restrict__ x_scale, int router_blocks) {
+    uint8_t* __restrict__ x_q, void* __restrict__ x_scale, int router_blocks) {
   static_assert(TOK == 16 || (TOK == 4 && !TAIL), "a chain holds 16 or 4 tokens");
-  static_assert(!QX || sizeof(XT) == 2, "x is quantised from bf16");
+  static_assert(QX == kQuantNone || sizeof(XT) == 2, "x is quantised from bf16");
   const int n_waves = static_cast<int>(blockDim.x) >> 6;
-  if constexpr (QX) {
+  if constexpr (QX != kQuantNone) {
     if (static_cast<int>(blockIdx.x) >= router_blocks) {
-      router_quant_rows(x, static_cast<int>(blockIdx.x) - router_blocks, n_waves, tokens, d_model,
-                        x_q, x_scale);
+      router_quant_rows<QX>(x, static_cast<int>(blockIdx.x) - router_blocks, n_waves, tokens, d_model,
+                            x_q, x_scale);
       return;
     }
   }
@@ -681,16 +696,16 @@ struct alignas(16) RouterStagedLds {
   float w[2][kDc][16 * NT + 8];
 };
 
-template <int NT, bool WV, typename XT, typename WT, bool QX>
+template <int NT, bool WV, typename XT, typename WT, int QX>
 __global__ __launch_bounds__(256) void router_staged_kernel(
     const XT* __restrict__ x, const WT* __restrict__ w, const float* __restrict__ bias,
     int64_t tokens, int d_model, int n_experts, int top_k, int mode, float rsf,
     float* __restrict__ logits, int32_t* __restrict__ top_idx, float* __restrict__ gates,
-    uint8_t* __restrict__ x_q, float* __restrict__ x_scale, int router_blocks) {
-  if constexpr (QX) {
+    uint8_t* __restrict__ x_q, void* __restrict__ x_scale, int router_blocks) {
+  if constexpr (QX != kQuantNone) {
     if (static_cast<int>(blockIdx.x) >= router_blocks) {
-      router_quant_rows(x, static_cast<int>(blockIdx.x) - router_blocks, 4, tokens, d_model, x_q,
-                        x_scale);
+      router_quant_rows<QX>(x, static_cast<int>(blockIdx.x) - router_blocks, 4, tokens, d_model, x_q,
+                            x_scale);
       return;
     }
   }
@@ -953,10 +968,11 @@ int stream_cus(hipStream_t s) {
   return cus > 0 ? cus : 0;
 }
 
-// Optional e4m3 quantisation of x in the router's launch (router_kernel QX).
+// Optional quantisation of x in the router's launch (router_kernel QX).
 struct XQuant {
+  QuantX to = kQuantNone;
   uint8_t* q = nullptr;
-  float* scale = nullptr;
+  void* scale = nullptr;
 };
 
 template <int MT, int TOK, bool TAIL, typename XT, typename WT>
@@ -965,20 +981,19 @@ void launch_router_tok(const void* x, const void* w, const float* bias, int64_t 
                        int32_t* top_idx, float* gates, hipStream_t stream, XQuant xq) {
   const int waves = (n_experts + 15) / 16 * router_groups(MT);
   const int rblocks = static_cast<int>(ceil_div(tokens, TOK * router_groups(MT)));
+  const auto launch = [&](auto QX) {
+    constexpr int qx = decltype(QX)::value;
+    const int64_t qblocks = qx != kQuantNone ? ceil_div(tokens, waves) : 0;
+    hipLaunchKernelGGL((router_kernel<MT, TOK, TAIL, XT, WT, qx>),
+                       dim3(static_cast<unsigned>(rblocks + qblocks)), dim3(64 * waves), 0, stream,
+                       static_cast<const XT*>(x), static_cast<const WT*>(w), bias, tokens, d_model,
+                       n_experts, top_k, mode, rsf, logits, top_idx, gates, xq.q, xq.scale, rblocks);
+  };
   if constexpr (sizeof(XT) == 2) {
-    if (xq.q != nullptr) {
-      hipLaunchKernelGGL((router_kernel<MT, TOK, TAIL, XT, WT, true>),
-                         dim3(static_cast<unsigned>(rblocks + ceil_div(tokens, waves))),
-                         dim3(64 * waves), 0, stream, static_cast<const XT*>(x),
-                         static_cast<const WT*>(w), bias, tokens, d_model, n_experts, top_k, mode,
-                         rsf, logits, top_idx, gates, xq.q, xq.scale, rblocks);
-      return;
-    }
+    if (xq.to == kQuantE4m3) return launch(IntC<kQuantE4m3>());
+    if (xq.to == kQuantMxfp4) return launch(IntC<kQuantMxfp4>());
   }
-  hipLaunchKernelGGL((router_kernel<MT, TOK, TAIL, XT, WT, false>), dim3(static_cast<unsigned>(rblocks)),
-                     dim3(64 * waves), 0, stream, static_cast<const XT*>(x),
-                     static_cast<const WT*>(w), bias, tokens, d_model, n_experts, top_k, mode, rsf,
-                     logits, top_idx, gates, nullptr, nullptr, rblocks);
+  launch(IntC<kQuantNone>());
 }
 
 template <int NT, bool WV, typename XT, typename WT>
@@ -987,20 +1002,19 @@ void launch_router_staged(const void* x, const void* w, const float* bias, int64
                           float* logits, int32_t* top_idx, float* gates, hipStream_t stream,
                           XQuant xq) {
   const int rblocks = static_cast<int>(ceil_div(tokens, RouterStagedLds<NT, WV>::kTB));
+  const auto launch = [&](auto QX) {
+    constexpr int qx = decltype(QX)::value;
+    const int64_t qblocks = qx != kQuantNone ? ceil_div(tokens, 4) : 0;
+    hipLaunchKernelGGL((router_staged_kernel<NT, WV, XT, WT, qx>),
+                       dim3(static_cast<unsigned>(rblocks + qblocks)), dim3(256), 0, stream,
+                       static_cast<const XT*>(x), static_cast<const WT*>(w), bias, tokens, d_model,
+                       n_experts, top_k, mode, rsf, logits, top_idx, gates, xq.q, xq.scale, rblocks);
+  };
   if constexpr (sizeof(XT) == 2) {
-    if (xq.q != nullptr) {
-      hipLaunchKernelGGL((router_staged_kernel<NT, WV, XT, WT, true>),
-                         dim3(static_cast<unsigned>(rblocks + ceil_div(tokens, 4))), dim3(256), 0,
-                         stream, static_cast<const XT*>(x), static_cast<const WT*>(w), bias, tokens,
-                         d_model, n_experts, top_k, mode, rsf, logits, top_idx, gates, xq.q,
-                         xq.scale, rblocks);
-      return;
-    }
+    if (xq.to == kQuantE4m3) return launch(IntC<kQuantE4m3>());
+    if (xq.to == kQuantMxfp4) return launch(IntC<kQuantMxfp4>());
   }
-  hipLaunchKernelGGL((router_staged_kernel<NT, WV, XT, WT, false>), dim3(static_cast<unsigned>(rblocks)),
-                     dim3(256), 0, stream, static_cast<const XT*>(x), static_cast<const WT*>(w),
-                     bias, tokens, d_model, n_experts, top_k, mode, rsf, logits, top_idx, gates,
-                     nullptr, nullptr, rblocks);
+  launch(IntC<kQuantNone>());
 }
 
 // Chains of 4 tokens while they leave at most 1.5 waves per SIMD: they are
@@ -1043,8 +1057,7 @@ void launch_router(const void* x, const void* w, const float* bias, int64_t toke
 template <int MT>
 void dispatch_router(int x_dtype, int w_dtype, const void* x, const void* w, const float* bias,
                      int64_t tokens, int d_model, int n_experts, int top_k, int mode, float rsf,
-                     float* logits, int32_t* top_idx, float* gates, hipStream_t s,
-                     XQuant xq = XQuant()) {
+                     float* logits, int32_t* top_idx, float* gates, hipStream_t s, XQuant xq) {
   if (x_dtype == HMOE_BF16 && w_dtype == HMOE_F32)
     launch_router<MT, uint16_t, float>(x, w, bias, tokens, d_model, n_experts, top_k, mode, rsf, logits, top_idx, gates, s, xq);
   else if (x_dtype == HMOE_F32 && w_dtype == HMOE_F32)
@@ -1053,6 +1066,20 @@ void dispatch_router(int x_dtype, int w_dtype, const void* x, const void* w, con
     launch_router<MT, uint16_t, uint16_t>(x, w, bias, tokens, d_model, n_experts, top_k, mode, rsf, logits, top_idx, gates, s, xq);
   else
     launch_router<MT, float, uint16_t>(x, w, bias, tokens, d_model, n_experts, top_k, mode, rsf, logits, top_idx, gates, s, xq);
+}
+
+void route_by_experts(int x_dtype, int w_dtype, const void* x, const void* w, const float* bias,
+                      int64_t tokens, int d_model, int n_experts, int top_k, int mode, float rsf,
+                      float* logits, int32_t* top_idx, float* gates, hipStream_t s, XQuant xq) {
+  const auto run = [&](auto MT) {
+    dispatch_router<decltype(MT)::value>(x_dtype, w_dtype, x, w, bias, tokens, d_model, n_experts, top_k, mode,
+                                         rsf, logits, top_idx, gates, s, xq);
+  };
+  if (n_experts <= 16) run(IntC<1>());
+  else if (n_experts <= 32) run(IntC<2>());
+  else if (n_experts <= 64) run(IntC<4>());
+  else if (n_experts <= 128) run(IntC<8>());
+  else run(IntC<16>());
 }
 
 int validate_routing(int64_t tokens, int n_experts, int top_k, int mode) {
@@ -1084,16 +1111,8 @@ extern "C" int hmoe_router(const void* x, int x_dtype, const void* router_w, int
   HMOE_REQUIRE(x && router_w && logits && top_idx && gates, "router: null pointer argument");
   hipStream_t s = static_cast<hipStream_t>(stream);
   const float rsf = routed_scaling_factor;
-  if (n_experts <= 16)
-    dispatch_router<1>(x_dtype, w_dtype, x, router_w, bias, tokens, d_model, n_experts, top_k, mode, rsf, logits, top_idx, gates, s);
-  else if (n_experts <= 32)
-    dispatch_router<2>(x_dtype, w_dtype, x, router_w, bias, tokens, d_model, n_experts, top_k, mode, rsf, logits, top_idx, gates, s);
-  else if (n_experts <= 64)
-    dispatch_router<4>(x_dtype, w_dtype, x, router_w, bias, tokens, d_model, n_experts, top_k, mode, rsf, logits, top_idx, gates, s);
-  else if (n_experts <= 128)
-    dispatch_router<8>(x_dtype, w_dtype, x, router_w, bias, tokens, d_model, n_experts, top_k, mode, rsf, logits, top_idx, gates, s);
-  else
-    dispatch_router<16>(x_dtype, w_dtype, x, router_w, bias, tokens, d_model, n_experts, top_k, mode, rsf, logits, top_idx, gates, s);
+  route_by_experts(x_dtype, w_dtype, x, router_w, bias, tokens, d_model, n_experts, top_k, mode, rsf, logits,
+                   top_idx, gates, s, XQuant());
   return check_launch("hmoe_router");
 }
 
@@ -1114,20 +1133,34 @@ extern "C" int hmoe_router_quant_fp8(const void* x, int x_dtype, const void* rou
                "router_quant_fp8: null pointer argument");
   hipStream_t s = static_cast<hipStream_t>(stream);
   const float rsf = routed_scaling_factor;
-  XQuant xq;
-  xq.q = x_q;
-  xq.scale = x_scale;
-  if (n_experts <= 16)
-    dispatch_router<1>(x_dtype, w_dtype, x, router_w, bias, tokens, d_model, n_experts, top_k, mode, rsf, logits, top_idx, gates, s, xq);
-  else if (n_experts <= 32)
-    dispatch_router<2>(x_dtype, w_dtype, x, router_w, bias, tokens, d_model, n_experts, top_k, mode, rsf, logits, top_idx, gates, s, xq);
-  else if (n_experts <= 64)
-    dispatch_router<4>(x_dtype, w_dtype, x, router_w, bias, tokens, d_model, n_experts, top_k, mode, rsf, logits, top_idx, gates, s, xq);
-  else if (n_experts <= 128)
-    dispatch_router<8>(x_dtype, w_dtype, x, router_w, bias, tokens, d_model, n_experts, top_k, mode, rsf, logits, top_idx, gates, s, xq);
-  else
-    dispatch_router<16>(x_dtype, w_dtype, x, router_w, bias, tokens, d_model, n_experts, top_k, mode, rsf, logits, top_idx, gates, s, xq);
+  const XQuant xq{kQuantE4m3, x_q, x_scale};
+  route_by_experts(x_dtype, w_dtype, x, router_w, bias, tokens, d_model, n_experts, top_k, mode, rsf, logits,
+                   top_idx, gates, s, xq);
   return check_launch("hmoe_router_quant_fp8");
+}
+
+extern "C" int hmoe_router_quant_mxfp4(const void* x, int x_dtype, const void* router_w, int w_dtype,
+                                       const float* bias, int64_t tokens, int d_model, int n_experts,
+                                       int top_k, int mode, float routed_scaling_factor,
+                                       float* logits, int32_t* top_idx, float* gates, uint8_t* x_q,
+                                       uint8_t* x_exp, hmoe_stream_t stream) {
+  using namespace hmoe;
+  if (int rc = validate_routing(tokens, n_experts, top_k, mode)) return rc;
+  HMOE_REQUIRE_CODE(d_model >= kMxBlock && d_model % kMxBlock == 0, HMOE_ERR_UNSUPPORTED,
+                    "router_quant_mxfp4: d_model must be a multiple of 32 (got %d)", d_model);
+  HMOE_REQUIRE(x_dtype == HMOE_BF16, "router_quant_mxfp4: x dtype must be BF16");
+  HMOE_REQUIRE(w_dtype == HMOE_F32 || w_dtype == HMOE_BF16,
+               "router_quant_mxfp4: weight dtype must be F32 or BF16");
+  if (tokens == 0) return HMOE_OK;
+  HMOE_REQUIRE(x && router_w && logits && top_idx && gates && x_q && x_exp,
+               "router_quant_mxfp4: null pointer argument");
+  HMOE_REQUIRE_ALIGNED("router_quant_mxfp4", 16, x, x_q);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const float rsf = routed_scaling_factor;
+  const XQuant xq{kQuantMxfp4, x_q, x_exp};
+  route_by_experts(x_dtype, w_dtype, x, router_w, bias, tokens, d_model, n_experts, top_k, mode, rsf, logits,
+                   top_idx, gates, s, xq);
+  return check_launch("hmoe_router_quant_mxfp4");
 }
 
 extern "C" int hmoe_router_from_logits(const float* logits, const float* bias, int64_t tokens,

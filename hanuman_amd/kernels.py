@@ -58,13 +58,8 @@ def rows_cap(tokens: int, top_k: int, n_experts: int, cap: int) -> int:
 
 # ---------------------------------------------------------------- router --
 
-def router(x: torch.Tensor, router_w: torch.Tensor, bias: torch.Tensor | None, top_k: int,
-           mode: int = _lib.ROUTE_SIGMOID_BIAS, routed_scaling_factor: float = 1.0):
-    """Router logits, top-k indices and gates (``moe.py:175-192``).
-
-    ``x [T,D]``, ``router_w [D,N]``, ``bias [N]`` float32 or None.
-    Returns (logits f32 [T,N], top_idx i32 [T,K], gates f32 [T,K]).
-    """
+def _router_operands(x, router_w, bias, top_k: int):
+    """The sizes ``T, D, N`` and the empty outputs of a router call, its tensors checked."""
     _check(x, "x", 2)
     _check(router_w, "router_w", 2)
     T, D = x.shape
@@ -79,6 +74,17 @@ def router(x: torch.Tensor, router_w: torch.Tensor, bias: torch.Tensor | None, t
     logits = torch.empty((T, N), dtype=torch.float32, device=dev)
     top_idx = torch.empty((T, top_k), dtype=torch.int32, device=dev)
     gates = torch.empty((T, top_k), dtype=torch.float32, device=dev)
+    return T, D, N, logits, top_idx, gates
+
+
+def router(x: torch.Tensor, router_w: torch.Tensor, bias: torch.Tensor | None, top_k: int,
+           mode: int = _lib.ROUTE_SIGMOID_BIAS, routed_scaling_factor: float = 1.0):
+    """Router logits, top-k indices and gates (``moe.py:175-192``).
+
+    ``x [T,D]``, ``router_w [D,N]``, ``bias [N]`` float32 or None.
+    Returns (logits f32 [T,N], top_idx i32 [T,K], gates f32 [T,K]).
+    """
+    T, D, N, logits, top_idx, gates = _router_operands(x, router_w, bias, top_k)
     call("hmoe_router", _ptr(x), _dtype_code(x), _ptr(router_w), _dtype_code(router_w),
          _ptr(bias), T, D, N, top_k, mode, float(routed_scaling_factor), _ptr(logits),
          _ptr(top_idx), _ptr(gates), _stream())
@@ -94,27 +100,36 @@ def router_quant_fp8(x: torch.Tensor, router_w: torch.Tensor, bias: torch.Tensor
     (logits, top_idx, gates, x_q uint8 [T,D], x_scale f32 [T]), bit-identical
     to the two calls."""
     _check(x, "x", 2)
-    _check(router_w, "router_w", 2)
     if x.dtype != torch.bfloat16:
         raise TypeError("router_quant_fp8 takes bf16 tokens")
-    T, D = x.shape
-    if router_w.shape[0] != D:
-        raise ValueError(f"router_w has {router_w.shape[0]} rows, x has d_model {D}")
-    N = router_w.shape[1]
-    if bias is not None:
-        _check(bias, "bias", 1)
-        if bias.dtype != torch.float32 or bias.shape[0] != N:
-            raise ValueError("bias must be float32 [n_experts]")
+    T, D, N, logits, top_idx, gates = _router_operands(x, router_w, bias, top_k)
     dev = x.device
-    logits = torch.empty((T, N), dtype=torch.float32, device=dev)
-    top_idx = torch.empty((T, top_k), dtype=torch.int32, device=dev)
-    gates = torch.empty((T, top_k), dtype=torch.float32, device=dev)
     x_q = torch.empty((T, D), dtype=torch.uint8, device=dev)
     x_s = torch.empty(T, dtype=torch.float32, device=dev)
     call("hmoe_router_quant_fp8", _ptr(x), _dtype_code(x), _ptr(router_w), _dtype_code(router_w),
          _ptr(bias), T, D, N, top_k, mode, float(routed_scaling_factor), _ptr(logits),
          _ptr(top_idx), _ptr(gates), _ptr(x_q), _ptr(x_s), _stream())
     return logits, top_idx, gates, x_q, x_s
+
+
+def router_quant_mxfp4(x: torch.Tensor, router_w: torch.Tensor, bias: torch.Tensor | None,
+                       top_k: int, mode: int = _lib.ROUTE_SIGMOID_BIAS,
+                       routed_scaling_factor: float = 1.0):
+    """:func:`router` and :func:`quantize_rows_mxfp4` of ``x`` (bf16 ``[T,D]``) in one
+    launch, as :func:`router_quant_fp8`.  Returns (logits, top_idx, gates, x_q uint8
+    [T,D/2], x_exp uint8 [T,D/32]), bit-identical to the two calls."""
+    dev = _current_device("router_quant_mxfp4", x, 2)
+    if x.dtype != torch.bfloat16:
+        raise TypeError("router_quant_mxfp4 takes bf16 tokens")
+    T, D, N, logits, top_idx, gates = _router_operands(x, router_w, bias, top_k)
+    for t in (router_w,) if bias is None else (router_w, bias):
+        _same_device("router_quant_mxfp4", t, dev)
+    x_q = torch.empty((T, D // 2), dtype=torch.uint8, device=dev)
+    x_e = x_q.new_empty((T, D // 32))
+    call("hmoe_router_quant_mxfp4", _ptr(x), _dtype_code(x), _ptr(router_w), _dtype_code(router_w),
+         _ptr(bias), T, D, N, top_k, mode, float(routed_scaling_factor), _ptr(logits),
+         _ptr(top_idx), _ptr(gates), _ptr(x_q), _ptr(x_e), _stream())
+    return logits, top_idx, gates, x_q, x_e
 
 
 def router_from_logits(logits: torch.Tensor, bias: torch.Tensor | None, top_k: int,

@@ -104,15 +104,20 @@ class DeviceLayer:
         return K.router(self.x, self.router_w, None, wl.top_k, self.mode)
 
     def route_quant(self):
-        """The router and, for fp8 experts gathering from per-token codes, x's
-        e4m3 quantisation in the same launch (``hmoe_router_quant_fp8``: the
-        quantisation runs beside the router's float64 MFMA chains).  Returns
-        (logits, top_idx, gates, (x_q, x_scale) or None)."""
+        """The router and, for fp8 experts gathering from per-token codes and for
+        mxfp4 experts on bf16 tokens, x's quantisation in the same launch
+        (``hmoe_router_quant_fp8``, ``hmoe_router_quant_mxfp4``: it runs beside the
+        router's float64 MFMA chains).  Returns (logits, top_idx, gates, (x_q,
+        x_scale) or None)."""
         wl = self.wl
         if self.fp8_gather and self.logits_in is None:
             logits, top_idx, gates, x_q, x_s = K.router_quant_fp8(self.x, self.router_w, None,
                                                                    wl.top_k, self.mode)
             return logits, top_idx, gates, (x_q, x_s)
+        if self.mxfp4 and wl.expert == "swiglu" and self.x.dtype == torch.bfloat16 and self.logits_in is None:
+            logits, top_idx, gates, x_q, x_e = K.router_quant_mxfp4(self.x, self.router_w, None,
+                                                                     wl.top_k, self.mode)
+            return logits, top_idx, gates, (x_q, x_e)
         return (*self.route(), None)
 
     def experts_fp8(self, plan, xq=None):
@@ -134,10 +139,11 @@ class DeviceLayer:
         ys = K.grouped_down_fp8_mx(h_q, h_e, plan.offsets, self.w_down, self.w_down_scale)
         return xs_q, xs_s, h_q, h_e, ys
 
-    def experts_mxfp4(self, plan):
+    def experts_mxfp4(self, plan, xq=None):
         """MXFP4 tokens and expert GEMMs: (x_q, x_exp, h_q, h_exp, ys), codes and biased
-        exponents of the tokens and of h."""
-        x_q, x_e = K.quantize_rows_mxfp4(self.x)
+        exponents of the tokens and of h.  ``xq``: the tokens' when the router's launch
+        made them."""
+        x_q, x_e = xq if xq is not None else K.quantize_rows_mxfp4(self.x)
         h_q, h_e = K.grouped_gate_up_mxfp4_gather(x_q, x_e, plan, self.w_gate_up, self.w_gate_up_exp)
         ys = K.grouped_down_mxfp4(h_q, h_e, plan.offsets, self.w_down, self.w_down_exp)
         return x_q, x_e, h_q, h_e, ys
@@ -153,7 +159,7 @@ class DeviceLayer:
             extra = {"xs_scale": xs_s, "h_q": h_q, "h_exp": h_e,
                      "xs_per_token": self.fp8_gather}
         elif self.mxfp4 and wl.expert == "swiglu":
-            x_q, x_e, h_q, h_e, ys = self.experts_mxfp4(plan)
+            x_q, x_e, h_q, h_e, ys = self.experts_mxfp4(plan, xq)
             xs = None
             extra = {"x_q": x_q, "x_exp": x_e, "h_q": h_q, "h_exp": h_e}
         elif self.f32:

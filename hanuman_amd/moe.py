@@ -423,8 +423,12 @@ class MoE:
         mode = _lib.ROUTE_SIGMOID_BIAS if self.routing == "sigmoid" else _lib.ROUTE_SOFTMAX
         rsf = self.routed_scaling_factor if self.routing == "sigmoid" else 1.0
         bias = self.bias.value if self.routing == "sigmoid" else None
-        logits, top_idx, gates = K.router(x2, self.router.value.float().contiguous(),
-                                          bias, Kk, mode, rsf)
+        router_w = self.router.value.float().contiguous()
+        x_q = None
+        if self.expert_dtype == "mxfp4" and x2.dtype == torch.bfloat16:
+            logits, top_idx, gates, *x_q = K.router_quant_mxfp4(x2, router_w, bias, Kk, mode, rsf)
+        else:
+            logits, top_idx, gates = K.router(x2, router_w, bias, Kk, mode, rsf)
         cap = K.capacity(T, Kk, N, self.capacity_factor)
         plan = K.dispatch_plan(top_idx, N, cap)
         if self.dtype == torch.float32:
@@ -445,8 +449,8 @@ class MoE:
             return out.reshape(B, S, D), losses, counts, saved
         if self.expert_dtype == "mxfp4":
             gate_up, gate_up_exp, down, down_exp = self._packed_mxfp4()
-            h_q, h_exp = K.grouped_gate_up_mxfp4_gather(*K.quantize_rows_mxfp4(x2), plan, gate_up,
-                                                        gate_up_exp)
+            h_q, h_exp = K.grouped_gate_up_mxfp4_gather(*(x_q or K.quantize_rows_mxfp4(x2)), plan,
+                                                        gate_up, gate_up_exp)
             ys = K.grouped_down_mxfp4(h_q, h_exp, plan.offsets, down, down_exp)
             if x2.dtype == torch.float32 and self.n_shared_experts > 0:
                 shared = self._shared_ffn_promoted(x2)

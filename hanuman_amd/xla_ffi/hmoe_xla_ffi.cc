@@ -579,6 +579,41 @@ bool Mxfp4Operand(const Q& q, const E& e) {
 
 }  // namespace
 
+// The router and the quantisation of x in one launch: x [T, D] bf16, router_w [D, N]
+// (f32/bf16), bias [N] f32 -> logits, top_idx, gates as hmoe_router, x_q [T, D / 2], x_exp
+// [T, D / 32] as hmoe_quantize_rows_mxfp4.
+static ffi::Error RouterQuantMxfp4Impl(hipStream_t stream, ffi::Buffer<ffi::BF16> x,
+                                       ffi::AnyBuffer w, ffi::Buffer<ffi::F32> bias, int64_t mode,
+                                       float rsf, ffi::ResultBuffer<ffi::F32> logits,
+                                       ffi::ResultBuffer<ffi::S32> top_idx,
+                                       ffi::ResultBuffer<ffi::F32> gates,
+                                       ffi::ResultBuffer<ffi::U8> x_q,
+                                       ffi::ResultBuffer<ffi::U8> x_exp) {
+  const int wd = DtypeCode(w.element_type());
+  if (wd < 0) return BadDtype("hmoe_router_quant_mxfp4 router_w");
+  if (x.dimensions().size() != 2 || w.dimensions().size() != 2 || Rows(w) != Cols(x) ||
+      !Mxfp4Rows(*x_q, *x_exp, Rows(x), Cols(x)))
+    return BadMxfp4("hmoe_router_quant_mxfp4");
+  return Status(hmoe_router_quant_mxfp4(
+      x.untyped_data(), HMOE_BF16, w.untyped_data(), wd, bias.typed_data(), Rows(x),
+      static_cast<int>(Cols(x)), static_cast<int>(Cols(w)), static_cast<int>(Cols(*top_idx)),
+      static_cast<int>(mode), rsf, logits->typed_data(), top_idx->typed_data(), gates->typed_data(),
+      x_q->typed_data(), x_exp->typed_data(), S(stream)));
+}
+XLA_FFI_DEFINE_HANDLER_SYMBOL(HmoeRouterQuantMxfp4, RouterQuantMxfp4Impl,
+                              ffi::Ffi::Bind()
+                                  .Ctx<ffi::PlatformStream<hipStream_t>>()
+                                  .Arg<ffi::Buffer<ffi::BF16>>()
+                                  .Arg<ffi::AnyBuffer>()
+                                  .Arg<ffi::Buffer<ffi::F32>>()
+                                  .Attr<int64_t>("mode")
+                                  .Attr<float>("routed_scaling_factor")
+                                  .Ret<ffi::Buffer<ffi::F32>>()
+                                  .Ret<ffi::Buffer<ffi::S32>>()
+                                  .Ret<ffi::Buffer<ffi::F32>>()
+                                  .Ret<ffi::Buffer<ffi::U8>>()
+                                  .Ret<ffi::Buffer<ffi::U8>>());
+
 // a [R, C] (f32/bf16) -> q [R, C / 2], exps [R, C / 32].
 static ffi::Error QuantizeRowsMxfp4Impl(hipStream_t stream, ffi::AnyBuffer a, ffi::ResultBuffer<ffi::U8> q,
                                         ffi::ResultBuffer<ffi::U8> exps) {

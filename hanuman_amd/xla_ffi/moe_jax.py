@@ -74,6 +74,7 @@ TARGETS = {
     "hmoe_grouped_gate_up_fp8_qh": "HmoeGroupedGateUpFp8Qh",
     "hmoe_grouped_gate_up_fp8_gather_qh": "HmoeGroupedGateUpFp8GatherQh",
     "hmoe_grouped_down_fp8_mx": "HmoeGroupedDownFp8Mx",
+    "hmoe_router_quant_mxfp4": "HmoeRouterQuantMxfp4",
     "hmoe_quantize_rows_mxfp4": "HmoeQuantizeRowsMxfp4",
     "hmoe_dequantize_rows_mxfp4": "HmoeDequantizeRowsMxfp4",
     "hmoe_pack_mxfp4_gate_up": "HmoePackMxfp4GateUp",

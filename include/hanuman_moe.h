@@ -397,6 +397,14 @@ int hmoe_grouped_wgrad_down_f32(const float* h, const float* d_ys, const int32_t
  * byte's low half), exps [rows, cols / 32] uint8.  cols % 32 == 0. */
 int hmoe_quantize_rows_mxfp4(const void* a, int a_dtype, int64_t rows, int cols, uint8_t* q,
                              uint8_t* exps, hmoe_stream_t stream);
+/* hmoe_router (moe.py:175-192) and hmoe_quantize_rows_mxfp4 of its tokens in one launch, as
+ * hmoe_router_quant_fp8: x [T,D] HMOE_BF16 only, D % 32 == 0, outputs bit-identical to the
+ * two calls.  x_q [T, D/2], x_exp [T, D/32] uint8. */
+int hmoe_router_quant_mxfp4(const void* x, int x_dtype, const void* router_w, int w_dtype,
+                            const float* bias, int64_t tokens, int d_model, int n_experts,
+                            int top_k, int mode, float routed_scaling_factor, float* logits,
+                            int32_t* top_idx, float* gates, uint8_t* x_q, uint8_t* x_exp,
+                            hmoe_stream_t stream);
 /* The values of such rows, out [rows, cols] (F32/BF16; exact in both). */
 int hmoe_dequantize_rows_mxfp4(const uint8_t* q, const uint8_t* exps, int64_t rows, int cols,
                                void* out, int out_dtype, hmoe_stream_t stream);

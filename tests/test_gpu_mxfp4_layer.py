@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import mxfp4_reference as R
-from hanuman_amd import MoE, kernels as K, workloads as W
+from hanuman_amd import MoE, _lib, kernels as K, workloads as W
 from hanuman_amd.layer import DeviceLayer
 
 pytestmark = pytest.mark.gpu
@@ -141,3 +141,26 @@ def test_layer_captured(gpu):
         torch.cuda.synchronize()
         for k in got:
             assert torch.equal(got[k], want[k]), k
+
+
+@pytest.mark.parametrize("T,D,N", [(1, 32, 8), (5, 96, 4), (37, 256, 16), (300, 4128, 32), (1000, 2048, 64),
+                                   (6145, 1056, 16), (6151, 160, 12), (1537, 288, 64), (700, 64, 256),
+                                   (4100, 64, 30)])
+@pytest.mark.parametrize("wd", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_router_with_quantisation(gpu, T, D, N, wd):
+    """The one launch gives the bits of the router and of the quantisation; rows of a wide
+    range and one of zeros."""
+    print(f"router quant T{T} D{D} N{N}", flush=True)
+    g = torch.Generator(device="cpu").manual_seed(T + D)
+    x = torch.randn(T, D, generator=g) * torch.exp(torch.rand(T, 1, generator=g) * 18 - 12)
+    x[T // 3] = 0
+    x = x.bfloat16().to(gpu)
+    w = torch.randn(D, N, generator=g).mul(0.1).to(gpu, wd)
+    bias = torch.randn(N, generator=g).mul(0.05).to(gpu)
+    got = K.router_quant_mxfp4(x, w, bias, 3, _lib.ROUTE_SIGMOID_BIAS, 2.5)
+    ref = (*K.router(x, w, bias, 3, _lib.ROUTE_SIGMOID_BIAS, 2.5), *K.quantize_rows_mxfp4(x))
+    torch.cuda.synchronize()
+    for i, (a, b) in enumerate(zip(got, ref)):
+        assert a.dtype == b.dtype and torch.equal(a, b), i
+    want_q, want_e = R.quantise(x.float().cpu().numpy())
+    assert np.array_equal(got[3].cpu().numpy(), want_q) and np.array_equal(got[4].cpu().numpy(), want_e)

@@ -141,3 +141,24 @@ def test_limits():
         expect(UNSUPPORTED, "d_ff", name, *args(128, 1 << 30))
     expect(INVALID, "too large", "hmoe_unpack_mxfp4", P, P, 1024, 1 << 19, 128, P, BF16, S)
     assert _lib.lib().hmoe_grouped_mxfp4_form((1 << 30) + 1, 4, 256, 256, 256) == -1
+
+
+def test_router_quant():
+    name = "hmoe_router_quant_mxfp4"
+
+    def args(p=P, xt=BF16, wt=F32, t=8, d=64, n=8, k=2, mode=_lib.ROUTE_SOFTMAX):
+        return p, xt, p, wt, None, t, d, n, k, mode, 1.0, p, p, p, p, p, S
+    expect(UNSUPPORTED, "d_model", name, *args(d=40))
+    expect(UNSUPPORTED, "d_model", name, *args(d=0))
+    expect(INVALID, "dtype", name, *args(xt=F32))
+    expect(INVALID, "dtype", name, *args(wt=E4M3))
+    expect(INVALID, "n_experts", name, *args(n=257))
+    expect(INVALID, "top_k", name, *args(k=9))
+    expect(INVALID, "mode", name, *args(mode=7))
+    expect(INVALID, "tokens", name, *args(t=-1))
+    expect(INVALID, "null", name, *args(p=None))
+    expect(INVALID, "aligned", name, *args(p=ODD))
+    expect(OK, None, name, *args(p=None, t=0))
+    x = torch.zeros((8, 64), dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="GPU"):
+        K.router_quant_mxfp4(x, torch.zeros((64, 8)), None, 2)
