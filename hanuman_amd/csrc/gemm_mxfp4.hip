@@ -112,13 +112,12 @@ __device__ __forceinline__ uint32_t quantise_h(const f32x16& g, const f32x16& u,
   // lanes L and L + 32 hold the row's other values
   const auto sw = __builtin_amdgcn_permlane32_swap(amax, amax, false, false);
   const uint32_t e = mxfp4_exponent(sw[0] > sw[1] ? sw[0] : sw[1]);
-  const float inv = mxfp4_inverse(e);
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     float v[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] = h[8 * j + k];
-    w[j] = mxfp4_codes8(v, inv);
+    w[j] = mxfp4_codes8(v, e);
   }
   return e;
 }
@@ -137,25 +136,6 @@ __device__ __forceinline__ void store_h_block(const f32x16& g, const f32x16& u, 
   __builtin_amdgcn_raw_buffer_store_b64(join_codes(t[0], t[1]), q_out, (row * d_ff + hcol) / 2 + 8 * half, 0, 0);
   if (half == 0)
     __builtin_amdgcn_raw_buffer_store_b8(static_cast<uint8_t>(e), e_out, row * (d_ff / 32) + hcol / 32, 0, 0);
-}
-
-// Two blocks side by side: lanes 0..31 store the first's 16 bytes of their row and both
-// exponents, lanes 32..63 the second's.
-__device__ __forceinline__ void store_h_blocks(const f32x16 (&acc)[4], __amdgpu_buffer_rsrc_t q_out,
-                                               __amdgpu_buffer_rsrc_t e_out, int row, int hcol, int d_ff,
-                                               int half) {
-  uint32_t w0[2], w1[2];
-  const uint32_t e0 = quantise_h(acc[0], acc[1], w0);
-  const uint32_t e1 = quantise_h(acc[2], acc[3], w1);
-  // (lanes 0..31 give their halves of block 1 for the others' of block 0)
-  const auto a = __builtin_amdgcn_permlane32_swap(w0[0], w1[0], false, false);
-  const auto b = __builtin_amdgcn_permlane32_swap(w0[1], w1[1], false, false);
-  const u32x2_t lo = join_codes(a[0], a[1]), hi = join_codes(b[0], b[1]);
-  const u32x4 codes = {lo[0], lo[1], hi[0], hi[1]};
-  __builtin_amdgcn_raw_buffer_store_b128(codes, q_out, (row * d_ff + hcol) / 2 + 16 * half, 0, 0);
-  if (half == 0)
-    __builtin_amdgcn_raw_buffer_store_b16(static_cast<uint16_t>(e0 | (e1 << 8)), e_out,
-                                          row * (d_ff / 32) + hcol / 32, 0, 0);
 }
 
 // 32 bf16 columns of a row: lanes L and L + 32 trade groups, after which lane L < 32
@@ -325,58 +305,60 @@ __global__ __launch_bounds__(256) void grouped_mxfp4_rows(
 }
 
 // ---- tiles for experts with many rows ------------------------------------------
-// Two workgroups of four waves share a CU, each looping over BM x 256 tiles: while one
-// is in its epilogue (the SwiGLU's exponentials and reciprocals alone take a quarter of
-// the products' time), switches tiles or waits at its barrier, the other's products run.
-// A K step is 128 values = 64 bytes of every row; the operands go from global memory
-// into a ring of three LDS stages (buffer_load ... lds), two steps ahead and on into
-// the next tile, one barrier a step.  A's part of a stage has 64-byte rows whose 16-byte
-// chunk c sits at c ^ swz64(r), so that 16 lanes of a fragment read cover all banks;
-// B's is the operand's own blocks of 1 KB, read lane by lane, and its exponents are a
-// run of 1 KB, put down in the order in which a lane reads four words.  A's exponents, 16 bytes of every row, come for up to four steps at once
-// into one of two regions (three with 64 rows, where a tile may be a single step).  The
-// last column tile may be 128 columns wide: the waves of the other half load and compute
-// the first half's again and store nothing.
+// Workgroups of four waves, two (BM 128) or three (BM 64) a CU, each looping over BM x 256
+// tiles: while one is in its epilogue (the SwiGLU's exponentials and reciprocals alone take
+// a quarter of the products' time), switches tiles or waits at its barrier, the others'
+// products run.  A wave has all of the tile's rows and 64 of its columns, so B's fragments
+// are read by one wave only and go from memory straight into registers, 1 KB an
+// instruction, each loaded for the next step as soon as its products are issued.  A goes
+// through LDS (buffer_load ... lds), two stages of 256 values = 128 bytes of every row, the
+// next stage's loads issued behind the one barrier of a step: whole lines (64-byte pieces
+// of rows come at 31 bytes a cycle and CU, 128-byte ones at 55), and 16-byte chunk c of row
+// r sits at c ^ swz128(r), so that 16 lanes of a fragment read cover all banks.  A's
+// exponents, 16 bytes of every row, come for two steps at once into one of two regions.
+// Where K is an odd multiple of 128 the last step is half a one.  The last column tile may
+// be 128 columns wide: waves 2 and 3 then load and compute the others' again and store
+// nothing.
 //
-// What bounds the large products is power: with these operands the matrix cores alone,
-// fed from registers, run at 1.65 GHz and 6.5 PFLOP/s.  Gate/up of 131072 rows, D 2048, F
-// 1024 (1.1 TFLOP) takes 333 us, 300 of them in the loop at 1.6 to 1.8 GHz, 1580 cycles for
-// two workgroups' steps (1024 of MFMA).  One workgroup of eight waves on 256 x 256 tiles (a
-// third less from L2) took 336 us at 1.8 GHz and 1750 cycles, four waves of 128 x 128
-// (a third less from LDS too) 400 us, the 16 x 16 x 128 MFMA 1900 cycles at 1.95 GHz, all
-// about 300 us in the loop.
+// Gate/up of 131072 rows, D 2048, F 1024 (1.1 TFLOP) takes 300 us, down 170 us.  What bounds
+// them is power: with these operands the matrix cores alone, fed from registers, run at
+// 1.65 GHz and 6.5 PFLOP/s (170 us), and with operands of zeros the same launches take 222
+// and 126 us.  With B through LDS too (2 x 2 waves, steps of 128 values, three stages) it
+// was 326 and 187 us, 265 and 148 with zeros: an LDS that moved as much as it can while the
+// products last, and half lines of A.  One workgroup of eight waves on 128 x 512 takes 301
+// and 176 us, row-tile groups of 4 and 16 and a raised wave priority around the products
+// the same as this, A's loads spread over the step 305 and 174.
 constexpr int kTileThreads = 256;
-constexpr int kStages = 3;
 constexpr int kNumXcd = 8;
 constexpr int kTileN = 256;
 constexpr int kTileGroup = 8;
 
-template <int BM>
+template <int BM, bool GATE_UP>
 struct TileCfg {
-  static constexpr int kA = BM * 64, kB = kTileN * 64, kExB = kTileN * 4;
-  static constexpr int kStage = kA + kB + kExB;
-  static constexpr int kExA = BM * 16;
-  static constexpr int kRegions = BM == 64 ? 3 : 2;
-  static constexpr int kLds = kStages * kStage + kRegions * kExA;
-  static constexpr int kNA = BM / 64, kNB = kTileN / 64;  // DMA instructions a wave and step
-  static constexpr int kFR = BM / 64;                      // row fragments a wave
-  static_assert(2 * kLds <= 160 * 1024, "two workgroups a CU");
+  static constexpr int kA = BM * 128, kExA = BM * 16;  // a stage, a region of exponents
+  static constexpr int kLds = 2 * (kA + kExA) + (GATE_UP ? 0 : 4 * 4096);  // (ys: 4 KB a wave)
+  static constexpr int kFR = BM / 32;             // row fragments; DMA instructions a wave and step
+  static constexpr int kPerCu = BM == 64 ? 3 : 2;
+  static_assert(kPerCu * kLds <= 160 * 1024, "workgroups a CU");
 };
 
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
 
-__device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, uint8_t* dst, uint32_t voff, int soff) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr_t)dst, 16, voff, soff, 0, 0);
-}
-__device__ __forceinline__ void dma4(__amdgpu_buffer_rsrc_t r, uint8_t* dst, uint32_t voff, int soff) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr_t)dst, 4, voff, soff, 0, 0);
+__device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, uint8_t* dst, uint32_t voff) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr_t)dst, 16, voff, 0, 0, 0);
 }
 
 // A use that later code is not moved before.  (A function of its own, like dma16:
 // where the operand's type depends on a template the host pass drops the kernel.)
 __device__ __forceinline__ void use_here(const f32x16& v) { asm volatile("" ::"v"(v)); }
 
-__device__ __forceinline__ int swz64(int r) { return (r >> 2) & 3; }
+__device__ __forceinline__ int swz128(int r) { return (r >> 1) & 7; }
+
+// Memory accesses are not moved past it by the compiler.
+__device__ __forceinline__ void fence() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
 
 // s_waitcnt vmcnt(N) lgkmcnt(0)
 template <int N>
@@ -453,18 +435,14 @@ struct TileCursor {
   }
 };
 
-// Steps of the group that starts with `left` steps to go: four, but no group of one
-// after another (the steps in the ring then span two groups at most).
-__device__ __forceinline__ int group_steps(int left) { return left == 5 ? 3 : left < 4 ? left : 4; }
-
 template <int BM, bool GATE_UP, bool GATHER>
-__global__ __launch_bounds__(kTileThreads, 2) void grouped_mxfp4_tiles(
+__global__ __launch_bounds__(kTileThreads, BM == 64 ? 3 : 2) void grouped_mxfp4_tiles(
     const uint8_t* __restrict__ A, const uint8_t* __restrict__ a_exp, const uint8_t* __restrict__ B,
     const uint8_t* __restrict__ b_exp, const int32_t* __restrict__ offsets, int n_experts, int kdim, int ncols,
     uint8_t* __restrict__ C, uint8_t* __restrict__ c_exp, const int32_t* __restrict__ gather_src, int gather_k,
     int gather_rows) {
-  typedef TileCfg<BM> Cfg;
-  constexpr int kNA = Cfg::kNA, kNB = Cfg::kNB, kFR = Cfg::kFR;
+  typedef TileCfg<BM, GATE_UP> Cfg;
+  constexpr int kFR = Cfg::kFR;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -479,191 +457,202 @@ __global__ __launch_bounds__(kTileThreads, 2) void grouped_mxfp4_tiles(
   const int first = lo + static_cast<int>(blockIdx.x) / kNumXcd;
   if (first >= hi) return;  // uniform per workgroup
   const int ks = kdim / 128;
+  const int nb = (ks + 1) / 2;  // steps of 256 values
   const int row_bytes = kdim / 2, ex_bytes = kdim / 32;
-  const int iters = (hi - first + per_xcd - 1) / per_xcd * ks;
 
   // ---- load side -----------------------------------------------------------------
-  // A: instruction j of wave w fills rows 16 (w kNA + j) + lane / 4, chunk (lane & 3)
-  // ^ swz64(row).  B: blocks of 1 KB, block b = 2 (column / 32) + (64 values of the
-  // step), instruction j of wave w block w kNB + j; its exponents 256 bytes a wave.
-  static_assert(kNB == 4, "two blocks of columns a wave");
+  // A: instruction j of wave w fills rows (BM / 4) w + 8 j + lane / 8, chunk (lane & 7) ^
+  // swz128(row) of the row's 128 bytes.
   TileCursor<BM> ld;
   ld.find(offsets, n_experts, first / n_tiles_n);
-  TileCursor<BM> cur = ld;
-  const int a_row = 16 * wave * kNA + (lane >> 2);
-  const int a_byte = ((lane & 3) ^ ((lane >> 4) & 3)) * 16;
+  TileCursor<BM> cur = ld, nx = ld;
+  const int a_row = (BM / 4) * wave + (lane >> 3);
   __amdgpu_buffer_rsrc_t a_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(A), 0,
                                                                     GATHER ? gather_rows * row_bytes : 0, kBufferWord3);
   __amdgpu_buffer_rsrc_t ae_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(a_exp), 0,
                                                                      GATHER ? gather_rows * ex_bytes : 0, kBufferWord3);
   __amdgpu_buffer_rsrc_t b_rsrc = a_rsrc, be_rsrc = a_rsrc;
-  uint32_t a_voff[kNA], ae_voff = 0;
+  uint32_t a_voff[kFR], ae_voff = 0;
   const int b_col = (kdim / 64) * 1024;  // bytes of 32 columns
-  // (words of a half's columns c, c + 32, c + 64, c + 96 together, as a lane reads them)
-  const int ex_word = (wave & 1) * 64 + lane;
-  const uint32_t be_voff = static_cast<uint32_t>(((ex_word & 3) * 32 + (ex_word >> 2)) * 4);
-  int b_wave = 0, be_wave = 0;       // where this wave's part of B's tile begins
-  const bool ex_a = wave < BM / 64;  // the waves that bring A's exponents
-  int ld_kb = 0, ld_left = 0, ld_g = 0, ld_t = first, ld_region = Cfg::kRegions - 1, ld_stage = 0;
-  int32_t pf_src[kNA], pf_ex = 0;  // GATHER: sources of this lane's rows
+  int b_wave = 0, be_wave = 0;           // where this wave's columns begin
+  const bool ex_a = wave < BM / 64;      // the waves that bring A's exponents
+  int ld_kb = 0, ld_t = first, ld_region = 1, ld_stage = 0;
+  int32_t pf_src[kFR], pf_ex = 0;  // GATHER: sources of this lane's rows of the tile after, nx
+  auto a_byte = [&](int j) __attribute__((always_inline)) {
+    return static_cast<uint32_t>(((lane & 7) ^ swz128(8 * j + (lane >> 3))) * 16);
+  };
   auto fetch_src = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < kNA; ++j) {
-      const int r = a_row + 16 * j;
-      pf_src[j] = gather_src[ld.row0 + (r < ld.rows ? r : ld.rows - 1)];
+    for (int j = 0; j < kFR; ++j) {
+      const int r = a_row + 8 * j;
+      pf_src[j] = gather_src[nx.row0 + (r < nx.rows ? r : nx.rows - 1)];
     }
     const int r = 64 * wave + lane;
-    if (ex_a) pf_ex = gather_src[ld.row0 + (r < ld.rows ? r : ld.rows - 1)];
+    if (ex_a) pf_ex = gather_src[nx.row0 + (r < nx.rows ? r : nx.rows - 1)];
   };
   auto token = [&](int32_t slot) __attribute__((always_inline)) {
     const int tk = slot >= 0 ? slot / gather_k : 0;  // a row without a source reads token 0
     return static_cast<uint32_t>(tk < gather_rows ? tk : gather_rows - 1);
   };
+  // Tile ld_t becomes the one that is loaded.
   auto set_load_tile = [&]() __attribute__((always_inline)) {
-    ld.move(offsets, ld_t, n_tiles_n);
-    if (GATHER) fetch_src();
-    const int64_t block = static_cast<int64_t>(ld.e) * (ncols / 32) + ld.n0 / 32;
-    const int width = ncols - ld.n0 < kTileN ? ncols - ld.n0 : kTileN;
-    const int part = 64 * wave < width ? wave : wave - 2;  // (a tile of 128 columns: waves 0 and 1 again)
-    b_wave = part * 2 * b_col;
-    be_wave = (part >> 1) * 512;
-    b_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(B + block * b_col), 0, width * row_bytes,
-                                               kBufferWord3);
-    be_rsrc = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<uint8_t*>(b_exp + (static_cast<int64_t>(ld.e) * ks * ncols + ld.n0) * 4), 0,
-        ((ks - 1) * ncols + width) * 4, kBufferWord3);
     if (GATHER) {
+      ld = nx;
 #pragma unroll
-      for (int j = 0; j < kNA; ++j) a_voff[j] = token(pf_src[j]) * static_cast<uint32_t>(row_bytes) + a_byte;
+      for (int j = 0; j < kFR; ++j) a_voff[j] = token(pf_src[j]) * static_cast<uint32_t>(row_bytes) + a_byte(j);
       ae_voff = token(pf_ex) * static_cast<uint32_t>(ex_bytes);
+      if (ld_t + per_xcd < hi) {
+        nx.move(offsets, ld_t + per_xcd, n_tiles_n);
+        fetch_src();
+      }
     } else {
+      ld.move(offsets, ld_t, n_tiles_n);
       // rows past the segment repeat its last one; their results are not stored
       a_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(A + static_cast<int64_t>(ld.row0) * row_bytes),
                                                  0, ld.rows * row_bytes, kBufferWord3);
       ae_rsrc = __builtin_amdgcn_make_buffer_rsrc(
           const_cast<uint8_t*>(a_exp + static_cast<int64_t>(ld.row0) * ex_bytes), 0, ld.rows * ex_bytes, kBufferWord3);
 #pragma unroll
-      for (int j = 0; j < kNA; ++j) {
-        const int r = a_row + 16 * j;
-        a_voff[j] = static_cast<uint32_t>((r < ld.rows ? r : ld.rows - 1) * row_bytes + a_byte);
+      for (int j = 0; j < kFR; ++j) {
+        const int r = a_row + 8 * j;
+        a_voff[j] = static_cast<uint32_t>((r < ld.rows ? r : ld.rows - 1) * row_bytes) + a_byte(j);
       }
       const int r = 64 * wave + lane;
       ae_voff = static_cast<uint32_t>((r < ld.rows ? r : ld.rows - 1) * ex_bytes);
     }
+    const int64_t block = static_cast<int64_t>(ld.e) * (ncols / 32) + ld.n0 / 32;
+    const int width = ncols - ld.n0 < kTileN ? ncols - ld.n0 : kTileN;
+    const int part = 64 * wave < width ? wave : wave - 2;  // (a tile of 128 columns: waves 0 and 1 again)
+    b_wave = part * 2 * b_col;
+    be_wave = part * 256;
+    b_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(B + block * b_col), 0, width * row_bytes,
+                                               kBufferWord3);
+    be_rsrc = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t*>(b_exp + (static_cast<int64_t>(ld.e) * ks * ncols + ld.n0) * 4), 0,
+        ((ks - 1) * ncols + width) * 4, kBufferWord3);
     ld_kb = 0;
   };
-  // One step into the ring.  (Every step loaded: the last one again, into a stage that
-  // nothing reads, so that a step always issues as many.)
-  auto issue = [&]() __attribute__((always_inline)) {
-    if (ld_g < iters && ld_left == 0) {
-      if (ld_kb == ks) {
-        ld_t += per_xcd;
-        set_load_tile();
-      }
-      ld_left = group_steps(ks - ld_kb);
-      ld_region = ld_region + 1 == Cfg::kRegions ? 0 : ld_region + 1;
-      // (what a short group reads past a row's end is not used; past the buffer it is
-      // not read)
+  auto issue_a = [&]() __attribute__((always_inline)) {
+    if ((ld_kb & 1) == 0) {
+      ld_region ^= 1;
+      // (what it reads past a row's end is not used; past the buffer it is not read)
       if (ex_a)
-        dma16(ae_rsrc, smem + kStages * Cfg::kStage + ld_region * Cfg::kExA + wave * 1024,
-              ae_voff + static_cast<uint32_t>(ld_kb * 4), 0);
+        dma16(ae_rsrc, smem + 2 * Cfg::kA + ld_region * Cfg::kExA + wave * 1024,
+              ae_voff + static_cast<uint32_t>(ld_kb * 8));
     }
-    const int kb = ld_g < iters ? ld_kb : ld_kb - 1;
-    uint8_t* st = smem + ld_stage * Cfg::kStage;
 #pragma unroll
-    for (int j = 0; j < kNA; ++j) dma16(a_rsrc, st + (wave * kNA + j) * 1024, a_voff[j], kb * 64);
+    for (int j = 0; j < kFR; ++j)
+      dma16(a_rsrc, smem + ld_stage * Cfg::kA + (wave * kFR + j) * 1024, a_voff[j] + static_cast<uint32_t>(ld_kb * 128));
+    ld_stage ^= 1;
+    fence();  // (the waits count B's loads behind these)
+  };
+  u32x4 fb[4][2];
+  uint32_t eb[2][2];
+  // B of the step that is loaded.  (Past the tile's last value: the last again, not used.)
+  auto load_b = [&](int q) __attribute__((always_inline)) {
+    const int k64 = 4 * ld_kb + q < 2 * ks ? 4 * ld_kb + q : 2 * ks - 1;
 #pragma unroll
-    for (int j = 0; j < kNB; ++j)
-      dma16(b_rsrc, st + Cfg::kA + (wave * kNB + j) * 1024, static_cast<uint32_t>(lane * 16),
-            b_wave + (j >> 1) * b_col + kb * 2048 + (j & 1) * 1024);
-    dma4(be_rsrc, st + Cfg::kA + Cfg::kB + wave * 256, be_voff, be_wave + kb * ncols * 4);
-    if (ld_g < iters) {
-      ++ld_g;
-      ++ld_kb;
-      --ld_left;
-    }
-    ld_stage = ld_stage + 1 == kStages ? 0 : ld_stage + 1;
+    for (int j = 0; j < 2; ++j)
+      fb[q][j] = __builtin_amdgcn_raw_buffer_load_b128(b_rsrc, lane * 16, b_wave + j * b_col + k64 * 1024, 0);
+  };
+  auto load_eb = [&](int t) __attribute__((always_inline)) {
+    const int k128 = 2 * ld_kb + t < ks ? 2 * ld_kb + t : ks - 1;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      eb[t][j] = __builtin_amdgcn_raw_buffer_load_b32(be_rsrc, (lane & 31) * 4, be_wave + j * 128 + k128 * ncols * 4, 0);
   };
 
   // ---- compute side ----------------------------------------------------------------
-  // Wave w: rows (BM / 2) (w & 1) .. and columns 128 (w >> 1) .. of the tile.
-  const int wm = wave & 1, wn = wave >> 1;
+  // Wave w: all rows and columns 64 w .. of the tile.
   const int frow = lane & 31, half = lane >> 5;
-  const int fsw = swz64(frow);
-  const int a_off = (wm * (BM / 2) + frow) * 64;
-  const int b_off = Cfg::kA + wn * 8192 + lane * 16;
-  const int be_off = Cfg::kA + Cfg::kB + wn * 512 + frow * 16;
-  const int ae_off = kStages * Cfg::kStage + (wm * (BM / 2) + frow) * 16;
-  f32x16 acc[kFR][4];
-  int stage = 0, region = Cfg::kRegions - 1, left = 0, in_group = 0;
-  auto step = [&]() __attribute__((always_inline)) {
-    const uint8_t* st = smem + stage * Cfg::kStage;
-    u32x4 fa[2][kFR], fb[2][4];
-    int exa[kFR], exb[4];
-    const u32x4 exw = *reinterpret_cast<const u32x4*>(st + be_off);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) exb[j] = static_cast<int>(exw[j] >> (8 * half));
-#pragma unroll
-    for (int i = 0; i < kFR; ++i)
-      exa[i] = static_cast<int>(*reinterpret_cast<const uint32_t*>(smem + ae_off + region * Cfg::kExA + i * 512 +
-                                                                   in_group * 4) >>
-                                (8 * half));
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) fb[q][j] = *reinterpret_cast<const u32x4*>(st + b_off + j * 2048 + q * 1024);
+  const int fsw = swz128(frow);
+  f32x16 acc[kFR][2];
+  int stage = 0, region = 1;
+  constexpr int kNewer = 12;  // loads of B and its exponents in a step, behind A's
+
+  // One step: 64 nq values of this tile, the loads of the next step behind them.
+  auto step = [&](int kb, auto NQ) __attribute__((always_inline)) {
+    constexpr int nq = decltype(NQ)::value;
+    // this wave's loads of A have landed; after the barrier every wave's have, and every
+    // wave is done with the step before, whose stage the next loads take
+    wait_vm_lgkm0<kNewer>();
+    __builtin_amdgcn_s_barrier();
+    fence();
+    // on to the next step (after the last tile's last one: it again)
+    if (ld_kb + 1 < nb) {
+      ++ld_kb;
+    } else if (ld_t + per_xcd < hi) {
+      ld_t += per_xcd;
+      set_load_tile();
+    }
+    issue_a();
+    if ((kb & 1) == 0) region ^= 1;
+    const uint8_t* st = smem + stage * Cfg::kA + frow * 128;
+    const uint8_t* se = smem + 2 * Cfg::kA + region * Cfg::kExA + frow * 16 + (kb & 1) * 8;
+    u32x2_t exw[kFR];
+    u32x4 fa[2][kFR];
+    auto read_a = [&](int q) __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i < kFR; ++i)
-        fa[q][i] = *reinterpret_cast<const u32x4*>(st + a_off + i * 2048 + (((2 * q + half) ^ fsw) * 16));
+        fa[q & 1][i] = *reinterpret_cast<const u32x4*>(st + i * 4096 + (((2 * q + half) ^ fsw) * 16));
+    };
+    read_a(0);
+#pragma unroll
+    for (int i = 0; i < kFR; ++i) exw[i] = *reinterpret_cast<const u32x2_t*>(se + i * 512);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      if (q < nq) {
+        // (kept ahead of the products, or each fragment is waited for)
+        if (q + 1 < nq) read_a(q + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        int ea[kFR], ebs[2];
+#pragma unroll
+        for (int i = 0; i < kFR; ++i) ea[i] = static_cast<int>(exw[i][q >> 1] >> (8 * half));
+#pragma unroll
+        for (int j = 0; j < 2; ++j) ebs[j] = static_cast<int>(eb[q >> 1][j] >> (8 * half));
+#pragma unroll
+        for (int i = 0; i < kFR; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            acc[i][j] = (q & 1) ? mfma_fp4<2>(fb[q][j], fa[q & 1][i], acc[i][j], ebs[j], ea[i])
+                                : mfma_fp4<0>(fb[q][j], fa[q & 1][i], acc[i][j], ebs[j], ea[i]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      load_b(q);
+      if (q & 1) load_eb(q >> 1);
+      fence();
     }
 #pragma unroll
     for (int i = 0; i < kFR; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = mfma_fp4<0>(fb[0][j], fa[0][i], acc[i][j], exb[j], exa[i]);
-#pragma unroll
-    for (int i = 0; i < kFR; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = mfma_fp4<2>(fb[1][j], fa[1][i], acc[i][j], exb[j], exa[i]);
-    // used here, before the barrier, so that the products are not moved past it
-#pragma unroll
-    for (int i = 0; i < kFR; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) use_here(acc[i][j]);
+      for (int j = 0; j < 2; ++j) use_here(acc[i][j]);
+    stage ^= 1;
   };
 
-  ld.move(offsets, first, n_tiles_n);
+  if (GATHER) {
+    nx.move(offsets, first, n_tiles_n);
+    fetch_src();
+  }
   set_load_tile();
-  issue();
-  issue();
-  int g = 0;
+  issue_a();
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    load_b(q);
+    if (q & 1) load_eb(q >> 1);
+  }
   for (int t = first; t < hi; t += per_xcd) {
 #pragma unroll
     for (int i = 0; i < kFR; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+      for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
-    for (int kb = 0; kb < ks; ++kb, ++g) {
-      // this wave's loads of step g have landed (step g + 1's may fly); after the
-      // barrier every wave's have, and every wave is done with step g - 1, whose stage
-      // the next loads take
-      wait_vm_lgkm0<kNA + kNB + 1>();
-      __builtin_amdgcn_s_barrier();
-      issue();
-      if (left == 0) {
-        left = group_steps(ks - kb);
-        region = region + 1 == Cfg::kRegions ? 0 : region + 1;
-        in_group = 0;
-      }
-      step();
-      --left;
-      ++in_group;
-      stage = stage + 1 == kStages ? 0 : stage + 1;
-    }
+    int kb = 0;
+    for (; 2 * kb + 1 < ks; ++kb) step(kb, std::integral_constant<int, 4>{});
+    if (2 * kb < ks) step(kb, std::integral_constant<int, 2>{});  // 128 values
     cur.move(offsets, t, n_tiles_n);
     const int64_t r0 = cur.row0;
-    const int row = wm * (BM / 2) + frow;
-    const bool mine = cur.n0 + wn * 128 < ncols;  // uniform per wave
+    const bool mine = cur.n0 + wave * 64 < ncols;  // uniform per wave
     if constexpr (GATE_UP) {
       const int d_ff = ncols / 2;
       const __amdgpu_buffer_rsrc_t q_out =
@@ -672,21 +661,14 @@ __global__ __launch_bounds__(kTileThreads, 2) void grouped_mxfp4_tiles(
           __builtin_amdgcn_make_buffer_rsrc(c_exp + r0 * (d_ff / 32), 0, cur.rows * (d_ff / 32), kBufferWord3);
 #pragma unroll
       for (int i = 0; i < kFR; ++i)
-        if (mine) store_h_blocks(acc[i], q_out, e_out, row + 32 * i, cur.n0 / 2 + wn * 64, d_ff, half);
+        if (mine) store_h_block(acc[i][0], acc[i][1], q_out, e_out, frow + 32 * i, cur.n0 / 2 + wave * 32, d_ff, half);
     } else {
       const __amdgpu_buffer_rsrc_t out =
           __builtin_amdgcn_make_buffer_rsrc(C + r0 * ncols * 2, 0, cur.rows * ncols * 2, kBufferWord3);
-      // through the stage of the last step, which every wave has read once all are here
-      // and which the next step's loads take after their barrier
-      uint8_t* const lds = smem + (stage == 0 ? kStages - 1 : stage - 1) * Cfg::kStage + wave * 4096;
-      __builtin_amdgcn_s_barrier();
+      uint8_t* const lds = smem + 2 * (Cfg::kA + Cfg::kExA) + wave * 4096;
 #pragma unroll
       for (int i = 0; i < kFR; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; j += 2)
-          if (mine)
-            store_y_blocks(acc[i][j], acc[i][j + 1], lds, out, wm * (BM / 2) + 32 * i, cur.n0 + wn * 128 + 32 * j, ncols,
-                         lane);
+        if (mine) store_y_blocks(acc[i][0], acc[i][1], lds, out, 32 * i, cur.n0 + wave * 64, ncols, lane);
     }
   }
   // nothing may still be writing into LDS when the workgroup ends
@@ -748,23 +730,26 @@ int check_product(const char* what, int n_experts, int64_t rows_cap, int d_model
   return HMOE_OK;
 }
 
-// Which kernel a product takes: the one with the least estimated time, from three
-// measured rates (MI355X, us, `steps` = K / 128):
-//   rows split four ways: 3.5, and 0.55 ns for every 32 rows x 64 columns x 128 values;
-//   64-row tiles:  4.2 + 0.5 a step while there is one a CU, 0.8 when there are two, and
-//     for every further two;
-//   128-row tiles: 5.0 + 0.7 and 1.23 alike.
-// None is faster than reading the experts' weights at 5.9 TB/s, which the first comes
-// nearest to.  Measured against each other (rows, 64, 128), us:
-//   gate/up 64 experts, D 2048, F 1024, top-8: 1 token 4.8, 11.6, 15.4; 48 tokens 24.0,
-//     25.0, 27.6; 512 tokens 39.9, 33.3, 35.9; 1000 tokens 68.7, 36.9, 35.9;
-//   32 experts, D 4096, F 2048, top-4: 300 tokens 68.2, 51.7, 64.1;
-//   24 experts, D 1152, F 640, top-3: 333 tokens 7.9, 8.9, 11.4; 800 tokens 13.2, 9.0,
-//     11.4; 2000 tokens 22.7, 16.6, 14.4;
-//   one segment, D 2048, F 1024: 64 rows 5.6, 11.9, 15.4; 2000 rows 19.4, 12.2, 15.7; 8000
-//     rows 64.7, 28.1, 23.7.
-// Below four steps the split has nothing to split: 2000 tokens on 8 experts, D 256, 8.7
-// against 5.5 with the waves side by side.
+// Which kernel a product takes: the one with the least estimated time, from measured
+// rates (MI355X, us, `steps` = K / 128):
+//   rows: 3.5, and 0.55 ns for every 32 rows x 64 columns x 128 values; or the experts'
+//     weights at 5.9 TB/s and, for every 64 columns, the rows at 8;
+//   64-row tiles: 3.6, and 0.36 a step or, when there are more of them, 0.32 for every one
+//     a CU has; or the weights and 1.5;
+//   128-row tiles: 4.2, 0.52 and 0.57.
+// Measured against each other (rows, 64, 128), us:
+//   gate/up 64 experts, D 2048, F 1024, top-8: 1 token 5.6, 8.8, 12.2; 8 tokens 15.0, 17.7,
+//     20.4; 48 tokens 24.0, 23.8, 25.1; 128 tokens 26.9, 24.3, 25.9; 1000 tokens 65, 32.8,
+//     36.1; 4000 tokens 208, 88, 82; 16384 tokens 790, 335, 296;
+//   32 experts, D 4096, F 2048, top-4: 100 tokens 47, 44.4, 45.2; 2000 tokens 239, 111, 92;
+//   24 experts, D 1152, F 640, top-3: 100 tokens 5.5, 7.3, 9.7; 333 tokens 8.0, 7.4, 9.8;
+//     2000 tokens 21.6, 13.2, 13.5;
+//   one segment, D 2048, F 1024: 200 rows 5.7, 9.0, 12.1; 1000 rows 9.9, 9.2, 12.4; 8000
+//     rows 53, 23.1, 21.7.
+// Rows split the reduction where there are few waves or it is long; below 16 steps waves
+// side by side that fill the chip are faster: down of 64 experts (8 steps), 32 tokens 12.1
+// against 13.3, of 128 experts, D 1024, F 512 (4 steps), 30 tokens 5.0 against 6.2.  Below
+// four steps there is nothing to split.
 enum Form { kRows1, kRows4, kTiles64, kTiles128 };
 
 // The experts that have rows, and the row tiles of all.  The counts are known only to
@@ -784,17 +769,18 @@ Form choose_form(int64_t rows, int n_experts, int kdim, int ncols, int cus) {
   const double n = live_experts(rows, n_experts);
   const double weights = n * ncols * kdim * (17.0 / 32.0) / 5.9e6;
   const double tiles32 = row_tiles(rows, n_experts, 32);
-  const double by_rows = std::max(3.5 + tiles32 * (ncols / 64) * steps * 0.55e-3, weights * (0.9 + 0.1 * tiles32 / n));
-  const auto by_tiles = [&](int bm, double start, double alone, double paired) {
+  const double re_read = static_cast<double>(rows) * (ncols / 64) * (kdim / 2) / 8e6;
+  const double waves = tiles32 * (ncols / 64);
+  const double by_rows = std::max(3.5 + waves * steps * 0.55e-3, weights + re_read);
+  const auto by_tiles = [&](int bm, double start, double alone, double busy) {
     const double tiles = row_tiles(rows, n_experts, bm) * static_cast<double>(ceil_div(ncols, kTileN));
-    const double step = tiles <= cus ? alone : paired * std::ceil(tiles / (2.0 * cus) - 0.02);
-    return std::max(start + steps * step, 1.1 * weights);
+    return std::max(start + steps * std::max(alone, busy * tiles / cus), weights + 1.5);
   };
-  const double by_64 = by_tiles(64, 4.2, 0.5, 0.8);
-  const double by_128 = steps > 1 ? by_tiles(128, 5.0, 0.7, 1.23) : by_64 + 1.0;
+  const double by_64 = by_tiles(64, 3.6, 0.36, 0.32);
+  const double by_128 = by_tiles(128, 4.2, 0.52, 0.57);
   // (a grid holds 65535 tiles along y)
   if (by_rows <= std::min(by_64, by_128) && max_row_tiles(rows, n_experts) <= 65535)
-    return steps < 4 ? kRows1 : kRows4;
+    return steps < 4 || (steps < 16 && waves >= 4.0 * cus) ? kRows1 : kRows4;
   return by_64 <= by_128 ? kTiles64 : kTiles128;
 }
 
@@ -812,10 +798,11 @@ int launch_product(const char* what, const uint8_t* a, const uint8_t* a_exp, con
   if (form == kTiles64 || form == kTiles128) {
     const auto launch = [&](auto BM) {
       constexpr int bm = decltype(BM)::value;
+      constexpr int lds = TileCfg<bm, GATE_UP>::kLds, per_cu = TileCfg<bm, GATE_UP>::kPerCu;
       static std::atomic<uint64_t> done{0};
-      if (int rc = allow_lds(what, grouped_mxfp4_tiles<bm, GATE_UP, GATHER>, TileCfg<bm>::kLds, dev, &done)) return rc;
-      hipLaunchKernelGGL((grouped_mxfp4_tiles<bm, GATE_UP, GATHER>), dim3(2 * cus), dim3(kTileThreads),
-                         TileCfg<bm>::kLds, s, a, a_exp, b, b_exp, offsets, n_experts, kdim, ncols, c, c_exp,
+      if (int rc = allow_lds(what, grouped_mxfp4_tiles<bm, GATE_UP, GATHER>, lds, dev, &done)) return rc;
+      hipLaunchKernelGGL((grouped_mxfp4_tiles<bm, GATE_UP, GATHER>), dim3(per_cu * cus), dim3(kTileThreads),
+                         lds, s, a, a_exp, b, b_exp, offsets, n_experts, kdim, ncols, c, c_exp,
                          gather_src, gather_k, gather_rows);
       return check_launch(what);
     };
@@ -837,8 +824,8 @@ int launch_product(const char* what, const uint8_t* a, const uint8_t* a_exp, con
 
 extern "C" int64_t hmoe_grouped_mxfp4_form(int64_t rows_cap, int n_experts, int kdim, int ncols, int cus) {
   using namespace hmoe;
-  if (rows_cap < 1 || rows_cap > kMaxRows || n_experts < 1 || n_experts > kMaxExperts || cus < 1 || kdim < 128 || kdim % 128 != 0 ||
-      ncols < 128 || ncols % 128 != 0) {
+  if (rows_cap < 1 || rows_cap > kMaxRows || n_experts < 1 || n_experts > kMaxExperts || cus < 1 || kdim < 128 ||
+      kdim % 128 != 0 || ncols < 128 || ncols % 128 != 0) {
     set_error("grouped_mxfp4_form: sizes that the products refuse");
     return -1;
   }

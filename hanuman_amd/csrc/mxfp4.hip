@@ -147,14 +147,13 @@ __global__ __launch_bounds__(256) void pack_mxfp4_kernel(const TW* __restrict__ 
 #pragma unroll
       for (int r = 0; r < 32; ++r) amax[j] = umax32(amax[j], __float_as_uint(v[j][r]) & 0x7fffffffu);
       const uint32_t ee = mxfp4_exponent(amax[j]);
-      const float inv = mxfp4_inverse(ee);
       u32x4 w;
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         float t[8];
 #pragma unroll
         for (int r = 0; r < 8; ++r) t[r] = v[j][g * 8 + r];
-        w[g] = mxfp4_codes8(t, inv);
+        w[g] = mxfp4_codes8(t, ee);
       }
       // column c of the master is operand row p
       const int c = c0 + i2 + j;

@@ -36,25 +36,22 @@ __device__ __forceinline__ uint32_t mxfp4_exponent(uint32_t amax_bits) {
   return amax_bits >= 0x7f800000u ? 255u : e;
 }
 
-// 2^(127 - E), and 0 for a NaN block.
-__device__ __forceinline__ float mxfp4_inverse(uint32_t e) {
-  return __uint_as_float(e < 255u ? (254u - e) << 23 : 0u);
-}
-
 // 2^(E - 127), NaN at 255 (2^-127 is below float32's normal numbers).
 __device__ __forceinline__ float mxfp4_scale(uint32_t e) {
   return __uint_as_float(e == 0u ? 0x00400000u : e == 255u ? 0x7fc00000u : e << 23);
 }
 
-// Codes of eight values of a block, value i in bits 4 i .. 4 i + 3.
-__device__ __forceinline__ uint32_t mxfp4_codes8(const float (&v)[8], float inv) {
+// Codes of eight values of a block with exponent e, value i in bits 4 i .. 4 i + 3.  (The
+// conversion divides by its scale operand, of which it takes the exponent field alone.)
+__device__ __forceinline__ uint32_t mxfp4_codes8(const float (&v)[8], uint32_t e) {
+  const float scale = __uint_as_float(e << 23);
   uint32_t w = 0;
-  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[0] * inv, v[1] * inv, 1.0f, 0);
-  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[2] * inv, v[3] * inv, 1.0f, 1);
-  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[4] * inv, v[5] * inv, 1.0f, 2);
-  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[6] * inv, v[7] * inv, 1.0f, 3);
-  // a NaN block: inf * 0 and NaN * 0 are NaN, whose code the format leaves open
-  return inv != 0.0f ? w : 0u;
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[0], v[1], scale, 0);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[2], v[3], scale, 1);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[4], v[5], scale, 2);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[6], v[7], scale, 3);
+  // (the codes of infinities and NaNs are left open)
+  return e != 255u ? w : 0u;
 }
 
 __device__ __forceinline__ uint32_t umax32(uint32_t a, uint32_t b) { return a > b ? a : b; }
@@ -73,7 +70,7 @@ __device__ __forceinline__ void quant_chunk_mxfp4(const Values& x, int64_t c, ui
   amax = umax32(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), 1)));
   amax = umax32(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), 2)));
   const uint32_t e = mxfp4_exponent(amax);
-  reinterpret_cast<uint32_t*>(q)[c] = mxfp4_codes8(v, mxfp4_inverse(e));
+  reinterpret_cast<uint32_t*>(q)[c] = mxfp4_codes8(v, e);
   if ((c & 3) == 0) exps[c >> 2] = static_cast<uint8_t>(e);
 }
 

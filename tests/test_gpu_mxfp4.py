@@ -213,13 +213,17 @@ def test_products(gpu, shape):
 
 
 FORMS = [
-    # the shape, and the form that its gate/up and down products take
-    ((6000, 3, 1, 128, 1280), 2, 1),    # one step a tile
-    ((8000, 2, 1, 256, 384), 2, 0),     # two
-    ((3000, 4, 2, 640, 384), 2, 2),     # five (groups of three and two), three
-    ((4000, 2, 1, 1152, 1152), 3, 3),   # nine; a last column tile of 128
-    ((2600, 2, 2, 512, 1152), 3, 2),    # a whole group of four
-    ((1500, 20, 2, 640, 1152), 2, 1),   # segments that end inside tiles
+    # the shape, and the form that its gate/up and down products take; tiles go in steps
+    # of 256 values
+    ((9000, 3, 1, 128, 256), 2, 0),     # half a step a tile
+    ((6000, 3, 1, 128, 1280), 2, 1),
+    ((8000, 2, 1, 256, 384), 2, 2),     # one step; one and a half
+    ((3000, 4, 2, 640, 384), 2, 2),     # two and a half
+    ((2600, 2, 2, 512, 1152), 2, 2),    # two; four and a half
+    ((1500, 20, 2, 640, 1152), 2, 2),   # segments that end inside tiles
+    ((4000, 2, 2, 1152, 1152), 3, 3),   # a last column tile of 128
+    ((20000, 2, 1, 384, 896), 3, 2),
+    ((40000, 2, 1, 128, 1152), 3, 3),   # half a step a tile of 128 rows
 ]
 
 
