@@ -56,6 +56,28 @@ __device__ __forceinline__ f32x16 mfma_fp4(const u32x4& b, const u32x4& a, const
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b8, a8, c, 4, 4, Q, eb, Q, ea);
 }
 
+// n / d for 0 <= n < 2^31 without a division: with 2^s the first power of two that is not
+// below d, mul = ceil(2^(31 + s) / d) is too large by less than 2^s / d, which n times over
+// is less than the 2^(31 + s) / d that the quotient could be off by.
+struct Divisor {
+  uint32_t mul;
+  int shift;
+};
+Divisor divisor(int d) {
+  int s = 0;
+  while ((int64_t(1) << s) < d) ++s;
+  return {static_cast<uint32_t>(((uint64_t(1) << (31 + s)) + d - 1) / d), s};
+}
+__device__ __forceinline__ int divide(int n, Divisor d) {
+  return static_cast<int>(__umulhi(static_cast<uint32_t>(n) * 2u, d.mul) >> d.shift);
+}
+
+// The token of a row's slot; a row without a source reads token 0.
+__device__ __forceinline__ int token_of(int32_t slot, Divisor top_k, int tokens) {
+  const int t = divide(slot > 0 ? slot : 0, top_k);
+  return t < tokens ? t : tokens - 1;
+}
+
 // Segment and row tile of the m_tile-th tile of `bm` rows; false past the last.
 // A wave looks at 64 experts at a time.
 struct RowTile {
@@ -102,15 +124,18 @@ __device__ __forceinline__ bool find_row_tile(const int32_t* __restrict__ offset
 // dwords 2 and 3.
 __device__ __forceinline__ uint32_t quantise_h(const f32x16& g, const f32x16& u, uint32_t (&w)[2]) {
   float h[16];
-  uint32_t amax = 0;
+  float amax = 0.0f;
 #pragma unroll
-  for (int k = 0; k < 16; ++k) {
+  for (int k = 0; k < 16; k += 2) {
     h[k] = swiglu_f32(g[k], u[k]);
-    const uint32_t b = __float_as_uint(h[k]) & 0x7fffffffu;
-    amax = amax > b ? amax : b;
+    h[k + 1] = swiglu_f32(g[k + 1], u[k + 1]);
+    // (NaN where either is)
+    amax = __builtin_elementwise_maximum(__builtin_elementwise_maximum(amax, __builtin_fabsf(h[k])),
+                                         __builtin_fabsf(h[k + 1]));
   }
   // lanes L and L + 32 hold the row's other values
-  const auto sw = __builtin_amdgcn_permlane32_swap(amax, amax, false, false);
+  const uint32_t am = __float_as_uint(amax);
+  const auto sw = __builtin_amdgcn_permlane32_swap(am, am, false, false);
   const uint32_t e = mxfp4_exponent(sw[0] > sw[1] ? sw[0] : sw[1]);
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
@@ -201,8 +226,8 @@ template <bool GATE_UP, bool GATHER, int SPLIT>
 __global__ __launch_bounds__(256) void grouped_mxfp4_rows(
     const uint8_t* __restrict__ A, const uint8_t* __restrict__ a_exp, const uint8_t* __restrict__ B,
     const uint8_t* __restrict__ b_exp, const int32_t* __restrict__ offsets, int n_experts, int kdim, int ncols,
-    uint8_t* __restrict__ C, uint8_t* __restrict__ c_exp, const int32_t* __restrict__ gather_src, int gather_k,
-    int gather_rows) {
+    uint8_t* __restrict__ C, uint8_t* __restrict__ c_exp, const int32_t* __restrict__ gather_src,
+    Divisor gather_k, int gather_rows) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int frow = lane & 31, half = lane >> 5;
@@ -211,11 +236,7 @@ __global__ __launch_bounds__(256) void grouped_mxfp4_rows(
   const int n0 = SPLIT == 1 ? (blockIdx.x * 4 + wave) * 64 : blockIdx.x * 64;
   if (n0 >= ncols) return;  // (SPLIT 1 only: no barrier follows there)
   int src = t.row0 + (frow < t.rows ? frow : t.rows - 1);  // rows past the segment repeat its last one
-  if (GATHER) {
-    const int slot = gather_src[src];
-    src = slot >= 0 ? slot / gather_k : 0;  // a row without a source reads token 0
-    src = src < gather_rows ? src : gather_rows - 1;
-  }
+  if (GATHER) src = token_of(gather_src[src], gather_k, gather_rows);
   const int groups = kdim / 128;
   const uint8_t* a = A + static_cast<int64_t>(src) * (kdim / 2) + half * 16;
   const uint8_t* ae = a_exp + static_cast<int64_t>(src) * (kdim / 32);
@@ -320,14 +341,24 @@ __global__ __launch_bounds__(256) void grouped_mxfp4_rows(
 // be 128 columns wide: waves 2 and 3 then load and compute the others' again and store
 // nothing.
 //
-// Gate/up of 131072 rows, D 2048, F 1024 (1.1 TFLOP) takes 300 us, down 170 us.  What bounds
+// Of two waves on a SIMD the older one's products go first, so that its workgroup took 23
+// thousand cycles a tile and the other 32, which then ended alone: they take turns by tile
+// (gate/up below 298 -> 285 us, down 172 -> 165; with 64 rows, taken where a workgroup has
+// few tiles, 512 tokens 28.8 -> 32.0, and not done).
+//
+// Gate/up of 131072 rows, D 2048, F 1024 (1.1 TFLOP) takes 285 us, down 165 us.  What bounds
 // them is power: with these operands the matrix cores alone, fed from registers, run at
-// 1.65 GHz and 6.5 PFLOP/s (170 us), and with operands of zeros the same launches take 222
-// and 126 us.  With B through LDS too (2 x 2 waves, steps of 128 values, three stages) it
-// was 326 and 187 us, 265 and 148 with zeros: an LDS that moved as much as it can while the
-// products last, and half lines of A.  One workgroup of eight waves on 128 x 512 takes 301
-// and 176 us, row-tile groups of 4 and 16 and a raised wave priority around the products
-// the same as this, A's loads spread over the step 305 and 174.
+// 1.65 GHz and 6.5 PFLOP/s (170 us), and with operands of zeros, at 2.4 GHz, the same
+// launches take 205 and 119 us.  In cycles it is what a CU has to do besides: a step's
+// loads come at 40 bytes a cycle and CU, and alone in its loop, while the other is in its
+// epilogue (4.6 thousand of 23 thousand cycles), a workgroup reaches half the rate.
+// Measured and not taken (us; gate/up and down, before the turns 300 and 170): B through LDS
+// too (2 x 2 waves, steps of 128 values, three stages) 326 and 187, an LDS and half lines of
+// A that kept pace with the products at best; one workgroup of eight waves on 128 x 512 301
+// and 176; loads and reads issued one by one behind each product, A two steps ahead, 293
+// and 173; the barrier ahead of a step's last products 290 and 169; the next tile brought
+// into L2 during the epilogue 306 and 175; row-tile groups of 2, 4 and 16 the same as of 8;
+// h stored from the accumulators, 16 bytes of a row at a time, 295.
 constexpr int kTileThreads = 256;
 constexpr int kNumXcd = 8;
 constexpr int kTileN = 256;
@@ -336,7 +367,8 @@ constexpr int kTileGroup = 8;
 template <int BM, bool GATE_UP>
 struct TileCfg {
   static constexpr int kA = BM * 128, kExA = BM * 16;  // a stage, a region of exponents
-  static constexpr int kLds = 2 * (kA + kExA) + (GATE_UP ? 0 : 4 * 4096);  // (ys: 4 KB a wave)
+  static constexpr int kOut = GATE_UP ? BM * 68 : 4 * 4096;  // h's codes and exponents; ys, 4 KB a wave
+  static constexpr int kLds = 2 * (kA + kExA) + kOut;
   static constexpr int kFR = BM / 32;             // row fragments; DMA instructions a wave and step
   static constexpr int kPerCu = BM == 64 ? 3 : 2;
   static_assert(kPerCu * kLds <= 160 * 1024, "workgroups a CU");
@@ -359,6 +391,15 @@ __device__ __forceinline__ void fence() {
   asm volatile("" ::: "memory");
   __builtin_amdgcn_sched_barrier(0);
 }
+
+// Of a CU's two workgroups one goes first.
+__device__ __forceinline__ void take_turn(int turn) {
+  if (turn == 0) __builtin_amdgcn_s_setprio(0);
+  else __builtin_amdgcn_s_setprio(1);
+}
+
+// s_waitcnt lgkmcnt(0)
+__device__ __forceinline__ void wait_lgkm0() { __builtin_amdgcn_s_waitcnt(0xc07f); }
 
 // s_waitcnt vmcnt(N) lgkmcnt(0)
 template <int N>
@@ -439,8 +480,8 @@ template <int BM, bool GATE_UP, bool GATHER>
 __global__ __launch_bounds__(kTileThreads, BM == 64 ? 3 : 2) void grouped_mxfp4_tiles(
     const uint8_t* __restrict__ A, const uint8_t* __restrict__ a_exp, const uint8_t* __restrict__ B,
     const uint8_t* __restrict__ b_exp, const int32_t* __restrict__ offsets, int n_experts, int kdim, int ncols,
-    uint8_t* __restrict__ C, uint8_t* __restrict__ c_exp, const int32_t* __restrict__ gather_src, int gather_k,
-    int gather_rows) {
+    uint8_t* __restrict__ C, uint8_t* __restrict__ c_exp, const int32_t* __restrict__ gather_src,
+    Divisor gather_k, int gather_rows) {
   typedef TileCfg<BM, GATE_UP> Cfg;
   constexpr int kFR = Cfg::kFR;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
@@ -488,11 +529,10 @@ __global__ __launch_bounds__(kTileThreads, BM == 64 ? 3 : 2) void grouped_mxfp4_
       pf_src[j] = gather_src[nx.row0 + (r < nx.rows ? r : nx.rows - 1)];
     }
     const int r = 64 * wave + lane;
-    if (ex_a) pf_ex = gather_src[nx.row0 + (r < nx.rows ? r : nx.rows - 1)];
+    pf_ex = gather_src[nx.row0 + (r < nx.rows ? r : nx.rows - 1)];
   };
   auto token = [&](int32_t slot) __attribute__((always_inline)) {
-    const int tk = slot >= 0 ? slot / gather_k : 0;  // a row without a source reads token 0
-    return static_cast<uint32_t>(tk < gather_rows ? tk : gather_rows - 1);
+    return static_cast<uint32_t>(token_of(slot, gather_k, gather_rows));
   };
   // Tile ld_t becomes the one that is loaded.
   auto set_load_tile = [&]() __attribute__((always_inline)) {
@@ -501,10 +541,8 @@ __global__ __launch_bounds__(kTileThreads, BM == 64 ? 3 : 2) void grouped_mxfp4_
 #pragma unroll
       for (int j = 0; j < kFR; ++j) a_voff[j] = token(pf_src[j]) * static_cast<uint32_t>(row_bytes) + a_byte(j);
       ae_voff = token(pf_ex) * static_cast<uint32_t>(ex_bytes);
-      if (ld_t + per_xcd < hi) {
-        nx.move(offsets, ld_t + per_xcd, n_tiles_n);
-        fetch_src();
-      }
+      if (ld_t + per_xcd < hi) nx.move(offsets, ld_t + per_xcd, n_tiles_n);
+      fetch_src();  // (on every path: a load that may not be issued is waited for at once)
     } else {
       ld.move(offsets, ld_t, n_tiles_n);
       // rows past the segment repeat its last one; their results are not stored
@@ -610,12 +648,20 @@ __global__ __launch_bounds__(kTileThreads, BM == 64 ? 3 : 2) void grouped_mxfp4_
         for (int i = 0; i < kFR; ++i) ea[i] = static_cast<int>(exw[i][q >> 1] >> (8 * half));
 #pragma unroll
         for (int j = 0; j < 2; ++j) ebs[j] = static_cast<int>(eb[q >> 1][j] >> (8 * half));
+        if (q == 0 && kb == 0) {  // (zeros as an operand, not written first)
+          const f32x16 zero = {};
 #pragma unroll
-        for (int i = 0; i < kFR; ++i)
+          for (int i = 0; i < kFR; ++i)
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
-            acc[i][j] = (q & 1) ? mfma_fp4<2>(fb[q][j], fa[q & 1][i], acc[i][j], ebs[j], ea[i])
-                                : mfma_fp4<0>(fb[q][j], fa[q & 1][i], acc[i][j], ebs[j], ea[i]);
+            for (int j = 0; j < 2; ++j) acc[i][j] = mfma_fp4<0>(fb[0][j], fa[0][i], zero, ebs[j], ea[i]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < kFR; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              acc[i][j] = (q & 1) ? mfma_fp4<2>(fb[q][j], fa[q & 1][i], acc[i][j], ebs[j], ea[i])
+                                  : mfma_fp4<0>(fb[q][j], fa[q & 1][i], acc[i][j], ebs[j], ea[i]);
+        }
       }
       __builtin_amdgcn_sched_barrier(0);
       load_b(q);
@@ -640,31 +686,54 @@ __global__ __launch_bounds__(kTileThreads, BM == 64 ? 3 : 2) void grouped_mxfp4_
     load_b(q);
     if (q & 1) load_eb(q >> 1);
   }
+  int turn = blockIdx.x < gridDim.x / 2;  // (workgroups i and i + gridDim / 2 share a CU)
   for (int t = first; t < hi; t += per_xcd) {
-#pragma unroll
-    for (int i = 0; i < kFR; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
     int kb = 0;
+    if (BM == 128) take_turn(turn ^= 1);
     for (; 2 * kb + 1 < ks; ++kb) step(kb, std::integral_constant<int, 4>{});
     if (2 * kb < ks) step(kb, std::integral_constant<int, 2>{});  // 128 values
     cur.move(offsets, t, n_tiles_n);
     const int64_t r0 = cur.row0;
-    const bool mine = cur.n0 + wave * 64 < ncols;  // uniform per wave
     if constexpr (GATE_UP) {
       const int d_ff = ncols / 2;
       const __amdgpu_buffer_rsrc_t q_out =
           __builtin_amdgcn_make_buffer_rsrc(C + r0 * (d_ff / 2), 0, cur.rows * (d_ff / 2), kBufferWord3);
       const __amdgpu_buffer_rsrc_t e_out =
           __builtin_amdgcn_make_buffer_rsrc(c_exp + r0 * (d_ff / 32), 0, cur.rows * (d_ff / 32), kBufferWord3);
+      // 64 bytes of every row's codes and four exponents are put together in LDS (each wave
+      // has 16 and one of them)
+      uint8_t* const codes = smem + 2 * (Cfg::kA + Cfg::kExA);
+      uint8_t* const exps = codes + BM * 64;
 #pragma unroll
-      for (int i = 0; i < kFR; ++i)
-        if (mine) store_h_block(acc[i][0], acc[i][1], q_out, e_out, frow + 32 * i, cur.n0 / 2 + wave * 32, d_ff, half);
+      for (int i = 0; i < kFR; ++i) {
+        uint32_t w[2];
+        const uint32_t e = quantise_h(acc[i][0], acc[i][1], w);
+        const auto sw = __builtin_amdgcn_permlane32_swap(w[0], w[1], false, false);
+        *reinterpret_cast<u32x2_t*>(codes + (32 * i + frow) * 64 + wave * 16 + half * 8) = join_codes(sw[0], sw[1]);
+        if (half == 0) exps[(32 * i + frow) * 4 + wave] = static_cast<uint8_t>(e);
+      }
+      wait_lgkm0();
+      __builtin_amdgcn_s_barrier();
+      fence();
+      const int width = ncols - cur.n0 < kTileN ? ncols - cur.n0 : kTileN;
+#pragma unroll
+      for (int m = 0; m < BM / 64; ++m) {
+        const int row = (BM / 4) * wave + 16 * m + (lane >> 2);
+        const u32x4 v = *reinterpret_cast<const u32x4*>(codes + row * 64 + (lane & 3) * 16);
+        if ((lane & 3) * 64 < width)
+          __builtin_amdgcn_raw_buffer_store_b128(v, q_out, (row * d_ff + cur.n0 / 2) / 2 + (lane & 3) * 16, 0, 0);
+      }
+      if (lane < BM / 4) {
+        const int row = (BM / 4) * wave + lane;
+        const uint32_t v = *reinterpret_cast<const uint32_t*>(exps + row * 4);
+        const int off = row * (d_ff / 32) + cur.n0 / 64;
+        if (width == kTileN) __builtin_amdgcn_raw_buffer_store_b32(v, e_out, off, 0, 0);
+        else __builtin_amdgcn_raw_buffer_store_b16(static_cast<uint16_t>(v), e_out, off, 0, 0);
+      }
     } else {
       const __amdgpu_buffer_rsrc_t out =
           __builtin_amdgcn_make_buffer_rsrc(C + r0 * ncols * 2, 0, cur.rows * ncols * 2, kBufferWord3);
+      const bool mine = cur.n0 + wave * 64 < ncols;  // uniform per wave
       uint8_t* const lds = smem + 2 * (Cfg::kA + Cfg::kExA) + wave * 4096;
 #pragma unroll
       for (int i = 0; i < kFR; ++i)
@@ -732,23 +801,23 @@ int check_product(const char* what, int n_experts, int64_t rows_cap, int d_model
 
 // Which kernel a product takes: the one with the least estimated time, from measured
 // rates (MI355X, us, `steps` = K / 128):
-//   rows: 3.5, and 0.55 ns for every 32 rows x 64 columns x 128 values; or the experts'
-//     weights at 5.9 TB/s and, for every 64 columns, the rows at 8;
-//   64-row tiles: 3.6, and 0.36 a step or, when there are more of them, 0.32 for every one
-//     a CU has; or the weights and 1.5;
-//   128-row tiles: 4.2, 0.52 and 0.57.
+//   rows: 3.5, and 0.55 ns for every 32 rows x 64 columns x 128 values (0.35 unsplit); or the
+//     experts' weights at 5.9 TB/s and, for every 64 columns, the rows at 8;
+//   64-row tiles, three a CU at a time: 3.6, and 0.34 a step for each that a CU has, 0.36 for
+//     one alone; or the weights and 1.5;
+//   128-row tiles, two a CU: 4.2, 0.545 and 0.52.
 // Measured against each other (rows, 64, 128), us:
-//   gate/up 64 experts, D 2048, F 1024, top-8: 1 token 5.6, 8.8, 12.2; 8 tokens 15.0, 17.7,
-//     20.4; 48 tokens 24.0, 23.8, 25.1; 128 tokens 26.9, 24.3, 25.9; 1000 tokens 65, 32.8,
-//     36.1; 4000 tokens 208, 88, 82; 16384 tokens 790, 335, 296;
-//   32 experts, D 4096, F 2048, top-4: 100 tokens 47, 44.4, 45.2; 2000 tokens 239, 111, 92;
-//   24 experts, D 1152, F 640, top-3: 100 tokens 5.5, 7.3, 9.7; 333 tokens 8.0, 7.4, 9.8;
-//     2000 tokens 21.6, 13.2, 13.5;
-//   one segment, D 2048, F 1024: 200 rows 5.7, 9.0, 12.1; 1000 rows 9.9, 9.2, 12.4; 8000
-//     rows 53, 23.1, 21.7.
+//   gate/up 64 experts, D 2048, F 1024, top-8: 1 token 5.6, 8.7, 11.8; 8 tokens 14.8, 17.8,
+//     20.4; 64 tokens 24.5, 23.5, 25.3; 128 tokens 26.4, 24.3, 26.0; 1000 tokens 63, 32.0,
+//     37; 1500 tokens 89, 40, 46; 4000 tokens 213, 86, 80; 16384 tokens 792, 330, 285;
+//   32 experts, D 4096, F 2048, top-4: 300 tokens 69, 49.8, 59.6; 2000 tokens 238, 111, 91;
+//   24 experts, D 1152, F 640, top-3: 100 tokens 5.5, 7.2, 9.2; 333 tokens 8.0, 7.2, 9.3;
+//     4000 tokens 34, 17.1, 22;
+//   one segment, D 2048, F 1024: 200 rows 5.8, 8.9, 11.8; 1000 rows 10.0, 9.0, 12.0; 8000
+//     rows 54, 22.9, 21.5.
 // Rows split the reduction where there are few waves or it is long; below 16 steps waves
-// side by side that fill the chip are faster: down of 64 experts (8 steps), 32 tokens 12.1
-// against 13.3, of 128 experts, D 1024, F 512 (4 steps), 30 tokens 5.0 against 6.2.  Below
+// side by side that fill the chip are faster: down of 64 experts (8 steps), 32 tokens 12.2
+// against 13.3, of 128 experts, D 1024, F 512 (4 steps), 30 tokens 5.0 against 6.1.  Below
 // four steps there is nothing to split.
 enum Form { kRows1, kRows4, kTiles64, kTiles128 };
 
@@ -771,17 +840,20 @@ Form choose_form(int64_t rows, int n_experts, int kdim, int ncols, int cus) {
   const double tiles32 = row_tiles(rows, n_experts, 32);
   const double re_read = static_cast<double>(rows) * (ncols / 64) * (kdim / 2) / 8e6;
   const double waves = tiles32 * (ncols / 64);
-  const double by_rows = std::max(3.5 + waves * steps * 0.55e-3, weights + re_read);
-  const auto by_tiles = [&](int bm, double start, double alone, double busy) {
+  const bool split = steps >= 16 || (steps >= 4 && waves < 4.0 * cus);
+  const double by_rows = std::max(3.5 + waves * steps * (split ? 0.55e-3 : 0.35e-3), weights + re_read);
+  const auto by_tiles = [&](int bm, int per_cu, double start, double alone, double busy) {
     const double tiles = row_tiles(rows, n_experts, bm) * static_cast<double>(ceil_div(ncols, kTileN));
-    return std::max(start + steps * std::max(alone, busy * tiles / cus), weights + 1.5);
+    const double whole = std::floor(tiles / (per_cu * cus)), rest = tiles - whole * per_cu * cus;
+    const double last = rest < 1.0 ? 0.0 : std::max(alone, busy * std::ceil(rest / cus - 0.02));
+    return std::max(start + steps * (whole * per_cu * busy + last), weights + 1.5);
   };
-  const double by_64 = by_tiles(64, 3.6, 0.36, 0.32);
-  const double by_128 = by_tiles(128, 4.2, 0.52, 0.57);
+  const double by_64 = by_tiles(64, TileCfg<64, true>::kPerCu, 3.6, 0.36, 0.34);
+  const double by_128 = by_tiles(128, TileCfg<128, true>::kPerCu, 4.2, 0.52, 0.545);
   // (a grid holds 65535 tiles along y)
   if (by_rows <= std::min(by_64, by_128) && max_row_tiles(rows, n_experts) <= 65535)
-    return steps < 4 || (steps < 16 && waves >= 4.0 * cus) ? kRows1 : kRows4;
-  return by_64 <= by_128 ? kTiles64 : kTiles128;
+    return split ? kRows4 : kRows1;
+  return 0.92 * by_64 <= by_128 ? kTiles64 : kTiles128;  // (the counts are estimates: 64 rows end more evenly)
 }
 
 template <bool GATE_UP, bool GATHER>
@@ -789,6 +861,7 @@ int launch_product(const char* what, const uint8_t* a, const uint8_t* a_exp, con
                    const uint8_t* b_exp, const int32_t* offsets, int n_experts, int64_t rows_cap, int kdim,
                    int ncols, uint8_t* c, uint8_t* c_exp, const int32_t* gather_src, int gather_k,
                    int gather_rows, hipStream_t s) {
+  const Divisor by_k = divisor(gather_k);
   HMOE_REQUIRE(static_cast<int64_t>(kdim / 128) * ncols * 4 < (int64_t(1) << 31), "%s: operand too large", what);
   HMOE_REQUIRE((ceil_div(rows_cap, 64) + n_experts) * ceil_div(ncols, kTileN) <= (int64_t(1) << 30),
                "%s: too many tiles", what);
@@ -803,7 +876,7 @@ int launch_product(const char* what, const uint8_t* a, const uint8_t* a_exp, con
       if (int rc = allow_lds(what, grouped_mxfp4_tiles<bm, GATE_UP, GATHER>, lds, dev, &done)) return rc;
       hipLaunchKernelGGL((grouped_mxfp4_tiles<bm, GATE_UP, GATHER>), dim3(per_cu * cus), dim3(kTileThreads),
                          lds, s, a, a_exp, b, b_exp, offsets, n_experts, kdim, ncols, c, c_exp,
-                         gather_src, gather_k, gather_rows);
+                         gather_src, by_k, gather_rows);
       return check_launch(what);
     };
     return form == kTiles64 ? launch(std::integral_constant<int, 64>{}) : launch(std::integral_constant<int, 128>{});
@@ -811,11 +884,11 @@ int launch_product(const char* what, const uint8_t* a, const uint8_t* a_exp, con
   const unsigned m_tiles = static_cast<unsigned>(max_row_tiles(rows_cap, n_experts));
   if (form == kRows4)
     hipLaunchKernelGGL((grouped_mxfp4_rows<GATE_UP, GATHER, 4>), dim3(ncols / 64, m_tiles), dim3(256), 0, s, a, a_exp,
-                       b, b_exp, offsets, n_experts, kdim, ncols, c, c_exp, gather_src, gather_k, gather_rows);
+                       b, b_exp, offsets, n_experts, kdim, ncols, c, c_exp, gather_src, by_k, gather_rows);
   else
     hipLaunchKernelGGL((grouped_mxfp4_rows<GATE_UP, GATHER, 1>),
                        dim3(static_cast<unsigned>(ceil_div(ncols, 256)), m_tiles), dim3(256), 0, s, a, a_exp, b, b_exp,
-                       offsets, n_experts, kdim, ncols, c, c_exp, gather_src, gather_k, gather_rows);
+                       offsets, n_experts, kdim, ncols, c, c_exp, gather_src, by_k, gather_rows);
   return check_launch(what);
 }
 

@@ -217,13 +217,13 @@ FORMS = [
     # of 256 values
     ((9000, 3, 1, 128, 256), 2, 0),     # half a step a tile
     ((6000, 3, 1, 128, 1280), 2, 1),
-    ((8000, 2, 1, 256, 384), 2, 2),     # one step; one and a half
-    ((3000, 4, 2, 640, 384), 2, 2),     # two and a half
-    ((2600, 2, 2, 512, 1152), 2, 2),    # two; four and a half
-    ((1500, 20, 2, 640, 1152), 2, 2),   # segments that end inside tiles
-    ((4000, 2, 2, 1152, 1152), 3, 3),   # a last column tile of 128
-    ((20000, 2, 1, 384, 896), 3, 2),
-    ((40000, 2, 1, 128, 1152), 3, 3),   # half a step a tile of 128 rows
+    ((8000, 2, 1, 256, 384), 2, 0),     # one step
+    ((3000, 4, 2, 640, 384), 2, 0),     # two and a half
+    ((2600, 2, 2, 512, 1152), 2, 2),    # two; four and a half, a last column tile of 128
+    ((1500, 20, 2, 640, 1152), 2, 0),   # segments that end inside tiles
+    ((7000, 1, 1, 1152, 1152), 3, 2),
+    ((10000, 1, 1, 1152, 640), 3, 3),   # a last column tile of 128
+    ((50000, 1, 1, 128, 1152), 3, 0),   # half a step a tile of 128 rows
 ]
 
 
