@@ -686,6 +686,7 @@ __global__ __launch_bounds__(kTileThreads, BM == 64 ? 3 : 2) void grouped_mxfp4_
     load_b(q);
     if (q & 1) load_eb(q >> 1);
   }
+  fence();
   int turn = blockIdx.x < gridDim.x / 2;  // (workgroups i and i + gridDim / 2 share a CU)
   for (int t = first; t < hi; t += per_xcd) {
     int kb = 0;
