@@ -164,3 +164,26 @@ def test_router_with_quantisation(gpu, T, D, N, wd):
         assert a.dtype == b.dtype and torch.equal(a, b), i
     want_q, want_e = R.quantise(x.float().cpu().numpy())
     assert np.array_equal(got[3].cpu().numpy(), want_q) and np.array_equal(got[4].cpu().numpy(), want_e)
+
+
+def test_module_captured(gpu):
+    """The module in a graph after a first call (which packs the masters), replayed with
+    eager calls between."""
+    layer = MoE(256, 384, 6, 2, 1, 0.02, 1.0, "bfloat16", rngs=0, expert_dtype="mxfp4", device=gpu)
+    x = torch.zeros((2, 150, 256), dtype=torch.bfloat16, device=gpu)
+    with torch.no_grad():
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            layer(x)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out, aux = layer(x)
+        for i in range(4):
+            x.copy_(torch.randn(x.shape, generator=torch.Generator(device=gpu).manual_seed(i), device=gpu))
+            graph.replay()
+            got, counts = out.clone(), aux["expert_counts"].clone()
+            want, want_aux = layer(x)
+            torch.cuda.synchronize()
+            assert torch.equal(got, want) and torch.equal(counts, want_aux["expert_counts"])
