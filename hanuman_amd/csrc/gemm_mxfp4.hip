@@ -637,17 +637,20 @@ __global__ __launch_bounds__(kTileThreads, BM == 64 ? 3 : 2) void grouped_mxfp4_
     read_a(0);
 #pragma unroll
     for (int i = 0; i < kFR; ++i) exw[i] = *reinterpret_cast<const u32x2_t*>(se + i * 512);
+    int ebs[2];
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       if (q < nq) {
         // (kept ahead of the products, or each fragment is waited for)
         if (q + 1 < nq) read_a(q + 1);
         __builtin_amdgcn_sched_barrier(0);
-        int ea[kFR], ebs[2];
+        int ea[kFR];
 #pragma unroll
         for (int i = 0; i < kFR; ++i) ea[i] = static_cast<int>(exw[i][q >> 1] >> (8 * half));
+        if ((q & 1) == 0) {  // (then the words themselves are free)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) ebs[j] = static_cast<int>(eb[q >> 1][j] >> (8 * half));
+          for (int j = 0; j < 2; ++j) ebs[j] = static_cast<int>(eb[q >> 1][j] >> (8 * half));
+        }
         if (q == 0 && kb == 0) {  // (zeros as an operand, not written first)
           const f32x16 zero = {};
 #pragma unroll
@@ -665,7 +668,7 @@ __global__ __launch_bounds__(kTileThreads, BM == 64 ? 3 : 2) void grouped_mxfp4_
       }
       __builtin_amdgcn_sched_barrier(0);
       load_b(q);
-      if (q & 1) load_eb(q >> 1);
+      if ((q & 1) == 0) load_eb(q >> 1);
       fence();
     }
 #pragma unroll
@@ -684,7 +687,7 @@ __global__ __launch_bounds__(kTileThreads, BM == 64 ? 3 : 2) void grouped_mxfp4_
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     load_b(q);
-    if (q & 1) load_eb(q >> 1);
+    if ((q & 1) == 0) load_eb(q >> 1);
   }
   fence();
   int turn = blockIdx.x < gridDim.x / 2;  // (workgroups i and i + gridDim / 2 share a CU)
