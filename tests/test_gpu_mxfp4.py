@@ -432,3 +432,52 @@ def test_zero_rows(gpu):
     assert h_q.shape == (0, 64) and h_e.shape == (0, 4)
     dn = [_to(t[None], gpu) for t in R.packed_operand(*R.quantise(rng.standard_normal((256, 128))))]
     assert K.grouped_down_mxfp4(h_q, h_e, off, *dn).shape == (0, 256)
+
+
+def test_rows_past_32_bits(gpu):
+    """Rows whose codes (2.2 GB) and results (9 GB) lie past 2^31 and 2^32 bytes: the last
+    ones as in a call of their own."""
+    rows, D, F, tail = 2_200_003, 2048, 128, 20_001
+    form = _lib.lib().hmoe_grouped_mxfp4_form
+    assert min(form(rows, 2, D, 2 * F, 256), form(tail, 1, D, 2 * F, 256), form(rows, 2, F, D, 256),
+               form(tail, 1, F, D, 256)) >= 2
+    g = torch.Generator(device=gpu).manual_seed(3)
+    x_q = torch.randint(0, 256, (rows, D // 2), dtype=torch.uint8, device=gpu, generator=g)
+    x_e = torch.randint(120, 128, (rows, D // 32), dtype=torch.uint8, device=gpu, generator=g)
+    gu = K.pack_mxfp4_gate_up(*(torch.randn((2, D, F), device=gpu, generator=g) * 0.05 for _ in range(2)))
+    dn = K.pack_mxfp4_down(torch.randn((2, F, D), device=gpu, generator=g))
+    off = torch.tensor([0, rows - tail, rows], dtype=torch.int32, device=gpu)
+    one = torch.tensor([0, tail], dtype=torch.int32, device=gpu)
+    h_q, h_e = K.grouped_gate_up_mxfp4(x_q, x_e, off, *gu)
+    last = [t[1:].contiguous() for t in gu]
+    w_q, w_e = K.grouped_gate_up_mxfp4(x_q[-tail:].contiguous(), x_e[-tail:].contiguous(), one, *last)
+    assert torch.equal(h_q[-tail:], w_q) and torch.equal(h_e[-tail:], w_e)
+    ys = K.grouped_down_mxfp4(h_q, h_e, off, *dn)
+    want = K.grouped_down_mxfp4(w_q, w_e, one, *(t[1:].contiguous() for t in dn))
+    assert torch.equal(ys[-tail:], want) and bool(want.isfinite().all()) and float(want.float().abs().max()) > 0
+    del ys
+    # and read back, 9 GB
+    back = K.dequantize_rows_mxfp4(x_q, x_e)[-3:]
+    assert torch.equal(back, K.dequantize_rows_mxfp4(x_q[-3:].contiguous(), x_e[-3:].contiguous()))
+
+
+def test_weights_past_32_bits(gpu):
+    """An operand of 4.3 GB: the last experts as in calls of their own."""
+    N, D, F, rows = 1024, 4096, 1024, 40
+    form = _lib.lib().hmoe_grouped_mxfp4_form
+    assert form(rows, N, D, 2 * F, 256) == form(3, 1, D, 2 * F, 256)
+    g = torch.Generator(device=gpu).manual_seed(4)
+    w_q = torch.randint(0, 256, (N, 2 * F // 32, D // 64, 64, 16), dtype=torch.uint8, device=gpu, generator=g)
+    w_e = torch.randint(115, 124, (N, D // 128, 2 * F, 4), dtype=torch.uint8, device=gpu, generator=g)
+    x_q, x_e = K.quantize_rows_mxfp4(torch.randn((rows, D), device=gpu, generator=g))
+    counts = torch.zeros(N, dtype=torch.int64)
+    counts[5], counts[600], counts[1022], counts[1023] = 20, 10, 7, 3
+    off = torch.cat([torch.zeros(1, dtype=torch.int64), counts.cumsum(0)]).to(gpu, torch.int32)
+    h_q, h_e = K.grouped_gate_up_mxfp4(x_q, x_e, off, w_q, w_e)
+    for e in (600, 1022, 1023):
+        lo, hi = int(off[e]), int(off[e + 1])
+        one = torch.tensor([0, hi - lo], dtype=torch.int32, device=gpu)
+        q, x = K.grouped_gate_up_mxfp4(x_q[lo:hi].contiguous(), x_e[lo:hi].contiguous(), one, w_q[e:e + 1], w_e[e:e + 1])
+        assert torch.equal(h_q[lo:hi], q) and torch.equal(h_e[lo:hi], x), e
+    back = K.unpack_mxfp4(w_q, w_e)
+    assert torch.equal(back[-1], K.unpack_mxfp4(w_q[-1:], w_e[-1:])[0])
