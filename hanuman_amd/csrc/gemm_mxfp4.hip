@@ -349,9 +349,9 @@ __global__ __launch_bounds__(256) void grouped_mxfp4_rows(
 // Gate/up of 131072 rows, D 2048, F 1024 (1.1 TFLOP) takes 285 us, down 165 us.  What bounds
 // them is power: with these operands the matrix cores alone, fed from registers, run at
 // 1.65 GHz and 6.5 PFLOP/s (170 us), and with operands of zeros, at 2.4 GHz, the same
-// launches take 205 and 119 us.  In cycles it is what a CU has to do besides: a step's
-// loads come at 40 bytes a cycle and CU, and alone in its loop, while the other is in its
-// epilogue (4.6 thousand of 23 thousand cycles), a workgroup reaches half the rate.
+// launches take 205 and 119 us (the products alone 113 and 57).  In cycles it is what a CU
+// has to do besides: gate/up with zeros takes 170 us with the products taken out, 161 with
+// all loads and reads taken out instead, 198 with every load a hit of the first cache.
 // Measured and not taken (us; gate/up and down, before the turns 300 and 170): B through LDS
 // too (2 x 2 waves, steps of 128 values, three stages) 326 and 187, an LDS and half lines of
 // A that kept pace with the products at best; one workgroup of eight waves on 128 x 512 301
@@ -457,19 +457,21 @@ struct TileCursor {
       before += total;
     }
   }
-  // On to tile t (t grows from call to call).
-  __device__ __forceinline__ void move(const int32_t* __restrict__ offsets, int t, int n_tiles_n) {
-    const int m_any = t / n_tiles_n;
+  // On to tile t (t grows from call to call; by_cols, by_group: the column tiles, a group's
+  // tiles).
+  __device__ __forceinline__ void move(const int32_t* __restrict__ offsets, int t, int n_tiles_n, Divisor by_cols,
+                                       Divisor by_group) {
+    const int m_any = divide(t, by_cols);
     while (m_any >= before + tiles) {
       before += tiles;
       expert(offsets, e + 1);
     }
     const int u = t - before * n_tiles_n;
-    const int g = u / (kTileGroup * n_tiles_n);
+    const int g = divide(u, by_group);
     const int left = tiles - g * kTileGroup;
     const int gm = left < kTileGroup ? left : kTileGroup;
     const int v = u - g * kTileGroup * n_tiles_n;
-    const int n_tile = v / gm;
+    const int n_tile = gm == kTileGroup ? v / kTileGroup : v / gm;
     row0 = seg0 + (g * kTileGroup + (v - n_tile * gm)) * BM;
     rows = seg1 - row0 < BM ? seg1 - row0 : BM;
     n0 = n_tile * kTileN;
@@ -481,7 +483,7 @@ __global__ __launch_bounds__(kTileThreads, BM == 64 ? 3 : 2) void grouped_mxfp4_
     const uint8_t* __restrict__ A, const uint8_t* __restrict__ a_exp, const uint8_t* __restrict__ B,
     const uint8_t* __restrict__ b_exp, const int32_t* __restrict__ offsets, int n_experts, int kdim, int ncols,
     uint8_t* __restrict__ C, uint8_t* __restrict__ c_exp, const int32_t* __restrict__ gather_src,
-    Divisor gather_k, int gather_rows) {
+    Divisor gather_k, int gather_rows, Divisor by_cols, Divisor by_group) {
   typedef TileCfg<BM, GATE_UP> Cfg;
   constexpr int kFR = Cfg::kFR;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
@@ -505,7 +507,7 @@ __global__ __launch_bounds__(kTileThreads, BM == 64 ? 3 : 2) void grouped_mxfp4_
   // A: instruction j of wave w fills rows (BM / 4) w + 8 j + lane / 8, chunk (lane & 7) ^
   // swz128(row) of the row's 128 bytes.
   TileCursor<BM> ld;
-  ld.find(offsets, n_experts, first / n_tiles_n);
+  ld.find(offsets, n_experts, divide(first, by_cols));
   TileCursor<BM> cur = ld, nx = ld;
   const int a_row = (BM / 4) * wave + (lane >> 3);
   __amdgpu_buffer_rsrc_t a_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(A), 0,
@@ -541,10 +543,10 @@ __global__ __launch_bounds__(kTileThreads, BM == 64 ? 3 : 2) void grouped_mxfp4_
 #pragma unroll
       for (int j = 0; j < kFR; ++j) a_voff[j] = token(pf_src[j]) * static_cast<uint32_t>(row_bytes) + a_byte(j);
       ae_voff = token(pf_ex) * static_cast<uint32_t>(ex_bytes);
-      if (ld_t + per_xcd < hi) nx.move(offsets, ld_t + per_xcd, n_tiles_n);
+      if (ld_t + per_xcd < hi) nx.move(offsets, ld_t + per_xcd, n_tiles_n, by_cols, by_group);
       fetch_src();  // (on every path: a load that may not be issued is waited for at once)
     } else {
-      ld.move(offsets, ld_t, n_tiles_n);
+      ld.move(offsets, ld_t, n_tiles_n, by_cols, by_group);
       // rows past the segment repeat its last one; their results are not stored
       a_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(A + static_cast<int64_t>(ld.row0) * row_bytes),
                                                  0, ld.rows * row_bytes, kBufferWord3);
@@ -679,7 +681,7 @@ __global__ __launch_bounds__(kTileThreads, BM == 64 ? 3 : 2) void grouped_mxfp4_
   };
 
   if (GATHER) {
-    nx.move(offsets, first, n_tiles_n);
+    nx.move(offsets, first, n_tiles_n, by_cols, by_group);
     fetch_src();
   }
   set_load_tile();
@@ -696,7 +698,7 @@ __global__ __launch_bounds__(kTileThreads, BM == 64 ? 3 : 2) void grouped_mxfp4_
     if (BM == 128) take_turn(turn ^= 1);
     for (; 2 * kb + 1 < ks; ++kb) step(kb, std::integral_constant<int, 4>{});
     if (2 * kb < ks) step(kb, std::integral_constant<int, 2>{});  // 128 values
-    cur.move(offsets, t, n_tiles_n);
+    cur.move(offsets, t, n_tiles_n, by_cols, by_group);
     const int64_t r0 = cur.row0;
     if constexpr (GATE_UP) {
       const int d_ff = ncols / 2;
@@ -876,11 +878,13 @@ int launch_product(const char* what, const uint8_t* a, const uint8_t* a_exp, con
     const auto launch = [&](auto BM) {
       constexpr int bm = decltype(BM)::value;
       constexpr int lds = TileCfg<bm, GATE_UP>::kLds, per_cu = TileCfg<bm, GATE_UP>::kPerCu;
+      const int n_tiles_n = static_cast<int>(ceil_div(ncols, kTileN));
+      const Divisor by_cols = divisor(n_tiles_n), by_group = divisor(kTileGroup * n_tiles_n);
       static std::atomic<uint64_t> done{0};
       if (int rc = allow_lds(what, grouped_mxfp4_tiles<bm, GATE_UP, GATHER>, lds, dev, &done)) return rc;
       hipLaunchKernelGGL((grouped_mxfp4_tiles<bm, GATE_UP, GATHER>), dim3(per_cu * cus), dim3(kTileThreads),
                          lds, s, a, a_exp, b, b_exp, offsets, n_experts, kdim, ncols, c, c_exp,
-                         gather_src, by_k, gather_rows);
+                         gather_src, by_k, gather_rows, by_cols, by_group);
       return check_launch(what);
     };
     return form == kTiles64 ? launch(std::integral_constant<int, 64>{}) : launch(std::integral_constant<int, 128>{});
