@@ -834,7 +834,8 @@ def _check_i32(name: str, what: str, t: torch.Tensor, numel: int, dev):
         return
     _check(t, what)
     _same_device(name, t, dev)
-    raise ValueError(f"{name}: {what} must be int32 [{numel}]")
+    if t.dtype != torch.int32 or t.numel() != numel:
+        raise ValueError(f"{name}: {what} must be int32 [{numel}]")
 
 
 def grouped_gate_up_mxfp4(xs_q: torch.Tensor, xs_exp: torch.Tensor, offsets: torch.Tensor,
