@@ -26,6 +26,7 @@ namespace {
 
 constexpr int kMaxExperts = 1024;
 constexpr int64_t kMaxRows = int64_t(1) << 30;
+constexpr int kMaxDim = 1 << 20;  // of D and F
 constexpr int kBufferWord3 = 0x00020000;
 constexpr int kNonTemporal = 2;  // cache policy of a buffer access
 
@@ -798,11 +799,19 @@ int check_product(const char* what, int n_experts, int64_t rows_cap, int d_model
                kMaxExperts, n_experts);
   // (2^30: a tile's rows and the tiles that a workgroup steps over are added in 32 bits)
   HMOE_REQUIRE(rows_cap >= 0 && rows_cap <= kMaxRows, "%s: rows_cap must be in [0, 2^30]", what);
-  HMOE_REQUIRE_CODE(d_model >= 128 && d_model % 128 == 0 && d_model <= (1 << 20), HMOE_ERR_UNSUPPORTED,
+  HMOE_REQUIRE_CODE(d_model >= 128 && d_model % 128 == 0 && d_model <= kMaxDim, HMOE_ERR_UNSUPPORTED,
                     "%s: d_model must be a multiple of 128 up to 2^20 (got %d)", what, d_model);
-  HMOE_REQUIRE_CODE(d_ff >= 128 && d_ff % 128 == 0 && d_ff <= (1 << 20), HMOE_ERR_UNSUPPORTED,
+  HMOE_REQUIRE_CODE(d_ff >= 128 && d_ff % 128 == 0 && d_ff <= kMaxDim, HMOE_ERR_UNSUPPORTED,
                     "%s: d_ff must be a multiple of 128 up to 2^20 (got %d)", what, d_ff);
   return HMOE_OK;
+}
+
+// What a launch cannot count in 32 bits, beyond the sizes that check_product looks at: an
+// expert's exponents in bytes, the tiles of the smaller tile form.
+const char* too_large(int64_t rows_cap, int n_experts, int kdim, int ncols) {
+  if (static_cast<int64_t>(kdim / 128) * ncols * 4 >= (int64_t(1) << 31)) return "operand too large";
+  if ((ceil_div(rows_cap, 64) + n_experts) * ceil_div(ncols, kTileN) > (int64_t(1) << 30)) return "too many tiles";
+  return nullptr;
 }
 
 // Which kernel a product takes: the one with the least estimated time, from measured
@@ -868,9 +877,8 @@ int launch_product(const char* what, const uint8_t* a, const uint8_t* a_exp, con
                    int ncols, uint8_t* c, uint8_t* c_exp, const int32_t* gather_src, int gather_k,
                    int gather_rows, hipStream_t s) {
   const Divisor by_k = divisor(gather_k);
-  HMOE_REQUIRE(static_cast<int64_t>(kdim / 128) * ncols * 4 < (int64_t(1) << 31), "%s: operand too large", what);
-  HMOE_REQUIRE((ceil_div(rows_cap, 64) + n_experts) * ceil_div(ncols, kTileN) <= (int64_t(1) << 30),
-               "%s: too many tiles", what);
+  const char* limit = too_large(rows_cap, n_experts, kdim, ncols);
+  HMOE_REQUIRE(limit == nullptr, "%s: %s", what, limit);
   int dev = 0, cus = 0;
   if (int rc = persistent_grid(what, s, &cus, &dev)) return rc;
   const Form form = choose_form(rows_cap, n_experts, kdim, ncols, cus);
@@ -906,7 +914,8 @@ int launch_product(const char* what, const uint8_t* a, const uint8_t* a_exp, con
 extern "C" int64_t hmoe_grouped_mxfp4_form(int64_t rows_cap, int n_experts, int kdim, int ncols, int cus) {
   using namespace hmoe;
   if (rows_cap < 1 || rows_cap > kMaxRows || n_experts < 1 || n_experts > kMaxExperts || cus < 1 || kdim < 128 ||
-      kdim % 128 != 0 || ncols < 128 || ncols % 128 != 0) {
+      kdim % 128 != 0 || kdim > kMaxDim || ncols < 128 || ncols % 128 != 0 || ncols > 2 * kMaxDim ||
+      too_large(rows_cap, n_experts, kdim, ncols) != nullptr) {
     set_error("grouped_mxfp4_form: sizes that the products refuse");
     return -1;
   }

@@ -434,8 +434,9 @@ int hmoe_unpack_mxfp4(const uint8_t* packed, const uint8_t* exps, int n_experts,
 /* The form in which the products below run `kdim` values of the reduction and `ncols`
  * columns (gate/up: 2 d_ff) on a device of `cus` CUs: 0 and 1, 32 rows from memory into
  * registers, the reduction split over four waves in 1; 2 and 3, tiles of 64 and 128 rows
- * through LDS.  -1 for sizes that they refuse.  A host-side query.  Forms 0, 2 and 3 sum
- * in the same order and give the same bits; 1 adds four parts. */
+ * through LDS.  -1 for sizes that they refuse (ncols: up to 2^20, gate/up 2^21) and for no
+ * rows.  A host-side query.  Forms 0, 2 and 3 sum in the same order and give the same bits;
+ * 1 adds four parts. */
 int64_t hmoe_grouped_mxfp4_form(int64_t rows_cap, int n_experts, int kdim, int ncols, int cus);
 
 /* h of rows r of expert e's segment [offsets[e], offsets[e+1]) as MXFP4 rows: with
@@ -443,7 +444,8 @@ int64_t hmoe_grouped_mxfp4_form(int64_t rows_cap, int n_experts, int kdim, int n
  * and quantised from there (h is rounded once, to its codes).  xs_q [rows_cap, D/2],
  * xs_exp [rows_cap, D/32], h_q [rows_cap, F/2], h_exp [rows_cap, F/32].  Rows past
  * offsets[N] are not written.  D % 128 == 0, F % 128 == 0, both up to 2^20, N <= 1024,
- * rows_cap <= 2^30. */
+ * rows_cap <= 2^30; an expert's exponents below 2^31 bytes (D * F < 2^35, down 2^36), and
+ * (rows_cap / 64 + N) * (2F / 256, down D / 256), each rounded up, at most 2^30. */
 int hmoe_grouped_gate_up_mxfp4(const uint8_t* xs_q, const uint8_t* xs_exp, const int32_t* offsets,
                                int n_experts, int64_t rows_cap, int d_model, int d_ff,
                                const uint8_t* w_packed, const uint8_t* w_exp, uint8_t* h_q,
