@@ -191,6 +191,9 @@ __device__ __forceinline__ void store_y_block(const f32x16& y, __amdgpu_buffer_r
   __builtin_amdgcn_raw_buffer_store_b128(hi, out, off + 32, 0, 0);
 }
 
+// Memory accesses are not moved past it by the compiler.
+__device__ __forceinline__ void order_memory() { asm volatile("" ::: "memory"); }
+
 // Two blocks side by side (64 columns, 32 rows), through 4 KB of LDS that only this
 // wave uses, so that a store instruction writes whole 128-byte lines: chunk c of row r
 // sits at c ^ (r & 7).  ys is far larger than the caches where tiles are taken, and kept
@@ -208,12 +211,14 @@ __device__ __forceinline__ void store_y_blocks(const f32x16& y0, const f32x16& y
     *reinterpret_cast<u32x4*>(p + (((4 * j + half) ^ (r & 7)) * 16)) = lo;
     *reinterpret_cast<u32x4*>(p + (((4 * j + 2 + half) ^ (r & 7)) * 16)) = hi;
   }
+  order_memory();  // (a lane reads what others wrote; a wave's LDS accesses run in their order)
 #pragma unroll
   for (int m = 0; m < 4; ++m) {
     const int rr = 8 * m + (lane >> 3);
     const u32x4 v = *reinterpret_cast<const u32x4*>(lds + rr * 128 + (((lane & 7) ^ (rr & 7)) * 16));
     __builtin_amdgcn_raw_buffer_store_b128(v, out, ((row0 + rr) * ldc + col + (lane & 7) * 8) * 2, 0, kNonTemporal);
   }
+  order_memory();  // (the next blocks' writes stay behind these reads)
 }
 
 // ---- few rows ---------------------------------------------------------------------
@@ -387,9 +392,9 @@ __device__ __forceinline__ void use_here(const f32x16& v) { asm volatile("" ::"v
 
 __device__ __forceinline__ int swz128(int r) { return (r >> 1) & 7; }
 
-// Memory accesses are not moved past it by the compiler.
+// order_memory, for instructions of every kind.
 __device__ __forceinline__ void fence() {
-  asm volatile("" ::: "memory");
+  order_memory();
   __builtin_amdgcn_sched_barrier(0);
 }
 
@@ -719,6 +724,7 @@ __global__ __launch_bounds__(kTileThreads, BM == 64 ? 3 : 2) void grouped_mxfp4_
         *reinterpret_cast<u32x2_t*>(codes + (32 * i + frow) * 64 + wave * 16 + half * 8) = join_codes(sw[0], sw[1]);
         if (half == 0) exps[(32 * i + frow) * 4 + wave] = static_cast<uint8_t>(e);
       }
+      fence();  // (the wait and the barrier are no memory accesses to the compiler)
       wait_lgkm0();
       __builtin_amdgcn_s_barrier();
       fence();
@@ -746,6 +752,7 @@ __global__ __launch_bounds__(kTileThreads, BM == 64 ? 3 : 2) void grouped_mxfp4_
       for (int i = 0; i < kFR; ++i)
         if (mine) store_y_blocks(acc[i][0], acc[i][1], lds, out, 32 * i, cur.n0 + wave * 64, ncols, lane);
     }
+    fence();  // (this tile's reads of LDS stay ahead of the next step's barrier)
   }
   // nothing may still be writing into LDS when the workgroup ends
   __builtin_amdgcn_s_waitcnt(0);

@@ -1,0 +1,85 @@
+"""The MXFP4 products in the forms that carry large calls: each test says which form its
+sizes take, and asserts it.  Forms 0 (32 rows a wave, from memory), 2 and 3 (tiles of 64 and
+128 rows through LDS) sum in the same order, so that pieces of a few rows give the tiles'
+bits; form 1 adds four parts and is held to float64."""
+import numpy as np
+import pytest
+import torch
+
+import mxfp4_reference as R
+from hanuman_amd import _lib, kernels as K
+from test_gpu_mxfp4 import _case, _check_down, _check_gate_up
+
+pytestmark = pytest.mark.gpu
+
+TILES = [2, 3]
+PIECE = 96
+
+
+def _form(gpu, rows, experts, kdim, ncols):
+    cus = torch.cuda.get_device_properties(gpu).multi_processor_count // 8 * 8
+    return _lib.lib().hmoe_grouped_mxfp4_form(rows, experts, kdim, ncols, cus)
+
+
+def _randn(gpu, seed, *shape):
+    return torch.randn(shape, generator=torch.Generator(device=gpu).manual_seed(seed), device=gpu)
+
+
+def _gate_up_operand(gpu, experts, d_model, d_ff):
+    return K.pack_mxfp4_gate_up(*(_randn(gpu, 70 + i, experts, d_model, d_ff) * 0.05 for i in range(2)))
+
+
+def _down_operand(gpu, experts, d_ff, d_model):
+    return K.pack_mxfp4_down(_randn(gpu, 80, experts, d_ff, d_model) * 0.05)
+
+
+def _in_pieces(gpu, product, q, exps, offsets, packed, packed_exp):
+    """The product of every segment, a few rows of one expert a call, on form 0."""
+    off = offsets.tolist()
+    kdim, ncols = q.shape[1] * 2, packed.shape[1] * 32
+    assert _form(gpu, PIECE, 1, kdim, ncols) == 0
+    outs = []
+    for e, (lo, hi) in enumerate(zip(off, off[1:])):
+        for r in range(lo, hi, PIECE):
+            n = min(PIECE, hi - r)
+            one = torch.tensor([0, n], dtype=torch.int32, device=gpu)
+            out = product(q[r:r + n].clone(), exps[r:r + n].clone(), one, packed[e:e + 1], packed_exp[e:e + 1])
+            outs.append(out if isinstance(out, tuple) else (out,))
+    return [torch.cat(t) for t in zip(*outs)]
+
+
+def _raw_gate_up(x_q, x_e, offsets, gu, h_q, h_e):
+    N, D, F = gu[0].shape[0], gu[0].shape[2] * 64, gu[0].shape[1] * 16
+    _lib.call("hmoe_grouped_gate_up_mxfp4", x_q.data_ptr(), x_e.data_ptr(), offsets.data_ptr(), N, h_q.shape[0], D, F,
+              gu[0].data_ptr(), gu[1].data_ptr(), h_q.data_ptr(), h_e.data_ptr(),
+              torch.cuda.current_stream().cuda_stream)
+
+
+@pytest.mark.parametrize("rows,experts,d_model,d_ff,gate_up,down", [
+    (12000, 3, 256, 1152, 2, 2),      # gate/up: one step of 256 a tile
+    (12000, 3, 128, 1152, 2, 2),      # half a step
+    (60000, 3, 256, 1152, 3, 3),
+    (60000, 3, 128, 1152, 3, 3),
+    (12000, 3, 2048, 256, 3, 2),      # down: one step
+    (60000, 3, 2048, 256, 3, 3),
+    (60000, 3, 2048, 128, 3, 3),      # half a step
+], ids=lambda v: str(v))
+def test_tiles_back_to_back(gpu, rows, experts, d_model, d_ff, gate_up, down):
+    """Tiles of a step or less, many a workgroup: what a tile puts into LDS for its rows'
+    ends follows the last tile's at once.  Against pieces of few rows, bit for bit."""
+    assert _form(gpu, rows, experts, d_model, 2 * d_ff) == gate_up
+    assert _form(gpu, rows, experts, d_ff, d_model) == down
+    off = torch.tensor([0, rows // 3 + 5, rows // 3 + 5 + rows // 2, rows], dtype=torch.int32, device=gpu)
+    if d_model <= 256:
+        x_q, x_e = K.quantize_rows_mxfp4(_randn(gpu, 1, rows, d_model))
+        gu = _gate_up_operand(gpu, experts, d_model, d_ff)
+        want = _in_pieces(gpu, K.grouped_gate_up_mxfp4, x_q, x_e, off, *gu)
+        for _ in range(3):
+            got = K.grouped_gate_up_mxfp4(x_q, x_e, off, *gu)
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    else:
+        h_q, h_e = K.quantize_rows_mxfp4(_randn(gpu, 2, rows, d_ff))
+        dn = _down_operand(gpu, experts, d_ff, d_model)
+        want, = _in_pieces(gpu, K.grouped_down_mxfp4, h_q, h_e, off, *dn)
+        for _ in range(3):
+            assert torch.equal(K.grouped_down_mxfp4(h_q, h_e, off, *dn), want)
