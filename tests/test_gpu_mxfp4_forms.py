@@ -83,3 +83,74 @@ def test_tiles_back_to_back(gpu, rows, experts, d_model, d_ff, gate_up, down):
         want, = _in_pieces(gpu, K.grouped_down_mxfp4, h_q, h_e, off, *dn)
         for _ in range(3):
             assert torch.equal(K.grouped_down_mxfp4(h_q, h_e, off, *dn), want)
+
+
+# ------------------------------------------------------- against float64 --
+
+def _float64(gpu, shape, seed, **kw):
+    """A layer's gathered gate/up and down products against float64, the gathered rows
+    against rows in the experts' order, and the plan."""
+    tokens, experts, active, d_model, d_ff = shape
+    x, plan, (gu_w, dn_w), (gu, dn) = _case(*shape, seed=seed, gpu=gpu, **kw)
+    x_q, x_e = K.quantize_rows_mxfp4(x.to(gpu))
+    h_q, h_e = K.grouped_gate_up_mxfp4_gather(x_q, x_e, plan, *gu)
+    _check_gate_up(h_q, h_e, R.values(x_q.cpu().numpy(), x_e.cpu().numpy()), plan, gu_w, d_ff, active)
+    kept = int(plan.offsets[-1])
+    src = (plan.perm_src.long() // active).clamp(min=0)
+    g_q, g_e = K.grouped_gate_up_mxfp4(x_q[src], x_e[src], plan.offsets, *gu)
+    assert torch.equal(g_q[:kept], h_q[:kept]) and torch.equal(g_e[:kept], h_e[:kept])
+    ys = K.grouped_down_mxfp4(h_q, h_e, plan.offsets, *dn)
+    _check_down(ys, R.values(h_q[:kept].cpu().numpy(), h_e[:kept].cpu().numpy()), plan.offsets.cpu().numpy(), dn_w)
+    return plan
+
+
+@pytest.mark.parametrize("shape,gate_up,down", [
+    ((12000, 3, 2, 640, 640), 3, 2),        # gathered, several experts, 128 rows a tile
+    ((14000, 12, 2, 640, 640), 2, 3),
+    ((3000, 70, 4, 384, 640), 2, 2),        # more experts than a wave has lanes
+    ((20000, 70, 2, 640, 640), 3, 2),
+    ((6000, 70, 2, 640, 256), 2, 2),
+    ((40, 4, 2, 2048, 2048), 1, 1),         # four groups of a wave's reduction at a time
+    ((9, 3, 2, 2176, 4224), 1, 1),          # and five, and nine
+], ids=lambda v: "x".join(map(str, v)) if isinstance(v, tuple) else str(v))
+def test_many_experts(gpu, shape, gate_up, down):
+    tokens, experts, active, d_model, d_ff = shape
+    assert _form(gpu, tokens * active, experts, d_model, 2 * d_ff) == gate_up
+    assert _form(gpu, tokens * active, experts, d_ff, d_model) == down
+    _float64(gpu, shape, seed=sum(shape))
+
+
+@pytest.mark.parametrize("shape,skew,gate_up,down", [
+    ((9000, 9, 1, 640, 640), 4.0, 2, 2),
+    ((12000, 6, 1, 640, 640), 4.0, 3, 2),
+    ((20000, 6, 1, 640, 640), 4.0, 2, 3),
+    ((12000, 12, 1, 640, 1152), 2.0, 2, 2),
+], ids=lambda v: "x".join(map(str, v)) if isinstance(v, tuple) else str(v))
+def test_skewed_experts(gpu, shape, skew, gate_up, down):
+    """Nearly all rows on the first experts, the last ones empty, segments of a few rows
+    between."""
+    tokens, experts, active, d_model, d_ff = shape
+    assert _form(gpu, tokens * active, experts, d_model, 2 * d_ff) == gate_up
+    assert _form(gpu, tokens * active, experts, d_ff, d_model) == down
+    plan = _float64(gpu, shape, seed=5, skew=skew)
+    counts = plan.counts.tolist()
+    assert 0 in counts and any(0 < c < 64 for c in counts)
+
+
+@pytest.mark.parametrize("where", ["first", "middle", "last"])
+@pytest.mark.parametrize("form", TILES)
+def test_experts_without_rows(gpu, form, where):
+    """66 experts, rows on three only, the others empty before, between and after them."""
+    rows, D, F = {2: 9000, 3: 60000}[form], 256, 1152
+    N = 66
+    assert _form(gpu, rows, N, D, 2 * F) == form
+    live = {"first": (0, 1, 2), "middle": (0, 63, 65), "last": (63, 64, 65)}[where]
+    counts = torch.zeros(N, dtype=torch.int64)
+    for e, c in zip(live, (rows - 3001, 3000, 1)):
+        counts[e] = c
+    off = torch.cat([torch.zeros(1, dtype=torch.int64), counts.cumsum(0)]).to(gpu, torch.int32)
+    x_q, x_e = K.quantize_rows_mxfp4(_randn(gpu, 1, rows, D))
+    gu = _gate_up_operand(gpu, N, D, F)
+    got = K.grouped_gate_up_mxfp4(x_q, x_e, off, *gu)
+    want = _in_pieces(gpu, K.grouped_gate_up_mxfp4, x_q, x_e, off, *gu)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
