@@ -154,3 +154,126 @@ def test_experts_without_rows(gpu, form, where):
     got = K.grouped_gate_up_mxfp4(x_q, x_e, off, *gu)
     want = _in_pieces(gpu, K.grouped_gate_up_mxfp4, x_q, x_e, off, *gu)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+# ---------------------------------------------------- what rows may be like --
+
+ROWS = {2: 12000, 3: 30000}     # of 4 experts: reductions of 384, 1152 columns of h or ys
+
+
+def _edge_sizes(gpu, form):
+    """Rows, experts and the sizes (D, F) whose gate/up and (F, D) whose down take `form`."""
+    rows, N, K_, cols = ROWS[form], 4, 384, 1152
+    assert _form(gpu, rows, N, K_, 2 * cols) == form and _form(gpu, rows, N, K_, cols) == form
+    return rows, N, K_, cols
+
+
+@pytest.mark.parametrize("form", TILES)
+def test_rows_past_the_segments_stay(gpu, form):
+    """Buffers with more rows than the segments, which end inside tiles: the others are left
+    as they were."""
+    rows, N, K_, cols = _edge_sizes(gpu, form)
+    kept = rows - 777
+    off = torch.tensor([0, 1, 1, kept // 2 + 7, kept], dtype=torch.int32, device=gpu)
+    q, e = K.quantize_rows_mxfp4(_randn(gpu, 1, rows, K_))
+    gu, dn = _gate_up_operand(gpu, N, K_, cols), _down_operand(gpu, N, K_, cols)
+    h_q = torch.full((rows, cols // 2), 0xA5, dtype=torch.uint8, device=gpu)
+    h_e = torch.full((rows, cols // 32), 0xA5, dtype=torch.uint8, device=gpu)
+    _raw_gate_up(q, e, off, gu, h_q, h_e)
+    want = _in_pieces(gpu, K.grouped_gate_up_mxfp4, q, e, off, *gu)
+    assert torch.equal(h_q[:kept], want[0]) and torch.equal(h_e[:kept], want[1])
+    assert (h_q[kept:] == 0xA5).all() and (h_e[kept:] == 0xA5).all()
+    ys = torch.full((rows, cols), 7.0, dtype=torch.bfloat16, device=gpu)
+    _lib.call("hmoe_grouped_down_mxfp4", q.data_ptr(), e.data_ptr(), off.data_ptr(), N, rows, K_, cols,
+              dn[0].data_ptr(), dn[1].data_ptr(), ys.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    want, = _in_pieces(gpu, K.grouped_down_mxfp4, q, e, off, *dn)
+    assert torch.equal(ys[:kept], want) and (ys[kept:] == 7.0).all()
+
+
+@pytest.mark.parametrize("start", [1, 3, 4])
+@pytest.mark.parametrize("form", TILES)
+def test_rows_inside_a_buffer(gpu, form, start):
+    """Rows that start at a later row of their buffers: codes at 16 bytes, exponents at words
+    only.  The rows before and behind hold NaN, which no result may show."""
+    rows, N, K_, cols = _edge_sizes(gpu, form)
+    off = torch.tensor([0, 5000, 5001, rows - 64, rows], dtype=torch.int32, device=gpu)
+    q, e = K.quantize_rows_mxfp4(_randn(gpu, 3, rows + start + 2, K_))
+    e[:start] = 255
+    e[start + rows:] = 255
+    a_q, a_e = q[start:start + rows], e[start:start + rows]
+    assert a_e.data_ptr() % 16 == start * 12 % 16 and a_q.data_ptr() % 16 == 0
+    gu, dn = _gate_up_operand(gpu, N, K_, cols), _down_operand(gpu, N, K_, cols)
+    got = K.grouped_gate_up_mxfp4(a_q, a_e, off, *gu)
+    want = _in_pieces(gpu, K.grouped_gate_up_mxfp4, a_q, a_e, off, *gu)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and (got[1] < 255).all()
+    ys = K.grouped_down_mxfp4(a_q, a_e, off, *dn)
+    assert torch.equal(ys, _in_pieces(gpu, K.grouped_down_mxfp4, a_q, a_e, off, *dn)[0]) and ys.isfinite().all()
+    # gathered from tokens that start there
+    src = torch.randperm(rows, generator=torch.Generator().manual_seed(1)).to(gpu, torch.int32)
+    plan = K.Plan(off.diff(), off, src.clone(), src, torch.ones(rows, dtype=torch.uint8, device=gpu), rows, rows, N, 1)
+    got = K.grouped_gate_up_mxfp4_gather(a_q, a_e, plan, *gu)
+    want = K.grouped_gate_up_mxfp4(a_q[src.long()], a_e[src.long()], off, *gu)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("form", TILES)
+def test_dropped_slots(gpu, form):
+    """A capacity that drops slots, so that the segments end before the rows do."""
+    rows, N, K_, cols = _edge_sizes(gpu, form)
+    tokens = rows // 2
+    gen = torch.Generator(device=gpu).manual_seed(6)
+    logits = torch.randn((tokens, N), generator=gen, device=gpu) - 1.5 * torch.arange(N, device=gpu)
+    top = logits.topk(2, dim=1).indices.int()
+    plan = K.dispatch_plan(top, N, rows // 3)
+    kept = int(plan.offsets[-1])
+    assert kept < plan.rows_cap and _form(gpu, plan.rows_cap, N, K_, 2 * cols) == form
+    x_q, x_e = K.quantize_rows_mxfp4(_randn(gpu, 4, tokens, K_))
+    gu = _gate_up_operand(gpu, N, K_, cols)
+    h_q = torch.full((plan.rows_cap, cols // 2), 0xA5, dtype=torch.uint8, device=gpu)
+    h_e = torch.full((plan.rows_cap, cols // 32), 0xA5, dtype=torch.uint8, device=gpu)
+    _lib.call("hmoe_grouped_gate_up_mxfp4_gather", x_q.data_ptr(), x_e.data_ptr(), tokens, 2, plan.perm_src.data_ptr(),
+              plan.offsets.data_ptr(), N, plan.rows_cap, K_, cols, gu[0].data_ptr(), gu[1].data_ptr(), h_q.data_ptr(),
+              h_e.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    src = plan.perm_src[:kept].long() // 2
+    want = _in_pieces(gpu, K.grouped_gate_up_mxfp4, x_q[src], x_e[src], plan.offsets, *gu)
+    assert torch.equal(h_q[:kept], want[0]) and torch.equal(h_e[:kept], want[1])
+    assert (h_q[kept:] == 0xA5).all() and (h_e[kept:] == 0xA5).all()
+
+
+@pytest.mark.parametrize("form", TILES)
+def test_nan_tokens(gpu, form):
+    """Tokens with a value that is not finite: their rows are NaN through both products, all
+    others as if they had been zeros."""
+    rows, N, K_, cols = _edge_sizes(gpu, form)
+    tokens = rows // 2
+    assert _form(gpu, rows, N, cols, K_) == form
+    x = _randn(gpu, 7, tokens, K_)
+    zeros = x.clone()
+    for t, c, v in ((3, 100, float("nan")), (17, 0, float("inf")), (tokens // 2, 383, float("-inf")), (tokens - 1, 31, float("nan"))):
+        x[t, c] = v
+        zeros[t] = 0
+    top = _randn(gpu, 8, tokens, N).topk(2, dim=1).indices.int()
+    plan = K.dispatch_plan(top, N, rows)
+    gu, dn = _gate_up_operand(gpu, N, K_, cols), _down_operand(gpu, N, cols, K_)
+
+    def run(v):
+        h = K.grouped_gate_up_mxfp4_gather(*K.quantize_rows_mxfp4(v), plan, *gu)
+        return (*h, K.grouped_down_mxfp4(*h, plan.offsets, *dn))
+
+    (h_q, h_e, ys), (z_q, z_e, zs) = run(x), run(zeros)
+    bad = ~x.isfinite().all(1)[plan.perm_src.long() // 2]
+    assert int(bad.sum()) == 8
+    assert (h_e[bad] == 255).all() and (h_q[bad] == 0).all() and ys[bad].isnan().all()
+    assert torch.equal(h_q[~bad], z_q[~bad]) and torch.equal(h_e[~bad], z_e[~bad]) and torch.equal(ys[~bad], zs[~bad])
+    assert ys[~bad].isfinite().all()
+
+
+def test_offsets_of_a_subclass(gpu):
+    """Index arrays that a module holds as parameters."""
+    off = torch.tensor([0, 5, 9], dtype=torch.int32, device=gpu)
+    q, e = K.quantize_rows_mxfp4(_randn(gpu, 1, 9, 256))
+    dn = _down_operand(gpu, 2, 256, 128)
+    held = torch.nn.Parameter(off, requires_grad=False)
+    assert torch.equal(K.grouped_down_mxfp4(q, e, held, *dn), K.grouped_down_mxfp4(q, e, off, *dn))
+    with pytest.raises(ValueError, match=r"offsets must be int32 \[3\]"):
+        K.grouped_down_mxfp4(q, e, torch.nn.Parameter(off[:2].clone(), requires_grad=False), *dn)
