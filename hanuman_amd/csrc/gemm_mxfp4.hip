@@ -40,8 +40,11 @@ __device__ __forceinline__ uint32_t pack_bf16x2_rne(float lo, float hi) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2_t));
 }
 
-// silu(g) u; the hardware's exponential and reciprocal are off by about one
-// float32 step each.
+// silu(g) u, off by at most (1.25 |g| + 8) 2^-24 of itself: the exponential's argument g
+// log2(e) is rounded once, a quarter more is log2(e)'s own rounding, and the hardware's
+// exponential and reciprocal are good to a float32 step, the sum and products to half a one.
+// Below g = -87.3 (1 + e^-g past 2^126) the reciprocal is subnormal and may come out as
+// zero: up to |g u| 2^-126 is lost there.  Sums past float32's range give infinity or NaN.
 __device__ __forceinline__ float swiglu_f32(float g, float u) {
   return g * __builtin_amdgcn_rcpf(1.0f + __expf(-g)) * u;
 }

@@ -441,9 +441,11 @@ int64_t hmoe_grouped_mxfp4_form(int64_t rows_cap, int n_experts, int kdim, int n
 
 /* h of rows r of expert e's segment [offsets[e], offsets[e+1]) as MXFP4 rows: with
  * g and u the float32 sums xs[r]·Wg[e] and xs[r]·Wu[e], h = silu(g) * u in float32
- * and quantised from there (h is rounded once, to its codes).  xs_q [rows_cap, D/2],
- * xs_exp [rows_cap, D/32], h_q [rows_cap, F/2], h_exp [rows_cap, F/32].  Rows past
- * offsets[N] are not written.  D % 128 == 0, F % 128 == 0, both up to 2^20, N <= 1024,
+ * and quantised from there (h is rounded once, to its codes; in float32 it is off by at
+ * most (1.25 |g| + 8) 2^-24 of itself, and by |g u| 2^-126 below g = -87.3).  A block of h
+ * whose sums pass float32's range is NaN.  xs_q [rows_cap, D/2], xs_exp [rows_cap, D/32],
+ * h_q [rows_cap, F/2], h_exp [rows_cap, F/32].  Rows past offsets[N] are not written.
+ * D % 128 == 0, F % 128 == 0, both up to 2^20, N <= 1024,
  * rows_cap <= 2^30; an expert's exponents below 2^31 bytes (D * F < 2^35, down 2^36), and
  * (rows_cap / 64 + N) * (2F / 256, down D / 256), each rounded up, at most 2^30. */
 int hmoe_grouped_gate_up_mxfp4(const uint8_t* xs_q, const uint8_t* xs_exp, const int32_t* offsets,

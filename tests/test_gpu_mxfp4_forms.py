@@ -277,3 +277,69 @@ def test_offsets_of_a_subclass(gpu):
     assert torch.equal(K.grouped_down_mxfp4(q, e, held, *dn), K.grouped_down_mxfp4(q, e, off, *dn))
     with pytest.raises(ValueError, match=r"offsets must be int32 \[3\]"):
         K.grouped_down_mxfp4(q, e, torch.nn.Parameter(off[:2].clone(), requires_grad=False), *dn)
+
+
+# ----------------------------------------------------- the ends of the SwiGLU --
+
+def _ones(gpu, rows, d_model):
+    """Rows of ones."""
+    return (torch.full((rows, d_model // 2), 0x22, dtype=torch.uint8, device=gpu),
+            torch.full((rows, d_model // 32), 127, dtype=torch.uint8, device=gpu))
+
+
+def _sums_operand(gpu, gate, gate_exp, up, up_exp):
+    """The operand of one expert with given codes [F, D] and exponents [F] of its columns."""
+    F, D = gate.shape
+    codes, exps = np.empty((2 * F, D), dtype=np.uint8), np.empty((2 * F, D // 32), dtype=np.uint8)
+    for p in range(2 * F):
+        which, c = R.gate_up_column(p, F)
+        codes[p], exps[p] = ((up[c], up_exp[c]) if which else (gate[c], gate_exp[c]))
+    return [torch.from_numpy(t[None]).to(gpu) for t in R.packed_operand(codes[:, 0::2] | (codes[:, 1::2] << 4), exps)]
+
+
+@pytest.mark.parametrize("rows,form", [(40, 0), (9000, 2), (60000, 3)])
+def test_far_negative_gates(gpu, rows, form):
+    """Gates from -60 to -90 with large up values.  Both sums are exact (at most 1536 halves of
+    a power of two), so that h is off by the SwiGLU's own roundings alone: the argument of the
+    exponential by half a step of |g| log2(e) and by log2(e)'s rounding, 1.25 |g| 2^-24 of h;
+    exponential and reciprocal by a step, the sum and two products by half a step, 7 of them,
+    and one for the products of these errors.  Where 1 + e^-g passes 2^126 its reciprocal may
+    be zero: |g u| 2^-126."""
+    D, F = 128, 2048
+    assert _form(gpu, rows, 1, D, 2 * F) == form
+    rng = np.random.default_rng(3)
+    t = np.concatenate([np.arange(60, 90.25, 0.5), [88.5, 87.0, 87.5]]).repeat(32)      # -g of each column
+    gate = np.zeros((F, D), dtype=np.uint8)
+    for c in range(F):
+        ones = int(t[c])
+        gate[c, :ones] = 0xA                                                            # -1
+        gate[c, ones:ones + int(2 * (t[c] - ones))] = 0x9                               # -1 / 2
+    up, up_exp = rng.integers(0, 16, (F, D), dtype=np.uint8), np.where(t < 87, 207, 227).astype(np.uint8)
+    gu = _sums_operand(gpu, gate, np.full(F, 127, dtype=np.uint8), up, up_exp)
+    h_q, h_e = K.grouped_gate_up_mxfp4(*_ones(gpu, rows, D), torch.tensor([0, rows], dtype=torch.int32, device=gpu), *gu)
+    assert (h_q == h_q[:1]).all() and (h_e == h_e[:1]).all()
+    u = np.where(up >= 8, -1.0, 1.0) * R.SIZES[up & 7] * np.ldexp(1.0, up_exp.astype(int) - 127)[:, None]
+    g, u = -t[None], u.sum(1)[None]
+    h = g / (1.0 + np.exp(-g)) * u
+    bound = np.abs(h) * (1.25 * np.abs(g) + 8) * 2.0**-24 + np.where(t > 126 * np.log(2), np.abs(g * u) * 2.0**-126, 0.0)
+    R.check_quantised(h_q[:1].cpu().numpy(), h_e[:1].cpu().numpy(), h, bound)
+    assert (h_e[0, :54] > 0).all()      # (down to -86.5 h is not lost)
+
+
+@pytest.mark.parametrize("rows,form", [(40, 0), (9000, 2), (60000, 3)])
+def test_sums_past_float32(gpu, rows, form):
+    """Gate sums of both signs and up sums past float32's range: NaN in their blocks alone."""
+    D, F = 128, 2048
+    assert _form(gpu, rows, 1, D, 2 * F) == form
+    gate, up = np.full((F, D), 0x1, dtype=np.uint8), np.full((F, D), 0x2, dtype=np.uint8)
+    gate_exp, up_exp = np.full(F, 123, dtype=np.uint8), np.full(F, 127, dtype=np.uint8)     # g = 4, u = 128
+    gate[64 + 5], gate_exp[64 + 5] = 0x7, 254
+    gate[992 + 31], gate_exp[992 + 31] = 0xF, 254
+    up[2016], up_exp[2016] = 0x7, 254
+    gu = _sums_operand(gpu, gate, gate_exp, up, up_exp)
+    h_q, h_e = K.grouped_gate_up_mxfp4(*_ones(gpu, rows, D), torch.tensor([0, rows], dtype=torch.int32, device=gpu), *gu)
+    nan = torch.zeros(F // 32, dtype=torch.bool, device=gpu)
+    nan[[2, 31, 63]] = True
+    assert (h_e[:, nan] == 255).all() and (h_q.reshape(rows, -1, 16)[:, nan] == 0).all()
+    # 4 / (1 + e^-4) * 128 = 502.8: a scale of 2^7, of which it is 3.93, code 6 (4)
+    assert (h_e[:, ~nan] == 127 + 7).all() and (h_q.reshape(rows, -1, 16)[:, ~nan] == 0x66).all()
