@@ -708,7 +708,8 @@ def grouped_down_fp8_mx(h_q: torch.Tensor, h_exp: torch.Tensor, offsets: torch.T
 # ---------------------------------------------------------- MXFP4 experts --
 # 32 values of a row share a power-of-two scale (an E8M0 byte), each is a 4-bit
 # e2m1 code; ``hmoe_quantize_rows_mxfp4`` has the rule.  Served weights only: there
-# is no backward, as for the e4m3 experts.
+# is no backward, as for the e4m3 experts.  A tensor that starts inside a buffer has to
+# start at 16 bytes, exponents at 4 (any row of such a matrix does).
 
 _U8, _TENSOR = torch.uint8, torch.Tensor
 

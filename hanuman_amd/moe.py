@@ -166,6 +166,12 @@ def ragged_dispatch(x_flat: torch.Tensor, top_idx: torch.Tensor, weights: torch.
     return K.combine(ys, plan, weights.float().contiguous(), None, torch.float32)
 
 
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """``t`` where the MXFP4 calls can read it: a tensor that starts inside a buffer (a
+    flat one of parameters, say) is copied unless it starts at 16 bytes."""
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 class MoE:
     """Mixture of Experts with aux-loss-free sigmoid routing (``moe.py:116-294``).
 
@@ -312,7 +318,8 @@ class MoE:
         """The routed experts' MXFP4 operands (codes and exponents of gate/up, of down)."""
         wg, wu, wd = self.expert_w_gate.value, self.expert_w_up.value, self.expert_w_down.value
         return self._mxfp4_pack.get((wg, wu, wd), lambda: (
-            *K.pack_mxfp4_gate_up(wg.detach(), wu.detach()), *K.pack_mxfp4_down(wd.detach())))
+            *K.pack_mxfp4_gate_up(_aligned(wg.detach()), _aligned(wu.detach())),
+            *K.pack_mxfp4_down(_aligned(wd.detach()))))
 
     def _packed_shared(self, masters=None):
         """One ``(gate_up, down)`` of packed operands per shared expert."""
@@ -425,6 +432,8 @@ class MoE:
         bias = self.bias.value if self.routing == "sigmoid" else None
         router_w = self.router.value.float().contiguous()
         x_q = None
+        if self.expert_dtype == "mxfp4":
+            x2 = _aligned(x2)
         if self.expert_dtype == "mxfp4" and x2.dtype == torch.bfloat16:
             logits, top_idx, gates, *x_q = K.router_quant_mxfp4(x2, router_w, bias, Kk, mode, rsf)
         else:
