@@ -355,12 +355,17 @@ __global__ __launch_bounds__(256) void grouped_mxfp4_rows(
 // (gate/up below 298 -> 285 us, down 172 -> 165; with 64 rows, taken where a workgroup has
 // few tiles, 512 tokens 28.8 -> 32.0, and not done).
 //
-// Gate/up of 131072 rows, D 2048, F 1024 (1.1 TFLOP) takes 285 us, down 165 us.  What bounds
-// them is power: with these operands the matrix cores alone, fed from registers, run at
-// 1.65 GHz and 6.5 PFLOP/s (170 us), and with operands of zeros, at 2.4 GHz, the same
-// launches take 205 and 119 us (the products alone 113 and 57).  In cycles it is what a CU
-// has to do besides: gate/up with zeros takes 170 us with the products taken out, 161 with
-// all loads and reads taken out instead, 198 with every load a hit of the first cache.
+// Gate/up of 131072 rows, D 2048, F 1024 (1.1 TFLOP) takes 277 to 285 us; down 157 to 165
+// us launched again and again and 203 behind the gate/up product (an output of 537 MB waits
+// for what lies written in the caches).  With these operands the matrix cores alone, fed from
+// registers, run at 1.65 GHz and 6.5 PFLOP/s (170 us) at the package's power limit; with
+// operands of zeros, at 2.4 GHz, the same launches take 205 and 119 us (the products alone
+// 113 and 57).  Power is not all: the matrix cores are busy in 54 % of gate/up's cycles (1.75
+// GHz) and 34 % of down's behind it (1.96 GHz).  A tile ends in a phase without a product
+// (the SwiGLU and quantisation; packing and stores), every 8 steps of K 2048 and every 4 of
+// K 1024, which only another workgroup's products cover.  Gate/up with zeros takes 170 us
+// with the products taken out, 161 with all loads and reads taken out instead, 198 with
+// every load a hit of the first cache.
 // Measured and not taken (us; gate/up and down, before the turns 300 and 170): B through LDS
 // too (2 x 2 waves, steps of 128 values, three stages) 326 and 187, an LDS and half lines of
 // A that kept pace with the products at best; one workgroup of eight waves on 128 x 512 301
@@ -844,6 +849,11 @@ const char* too_large(int64_t rows_cap, int n_experts, int kdim, int ncols) {
 // side by side that fill the chip are faster: down of 64 experts (8 steps), 32 tokens 12.2
 // against 13.3, of 128 experts, D 1024, F 512 (4 steps), 30 tokens 5.0 against 6.1.  Below
 // four steps there is nothing to split.
+// The rule does not always choose the fastest (forms 0, 1, 2, 3 measured, us): a split that is
+// taken below 4 waves a CU and charged 0.55 lets down of 64 experts, D 2048, F 1024, go to 64-row
+// tiles at 4 and 5 tokens (4.4, 4.5, 6.0, 7.6) and of 128 experts, D 2048, F 768, at 3 and 4
+// (4.4, 4.4, 5.8, 7.2; 5.1, 5.0, 5.8, 7.2); where the weights bound both sides, gate/up of 128
+// experts, D 4096, F 1536, 16 tokens goes there too (84.9, 75.1, 79.9, 80.7).
 enum Form { kRows1, kRows4, kTiles64, kTiles128 };
 
 // The experts that have rows, and the row tiles of all.  The counts are known only to

@@ -5,7 +5,8 @@
 // The scale is the smallest power of two at which the block's largest value
 // rounds to 6 or less: with amax = m 2^a, 1 <= m < 2, that is 2^(a - 2) where m <
 // 1.75 (then amax is below 7 scale units, which rounds to 6 at most) and 2^(a - 1)
-// above.  (Always 2^(a - 2) would cut values of 7 to 8 units to 6.)  Adding a
+// above.  (Always 2^(a - 2), as in the conversion that the OCP Microscaling Formats
+// specification describes, would cut values of 7 to 8 units to 6.)  Adding a
 // quarter to the mantissa field carries into the exponent exactly where m >= 1.75.
 // Scaling by a power of two is exact, so a code is one rounding (nearest, ties to
 // the even code) of the value.  A block with a value that is not finite gets E =

@@ -387,7 +387,9 @@ int hmoe_grouped_wgrad_down_f32(const float* h, const float* d_ys, const int32_t
  * E8M0 byte E for 2^(E - 127), and each value is an e2m1 code (0, 0.5, 1, 1.5, 2,
  * 3, 4, 6 and their negatives).  The scale is the smallest power of two at which
  * the block's largest value rounds to 6 or less (E >= 0), a code is the value over
- * the scale rounded to nearest, ties to the even code.  A block with a value that
+ * the scale rounded to nearest, ties to the even code.  (The OCP Microscaling Formats
+ * specification's own conversion takes 2^floor(log2 max) / 4 always and cuts to 6: where the
+ * largest value's mantissa is 1.75 or more, exponent and codes differ.)  A block with a value that
  * is not finite has E = 255 and zero codes and stands for NaN; a product with it is
  * NaN.  A value past the format's range (a block whose largest is 1.75 * 2^127 or
  * more) reads back as infinity.  Codes and values are 16-byte aligned, exponents 4-byte
