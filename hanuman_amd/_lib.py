@@ -18,7 +18,7 @@ HEADER = PKG.parent / "include" / "hanuman_moe.h"
 
 # hmoe status codes and enums (hanuman_moe.h)
 OK, ERR_INVALID, ERR_UNSUPPORTED, ERR_HIP, ERR_WORKSPACE = 0, 1, 2, 3, 4
-F32, BF16, FP8_E4M3 = 0, 1, 2
+F32, BF16, FP8_E4M3, I8 = 0, 1, 2, 3
 ROUTE_SIGMOID_BIAS, ROUTE_SOFTMAX = 0, 1
 GEMM_TILE_M = 256
 
@@ -96,6 +96,23 @@ SIGNATURES = {
                                                  _i32, _vp, _vp, _vp, _vp, _vp]),
     "hmoe_grouped_down_mxfp4": (_i32, [_vp, _vp, _vp, _i32, _i64, _i32, _i32, _vp, _vp, _vp,
                                        _vp]),
+    "hmoe_add_rms_norm": (_i32, [_vp, _i32, _vp, _i32, _vp, _i32, _f32, _i64, _i32, _vp, _vp, _i32,
+                                 _vp, _vp, _i32, _vp, _vp]),
+    "hmoe_add_rms_norm_bwd_workspace_bytes": (_sz, [_i64, _i32]),
+    "hmoe_add_rms_norm_bwd": (_i32, [_vp, _i32, _vp, _i32, _vp, _i32, _vp, _vp, _i64, _i32, _vp,
+                                     _vp, _vp, _sz, _vp]),
+    "hmoe_quantize_rows_i8": (_i32, [_vp, _i32, _i64, _i32, _vp, _i32, _vp, _vp, _vp]),
+    "hmoe_dequantize_rows_i8": (_i32, [_vp, _vp, _i64, _i32, _vp, _i32, _vp]),
+    "hmoe_dequantize_rows_fp8": (_i32, [_vp, _vp, _i64, _i32, _vp, _i32, _vp]),
+    "hmoe_packed_i8_gate_up_bytes": (_sz, [_i32, _i32, _i32]),
+    "hmoe_pack_i8_gate_up": (_i32, [_vp, _vp, _i32, _i32, _i32, _i32, _vp, _vp, _vp]),
+    "hmoe_packed_i8_down_bytes": (_sz, [_i32, _i32, _i32]),
+    "hmoe_pack_i8_down": (_i32, [_vp, _i32, _i32, _i32, _i32, _vp, _vp, _vp]),
+    "hmoe_grouped_i8_form": (_i64, [_i64, _i32, _i32, _i32, _i32]),
+    "hmoe_grouped_gate_up_i8": (_i32, [_vp, _vp, _vp, _i32, _i64, _i32, _i32, _vp, _vp, _vp, _vp]),
+    "hmoe_grouped_gate_up_i8_gather": (_i32, [_vp, _vp, _i64, _i32, _vp, _vp, _i32, _i64, _i32,
+                                              _i32, _vp, _vp, _vp, _vp]),
+    "hmoe_grouped_down_i8": (_i32, [_vp, _vp, _vp, _i32, _i64, _i32, _i32, _vp, _vp, _vp, _vp]),
     "hmoe_aux_workspace_bytes": (_sz, [_i32, _i32, _i32]),
     "hmoe_router_aux": (_i32, [_vp, _vp, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _sz, _vp]),
     "hmoe_combine_bwd": (_i32, [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _f32, _vp]),

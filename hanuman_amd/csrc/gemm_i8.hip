@@ -1,0 +1,492 @@
+// Grouped products of int8 rows with int8 expert weights (model/moe.py:67-74 on 8-bit
+// operands; the reference has no such path):
+//
+//   C[r, n] = a_scale[r] b_scale_e[n] sum_k A[r, k] B_e[n, k]   for rows r of expert e's segment
+//
+// on v_mfma_i32_32x32x32_i8.  The sums are exact: 32768 products of at most 2^14 stay below
+// 2^31.  They are rounded to float32 once, then come the two scales, and for gate/up the
+// SwiGLU, all in float32; h and ys are rounded to bf16 once.
+//
+// The operand keeps a lane's 16 bytes of a fragment together: lane 32 h + r of block (p /
+// 32, k / 32) has the 16 codes of row r from column 16 h on, so a fragment is one 1 KB run
+// of memory.  (Which of the instruction's 32 products a value takes part in does not matter,
+// as long as both operands agree.)
+#include <type_traits>
+
+#include "grouped_tiles.h"
+#include "quant_mxfp4.h"
+#include "rows.h"
+
+namespace hmoe {
+namespace {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x16 __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ i32x16 mfma_i8(const u32x4& b, const u32x4& a, const i32x16& c) {
+  return __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, b), __builtin_bit_cast(i32x4, a), c, 0, 0, 0);
+}
+
+// Sums of 32 columns to values: `cols` are the columns' scales.  Lane L holds row L % 32 and
+// columns 8 q + 4 (L / 32) + 0..3 (q = 0..3).
+__device__ __forceinline__ f32x16 scaled(const i32x16& acc, const float* __restrict__ cols, float row, int half) {
+  f32x16 y;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const f32x4 c = *reinterpret_cast<const f32x4*>(cols + 8 * q + 4 * half);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[4 * q + i] = static_cast<float>(acc[4 * q + i]) * c[i] * row;
+  }
+  return y;
+}
+__device__ __forceinline__ f32x16 swiglu16(const f32x16& g, const f32x16& u) {
+  f32x16 h;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) h[i] = swiglu_f32(g[i], u[i]);
+  return h;
+}
+
+// ---- few rows ---------------------------------------------------------------------
+// 32 rows x 64 columns a wave, operands straight from memory into registers: with few
+// rows an expert every weight is used once or twice, and a fragment is one run of 1 KB.
+// A workgroup is four waves: side by side (SPLIT 1), or on a quarter of the reduction
+// each, joined in LDS (SPLIT 4; the sums are exact, so the order does not matter).
+template <bool GATE_UP, bool GATHER, int SPLIT>
+__global__ __launch_bounds__(256) void grouped_i8_rows(
+    const int8_t* __restrict__ A, const float* __restrict__ a_scale, const int8_t* __restrict__ B,
+    const float* __restrict__ b_scale, const int32_t* __restrict__ offsets, int n_experts, int kdim, int ncols,
+    uint16_t* __restrict__ C, const int32_t* __restrict__ gather_src, Divisor gather_k, int gather_rows) {
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int frow = lane & 31, half = lane >> 5;
+  RowTile t;
+  if (!find_row_tile(offsets, n_experts, 32, blockIdx.y, t)) return;
+  const int n0 = SPLIT == 1 ? (blockIdx.x * 4 + wave) * 64 : blockIdx.x * 64;
+  if (n0 >= ncols) return;  // (SPLIT 1 only: no barrier follows there)
+  int src = t.row0 + (frow < t.rows ? frow : t.rows - 1);  // rows past the segment repeat its last one
+  if (GATHER) src = token_of(gather_src[src], gather_k, gather_rows);
+  const int groups = kdim / 128;
+  const int8_t* a = A + static_cast<int64_t>(src) * kdim + half * 16;
+  const int64_t frag = (static_cast<int64_t>(t.e) * (ncols / 32) + n0 / 32) * (kdim / 32);
+  const int8_t* b0 = B + frag * 1024 + lane * 16;
+  const int8_t* b1 = b0 + static_cast<int64_t>(kdim / 32) * 1024;
+  const float row_scale = a_scale[src];
+  i32x16 acc0 = {}, acc1 = {};
+  struct Group {
+    u32x4 fa[4], f0[4], f1[4];
+  };
+  auto load = [&](Group& p, int k) __attribute__((always_inline)) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      p.fa[q] = *reinterpret_cast<const u32x4*>(a + k * 128 + q * 32);
+      p.f0[q] = *reinterpret_cast<const u32x4*>(b0 + static_cast<int64_t>(k) * 4096 + q * 1024);
+      p.f1[q] = *reinterpret_cast<const u32x4*>(b1 + static_cast<int64_t>(k) * 4096 + q * 1024);
+    }
+  };
+  auto use = [&](const Group& p) __attribute__((always_inline)) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      acc0 = mfma_i8(p.f0[q], p.fa[q], acc0);
+      acc1 = mfma_i8(p.f1[q], p.fa[q], acc1);
+    }
+  };
+  int k = SPLIT == 1 ? 0 : groups * wave / SPLIT;
+  const int end = SPLIT == 1 ? groups : groups * (wave + 1) / SPLIT;
+  for (; k + 2 <= end; k += 2) {
+    Group p[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) load(p[j], k + j);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) use(p[j]);
+  }
+  for (; k < end; ++k) {
+    Group p;
+    load(p, k);
+    use(p);
+  }
+  if constexpr (SPLIT > 1) {
+    // wave 0 adds the others' sums
+    __shared__ i32x4 part[SPLIT - 1][8][64];
+    if (wave > 0) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        part[wave - 1][r][lane] = i32x4{acc0[4 * r], acc0[4 * r + 1], acc0[4 * r + 2], acc0[4 * r + 3]};
+        part[wave - 1][4 + r][lane] = i32x4{acc1[4 * r], acc1[4 * r + 1], acc1[4 * r + 2], acc1[4 * r + 3]};
+      }
+    }
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int w = 0; w < SPLIT - 1; ++w)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const i32x4 p0 = part[w][r][lane], p1 = part[w][4 + r][lane];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          acc0[4 * r + i] += p0[i];
+          acc1[4 * r + i] += p1[i];
+        }
+      }
+  }
+  const int64_t r0 = t.row0;
+  const float* cs = b_scale + static_cast<int64_t>(t.e) * ncols + n0;
+  const f32x16 y0 = scaled(acc0, cs, row_scale, half), y1 = scaled(acc1, cs + 32, row_scale, half);
+  const int ldc = GATE_UP ? ncols / 2 : ncols;
+  const __amdgpu_buffer_rsrc_t out =
+      __builtin_amdgcn_make_buffer_rsrc(C + r0 * ldc, 0, t.rows * ldc * 2, kBufferWord3);
+  if constexpr (GATE_UP) {
+    store_y_block(swiglu16(y0, y1), out, frow, n0 / 2, ldc, half);
+  } else {
+    store_y_block(y0, out, frow, n0, ldc, half);
+    store_y_block(y1, out, frow, n0 + 32, ldc, half);
+  }
+}
+
+// ---- tiles for experts with many rows ------------------------------------------
+// Workgroups of four waves, two (BM 128) or three (BM 64) a CU, each looping over BM x 256
+// tiles: while one is in its epilogue, switches tiles or waits at its barrier, the others'
+// products run.  A wave has all of the tile's rows and 64 of its columns, so B's fragments
+// are read by one wave only and go from memory straight into registers, 1 KB an
+// instruction, each loaded for the next step as soon as its products are issued.  A goes
+// through LDS (buffer_load ... lds), two stages of 128 values of every row, the next
+// stage's loads issued behind the one barrier of a step: whole lines, and 16-byte chunk c of
+// row r sits at c ^ swz128(r), so that 16 lanes of a fragment read cover all banks.  The
+// last column tile may be 128 columns wide: waves 2 and 3 then load and compute the others'
+// again and store nothing.
+constexpr int kTileThreads = 256;
+
+template <int BM, bool GATE_UP>
+struct TileCfg {
+  static constexpr int kA = BM * 128;              // a stage
+  static constexpr int kOut = 4 * 4096;            // 4 KB a wave for the rows that are stored
+  static constexpr int kLds = 2 * kA + kOut;
+  static constexpr int kFR = BM / 32;              // row fragments; DMA instructions a wave and step
+  static constexpr int kPerCu = BM == 64 ? 3 : 2;
+  static_assert(kPerCu * kLds <= 160 * 1024, "workgroups a CU");
+};
+
+__device__ __forceinline__ void use_here(const i32x16& v) { asm volatile("" ::"v"(v)); }
+
+// Of a CU's two workgroups one goes first.
+__device__ __forceinline__ void take_turn(int turn) {
+  if (turn == 0) __builtin_amdgcn_s_setprio(0);
+  else __builtin_amdgcn_s_setprio(1);
+}
+
+template <int BM, bool GATE_UP, bool GATHER>
+__global__ __launch_bounds__(kTileThreads, BM == 64 ? 3 : 2) void grouped_i8_tiles(
+    const int8_t* __restrict__ A, const float* __restrict__ a_scale, const int8_t* __restrict__ B,
+    const float* __restrict__ b_scale, const int32_t* __restrict__ offsets, int n_experts, int kdim, int ncols,
+    uint16_t* __restrict__ C, const int32_t* __restrict__ gather_src, Divisor gather_k, int gather_rows,
+    Divisor by_cols, Divisor by_group) {
+  typedef TileCfg<BM, GATE_UP> Cfg;
+  constexpr int kFR = Cfg::kFR;
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n_tiles_n = (ncols + kTileN - 1) / kTileN;
+  const int total = count_row_tiles(offsets, n_experts, BM) * n_tiles_n;
+  // the tiles are split evenly over the XCDs (workgroup i runs on XCD i % 8)
+  const int xcd = blockIdx.x % kNumXcd;
+  const int per_xcd = gridDim.x / kNumXcd;
+  const int lo = static_cast<int>((static_cast<int64_t>(total) * xcd) / kNumXcd);
+  const int hi = static_cast<int>((static_cast<int64_t>(total) * (xcd + 1)) / kNumXcd);
+  const int first = lo + static_cast<int>(blockIdx.x) / kNumXcd;
+  if (first >= hi) return;  // uniform per workgroup
+  const int ks = kdim / 128;  // steps
+  const int row_bytes = kdim;
+
+  // ---- load side -----------------------------------------------------------------
+  // A: instruction j of wave w fills rows (BM / 4) w + 8 j + lane / 8, chunk (lane & 7) ^
+  // swz128(row) of the row's 128 bytes.
+  TileCursor<BM> ld;
+  ld.find(offsets, n_experts, divide(first, by_cols));
+  TileCursor<BM> cur = ld, nx = ld;
+  const int a_row = (BM / 4) * wave + (lane >> 3);
+  __amdgpu_buffer_rsrc_t a_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(A), 0,
+                                                                    GATHER ? gather_rows * row_bytes : 0, kBufferWord3);
+  __amdgpu_buffer_rsrc_t b_rsrc = a_rsrc;
+  uint32_t a_voff[kFR];
+  const int b_col = (kdim / 32) * 1024;  // bytes of 32 columns
+  int b_wave = 0;                        // where this wave's columns begin
+  int ld_kb = 0, ld_t = first, ld_stage = 0;
+  int32_t pf_src[kFR];  // GATHER: sources of this lane's rows of the tile after, nx
+  auto a_byte = [&](int j) __attribute__((always_inline)) {
+    return static_cast<uint32_t>(((lane & 7) ^ swz128(8 * j + (lane >> 3))) * 16);
+  };
+  auto fetch_src = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < kFR; ++j) {
+      const int r = a_row + 8 * j;
+      pf_src[j] = gather_src[nx.row0 + (r < nx.rows ? r : nx.rows - 1)];
+    }
+  };
+  // Tile ld_t becomes the one that is loaded.
+  auto set_load_tile = [&]() __attribute__((always_inline)) {
+    if (GATHER) {
+      ld = nx;
+#pragma unroll
+      for (int j = 0; j < kFR; ++j)
+        a_voff[j] = static_cast<uint32_t>(token_of(pf_src[j], gather_k, gather_rows)) * static_cast<uint32_t>(row_bytes) +
+                    a_byte(j);
+      if (ld_t + per_xcd < hi) nx.move(offsets, ld_t + per_xcd, n_tiles_n, by_cols, by_group);
+      fetch_src();  // (on every path: a load that may not be issued is waited for at once)
+    } else {
+      ld.move(offsets, ld_t, n_tiles_n, by_cols, by_group);
+      // rows past the segment repeat its last one; their results are not stored
+      a_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(A + static_cast<int64_t>(ld.row0) * row_bytes), 0,
+                                                 ld.rows * row_bytes, kBufferWord3);
+#pragma unroll
+      for (int j = 0; j < kFR; ++j) {
+        const int r = a_row + 8 * j;
+        a_voff[j] = static_cast<uint32_t>((r < ld.rows ? r : ld.rows - 1) * row_bytes) + a_byte(j);
+      }
+    }
+    const int64_t block = static_cast<int64_t>(ld.e) * (ncols / 32) + ld.n0 / 32;
+    const int width = ncols - ld.n0 < kTileN ? ncols - ld.n0 : kTileN;
+    const int part = 64 * wave < width ? wave : wave - 2;  // (a tile of 128 columns: waves 0 and 1 again)
+    b_wave = part * 2 * b_col;
+    b_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(B + block * b_col), 0, width * row_bytes,
+                                               kBufferWord3);
+    ld_kb = 0;
+  };
+  auto issue_a = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < kFR; ++j)
+      dma16(a_rsrc, smem + ld_stage * Cfg::kA + (wave * kFR + j) * 1024, a_voff[j] + static_cast<uint32_t>(ld_kb * 128));
+    ld_stage ^= 1;
+    fence();  // (the waits count B's loads behind these)
+  };
+  u32x4 fb[4][2];
+  // B of the step that is loaded.
+  auto load_b = [&](int q) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      fb[q][j] = __builtin_amdgcn_raw_buffer_load_b128(b_rsrc, lane * 16, b_wave + j * b_col + (4 * ld_kb + q) * 1024, 0);
+  };
+
+  // ---- compute side ----------------------------------------------------------------
+  // Wave w: all rows and columns 64 w .. of the tile.
+  const int frow = lane & 31, half = lane >> 5;
+  const int fsw = swz128(frow);
+  i32x16 acc[kFR][2];
+  int stage = 0;
+  constexpr int kNewer = 8;  // loads of B in a step, behind A's
+
+  // One step: 128 values of this tile, the loads of the next step behind them.
+  auto step = [&](int kb) __attribute__((always_inline)) {
+    // this wave's loads of A have landed; after the barrier every wave's have, and every
+    // wave is done with the step before, whose stage the next loads take
+    wait_vm_lgkm0<kNewer>();
+    __builtin_amdgcn_s_barrier();
+    fence();
+    // on to the next step (after the last tile's last one: it again)
+    if (ld_kb + 1 < ks) {
+      ++ld_kb;
+    } else if (ld_t + per_xcd < hi) {
+      ld_t += per_xcd;
+      set_load_tile();
+    }
+    issue_a();
+    const uint8_t* st = smem + stage * Cfg::kA + frow * 128;
+    u32x4 fa[2][kFR];
+    auto read_a = [&](int q) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < kFR; ++i)
+        fa[q & 1][i] = *reinterpret_cast<const u32x4*>(st + i * 4096 + (((2 * q + half) ^ fsw) * 16));
+    };
+    read_a(0);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      // (kept ahead of the products, or each fragment is waited for)
+      if (q + 1 < 4) read_a(q + 1);
+      __builtin_amdgcn_sched_barrier(0);
+      if (q == 0 && kb == 0) {  // (zeros as an operand, not written first)
+        const i32x16 zero = {};
+#pragma unroll
+        for (int i = 0; i < kFR; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) acc[i][j] = mfma_i8(fb[0][j], fa[0][i], zero);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kFR; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) acc[i][j] = mfma_i8(fb[q][j], fa[q & 1][i], acc[i][j]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      load_b(q);
+      fence();
+    }
+#pragma unroll
+    for (int i = 0; i < kFR; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) use_here(acc[i][j]);
+    stage ^= 1;
+  };
+
+  if (GATHER) {
+    nx.move(offsets, first, n_tiles_n, by_cols, by_group);
+    fetch_src();
+  }
+  set_load_tile();
+  issue_a();
+#pragma unroll
+  for (int q = 0; q < 4; ++q) load_b(q);
+  fence();
+  int turn = blockIdx.x < gridDim.x / 2;  // (workgroups i and i + gridDim / 2 share a CU)
+  for (int t = first; t < hi; t += per_xcd) {
+    if (BM == 128) take_turn(turn ^= 1);
+    for (int kb = 0; kb < ks; ++kb) step(kb);
+    cur.move(offsets, t, n_tiles_n, by_cols, by_group);
+    const int64_t r0 = cur.row0;
+    const int ldc = GATE_UP ? ncols / 2 : ncols;
+    const __amdgpu_buffer_rsrc_t out =
+        __builtin_amdgcn_make_buffer_rsrc(C + r0 * ldc, 0, cur.rows * ldc * 2, kBufferWord3);
+    const bool mine = cur.n0 + wave * 64 < ncols;  // uniform per wave
+    if (mine) {
+      const float* cs = b_scale + static_cast<int64_t>(cur.e) * ncols + cur.n0 + wave * 64;
+      uint8_t* const lds = smem + 2 * Cfg::kA + wave * 4096;
+#pragma unroll
+      for (int i = 0; i < kFR; ++i) {
+        const int r = 32 * i + frow < cur.rows ? 32 * i + frow : cur.rows - 1;
+        int src = cur.row0 + r;
+        if (GATHER) src = token_of(gather_src[src], gather_k, gather_rows);
+        const float row_scale = a_scale[src];
+        const f32x16 y0 = scaled(acc[i][0], cs, row_scale, half), y1 = scaled(acc[i][1], cs + 32, row_scale, half);
+        if constexpr (GATE_UP)
+          store_y_block(swiglu16(y0, y1), out, 32 * i + frow, cur.n0 / 2 + wave * 32, ldc, half);
+        else
+          store_y_blocks(y0, y1, lds, out, 32 * i, cur.n0 + wave * 64, ldc, lane);
+      }
+    }
+    fence();  // (this tile's reads of LDS stay ahead of the next step's barrier)
+  }
+  // nothing may still be writing into LDS when the workgroup ends
+  __builtin_amdgcn_s_waitcnt(0);
+}
+
+// The checks that the products share.
+int check_product(const char* what, int n_experts, int64_t rows_cap, int d_model, int d_ff) {
+  HMOE_REQUIRE(n_experts >= 1 && n_experts <= kMaxExperts, "%s: n_experts must be in [1, %d] (got %d)", what,
+               kMaxExperts, n_experts);
+  // (2^30: a tile's rows and the tiles that a workgroup steps over are added in 32 bits)
+  HMOE_REQUIRE(rows_cap >= 0 && rows_cap <= kMaxRows, "%s: rows_cap must be in [0, 2^30]", what);
+  HMOE_REQUIRE_CODE(d_model >= 128 && d_model % 128 == 0 && d_model <= kMaxRowCols, HMOE_ERR_UNSUPPORTED,
+                    "%s: d_model must be a multiple of 128 up to %d (got %d)", what, kMaxRowCols, d_model);
+  HMOE_REQUIRE_CODE(d_ff >= 128 && d_ff % 128 == 0 && d_ff <= kMaxRowCols, HMOE_ERR_UNSUPPORTED,
+                    "%s: d_ff must be a multiple of 128 up to %d (got %d)", what, kMaxRowCols, d_ff);
+  return HMOE_OK;
+}
+
+// What a launch cannot count in 32 bits beyond that: the tiles of the smaller tile form.
+// (An expert's columns of a tile are 256 x 32768 bytes, its rows 128 x 65536 x 2.)
+bool too_many_tiles(int64_t rows_cap, int n_experts, int ncols) {
+  return (ceil_div(rows_cap, 64) + n_experts) * ceil_div(ncols, kTileN) > (int64_t(1) << 30);
+}
+
+enum Form { kRows1, kRows4, kTiles64, kTiles128 };
+
+Form choose_form(int64_t rows, int n_experts, int kdim, int ncols, int cus) {
+  const double n = live_experts(rows, n_experts), mean = rows / n;
+  const bool split = kdim >= 1024;
+  (void)ncols;
+  (void)cus;
+  if (mean <= 32 && max_row_tiles(rows, n_experts) <= 65535) return split ? kRows4 : kRows1;
+  return mean <= 256 ? kTiles64 : kTiles128;
+}
+
+template <bool GATE_UP, bool GATHER>
+int launch_product(const char* what, const int8_t* a, const float* a_scale, const int8_t* b, const float* b_scale,
+                   const int32_t* offsets, int n_experts, int64_t rows_cap, int kdim, int ncols, void* c,
+                   const int32_t* gather_src, int gather_k, int gather_rows, hipStream_t s) {
+  const Divisor by_k = divisor(gather_k);
+  HMOE_REQUIRE(!too_many_tiles(rows_cap, n_experts, ncols), "%s: too many tiles", what);
+  uint16_t* const out = static_cast<uint16_t*>(c);
+  int dev = 0, cus = 0;
+  if (int rc = persistent_grid(what, s, &cus, &dev)) return rc;
+  const Form form = choose_form(rows_cap, n_experts, kdim, ncols, cus);
+  if (form == kTiles64 || form == kTiles128) {
+    const auto launch = [&](auto BM) {
+      constexpr int bm = decltype(BM)::value;
+      constexpr int lds = TileCfg<bm, GATE_UP>::kLds, per_cu = TileCfg<bm, GATE_UP>::kPerCu;
+      const int n_tiles_n = static_cast<int>(ceil_div(ncols, kTileN));
+      const Divisor by_cols = divisor(n_tiles_n), by_group = divisor(kTileGroup * n_tiles_n);
+      static std::atomic<uint64_t> done{0};
+      if (int rc = allow_lds(what, grouped_i8_tiles<bm, GATE_UP, GATHER>, lds, dev, &done)) return rc;
+      hipLaunchKernelGGL((grouped_i8_tiles<bm, GATE_UP, GATHER>), dim3(per_cu * cus), dim3(kTileThreads), lds, s, a,
+                         a_scale, b, b_scale, offsets, n_experts, kdim, ncols, out, gather_src, by_k, gather_rows,
+                         by_cols, by_group);
+      return check_launch(what);
+    };
+    return form == kTiles64 ? launch(std::integral_constant<int, 64>{}) : launch(std::integral_constant<int, 128>{});
+  }
+  const unsigned m_tiles = static_cast<unsigned>(max_row_tiles(rows_cap, n_experts));
+  if (form == kRows4)
+    hipLaunchKernelGGL((grouped_i8_rows<GATE_UP, GATHER, 4>), dim3(ncols / 64, m_tiles), dim3(256), 0, s, a, a_scale,
+                       b, b_scale, offsets, n_experts, kdim, ncols, out, gather_src, by_k, gather_rows);
+  else
+    hipLaunchKernelGGL((grouped_i8_rows<GATE_UP, GATHER, 1>),
+                       dim3(static_cast<unsigned>(ceil_div(ncols, 256)), m_tiles), dim3(256), 0, s, a, a_scale, b,
+                       b_scale, offsets, n_experts, kdim, ncols, out, gather_src, by_k, gather_rows);
+  return check_launch(what);
+}
+
+}  // namespace
+}  // namespace hmoe
+
+extern "C" int64_t hmoe_grouped_i8_form(int64_t rows_cap, int n_experts, int kdim, int ncols, int cus) {
+  using namespace hmoe;
+  if (rows_cap < 1 || rows_cap > kMaxRows || n_experts < 1 || n_experts > kMaxExperts || cus < 1 || kdim < 128 ||
+      kdim % 128 != 0 || kdim > kMaxRowCols || ncols < 128 || ncols % 128 != 0 || ncols > 2 * kMaxRowCols ||
+      too_many_tiles(rows_cap, n_experts, ncols)) {
+    set_error("grouped_i8_form: sizes that the products refuse");
+    return -1;
+  }
+  return choose_form(rows_cap, n_experts, kdim, ncols, cus);
+}
+
+extern "C" int hmoe_grouped_gate_up_i8(const int8_t* xs_q, const float* xs_scale, const int32_t* offsets,
+                                       int n_experts, int64_t rows_cap, int d_model, int d_ff, const int8_t* w_packed,
+                                       const float* w_scales, void* h, hmoe_stream_t stream) {
+  using namespace hmoe;
+  const char* what = "grouped_gate_up_i8";
+  if (int rc = check_product(what, n_experts, rows_cap, d_model, d_ff)) return rc;
+  if (rows_cap == 0) return HMOE_OK;
+  HMOE_REQUIRE(xs_q && xs_scale && offsets && w_packed && w_scales && h, "%s: null pointer argument", what);
+  HMOE_REQUIRE_ALIGNED(what, 16, xs_q, w_packed, w_scales, h);
+  return launch_product<true, false>(what, xs_q, xs_scale, w_packed, w_scales, offsets, n_experts, rows_cap, d_model,
+                                     2 * d_ff, h, nullptr, 1, 1, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int hmoe_grouped_gate_up_i8_gather(const int8_t* x_q, const float* x_scale, int64_t tokens, int top_k,
+                                              const int32_t* perm_src, const int32_t* offsets, int n_experts,
+                                              int64_t rows_cap, int d_model, int d_ff, const int8_t* w_packed,
+                                              const float* w_scales, void* h, hmoe_stream_t stream) {
+  using namespace hmoe;
+  const char* what = "grouped_gate_up_i8_gather";
+  if (int rc = check_product(what, n_experts, rows_cap, d_model, d_ff)) return rc;
+  HMOE_REQUIRE(tokens >= 0 && top_k >= 1 && (tokens >= 1 || rows_cap == 0),
+               "%s: need tokens >= 0, top_k >= 1 (tokens >= 1 with rows)", what);
+  HMOE_REQUIRE(tokens < (int64_t(1) << 31) && tokens * d_model < (int64_t(1) << 31),
+               "%s: x_q must be smaller than 2 GiB", what);
+  if (rows_cap == 0) return HMOE_OK;
+  HMOE_REQUIRE(x_q && x_scale && perm_src && offsets && w_packed && w_scales && h, "%s: null pointer argument", what);
+  HMOE_REQUIRE_ALIGNED(what, 16, x_q, w_packed, w_scales, h);
+  return launch_product<true, true>(what, x_q, x_scale, w_packed, w_scales, offsets, n_experts, rows_cap, d_model,
+                                    2 * d_ff, h, perm_src, top_k, static_cast<int>(tokens),
+                                    static_cast<hipStream_t>(stream));
+}
+
+extern "C" int hmoe_grouped_down_i8(const int8_t* h_q, const float* h_scale, const int32_t* offsets, int n_experts,
+                                    int64_t rows_cap, int d_ff, int d_model, const int8_t* w_packed,
+                                    const float* w_scales, void* ys, hmoe_stream_t stream) {
+  using namespace hmoe;
+  const char* what = "grouped_down_i8";
+  if (int rc = check_product(what, n_experts, rows_cap, d_model, d_ff)) return rc;
+  if (rows_cap == 0) return HMOE_OK;
+  HMOE_REQUIRE(h_q && h_scale && offsets && w_packed && w_scales && ys, "%s: null pointer argument", what);
+  HMOE_REQUIRE_ALIGNED(what, 16, h_q, w_packed, w_scales, ys);
+  return launch_product<false, false>(what, h_q, h_scale, w_packed, w_scales, offsets, n_experts, rows_cap, d_ff,
+                                      d_model, ys, nullptr, 1, 1, static_cast<hipStream_t>(stream));
+}

@@ -87,8 +87,8 @@ __device__ __forceinline__ void load_row_regs(const TI* __restrict__ row, int ch
   scales_from_amax(amax, s, inv);
 }
 
-template <typename TI>
-__device__ __forceinline__ uint2 quant8_e4m3(const Chunk8<TI>& v, float inv) {
+template <typename Values>
+__device__ __forceinline__ uint2 quant8_e4m3(const Values& v, float inv) {
   float q[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) q[i] = fminf(fmaxf(v.get(i) * inv, -kE4m3Max), kE4m3Max);

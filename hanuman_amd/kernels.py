@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 from dataclasses import dataclass
+from typing import NamedTuple
 
 import torch
 
@@ -893,6 +894,251 @@ def grouped_down_mxfp4(h_q: torch.Tensor, h_exp: torch.Tensor, offsets: torch.Te
     ys = h_q.new_empty((rows, D), dtype=torch.bfloat16)
     call("hmoe_grouped_down_mxfp4", h_q.data_ptr(), h_exp.data_ptr(), offsets.data_ptr(), N, rows, F, D,
          w_packed.data_ptr(), w_exp.data_ptr(), ys.data_ptr(), _stream())
+    return ys
+
+
+# ----------------------------------------------------------- norm and residual --
+
+class NormOut(NamedTuple):
+    """What :func:`add_rms_norm` gives: the normed rows ``y``, the ``sum`` that was normed
+    (``x`` itself without a residual), its reciprocal root mean square ``rstd`` float32
+    ``[rows]``, and 8-bit codes ``q`` of ``y`` with their ``scale`` ``[rows]`` (or None)."""
+    y: torch.Tensor
+    sum: torch.Tensor
+    rstd: torch.Tensor
+    q: torch.Tensor | None
+    scale: torch.Tensor | None
+
+
+def _norm_operand(name: str, what: str, t: torch.Tensor, dev, shape: tuple) -> int:
+    """The dtype code of a float32 or bf16 operand of that shape on the call's device."""
+    _check(t, what)
+    _same_device(name, t, dev)
+    if t.shape != shape:
+        raise ValueError(f"{name}: {what} must have shape {tuple(shape)} (got {tuple(t.shape)})")
+    return _dtype_code(t)
+
+
+_QUANT = {None: 0, "e4m3": _lib.FP8_E4M3, "int8": _lib.I8}
+
+
+def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None,
+                 eps: float = 1e-6, *, out_dtype: torch.dtype | None = None,
+                 quant: str | None = None) -> NormOut:
+    """``y = sum * rsqrt(mean(sum^2) + eps) * weight`` of ``sum = x + residual`` (``[rows,
+    cols]``, rounded to the residual's type; ``x`` where there is none), ``weight [cols]``,
+    each float32 or bf16.  ``y`` has ``out_dtype`` (``x``'s by default).  ``quant``:
+    "int8" or "e4m3" for the codes and scales of ``y`` as well, those of
+    :func:`quantize_rows_i8` or :func:`quantize_rows_fp8`."""
+    name = "add_rms_norm"
+    dev = _current_device(name, x, 2)
+    shape = x.shape
+    x_code = _dtype_code(x)
+    w_code = _norm_operand(name, "weight", weight, dev, shape[1:])
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    if out_dtype not in _DT:
+        raise TypeError(f"unsupported dtype {out_dtype}; expected float32 or bfloat16")
+    if quant not in _QUANT:
+        raise ValueError(f"{name}: quant must be None, 'e4m3' or 'int8' (got {quant!r})")
+    r_code, total = 0, x
+    if residual is not None:
+        r_code = _norm_operand(name, "residual", residual, dev, shape)
+        total = torch.empty_like(residual)
+    y = x.new_empty(shape, dtype=out_dtype)
+    rstd = x.new_empty(shape[:1], dtype=torch.float32)
+    q = scale = None
+    if quant is not None:
+        q = x.new_empty(shape, dtype=torch.int8 if quant == "int8" else _U8)
+        scale = torch.empty_like(rstd)
+    call("hmoe_add_rms_norm", x.data_ptr(), x_code, _ptr(residual), r_code, weight.data_ptr(), w_code, float(eps),
+         shape[0], shape[1], None if residual is None else total.data_ptr(), y.data_ptr(), _DT[out_dtype],
+         rstd.data_ptr(), _ptr(q), _QUANT[quant], _ptr(scale), _stream())
+    return NormOut(y, total, rstd, q, scale)
+
+
+def add_rms_norm_bwd(dy: torch.Tensor, total: torch.Tensor, weight: torch.Tensor, rstd: torch.Tensor,
+                     d_sum: torch.Tensor | None = None, need_weight: bool = True):
+    """Gradients of :func:`add_rms_norm` from its ``sum`` and ``rstd``, for the cotangents
+    ``dy`` of ``y`` and ``d_sum`` of ``sum`` (None: none): ``(dx, d_weight)``, ``dx`` in
+    ``sum``'s type (the gradient of ``x`` and of the residual), ``d_weight`` float32
+    ``[cols]`` (None where not wanted)."""
+    name = "add_rms_norm_bwd"
+    dev = _current_device(name, total, 2)
+    shape = total.shape
+    s_code = _dtype_code(total)
+    g_code = _norm_operand(name, "dy", dy, dev, shape)
+    w_code = _norm_operand(name, "weight", weight, dev, shape[1:])
+    if _norm_operand(name, "rstd", rstd, dev, shape[:1]) != _lib.F32:
+        raise TypeError(f"{name}: rstd must be float32")
+    if d_sum is not None and _norm_operand(name, "d_sum", d_sum, dev, shape) != s_code:
+        raise TypeError(f"{name}: d_sum must have sum's dtype")
+    dx = torch.empty_like(total)
+    dw, ws, ws_bytes = None, None, 0
+    if need_weight:
+        dw = total.new_empty(shape[1:], dtype=torch.float32)
+        ws_bytes = _lib.lib().hmoe_add_rms_norm_bwd_workspace_bytes(shape[0], shape[1])
+        ws = total.new_empty(ws_bytes, dtype=_U8)
+    call("hmoe_add_rms_norm_bwd", dy.data_ptr(), g_code, total.data_ptr(), s_code, weight.data_ptr(), w_code,
+         rstd.data_ptr(), _ptr(d_sum), shape[0], shape[1], dx.data_ptr(), _ptr(dw), _ptr(ws), ws_bytes, _stream())
+    return dx, dw
+
+
+# ----------------------------------------------------------------- int8 experts --
+# A row's scale is its largest value over 127 (``hmoe_quantize_rows_i8`` has the rule), a
+# weight's row the reduction of one output column.  Served weights only, as for the e4m3
+# and MXFP4 experts.  Operands start at 16 bytes (any row of such a matrix does).
+
+_I8, _F32 = torch.int8, torch.float32
+
+
+def _codes(name: str, what: str, dev, t: torch.Tensor, dtype: torch.dtype, shape: tuple):
+    """Checks a tensor of codes or scales: its type, contiguous, on the call's device, of
+    that size."""
+    if (t.__class__ is _TENSOR and t.dtype is dtype and t.shape == shape and t.is_contiguous()
+            and t.device == dev):
+        return
+    _check(t, what)
+    if t.dtype != dtype or t.shape != shape:
+        raise ValueError(f"{name}: {what} must be {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+    _same_device(name, t, dev)
+
+
+def quantize_rows_i8(a: torch.Tensor, offsets: torch.Tensor | None = None):
+    """int8 codes and scales of the rows of a float32 or bf16 matrix ``[rows, cols]``; rows
+    at or past ``offsets[-1]`` are not read when offsets are given (codes left as
+    allocated, scale 1)."""
+    name = "quantize_rows_i8"
+    dev = _current_device(name, a, 2)
+    rows, cols = a.shape
+    q = a.new_empty((rows, cols), dtype=_I8)
+    scale = a.new_empty((rows,), dtype=_F32)
+    n = 0
+    if offsets is not None:
+        _check_i32(name, "offsets", offsets, offsets.numel(), dev)
+        n = offsets.numel() - 1
+    call("hmoe_quantize_rows_i8", a.data_ptr(), _dtype_code(a), rows, cols, _ptr(offsets), n, q.data_ptr(),
+         scale.data_ptr(), _stream())
+    return q, scale
+
+
+def _dequantize_rows(name: str, q: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype,
+                     out_dtype: torch.dtype) -> torch.Tensor:
+    dev = _current_device(name, q, 2)
+    _codes(name, "q", dev, q, dtype, q.shape)
+    _codes(name, "scale", dev, scale, _F32, q.shape[:1])
+    if out_dtype not in _DT:
+        raise TypeError(f"unsupported dtype {out_dtype}; expected float32 or bfloat16")
+    out = q.new_empty(q.shape, dtype=out_dtype)
+    call("hmoe_" + name, q.data_ptr(), scale.data_ptr(), q.shape[0], q.shape[1], out.data_ptr(), _DT[out_dtype],
+         _stream())
+    return out
+
+
+def dequantize_rows_i8(q: torch.Tensor, scale: torch.Tensor, out_dtype: torch.dtype = torch.bfloat16):
+    """The values ``[rows, cols]`` of int8 rows."""
+    return _dequantize_rows("dequantize_rows_i8", q, scale, _I8, out_dtype)
+
+
+def dequantize_rows_fp8(q: torch.Tensor, scale: torch.Tensor, out_dtype: torch.dtype = torch.bfloat16):
+    """The values ``[rows, cols]`` of e4m3 rows (:func:`quantize_rows_fp8`)."""
+    return _dequantize_rows("dequantize_rows_fp8", q, scale, _U8, out_dtype)
+
+
+def _i8_operand(N: int, rows: int, k: int, dev):
+    """Empty codes and scales of a packed operand (see ``hmoe_pack_i8_gate_up``)."""
+    codes = torch.empty((N, rows // 32, k // 32, 64, 16), dtype=_I8, device=dev)
+    return codes, torch.empty((N, rows), dtype=_F32, device=dev)
+
+
+def pack_i8_gate_up(w_gate: torch.Tensor, w_up: torch.Tensor):
+    """int8 gate/up operand of ``[N,D,F]`` masters, quantised along ``D``: codes ``[N,
+    2F/32, D/32, 64, 16]`` and scales ``[N, 2F]`` in the operand's row order."""
+    name = "pack_i8_gate_up"
+    dev = _current_device(name, w_gate, 3)
+    _check(w_up, "w_up", 3)
+    _same_device(name, w_up, dev)
+    if w_gate.shape != w_up.shape or w_gate.dtype != w_up.dtype:
+        raise ValueError("w_gate and w_up must have the same shape and dtype")
+    N, D, F = w_gate.shape
+    out, scales = _i8_operand(N, 2 * F, D, dev)
+    call("hmoe_pack_i8_gate_up", w_gate.data_ptr(), w_up.data_ptr(), _dtype_code(w_gate), N, D, F, out.data_ptr(),
+         scales.data_ptr(), _stream())
+    return out, scales
+
+
+def pack_i8_down(w_down: torch.Tensor):
+    """int8 down operand of the ``[N,F,D]`` master, quantised along ``F``: codes ``[N,
+    D/32, F/32, 64, 16]`` and scales ``[N, D]``."""
+    dev = _current_device("pack_i8_down", w_down, 3)
+    N, F, D = w_down.shape
+    out, scales = _i8_operand(N, D, F, dev)
+    call("hmoe_pack_i8_down", w_down.data_ptr(), _dtype_code(w_down), N, F, D, out.data_ptr(), scales.data_ptr(),
+         _stream())
+    return out, scales
+
+
+def _i8_sizes(name: str, packed: torch.Tensor, scales: torch.Tensor, dev):
+    """``N, rows, K`` of a packed int8 operand, its tensors checked."""
+    if packed.dim() != 5:
+        raise ValueError(f"{name}: a packed operand has 5 dims (got {tuple(packed.shape)})")
+    N, r, k = packed.shape[:3]
+    _codes(name, "packed codes", dev, packed, _I8, (N, r, k, 64, 16))
+    _codes(name, "packed scales", dev, scales, _F32, (N, 32 * r))
+    return N, 32 * r, 32 * k
+
+
+def grouped_gate_up_i8(xs_q: torch.Tensor, xs_scale: torch.Tensor, offsets: torch.Tensor,
+                       w_packed: torch.Tensor, w_scales: torch.Tensor) -> torch.Tensor:
+    """bf16 ``h = silu(g) * u`` of int8 rows in the experts' order.  Rows past
+    ``offsets[-1]`` are not written."""
+    name = "grouped_gate_up_i8"
+    dev = _current_device(name, xs_q, 2)
+    N, F2, D = _i8_sizes(name, w_packed, w_scales, dev)
+    rows, F = xs_q.shape[0], F2 // 2
+    _codes(name, "xs_q", dev, xs_q, _I8, (rows, D))
+    _codes(name, "xs_scale", dev, xs_scale, _F32, (rows,))
+    _check_i32(name, "offsets", offsets, N + 1, dev)
+    h = xs_q.new_empty((rows, F), dtype=torch.bfloat16)
+    call("hmoe_grouped_gate_up_i8", xs_q.data_ptr(), xs_scale.data_ptr(), offsets.data_ptr(), N, rows, D, F,
+         w_packed.data_ptr(), w_scales.data_ptr(), h.data_ptr(), _stream())
+    return h
+
+
+def grouped_gate_up_i8_gather(x_q: torch.Tensor, x_scale: torch.Tensor, plan: Plan,
+                              w_packed: torch.Tensor, w_scales: torch.Tensor) -> torch.Tensor:
+    """:func:`grouped_gate_up_i8` gathering its rows from the quantised tokens through
+    ``perm_src``."""
+    name = "grouped_gate_up_i8_gather"
+    dev = _current_device(name, x_q, 2)
+    N, F2, D = _i8_sizes(name, w_packed, w_scales, dev)
+    T, F = x_q.shape[0], F2 // 2
+    _codes(name, "x_q", dev, x_q, _I8, (T, D))
+    _codes(name, "x_scale", dev, x_scale, _F32, (T,))
+    if plan.n_experts != N or plan.slot_pos.numel() != T * plan.top_k:
+        raise ValueError(f"{name}: the plan is of other tokens or experts")
+    _check_i32(name, "offsets", plan.offsets, N + 1, dev)
+    _check_i32(name, "perm_src", plan.perm_src, plan.rows_cap, dev)
+    h = x_q.new_empty((plan.rows_cap, F), dtype=torch.bfloat16)
+    call("hmoe_grouped_gate_up_i8_gather", x_q.data_ptr(), x_scale.data_ptr(), T, plan.top_k,
+         plan.perm_src.data_ptr(), plan.offsets.data_ptr(), N, plan.rows_cap, D, F, w_packed.data_ptr(),
+         w_scales.data_ptr(), h.data_ptr(), _stream())
+    return h
+
+
+def grouped_down_i8(h_q: torch.Tensor, h_scale: torch.Tensor, offsets: torch.Tensor,
+                    w_packed: torch.Tensor, w_scales: torch.Tensor) -> torch.Tensor:
+    """bf16 ``ys`` of int8 rows times the int8 down operand.  Rows past ``offsets[-1]`` are
+    not written."""
+    name = "grouped_down_i8"
+    dev = _current_device(name, h_q, 2)
+    N, D, F = _i8_sizes(name, w_packed, w_scales, dev)
+    rows = h_q.shape[0]
+    _codes(name, "h_q", dev, h_q, _I8, (rows, F))
+    _codes(name, "h_scale", dev, h_scale, _F32, (rows,))
+    _check_i32(name, "offsets", offsets, N + 1, dev)
+    ys = h_q.new_empty((rows, D), dtype=torch.bfloat16)
+    call("hmoe_grouped_down_i8", h_q.data_ptr(), h_scale.data_ptr(), offsets.data_ptr(), N, rows, F, D,
+         w_packed.data_ptr(), w_scales.data_ptr(), ys.data_ptr(), _stream())
     return ys
 
 

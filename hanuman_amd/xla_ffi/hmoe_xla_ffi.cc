@@ -796,6 +796,274 @@ XLA_FFI_DEFINE_HANDLER_SYMBOL(HmoeGroupedDownMxfp4, GroupedDownMxfp4Impl,
                                   .Arg<ffi::Buffer<ffi::U8>>()
                                   .Ret<ffi::Buffer<ffi::BF16>>());
 
+// ---- root-mean-square norm with the residual's addition; int8 experts --------------
+static ffi::Error BadSizes(const char* what) {
+  return ffi::Error(ffi::ErrorCode::kInvalidArgument, std::string(what) + ": operands and results do not fit together");
+}
+template <typename X, typename Y>
+static bool SameRows(const X& x, const Y& y) {  // both [R, C]
+  return x.dimensions().size() == 2 && y.dimensions().size() == 2 && Rows(x) == Rows(y) && Cols(x) == Cols(y);
+}
+// Codes [N, rows / 32, K / 32, 64, 16] and scales [N, rows] of an int8 operand.
+template <typename Q, typename Sc>
+static bool I8Operand(const Q& q, const Sc& scales) {
+  auto d = q.dimensions();
+  auto s = scales.dimensions();
+  return d.size() == 5 && s.size() == 2 && d[3] == 64 && d[4] == 16 && s[0] == d[0] && s[1] == d[1] * 32;
+}
+// Codes [R, C] and scales [R] of int8 rows.
+template <typename Q, typename Sc>
+static bool I8Rows(const Q& q, const Sc& scale, int64_t rows, int64_t cols) {
+  return q.dimensions().size() == 2 && Rows(q) == rows && Cols(q) == cols &&
+         static_cast<int64_t>(scale.element_count()) == rows;
+}
+
+// x [R, C], residual [R, C] or of no elements, weight [C] -> sum (of no elements without a
+// residual), y [R, C], rstd [R] f32, q [R, C] (u8: e4m3, s8: int8) and scale [R] f32, both of no
+// elements where no codes are wanted.
+static ffi::Error AddRmsNormImpl(hipStream_t stream, ffi::AnyBuffer x, ffi::AnyBuffer residual,
+                                 ffi::AnyBuffer weight, float eps, ffi::Result<ffi::AnyBuffer> sum,
+                                 ffi::Result<ffi::AnyBuffer> y, ffi::ResultBuffer<ffi::F32> rstd,
+                                 ffi::Result<ffi::AnyBuffer> q, ffi::ResultBuffer<ffi::F32> scale) {
+  const char* what = "hmoe_add_rms_norm";
+  const int xd = DtypeCode(x.element_type()), rd = DtypeCode(residual.element_type());
+  const int wd = DtypeCode(weight.element_type()), yd = DtypeCode(y->element_type());
+  if (xd < 0 || rd < 0 || wd < 0 || yd < 0) return BadDtype(what);
+  const bool add = residual.element_count() > 0, codes = q->element_count() > 0;
+  const int qt = q->element_type() == ffi::DataType::S8 ? HMOE_I8 : HMOE_FP8_E4M3;
+  if (x.dimensions().size() != 2 || !SameRows(x, *y) || (add && (!SameRows(x, residual) || !SameRows(x, *sum))) ||
+      (add && sum->element_type() != residual.element_type()) ||
+      static_cast<int64_t>(weight.element_count()) != Cols(x) ||
+      static_cast<int64_t>(rstd->element_count()) != Rows(x) ||
+      (codes && (!I8Rows(*q, *scale, Rows(x), Cols(x)) ||
+                 (q->element_type() != ffi::DataType::S8 && q->element_type() != ffi::DataType::U8))))
+    return BadSizes(what);
+  return Status(hmoe_add_rms_norm(x.untyped_data(), xd, add ? residual.untyped_data() : nullptr, rd,
+                                  weight.untyped_data(), wd, eps, Rows(x), static_cast<int>(Cols(x)),
+                                  add ? sum->untyped_data() : nullptr, y->untyped_data(), yd, rstd->typed_data(),
+                                  codes ? q->untyped_data() : nullptr, qt, codes ? scale->typed_data() : nullptr,
+                                  S(stream)));
+}
+XLA_FFI_DEFINE_HANDLER_SYMBOL(HmoeAddRmsNorm, AddRmsNormImpl,
+                              ffi::Ffi::Bind()
+                                  .Ctx<ffi::PlatformStream<hipStream_t>>()
+                                  .Arg<ffi::AnyBuffer>()
+                                  .Arg<ffi::AnyBuffer>()
+                                  .Arg<ffi::AnyBuffer>()
+                                  .Attr<float>("eps")
+                                  .Ret<ffi::AnyBuffer>()
+                                  .Ret<ffi::AnyBuffer>()
+                                  .Ret<ffi::Buffer<ffi::F32>>()
+                                  .Ret<ffi::AnyBuffer>()
+                                  .Ret<ffi::Buffer<ffi::F32>>());
+
+// dy, sum [R, C], weight [C], rstd [R], d_sum [R, C] or of no elements -> dx [R, C] in sum's type,
+// d_weight [C] f32, workspace u8 (hmoe_add_rms_norm_bwd_workspace_bytes).
+static ffi::Error AddRmsNormBwdImpl(hipStream_t stream, ffi::AnyBuffer dy, ffi::AnyBuffer sum,
+                                    ffi::AnyBuffer weight, ffi::Buffer<ffi::F32> rstd, ffi::AnyBuffer d_sum,
+                                    ffi::Result<ffi::AnyBuffer> dx, ffi::ResultBuffer<ffi::F32> d_weight,
+                                    ffi::ResultBuffer<ffi::U8> workspace) {
+  const char* what = "hmoe_add_rms_norm_bwd";
+  const int gd = DtypeCode(dy.element_type()), sd = DtypeCode(sum.element_type());
+  const int wd = DtypeCode(weight.element_type());
+  if (gd < 0 || sd < 0 || wd < 0) return BadDtype(what);
+  const bool more = d_sum.element_count() > 0;
+  if (sum.dimensions().size() != 2 || !SameRows(sum, dy) || !SameRows(sum, *dx) || (more && !SameRows(sum, d_sum)) ||
+      dx->element_type() != sum.element_type() || (more && d_sum.element_type() != sum.element_type()) ||
+      static_cast<int64_t>(weight.element_count()) != Cols(sum) ||
+      static_cast<int64_t>(d_weight->element_count()) != Cols(sum) ||
+      static_cast<int64_t>(rstd.element_count()) != Rows(sum))
+    return BadSizes(what);
+  return Status(hmoe_add_rms_norm_bwd(dy.untyped_data(), gd, sum.untyped_data(), sd, weight.untyped_data(), wd,
+                                      rstd.typed_data(), more ? d_sum.untyped_data() : nullptr, Rows(sum),
+                                      static_cast<int>(Cols(sum)), dx->untyped_data(), d_weight->typed_data(),
+                                      workspace->untyped_data(), workspace->size_bytes(), S(stream)));
+}
+XLA_FFI_DEFINE_HANDLER_SYMBOL(HmoeAddRmsNormBwd, AddRmsNormBwdImpl,
+                              ffi::Ffi::Bind()
+                                  .Ctx<ffi::PlatformStream<hipStream_t>>()
+                                  .Arg<ffi::AnyBuffer>()
+                                  .Arg<ffi::AnyBuffer>()
+                                  .Arg<ffi::AnyBuffer>()
+                                  .Arg<ffi::Buffer<ffi::F32>>()
+                                  .Arg<ffi::AnyBuffer>()
+                                  .Ret<ffi::AnyBuffer>()
+                                  .Ret<ffi::Buffer<ffi::F32>>()
+                                  .Ret<ffi::Buffer<ffi::U8>>());
+
+// a [R, C] (f32/bf16), offsets [N+1] or of no elements -> q [R, C] s8, scale [R] f32.
+static ffi::Error QuantizeRowsI8Impl(hipStream_t stream, ffi::AnyBuffer a, ffi::Buffer<ffi::S32> offsets,
+                                     ffi::ResultBuffer<ffi::S8> q, ffi::ResultBuffer<ffi::F32> scale) {
+  const int d = DtypeCode(a.element_type());
+  if (d < 0) return BadDtype("hmoe_quantize_rows_i8");
+  if (a.dimensions().size() != 2 || !I8Rows(*q, *scale, Rows(a), Cols(a))) return BadSizes("hmoe_quantize_rows_i8");
+  const int64_t n = static_cast<int64_t>(offsets.element_count());
+  return Status(hmoe_quantize_rows_i8(a.untyped_data(), d, Rows(a), static_cast<int>(Cols(a)),
+                                      n > 0 ? offsets.typed_data() : nullptr, n > 0 ? static_cast<int>(n - 1) : 0,
+                                      q->typed_data(), scale->typed_data(), S(stream)));
+}
+XLA_FFI_DEFINE_HANDLER_SYMBOL(HmoeQuantizeRowsI8, QuantizeRowsI8Impl,
+                              ffi::Ffi::Bind()
+                                  .Ctx<ffi::PlatformStream<hipStream_t>>()
+                                  .Arg<ffi::AnyBuffer>()
+                                  .Arg<ffi::Buffer<ffi::S32>>()
+                                  .Ret<ffi::Buffer<ffi::S8>>()
+                                  .Ret<ffi::Buffer<ffi::F32>>());
+
+// q [R, C], scale [R] -> out [R, C] (f32/bf16).
+static ffi::Error DequantizeRowsI8Impl(hipStream_t stream, ffi::Buffer<ffi::S8> q, ffi::Buffer<ffi::F32> scale,
+                                       ffi::Result<ffi::AnyBuffer> out) {
+  const int d = DtypeCode(out->element_type());
+  if (d < 0) return BadDtype("hmoe_dequantize_rows_i8");
+  if (out->dimensions().size() != 2 || !I8Rows(q, scale, Rows(*out), Cols(*out)))
+    return BadSizes("hmoe_dequantize_rows_i8");
+  return Status(hmoe_dequantize_rows_i8(q.typed_data(), scale.typed_data(), Rows(q), static_cast<int>(Cols(q)),
+                                        out->untyped_data(), d, S(stream)));
+}
+XLA_FFI_DEFINE_HANDLER_SYMBOL(HmoeDequantizeRowsI8, DequantizeRowsI8Impl,
+                              ffi::Ffi::Bind()
+                                  .Ctx<ffi::PlatformStream<hipStream_t>>()
+                                  .Arg<ffi::Buffer<ffi::S8>>()
+                                  .Arg<ffi::Buffer<ffi::F32>>()
+                                  .Ret<ffi::AnyBuffer>());
+
+// q [R, C], scale [R] -> out [R, C] (f32/bf16).
+static ffi::Error DequantizeRowsFp8Impl(hipStream_t stream, ffi::Buffer<ffi::U8> q, ffi::Buffer<ffi::F32> scale,
+                                       ffi::Result<ffi::AnyBuffer> out) {
+  const int d = DtypeCode(out->element_type());
+  if (d < 0) return BadDtype("hmoe_dequantize_rows_fp8");
+  if (out->dimensions().size() != 2 || !I8Rows(q, scale, Rows(*out), Cols(*out)))
+    return BadSizes("hmoe_dequantize_rows_fp8");
+  return Status(hmoe_dequantize_rows_fp8(q.typed_data(), scale.typed_data(), Rows(q), static_cast<int>(Cols(q)),
+                                        out->untyped_data(), d, S(stream)));
+}
+XLA_FFI_DEFINE_HANDLER_SYMBOL(HmoeDequantizeRowsFp8, DequantizeRowsFp8Impl,
+                              ffi::Ffi::Bind()
+                                  .Ctx<ffi::PlatformStream<hipStream_t>>()
+                                  .Arg<ffi::Buffer<ffi::U8>>()
+                                  .Arg<ffi::Buffer<ffi::F32>>()
+                                  .Ret<ffi::AnyBuffer>());
+
+// w_gate, w_up [N, D, F] (f32/bf16) -> codes, scales of the gate/up operand.
+static ffi::Error PackI8GateUpImpl(hipStream_t stream, ffi::AnyBuffer wg, ffi::AnyBuffer wu,
+                                   ffi::ResultBuffer<ffi::S8> packed, ffi::ResultBuffer<ffi::F32> scales) {
+  const int d = DtypeCode(wg.element_type());
+  if (d < 0 || DtypeCode(wu.element_type()) != d) return BadDtype("hmoe_pack_i8_gate_up");
+  auto dims = wg.dimensions();
+  auto up = wu.dimensions();
+  auto out = packed->dimensions();
+  if (dims.size() != 3 || up.size() != 3 || up[0] != dims[0] || up[1] != dims[1] || up[2] != dims[2] ||
+      !I8Operand(*packed, *scales) || out[0] != dims[0] || out[1] * 16 != dims[2] || out[2] * 32 != dims[1])
+    return BadSizes("hmoe_pack_i8_gate_up");
+  return Status(hmoe_pack_i8_gate_up(wg.untyped_data(), wu.untyped_data(), d, static_cast<int>(dims[0]),
+                                     static_cast<int>(dims[1]), static_cast<int>(dims[2]), packed->typed_data(),
+                                     scales->typed_data(), S(stream)));
+}
+XLA_FFI_DEFINE_HANDLER_SYMBOL(HmoePackI8GateUp, PackI8GateUpImpl,
+                              ffi::Ffi::Bind()
+                                  .Ctx<ffi::PlatformStream<hipStream_t>>()
+                                  .Arg<ffi::AnyBuffer>()
+                                  .Arg<ffi::AnyBuffer>()
+                                  .Ret<ffi::Buffer<ffi::S8>>()
+                                  .Ret<ffi::Buffer<ffi::F32>>());
+
+// w_down [N, F, D] (f32/bf16) -> codes, scales of the down operand.
+static ffi::Error PackI8DownImpl(hipStream_t stream, ffi::AnyBuffer wd, ffi::ResultBuffer<ffi::S8> packed,
+                                 ffi::ResultBuffer<ffi::F32> scales) {
+  const int d = DtypeCode(wd.element_type());
+  if (d < 0) return BadDtype("hmoe_pack_i8_down");
+  auto dims = wd.dimensions();
+  auto out = packed->dimensions();
+  if (dims.size() != 3 || !I8Operand(*packed, *scales) || out[0] != dims[0] || out[1] * 32 != dims[2] ||
+      out[2] * 32 != dims[1])
+    return BadSizes("hmoe_pack_i8_down");
+  return Status(hmoe_pack_i8_down(wd.untyped_data(), d, static_cast<int>(dims[0]), static_cast<int>(dims[1]),
+                                  static_cast<int>(dims[2]), packed->typed_data(), scales->typed_data(), S(stream)));
+}
+XLA_FFI_DEFINE_HANDLER_SYMBOL(HmoePackI8Down, PackI8DownImpl,
+                              ffi::Ffi::Bind()
+                                  .Ctx<ffi::PlatformStream<hipStream_t>>()
+                                  .Arg<ffi::AnyBuffer>()
+                                  .Ret<ffi::Buffer<ffi::S8>>()
+                                  .Ret<ffi::Buffer<ffi::F32>>());
+
+// xs_q [rows, D], xs_scale [rows], offsets [N+1], gate/up operand -> h [rows, F] bf16.
+static ffi::Error GroupedGateUpI8Impl(hipStream_t stream, ffi::Buffer<ffi::S8> xs_q, ffi::Buffer<ffi::F32> xs_scale,
+                                      ffi::Buffer<ffi::S32> offsets, ffi::Buffer<ffi::S8> w,
+                                      ffi::Buffer<ffi::F32> w_scales, ffi::ResultBuffer<ffi::BF16> h) {
+  auto d = w.dimensions();
+  const int64_t n = static_cast<int64_t>(offsets.element_count()) - 1;
+  if (!I8Operand(w, w_scales) || d[0] != n || !I8Rows(xs_q, xs_scale, Rows(xs_q), d[2] * 32) ||
+      h->dimensions().size() != 2 || Rows(*h) != Rows(xs_q) || Cols(*h) != d[1] * 16)
+    return BadSizes("hmoe_grouped_gate_up_i8");
+  return Status(hmoe_grouped_gate_up_i8(xs_q.typed_data(), xs_scale.typed_data(), offsets.typed_data(),
+                                        static_cast<int>(n), Rows(xs_q), static_cast<int>(d[2] * 32),
+                                        static_cast<int>(d[1] * 16), w.typed_data(), w_scales.typed_data(),
+                                        h->untyped_data(), S(stream)));
+}
+XLA_FFI_DEFINE_HANDLER_SYMBOL(HmoeGroupedGateUpI8, GroupedGateUpI8Impl,
+                              ffi::Ffi::Bind()
+                                  .Ctx<ffi::PlatformStream<hipStream_t>>()
+                                  .Arg<ffi::Buffer<ffi::S8>>()
+                                  .Arg<ffi::Buffer<ffi::F32>>()
+                                  .Arg<ffi::Buffer<ffi::S32>>()
+                                  .Arg<ffi::Buffer<ffi::S8>>()
+                                  .Arg<ffi::Buffer<ffi::F32>>()
+                                  .Ret<ffi::Buffer<ffi::BF16>>());
+
+// x_q [T, D], x_scale [T], perm_src [rows], offsets [N+1], gate/up operand -> h [rows, F] bf16.
+static ffi::Error GroupedGateUpI8GatherImpl(hipStream_t stream, ffi::Buffer<ffi::S8> x_q,
+                                            ffi::Buffer<ffi::F32> x_scale, ffi::Buffer<ffi::S32> perm_src,
+                                            ffi::Buffer<ffi::S32> offsets, ffi::Buffer<ffi::S8> w,
+                                            ffi::Buffer<ffi::F32> w_scales, int64_t top_k,
+                                            ffi::ResultBuffer<ffi::BF16> h) {
+  auto d = w.dimensions();
+  const int64_t n = static_cast<int64_t>(offsets.element_count()) - 1;
+  const int64_t rows = static_cast<int64_t>(perm_src.element_count());
+  if (!I8Operand(w, w_scales) || d[0] != n || !I8Rows(x_q, x_scale, Rows(x_q), d[2] * 32) ||
+      h->dimensions().size() != 2 || Rows(*h) != rows || Cols(*h) != d[1] * 16)
+    return BadSizes("hmoe_grouped_gate_up_i8_gather");
+  return Status(hmoe_grouped_gate_up_i8_gather(
+      x_q.typed_data(), x_scale.typed_data(), Rows(x_q), static_cast<int>(top_k), perm_src.typed_data(),
+      offsets.typed_data(), static_cast<int>(n), rows, static_cast<int>(d[2] * 32), static_cast<int>(d[1] * 16),
+      w.typed_data(), w_scales.typed_data(), h->untyped_data(), S(stream)));
+}
+XLA_FFI_DEFINE_HANDLER_SYMBOL(HmoeGroupedGateUpI8Gather, GroupedGateUpI8GatherImpl,
+                              ffi::Ffi::Bind()
+                                  .Ctx<ffi::PlatformStream<hipStream_t>>()
+                                  .Arg<ffi::Buffer<ffi::S8>>()
+                                  .Arg<ffi::Buffer<ffi::F32>>()
+                                  .Arg<ffi::Buffer<ffi::S32>>()
+                                  .Arg<ffi::Buffer<ffi::S32>>()
+                                  .Arg<ffi::Buffer<ffi::S8>>()
+                                  .Arg<ffi::Buffer<ffi::F32>>()
+                                  .Attr<int64_t>("top_k")
+                                  .Ret<ffi::Buffer<ffi::BF16>>());
+
+// h_q [rows, F], h_scale [rows], offsets [N+1], down operand -> ys [rows, D] bf16.
+static ffi::Error GroupedDownI8Impl(hipStream_t stream, ffi::Buffer<ffi::S8> h_q, ffi::Buffer<ffi::F32> h_scale,
+                                    ffi::Buffer<ffi::S32> offsets, ffi::Buffer<ffi::S8> w,
+                                    ffi::Buffer<ffi::F32> w_scales, ffi::ResultBuffer<ffi::BF16> ys) {
+  auto d = w.dimensions();
+  const int64_t n = static_cast<int64_t>(offsets.element_count()) - 1;
+  if (!I8Operand(w, w_scales) || d[0] != n || !I8Rows(h_q, h_scale, Rows(h_q), d[2] * 32) ||
+      ys->dimensions().size() != 2 || Rows(*ys) != Rows(h_q) || Cols(*ys) != d[1] * 32)
+    return BadSizes("hmoe_grouped_down_i8");
+  return Status(hmoe_grouped_down_i8(h_q.typed_data(), h_scale.typed_data(), offsets.typed_data(),
+                                     static_cast<int>(n), Rows(h_q), static_cast<int>(d[2] * 32),
+                                     static_cast<int>(d[1] * 32), w.typed_data(), w_scales.typed_data(),
+                                     ys->untyped_data(), S(stream)));
+}
+XLA_FFI_DEFINE_HANDLER_SYMBOL(HmoeGroupedDownI8, GroupedDownI8Impl,
+                              ffi::Ffi::Bind()
+                                  .Ctx<ffi::PlatformStream<hipStream_t>>()
+                                  .Arg<ffi::Buffer<ffi::S8>>()
+                                  .Arg<ffi::Buffer<ffi::F32>>()
+                                  .Arg<ffi::Buffer<ffi::S32>>()
+                                  .Arg<ffi::Buffer<ffi::S8>>()
+                                  .Arg<ffi::Buffer<ffi::F32>>()
+                                  .Ret<ffi::Buffer<ffi::BF16>>());
+
 // float32 compute dtype: masters as they are.
 static ffi::Error GroupedGateUpF32Impl(hipStream_t stream, ffi::Buffer<ffi::F32> xs,
                                        ffi::Buffer<ffi::S32> offsets,

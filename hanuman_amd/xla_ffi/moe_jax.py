@@ -83,6 +83,16 @@ TARGETS = {
     "hmoe_grouped_gate_up_mxfp4": "HmoeGroupedGateUpMxfp4",
     "hmoe_grouped_gate_up_mxfp4_gather": "HmoeGroupedGateUpMxfp4Gather",
     "hmoe_grouped_down_mxfp4": "HmoeGroupedDownMxfp4",
+    "hmoe_add_rms_norm": "HmoeAddRmsNorm",
+    "hmoe_add_rms_norm_bwd": "HmoeAddRmsNormBwd",
+    "hmoe_quantize_rows_i8": "HmoeQuantizeRowsI8",
+    "hmoe_dequantize_rows_i8": "HmoeDequantizeRowsI8",
+    "hmoe_dequantize_rows_fp8": "HmoeDequantizeRowsFp8",
+    "hmoe_pack_i8_gate_up": "HmoePackI8GateUp",
+    "hmoe_pack_i8_down": "HmoePackI8Down",
+    "hmoe_grouped_gate_up_i8": "HmoeGroupedGateUpI8",
+    "hmoe_grouped_gate_up_i8_gather": "HmoeGroupedGateUpI8Gather",
+    "hmoe_grouped_down_i8": "HmoeGroupedDownI8",
     "hmoe_grouped_gate_up_f32": "HmoeGroupedGateUpF32",
     "hmoe_grouped_down_f32": "HmoeGroupedDownF32",
     "hmoe_combine": "HmoeCombine",
@@ -127,6 +137,7 @@ def _core():
             ("hmoe_aux_workspace_bytes", sz, [i32, i32, i32]),
             ("hmoe_aux_bwd_workspace_bytes", sz, [i32, i32, i32]),
             ("hmoe_router_dw_workspace_bytes", sz, [i64, i32, i32]),
+            ("hmoe_add_rms_norm_bwd_workspace_bytes", sz, [i64, i32]),
             ("hmoe_packed_gate_up_bytes", sz, [i32, i32, i32]),
             ("hmoe_packed_down_bytes", sz, [i32, i32, i32]),
             ("hmoe_grouped_swiglu_fused_workspace_bytes", sz, [i64, i32])):

@@ -37,7 +37,7 @@ enum {
   HMOE_ERR_WORKSPACE = 4    /* workspace too small                         */
 };
 
-enum { HMOE_F32 = 0, HMOE_BF16 = 1, HMOE_FP8_E4M3 = 2 };
+enum { HMOE_F32 = 0, HMOE_BF16 = 1, HMOE_FP8_E4M3 = 2, HMOE_I8 = 3 };
 
 enum {
   HMOE_ROUTE_SIGMOID_BIAS = 0, /* moe.py:179-192: top-k of sigmoid(l)+bias,
@@ -469,6 +469,97 @@ int hmoe_grouped_down_mxfp4(const uint8_t* h_q, const uint8_t* h_exp, const int3
                             int n_experts, int64_t rows_cap, int d_ff, int d_model,
                             const uint8_t* w_packed, const uint8_t* w_exp, void* ys,
                             hmoe_stream_t stream);
+
+/* ---- root-mean-square norm with the residual's addition (the reference's Block norms what
+ *      it gives the layer, model/transformer.py:14-24, 82-95; no counterpart in moe.py) -------- */
+
+/* sum = rnd(x + residual) in the residual's type, rstd = (mean_d sum^2 + eps)^(-1/2) of the
+ * rounded sum, y = rnd(sum * rstd * weight); float32 sums in a fixed order.  x, y, residual and
+ * weight are F32 or BF16 each, [rows, cols] and [cols].  Without a residual (NULL, then sum NULL
+ * too) the norm is x's.  rstd [rows] f32 (or NULL) is what the gradients need.  q (or NULL, then
+ * scale NULL too) [rows, cols] and scale [rows] f32: the 8-bit codes of the rounded y, HMOE_I8 by
+ * the rule of hmoe_quantize_rows_i8 or HMOE_FP8_E4M3 by that of hmoe_quantize_rows_fp8 (the same
+ * bits as those calls on y).  cols % 8 == 0, up to 32768; matrices 16-byte aligned, q 8-byte.
+ * sum may be x or residual where the types agree, y may be x: a row is read before it is written. */
+int hmoe_add_rms_norm(const void* x, int x_dtype, const void* residual, int residual_dtype,
+                      const void* weight, int w_dtype, float eps, int64_t rows, int cols, void* sum,
+                      void* y, int y_dtype, float* rstd, void* q, int q_type, float* scale,
+                      hmoe_stream_t stream);
+/* Its gradients for the cotangents dy of y and d_sum of sum (NULL: none), with n = sum * rstd:
+ *   dx [rows, cols] = d_sum + rstd * (dy * weight - n * mean_d(dy * weight * n)), in sum's type:
+ *      the gradient of x and of the residual;
+ *   d_weight [cols] f32 (NULL: not wanted) = sum over the rows of dy * n, in at most 1024 parts,
+ *      each summed row by row, then one after another.
+ * sum, d_sum and dx have one type, dy and weight their own (F32 or BF16).  Zero rows write a zero
+ * d_weight.  workspace >= hmoe_add_rms_norm_bwd_workspace_bytes where d_weight is wanted.  dx may
+ * be d_sum, sum or (of one type) dy. */
+size_t hmoe_add_rms_norm_bwd_workspace_bytes(int64_t rows, int cols);
+int hmoe_add_rms_norm_bwd(const void* dy, int dy_dtype, const void* sum, int sum_dtype,
+                          const void* weight, int w_dtype, const float* rstd, const void* d_sum,
+                          int64_t rows, int cols, void* dx, float* d_weight, void* workspace,
+                          size_t workspace_bytes, hmoe_stream_t stream);
+
+/* ---- int8 experts (no reference code): 8-bit rows times 8-bit weights ------------------------
+ *
+ * A row's scale is its largest |v| / 127 and a code v * (127 / largest) rounded to nearest even
+ * (float32, both quotients correctly rounded; a row of zeros has scale 1).  A weight's row is the
+ * reduction dimension of one output column.  A row with a value that is not finite has zero codes
+ * and a scale that is not finite: what is made of it is NaN.  Codes 16-byte aligned in the
+ * products, 8-byte elsewhere. */
+
+/* a [rows, cols] (F32/BF16) -> q [rows, cols] int8, scale [rows] f32.  With offsets != NULL, rows
+ * at or past offsets[n_experts] are not read: codes left untouched, scale 1.  cols % 8 == 0, up
+ * to 32768. */
+int hmoe_quantize_rows_i8(const void* a, int a_dtype, int64_t rows, int cols, const int32_t* offsets,
+                          int n_experts, int8_t* q, float* scale, hmoe_stream_t stream);
+/* The values of int8 and of e4m3 rows (code * scale in float32), out [rows, cols] (F32/BF16).
+ * cols % 8 == 0. */
+int hmoe_dequantize_rows_i8(const int8_t* q, const float* scale, int64_t rows, int cols, void* out,
+                            int out_dtype, hmoe_stream_t stream);
+int hmoe_dequantize_rows_fp8(const uint8_t* q, const float* scale, int64_t rows, int cols, void* out,
+                             int out_dtype, hmoe_stream_t stream);
+/* Expert masters (F32/BF16) quantised along the reduction into the products' operands.  Operand
+ * rows are those of hmoe_pack_gate_up (2F an expert, 32 gate and 32 up columns alternating) and
+ * hmoe_pack_down (D an expert).  With K the reduction (D, F):
+ *   codes  [N][rows / 32][K / 32][64][16]: bytes of lane 32 h + r hold the 16 codes of row r (of
+ *          the 32) from column 16 h (of the 32) on
+ *   scales [N][rows] f32
+ * D % 128 == 0, F % 128 == 0, both up to 32768, N <= 1024. */
+size_t hmoe_packed_i8_gate_up_bytes(int n_experts, int d_model, int d_ff);
+int hmoe_pack_i8_gate_up(const void* w_gate, const void* w_up, int w_dtype, int n_experts,
+                         int d_model, int d_ff, int8_t* packed, float* scales, hmoe_stream_t stream);
+size_t hmoe_packed_i8_down_bytes(int n_experts, int d_ff, int d_model);
+int hmoe_pack_i8_down(const void* w_down, int w_dtype, int n_experts, int d_ff, int d_model,
+                      int8_t* packed, float* scales, hmoe_stream_t stream);
+/* The form in which the products below run `kdim` values of the reduction and `ncols` columns
+ * (gate/up: 2 d_ff) on a device of `cus` CUs: 0 and 1, 32 rows from memory into registers, the
+ * reduction split over four waves in 1; 2 and 3, tiles of 64 and 128 rows through LDS.  -1 for
+ * sizes that they refuse and for no rows.  A host-side query: the sums are exact integers, so
+ * every form gives the same bits. */
+int64_t hmoe_grouped_i8_form(int64_t rows_cap, int n_experts, int kdim, int ncols, int cus);
+/* h[r, :] = bf16(silu(g) * u) of rows r of expert e's segment [offsets[e], offsets[e+1]), with g
+ * and u the integer sums of xs[r]·Wg[e] and xs[r]·Wu[e] rounded to float32, times the column's,
+ * then the row's scale; the SwiGLU in float32.  xs_q [rows_cap, D], xs_scale [rows_cap], h
+ * [rows_cap, F] bf16.  Rows past offsets[N] are not written.  D % 128 == 0, F % 128 == 0, both up
+ * to 32768, N <= 1024, rows_cap <= 2^30, (rows_cap / 64 + N) * (2F / 256, down D / 256), each
+ * rounded up, at most 2^30. */
+int hmoe_grouped_gate_up_i8(const int8_t* xs_q, const float* xs_scale, const int32_t* offsets,
+                            int n_experts, int64_t rows_cap, int d_model, int d_ff,
+                            const int8_t* w_packed, const float* w_scales, void* h,
+                            hmoe_stream_t stream);
+/* The same h with the rows gathered by the product's loads: x_q [tokens, D] and x_scale [tokens]
+ * are the quantised tokens and row r is token perm_src[r] / top_k (token 0 where perm_src[r] is
+ * -1).  tokens * D < 2^31. */
+int hmoe_grouped_gate_up_i8_gather(const int8_t* x_q, const float* x_scale, int64_t tokens, int top_k,
+                                   const int32_t* perm_src, const int32_t* offsets, int n_experts,
+                                   int64_t rows_cap, int d_model, int d_ff, const int8_t* w_packed,
+                                   const float* w_scales, void* h, hmoe_stream_t stream);
+/* ys[r, :] = bf16 of h[r]·Wd[e], scaled likewise, ys [rows_cap, D] bf16.  Rows past offsets[N]
+ * are not written. */
+int hmoe_grouped_down_i8(const int8_t* h_q, const float* h_scale, const int32_t* offsets,
+                         int n_experts, int64_t rows_cap, int d_ff, int d_model,
+                         const int8_t* w_packed, const float* w_scales, void* ys,
+                         hmoe_stream_t stream);
 
 /* ---- combine: moe.py:80-85 (replaces `ys[inv]` and the weighted einsum) - */
 
