@@ -12,6 +12,7 @@
 #include "hmoe_common.h"
 #include "quant_e4m3.h"
 #include "quant_mxfp4.h"
+#include "route_groups.h"
 
 namespace hmoe {
 namespace {
@@ -956,6 +957,64 @@ __global__ __launch_bounds__(256) void select_kernel_g8(const float* __restrict_
                    gates + tq * top_k);
 }
 
+// Selection and gates among the experts of the best groups from given logits.  A wave takes 64
+// >> log_lanes tokens, whose logits, one run of memory, go through LDS: a lane reads E of them
+// one after another (a word more every 32, so that the lanes' words are in different banks).
+template <int E>
+__global__ __launch_bounds__(256) void select_groups_kernel(const float* __restrict__ logits,
+                                                            const float* __restrict__ bias, int64_t tokens,
+                                                            GroupRule r, int32_t* __restrict__ top_idx,
+                                                            float* __restrict__ gates) {
+  extern __shared__ float stage[];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int per_wave = 64 >> r.log_lanes;
+  const int64_t t0 = (static_cast<int64_t>(blockIdx.x) * 4 + wave) * per_wave;
+  if (t0 >= tokens) return;  // uniform per wave; no barrier follows
+  const int count = static_cast<int>(tokens - t0 < per_wave ? tokens - t0 : per_wave) * r.n_experts;
+  float* mine = stage + wave * (per_wave * r.n_experts / 32 * 33 + 33);
+  const float* src = logits + t0 * r.n_experts;
+  for (int i = lane; i < count; i += 64) mine[i + (i >> 5)] = src[i];
+  const int64_t tok = t0 + (lane >> r.log_lanes);
+  const bool store = tok < tokens;
+  const int row = store ? static_cast<int>(tok - t0) * r.n_experts : 0;
+  // (a wave's LDS accesses run in their order)
+  asm volatile("" ::: "memory");
+  const auto get = [&](int e) __attribute__((always_inline)) {
+    const int i = row + e;
+    return mine[i + (i >> 5)];
+  };
+  const int64_t tq = store ? tok : t0;
+  select_in_groups<E>(get, bias, r, store, top_idx + tq * r.top_k, gates + tq * r.top_k);
+}
+
+template <int E>
+void launch_select_groups(const float* logits, const float* bias, int64_t tokens, int n_experts, int n_groups,
+                          int top_groups, int top_k, int mode, float rsf, int32_t* top_idx, float* gates,
+                          hipStream_t s) {
+  const GroupRule r = group_rule(n_experts, n_groups, top_groups, top_k, mode, rsf, E);
+  const int per_wave = 64 >> r.log_lanes;
+  const size_t lds = static_cast<size_t>(4) * (per_wave * n_experts / 32 * 33 + 33) * sizeof(float);
+  hipLaunchKernelGGL((select_groups_kernel<E>), dim3(static_cast<unsigned>(ceil_div(tokens, 4 * per_wave))), dim3(256),
+                     lds, s, logits, bias, tokens, r, top_idx, gates);
+}
+
+// E: as many keys a lane as leave a token eight lanes and more.
+void select_groups(const float* logits, const float* bias, int64_t tokens, int n_experts, int n_groups,
+                   int top_groups, int top_k, int mode, float rsf, int32_t* top_idx, float* gates, hipStream_t s) {
+  const auto run = [&](auto E) {
+    launch_select_groups<decltype(E)::value>(logits, bias, tokens, n_experts, n_groups, top_groups, top_k, mode, rsf,
+                                             top_idx, gates, s);
+  };
+  const int size = n_experts / n_groups;
+  int groups = 1;
+  while (groups < n_groups) groups *= 2;
+  const int keys = groups >= 8 ? size : (size * groups + 7) / 8;  // for one lane
+  if (keys <= 4) run(IntC<4>());
+  else if (keys <= 8) run(IntC<8>());
+  else if (keys <= 16) run(IntC<16>());
+  else run(IntC<32>());
+}
+
 // CU count of the stream's device (0 if it cannot be queried), cached per device.
 int stream_cus(hipStream_t s) {
   int dev = 0;
@@ -1094,6 +1153,21 @@ int validate_routing(int64_t tokens, int n_experts, int top_k, int mode) {
   return HMOE_OK;
 }
 
+int validate_groups(int n_experts, int top_k, int mode, int n_groups, int top_groups) {
+  HMOE_REQUIRE(n_groups >= 1 && n_groups <= kMaxGroups && n_experts % n_groups == 0,
+               "router: n_groups must divide n_experts and be in [1, %d] (got %d, n_experts %d)", kMaxGroups, n_groups,
+               n_experts);
+  HMOE_REQUIRE(top_groups >= 1 && top_groups <= n_groups, "router: top_groups must be in [1, n_groups] (got %d of %d)",
+               top_groups, n_groups);
+  const int size = n_experts / n_groups;
+  HMOE_REQUIRE(top_groups == n_groups || mode == HMOE_ROUTE_SOFTMAX || size >= 2,
+               "router: a group's score is the sum of two: groups need two experts (n_experts %d in %d groups)",
+               n_experts, n_groups);
+  HMOE_REQUIRE(top_k <= top_groups * size, "router: top_k %d of the %d experts that top_groups %d leave", top_k,
+               top_groups * size, top_groups);
+  return HMOE_OK;
+}
+
 }  // namespace
 }  // namespace hmoe
 
@@ -1181,4 +1255,40 @@ extern "C" int hmoe_router_from_logits(const float* logits, const float* bias, i
   else
     hipLaunchKernelGGL(select_kernel<4>, grid, dim3(256), 0, s, logits, bias, tokens, n_experts, top_k, mode, routed_scaling_factor, top_idx, gates);
   return check_launch("hmoe_router_from_logits");
+}
+
+extern "C" int hmoe_router_grouped(const void* x, int x_dtype, const void* router_w, int w_dtype, const float* bias,
+                                   int64_t tokens, int d_model, int n_experts, int top_k, int mode,
+                                   float routed_scaling_factor, int n_groups, int top_groups, float* logits,
+                                   int32_t* top_idx, float* gates, hmoe_stream_t stream) {
+  using namespace hmoe;
+  if (int rc = validate_routing(tokens, n_experts, top_k, mode)) return rc;
+  if (int rc = validate_groups(n_experts, top_k, mode, n_groups, top_groups)) return rc;
+  if (top_groups == n_groups)  // every expert is left
+    return hmoe_router(x, x_dtype, router_w, w_dtype, bias, tokens, d_model, n_experts, top_k, mode,
+                       routed_scaling_factor, logits, top_idx, gates, stream);
+  // the logits (and the largest one's expert, which is written over)
+  if (int rc = hmoe_router(x, x_dtype, router_w, w_dtype, nullptr, tokens, d_model, n_experts, 1, HMOE_ROUTE_SOFTMAX,
+                           1.0f, logits, top_idx, gates, stream))
+    return rc;
+  if (tokens == 0) return HMOE_OK;
+  select_groups(logits, mode == HMOE_ROUTE_SIGMOID_BIAS ? bias : nullptr, tokens, n_experts, n_groups, top_groups,
+                top_k, mode, routed_scaling_factor, top_idx, gates, static_cast<hipStream_t>(stream));
+  return check_launch("hmoe_router_grouped");
+}
+
+extern "C" int hmoe_router_grouped_from_logits(const float* logits, const float* bias, int64_t tokens, int n_experts,
+                                               int top_k, int mode, float routed_scaling_factor, int n_groups,
+                                               int top_groups, int32_t* top_idx, float* gates, hmoe_stream_t stream) {
+  using namespace hmoe;
+  if (int rc = validate_routing(tokens, n_experts, top_k, mode)) return rc;
+  if (int rc = validate_groups(n_experts, top_k, mode, n_groups, top_groups)) return rc;
+  if (top_groups == n_groups)
+    return hmoe_router_from_logits(logits, bias, tokens, n_experts, top_k, mode, routed_scaling_factor, top_idx, gates,
+                                   stream);
+  if (tokens == 0) return HMOE_OK;
+  HMOE_REQUIRE(logits && top_idx && gates, "router_grouped_from_logits: null pointer argument");
+  select_groups(logits, mode == HMOE_ROUTE_SIGMOID_BIAS ? bias : nullptr, tokens, n_experts, n_groups, top_groups,
+                top_k, mode, routed_scaling_factor, top_idx, gates, static_cast<hipStream_t>(stream));
+  return check_launch("hmoe_router_grouped_from_logits");
 }

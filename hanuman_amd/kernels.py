@@ -78,13 +78,33 @@ def _router_operands(x, router_w, bias, top_k: int):
     return T, D, N, logits, top_idx, gates
 
 
+def _whole_groups(name: str, n_experts: int, n_groups: int):
+    """Refuses groups that are no groups, where all of them are taken."""
+    if n_groups != 1 and (n_groups < 1 or n_experts % n_groups):
+        raise ValueError(f"{name}: n_groups must divide n_experts (got {n_groups}, {n_experts})")
+
+
 def router(x: torch.Tensor, router_w: torch.Tensor, bias: torch.Tensor | None, top_k: int,
-           mode: int = _lib.ROUTE_SIGMOID_BIAS, routed_scaling_factor: float = 1.0):
+           mode: int = _lib.ROUTE_SIGMOID_BIAS, routed_scaling_factor: float = 1.0,
+           n_groups: int = 1, top_groups: int | None = None):
     """Router logits, top-k indices and gates (``moe.py:175-192``).
 
-    ``x [T,D]``, ``router_w [D,N]``, ``bias [N]`` float32 or None.
+    ``x [T,D]``, ``router_w [D,N]``, ``bias [N]`` float32 or None.  ``n_groups``,
+    ``top_groups`` (None: all): the experts are taken from the ``top_groups`` best of
+    ``n_groups`` groups (``hmoe_router_grouped``).
     Returns (logits f32 [T,N], top_idx i32 [T,K], gates f32 [T,K]).
     """
+    top_groups = n_groups if top_groups is None else top_groups
+    if top_groups != n_groups:
+        dev = _current_device("router", x, 2)
+        T, D, N, logits, top_idx, gates = _router_operands(x, router_w, bias, top_k)
+        for t in (router_w,) if bias is None else (router_w, bias):
+            _same_device("router", t, dev)
+        call("hmoe_router_grouped", _ptr(x), _dtype_code(x), _ptr(router_w), _dtype_code(router_w),
+             _ptr(bias), T, D, N, top_k, mode, float(routed_scaling_factor), n_groups, top_groups,
+             _ptr(logits), _ptr(top_idx), _ptr(gates), _stream())
+        return logits, top_idx, gates
+    _whole_groups("router", router_w.shape[-1], n_groups)
     T, D, N, logits, top_idx, gates = _router_operands(x, router_w, bias, top_k)
     call("hmoe_router", _ptr(x), _dtype_code(x), _ptr(router_w), _dtype_code(router_w),
          _ptr(bias), T, D, N, top_k, mode, float(routed_scaling_factor), _ptr(logits),
@@ -134,8 +154,10 @@ def router_quant_mxfp4(x: torch.Tensor, router_w: torch.Tensor, bias: torch.Tens
 
 
 def router_from_logits(logits: torch.Tensor, bias: torch.Tensor | None, top_k: int,
-                       mode: int = _lib.ROUTE_SOFTMAX, routed_scaling_factor: float = 1.0):
-    """Top-k indices and gates from given float32 logits [T,N]."""
+                       mode: int = _lib.ROUTE_SOFTMAX, routed_scaling_factor: float = 1.0,
+                       n_groups: int = 1, top_groups: int | None = None):
+    """Top-k indices and gates from given float32 logits [T,N]; groups as for
+    :func:`router`."""
     _check(logits, "logits", 2)
     if logits.dtype != torch.float32:
         raise TypeError("logits must be float32")
@@ -146,6 +168,14 @@ def router_from_logits(logits: torch.Tensor, bias: torch.Tensor | None, top_k: i
             raise ValueError("bias must be float32 [n_experts]")
     top_idx = torch.empty((T, top_k), dtype=torch.int32, device=logits.device)
     gates = torch.empty((T, top_k), dtype=torch.float32, device=logits.device)
+    if top_groups is not None and top_groups != n_groups:
+        dev = _current_device("router_from_logits", logits, 2)
+        if bias is not None:
+            _same_device("router_from_logits", bias, dev)
+        call("hmoe_router_grouped_from_logits", _ptr(logits), _ptr(bias), T, N, top_k, mode,
+             float(routed_scaling_factor), n_groups, top_groups, _ptr(top_idx), _ptr(gates), _stream())
+        return top_idx, gates
+    _whole_groups("router_from_logits", N, n_groups)
     call("hmoe_router_from_logits", _ptr(logits), _ptr(bias), T, N, top_k, mode,
          float(routed_scaling_factor), _ptr(top_idx), _ptr(gates), _stream())
     return top_idx, gates

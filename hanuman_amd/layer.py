@@ -6,7 +6,7 @@ entirely through ``libhanuman_moe.so``; ``forward`` is the step ``bench.py``
 times and the GPU tests check.  With bf16 tokens and SwiGLU experts the
 permutation is fused into the gate/up GEMM (``xs`` is then ``None``); with
 fp8 experts on bf16 tokens the gate/up GEMM gathers from the per-token codes,
-with mxfp4 experts from the tokens' 4-bit rows.
+with mxfp4 experts from the tokens' 4-bit rows, with int8 experts from their int8 rows.
 """
 from __future__ import annotations
 
@@ -23,12 +23,13 @@ class DeviceLayer:
     def __init__(self, inp: Inputs, device: str | torch.device = "cuda",
                  fused_ffn: bool | None = None):
         wl: Workload = inp.wl
-        if wl.expert_dtype not in ("bf16", "fp8", "f32", "mxfp4"):
+        if wl.expert_dtype not in ("bf16", "fp8", "f32", "mxfp4", "int8"):
             raise NotImplementedError(f"{wl.name}: expert dtype {wl.expert_dtype} is not built")
         self.wl = wl
         self.fp8 = wl.expert_dtype == "fp8"
         self.f32 = wl.expert_dtype == "f32"
         self.mxfp4 = wl.expert_dtype == "mxfp4"
+        self.i8 = wl.expert_dtype == "int8"
         dev = torch.device(device)
         self.device = dev
         self.x = torch.from_numpy(inp.x).to(dev, _TORCH_DT[wl.x_dtype]).contiguous()
@@ -58,6 +59,8 @@ class DeviceLayer:
                 self.w_gate_up, self.w_gate_up_scale = K.pack_fp8_gate_up(wg, wu)
             elif self.mxfp4:
                 self.w_gate_up, self.w_gate_up_exp = K.pack_mxfp4_gate_up(wg, wu)
+            elif self.i8:
+                self.w_gate_up, self.w_gate_up_scale = K.pack_i8_gate_up(wg, wu)
             else:
                 self.w_gate_up = K.pack_gate_up(wg, wu)
             del wg, wu
@@ -66,12 +69,14 @@ class DeviceLayer:
                 self.w_down, self.w_down_scale = K.pack_fp8_down(wd)
             elif self.mxfp4:
                 self.w_down, self.w_down_exp = K.pack_mxfp4_down(wd)
+            elif self.i8:
+                self.w_down, self.w_down_scale = K.pack_i8_down(wd)
             else:
                 self.w_down = K.pack_down(wd)
             del wd
         # bf16 SwiGLU experts on bf16 tokens: the gate/up GEMM gathers its rows
         # from x itself (hmoe_grouped_gate_up_gather), no dispatched copy.
-        self.fused_dispatch = (wl.expert == "swiglu" and not self.fp8 and not self.mxfp4
+        self.fused_dispatch = (wl.expert == "swiglu" and not self.fp8 and not self.mxfp4 and not self.i8
                                and self.x.dtype == torch.bfloat16)
         # fp8 experts on bf16 tokens: x is quantised per token and the gate/up
         # GEMM gathers from its codes (hmoe_grouped_gate_up_fp8_gather).
@@ -148,6 +153,14 @@ class DeviceLayer:
         ys = K.grouped_down_mxfp4(h_q, h_e, plan.offsets, self.w_down, self.w_down_exp)
         return x_q, x_e, h_q, h_e, ys
 
+    def experts_i8(self, plan):
+        """int8 tokens and expert GEMMs: (x_q, x_scale, h_q, h_scale, ys), codes and scales of
+        the tokens and of h, which is quantised by rows between the products."""
+        x_q, x_s = K.quantize_rows_i8(self.x)
+        h = K.grouped_gate_up_i8_gather(x_q, x_s, plan, self.w_gate_up, self.w_gate_up_scale)
+        h_q, h_s = K.quantize_rows_i8(h, plan.offsets)
+        return x_q, x_s, h_q, h_s, K.grouped_down_i8(h_q, h_s, plan.offsets, self.w_down, self.w_down_scale)
+
     def forward(self) -> dict:
         wl = self.wl
         logits, top_idx, gates, xq = self.route_quant()
@@ -162,6 +175,10 @@ class DeviceLayer:
             x_q, x_e, h_q, h_e, ys = self.experts_mxfp4(plan, xq)
             xs = None
             extra = {"x_q": x_q, "x_exp": x_e, "h_q": h_q, "h_exp": h_e}
+        elif self.i8 and wl.expert == "swiglu":
+            x_q, x_s, h_q, h_s, ys = self.experts_i8(plan)
+            xs = None
+            extra = {"x_q": x_q, "x_scale": x_s, "h_q": h_q, "h_scale": h_s}
         elif self.f32:
             xs = K.permute_rows(self.x, plan, torch.float32)
             h = K.grouped_gate_up_f32(xs, plan.offsets, self.w_gate, self.w_up)

@@ -167,7 +167,7 @@ def ragged_dispatch(x_flat: torch.Tensor, top_idx: torch.Tensor, weights: torch.
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
-    """``t`` where the MXFP4 calls can read it: a tensor that starts inside a buffer (a
+    """``t`` where calls that load 16 bytes at a time can read it: a tensor that starts inside a buffer (a
     flat one of parameters, say) is copied unless it starts at 16 bytes."""
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
@@ -178,9 +178,12 @@ class MoE:
     Reference behaviour by default.  Keyword-only extensions (not in the
     reference): ``routing="softmax"`` (top-k of softmax, renormalised gates,
     no bias, no scaling), ``capacity_factor`` (per-expert capacity
-    ``ceil(CF*T*K/N)`` with token-order priority; ``None`` = dropless) and
-    ``expert_dtype="mxfp4"`` (the routed experts on 4-bit operands quantised from
-    the masters, tokens and ``h`` quantised on the way; bfloat16 compute otherwise.
+    ``ceil(CF*T*K/N)`` with token-order priority; ``None`` = dropless),
+    ``n_groups`` and ``top_groups`` (the experts of a token come from its
+    ``top_groups`` best of ``n_groups`` groups of experts, ``hmoe_router_grouped``;
+    None: all of them) and ``expert_dtype="mxfp4"`` or ``"int8"`` (the routed experts
+    on 4- or 8-bit operands quantised from the masters, tokens and ``h`` quantised on
+    the way; bfloat16 compute otherwise.
     For inference: a call that autograd would record is refused).  As everywhere
     in this module, operands are packed on the calling stream by the first call and
     by the first one after a master changed: other streams wait for that call, and a
@@ -191,22 +194,32 @@ class MoE:
                  n_shared_experts: int, router_init_std: float, routed_scaling_factor: float,
                  dtype, rngs, mesh=None, d_ff_shared: int | None = None, *,
                  routing: str = "sigmoid", capacity_factor: float | None = None,
-                 expert_dtype: str | None = None, device: str | torch.device | None = None):
+                 expert_dtype: str | None = None, n_groups: int = 1, top_groups: int | None = None,
+                 device: str | torch.device | None = None):
         if mesh is not None:
             size = getattr(getattr(mesh, "devices", None), "size", 1)
             if size > 1:
                 raise NotImplementedError("one GPU holds every expert; a multi-device mesh is not built")
         if routing not in ("sigmoid", "softmax"):
             raise ValueError(f"routing must be 'sigmoid' or 'softmax' (got {routing!r})")
-        if expert_dtype not in (None, "mxfp4"):
-            raise ValueError(f"expert_dtype must be None or 'mxfp4' (got {expert_dtype!r})")
-        if expert_dtype == "mxfp4":
+        if expert_dtype not in (None, "mxfp4", "int8"):
+            raise ValueError(f"expert_dtype must be None, 'mxfp4' or 'int8' (got {expert_dtype!r})")
+        if expert_dtype is not None:
             if _torch_dtype(dtype) != torch.bfloat16:
-                raise ValueError("mxfp4 experts belong to the bfloat16 compute dtype")
+                raise ValueError(f"{expert_dtype} experts belong to the bfloat16 compute dtype")
             # (256: the shared experts stay on the bf16 products)
             if d_model % 256 or d_ff % 128:
-                raise ValueError("a layer with mxfp4 experts needs d_model that is a multiple of 256 "
+                raise ValueError(f"a layer with {expert_dtype} experts needs d_model that is a multiple of 256 "
                                  f"and d_ff of 128 (got {d_model}, {d_ff})")
+        top_groups = n_groups if top_groups is None else top_groups
+        if n_groups < 1 or n_experts % n_groups or not 1 <= top_groups <= n_groups:
+            raise ValueError("n_groups must divide n_experts and top_groups be in [1, n_groups] "
+                             f"(got {n_groups}, {top_groups}; {n_experts} experts)")
+        if routing == "sigmoid" and top_groups < n_groups and n_experts // n_groups < 2:
+            raise ValueError("with sigmoid routing a group's score is the sum of two experts': groups need two")
+        if top_groups * (n_experts // n_groups) < n_active:
+            raise ValueError(f"{top_groups} groups of {n_experts // n_groups} experts hold fewer than the "
+                             f"{n_active} that a token takes")
         dev = torch.device(device) if device is not None else torch.device("cuda")
         self.mesh = mesh
         self.expert_axis_name = None
@@ -218,6 +231,7 @@ class MoE:
         self.routing = routing
         self.capacity_factor = capacity_factor
         self.expert_dtype = expert_dtype
+        self.n_groups, self.top_groups = n_groups, top_groups
         g = _generator(rngs, dev)
 
         def normal(shape, std):
@@ -241,6 +255,7 @@ class MoE:
         self._routed_pack = _PackCache()
         self._shared_pack = _PackCache()
         self._mxfp4_pack = _PackCache()
+        self._i8_pack = _PackCache()
         self._routed_bwd_pack = _PackCache()
         self._shared_bwd_pack = _PackCache()
         self._backward_expected = True   # there was one since the last joint pack
@@ -320,6 +335,12 @@ class MoE:
         return self._mxfp4_pack.get((wg, wu, wd), lambda: (
             *K.pack_mxfp4_gate_up(_aligned(wg.detach()), _aligned(wu.detach())),
             *K.pack_mxfp4_down(_aligned(wd.detach()))))
+
+    def _packed_i8(self):
+        """The routed experts' int8 operands (codes and scales of gate/up, of down)."""
+        wg, wu, wd = self.expert_w_gate.value, self.expert_w_up.value, self.expert_w_down.value
+        return self._i8_pack.get((wg, wu, wd), lambda: (
+            *K.pack_i8_gate_up(wg.detach(), wu.detach()), *K.pack_i8_down(wd.detach())))
 
     def _packed_shared(self, masters=None):
         """One ``(gate_up, down)`` of packed operands per shared expert."""
@@ -403,23 +424,47 @@ class MoE:
         differentiates the same outputs)."""
         if torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in self._params())):
             if self.expert_dtype is not None:
-                raise NotImplementedError("mxfp4 experts have no backward: call under torch.no_grad(), "
-                                          "or train the layer without expert_dtype")
+                raise NotImplementedError(f"{self.expert_dtype} experts have no backward: call under "
+                                          "torch.no_grad(), or train the layer without expert_dtype")
             out, z, bal, ent, counts = _MoEFunction.apply(self, x, *self._params())
             return out, {"router_z_loss": z, "balance_loss": bal, "mean_entropy": ent,
                          "expert_counts": counts}
         out, losses, counts, _ = self._forward(x, save=False)
-        aux = {
+        return out, self._aux(losses, counts)
+
+    @staticmethod
+    def _aux(losses, counts) -> dict:
+        return {
             "router_z_loss": losses[0],
             "balance_loss": losses[1],
             "mean_entropy": losses[2],
             "expert_counts": counts,
         }
-        return out, aux
 
-    def _forward(self, x: torch.Tensor, save: bool):
+    def behind_norm(self, norm, x: torch.Tensor, residual: torch.Tensor | None = None):
+        """The layer behind a block's norm (``model/transformer.py:91-95``): ``total = x +
+        residual`` (``x`` without one), and the layer of ``norm(total)``, ``norm`` an
+        :class:`hanuman_amd.RMSNorm`.  Returns ``(out [B,S,D] float32, total [B,S,D], aux)``;
+        the block's output is ``total + out``.  The addition, the norm and, for int8 experts,
+        the tokens' codes are one launch.  Under autograd it is ``norm`` and the layer as
+        two nodes."""
+        if x.dim() != 3:
+            raise ValueError(f"x must be [B, S, d_model] (got {tuple(x.shape)})")
+        tracked = (x, norm.scale.value, *self._params()) if residual is None else (
+            x, residual, norm.scale.value, *self._params())
+        if torch.is_grad_enabled() and any(t.requires_grad for t in tracked):
+            y, total = norm.with_sum(x, residual, out_dtype=self.dtype)
+            out, aux = self(y)
+            return out, total, aux
+        r = norm.rows(x, residual, out_dtype=self.dtype, quant="int8" if self.expert_dtype == "int8" else None)
+        out, losses, counts, _ = self._forward(r.y.view(x.shape), save=False,
+                                               codes=None if r.q is None else (r.q, r.scale))
+        return out, r.sum.view(x.shape), self._aux(losses, counts)
+
+    def _forward(self, x: torch.Tensor, save: bool, codes=None):
         """The forward; returns ``(out [B,S,D], losses [3], counts [N], saved)``
-        with ``saved`` the backward's residuals when ``save``."""
+        with ``saved`` the backward's residuals when ``save``.  ``codes``: the tokens'
+        int8 codes and scales where the caller has them."""
         _require_bf16_compute(self.dtype)
         if x.dim() != 3:
             raise ValueError(f"x must be [B, S, d_model] (got {tuple(x.shape)})")
@@ -432,12 +477,12 @@ class MoE:
         bias = self.bias.value if self.routing == "sigmoid" else None
         router_w = self.router.value.float().contiguous()
         x_q = None
-        if self.expert_dtype == "mxfp4":
+        if self.expert_dtype is not None:
             x2 = _aligned(x2)
-        if self.expert_dtype == "mxfp4" and x2.dtype == torch.bfloat16:
+        if self.expert_dtype == "mxfp4" and x2.dtype == torch.bfloat16 and self.top_groups == self.n_groups:
             logits, top_idx, gates, *x_q = K.router_quant_mxfp4(x2, router_w, bias, Kk, mode, rsf)
         else:
-            logits, top_idx, gates = K.router(x2, router_w, bias, Kk, mode, rsf)
+            logits, top_idx, gates = K.router(x2, router_w, bias, Kk, mode, rsf, self.n_groups, self.top_groups)
         cap = K.capacity(T, Kk, N, self.capacity_factor)
         plan = K.dispatch_plan(top_idx, N, cap)
         if self.dtype == torch.float32:
@@ -456,11 +501,16 @@ class MoE:
                          "plan": plan, "xs": xs, "h": h, "ys": ys, "h_shared": hs, "mode": mode,
                          "rsf": rsf, "batch": B, "seq": S}
             return out.reshape(B, S, D), losses, counts, saved
-        if self.expert_dtype == "mxfp4":
-            gate_up, gate_up_exp, down, down_exp = self._packed_mxfp4()
-            h_q, h_exp = K.grouped_gate_up_mxfp4_gather(*(x_q or K.quantize_rows_mxfp4(x2)), plan,
-                                                        gate_up, gate_up_exp)
-            ys = K.grouped_down_mxfp4(h_q, h_exp, plan.offsets, down, down_exp)
+        if self.expert_dtype is not None:
+            if self.expert_dtype == "mxfp4":
+                gate_up, gate_up_exp, down, down_exp = self._packed_mxfp4()
+                h_q, h_exp = K.grouped_gate_up_mxfp4_gather(*(x_q or K.quantize_rows_mxfp4(x2)), plan,
+                                                            gate_up, gate_up_exp)
+                ys = K.grouped_down_mxfp4(h_q, h_exp, plan.offsets, down, down_exp)
+            else:
+                gate_up, gate_up_scale, down, down_scale = self._packed_i8()
+                h = K.grouped_gate_up_i8_gather(*(codes or K.quantize_rows_i8(x2)), plan, gate_up, gate_up_scale)
+                ys = K.grouped_down_i8(*K.quantize_rows_i8(h, plan.offsets), plan.offsets, down, down_scale)
             if x2.dtype == torch.float32 and self.n_shared_experts > 0:
                 shared = self._shared_ffn_promoted(x2)
             else:

@@ -30,7 +30,7 @@ class Workload:
     expert: str = "swiglu"    # "swiglu" | "identity"
     zipf_bias: bool = False   # per-expert logit bias 3 * rank^-1.1
     router_w_dtype: str = "f32"
-    expert_dtype: str = "bf16"  # "bf16" | "fp8" | "mxfp4" | "f32" (float32 compute)
+    expert_dtype: str = "bf16"  # "bf16" | "fp8" | "mxfp4" | "int8" | "f32" (float32 compute)
     out_dtype: str = "f32"
     batch: int = 1
     weight_std: float = 0.02

@@ -95,6 +95,57 @@ XLA_FFI_DEFINE_HANDLER_SYMBOL(HmoeRouter, RouterImpl,
                                   .Ret<ffi::Buffer<ffi::S32>>()
                                   .Ret<ffi::Buffer<ffi::F32>>());
 
+// The same with the experts taken from the best groups.
+static ffi::Error RouterGroupedImpl(hipStream_t stream, ffi::AnyBuffer x, ffi::AnyBuffer w,
+                                    ffi::Buffer<ffi::F32> bias, int64_t mode, float rsf, int64_t n_groups,
+                                    int64_t top_groups, ffi::ResultBuffer<ffi::F32> logits,
+                                    ffi::ResultBuffer<ffi::S32> top_idx, ffi::ResultBuffer<ffi::F32> gates) {
+  const int xd = DtypeCode(x.element_type()), wd = DtypeCode(w.element_type());
+  if (xd < 0) return BadDtype("hmoe_router_grouped x");
+  if (wd < 0) return BadDtype("hmoe_router_grouped router_w");
+  return Status(hmoe_router_grouped(x.untyped_data(), xd, w.untyped_data(), wd, bias.typed_data(), Rows(x),
+                                    static_cast<int>(Cols(x)), static_cast<int>(Cols(w)),
+                                    static_cast<int>(Cols(*top_idx)), static_cast<int>(mode), rsf,
+                                    static_cast<int>(n_groups), static_cast<int>(top_groups), logits->typed_data(),
+                                    top_idx->typed_data(), gates->typed_data(), S(stream)));
+}
+XLA_FFI_DEFINE_HANDLER_SYMBOL(HmoeRouterGrouped, RouterGroupedImpl,
+                              ffi::Ffi::Bind()
+                                  .Ctx<ffi::PlatformStream<hipStream_t>>()
+                                  .Arg<ffi::AnyBuffer>()
+                                  .Arg<ffi::AnyBuffer>()
+                                  .Arg<ffi::Buffer<ffi::F32>>()
+                                  .Attr<int64_t>("mode")
+                                  .Attr<float>("routed_scaling_factor")
+                                  .Attr<int64_t>("n_groups")
+                                  .Attr<int64_t>("top_groups")
+                                  .Ret<ffi::Buffer<ffi::F32>>()
+                                  .Ret<ffi::Buffer<ffi::S32>>()
+                                  .Ret<ffi::Buffer<ffi::F32>>());
+
+// logits [T, N], bias [N] f32 -> top_idx [T, K] s32, gates [T, K] f32, from the best groups.
+static ffi::Error RouterGroupedFromLogitsImpl(hipStream_t stream, ffi::Buffer<ffi::F32> logits,
+                                              ffi::Buffer<ffi::F32> bias, int64_t mode, float rsf,
+                                              int64_t n_groups, int64_t top_groups,
+                                              ffi::ResultBuffer<ffi::S32> top_idx,
+                                              ffi::ResultBuffer<ffi::F32> gates) {
+  return Status(hmoe_router_grouped_from_logits(
+      logits.typed_data(), bias.typed_data(), Rows(logits), static_cast<int>(Cols(logits)),
+      static_cast<int>(Cols(*top_idx)), static_cast<int>(mode), rsf, static_cast<int>(n_groups),
+      static_cast<int>(top_groups), top_idx->typed_data(), gates->typed_data(), S(stream)));
+}
+XLA_FFI_DEFINE_HANDLER_SYMBOL(HmoeRouterGroupedFromLogits, RouterGroupedFromLogitsImpl,
+                              ffi::Ffi::Bind()
+                                  .Ctx<ffi::PlatformStream<hipStream_t>>()
+                                  .Arg<ffi::Buffer<ffi::F32>>()
+                                  .Arg<ffi::Buffer<ffi::F32>>()
+                                  .Attr<int64_t>("mode")
+                                  .Attr<float>("routed_scaling_factor")
+                                  .Attr<int64_t>("n_groups")
+                                  .Attr<int64_t>("top_groups")
+                                  .Ret<ffi::Buffer<ffi::S32>>()
+                                  .Ret<ffi::Buffer<ffi::F32>>());
+
 // The router and the per-token e4m3 quantisation of x in one launch (fp8
 // experts on bf16 tokens): x [T, D] bf16, router_w [D, N] (f32/bf16), bias
 // [N] f32 -> logits, top_idx, gates as hmoe_router, x_q [T, D] u8, x_scale

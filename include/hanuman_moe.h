@@ -87,6 +87,23 @@ int hmoe_router_from_logits(const float* logits, const float* bias, int64_t toke
                             float routed_scaling_factor, int32_t* top_idx,
                             float* gates, hmoe_stream_t stream);
 
+/* The same two with the selection limited to groups (no reference code; config.py:50 has an
+ * n_group that nothing reads).  The experts are n_groups groups of N / n_groups one after another.
+ * A key is the logit (HMOE_ROUTE_SOFTMAX) or sigmoid + bias; a group's score is its largest key, or
+ * with sigmoid the float32 sum of its two largest.  The experts are taken, by their keys, from the
+ * top_groups groups with the largest scores (the lower index first where equal; a score that is
+ * NaN is below all others); gates as above.  With top_groups == n_groups these are the calls
+ * above.  n_groups <= 64 divides N, top_k <= top_groups * (N / n_groups), with sigmoid groups of
+ * two experts at least.  hmoe_router_bwd and hmoe_router_aux take the results as they are. */
+int hmoe_router_grouped(const void* x, int x_dtype, const void* router_w, int w_dtype,
+                        const float* bias, int64_t tokens, int d_model, int n_experts, int top_k,
+                        int mode, float routed_scaling_factor, int n_groups, int top_groups,
+                        float* logits, int32_t* top_idx, float* gates, hmoe_stream_t stream);
+int hmoe_router_grouped_from_logits(const float* logits, const float* bias, int64_t tokens,
+                                    int n_experts, int top_k, int mode, float routed_scaling_factor,
+                                    int n_groups, int top_groups, int32_t* top_idx, float* gates,
+                                    hmoe_stream_t stream);
+
 /* ---- dispatch plan: moe.py:54-57,80 (replaces `argsort(slot_expert)`,
  *      `bincount`, `argsort(order)`) plus the capacity drop --------------- */
 
