@@ -958,33 +958,64 @@ __global__ __launch_bounds__(256) void select_kernel_g8(const float* __restrict_
 }
 
 // Selection and gates among the experts of the best groups from given logits.  A wave takes 64
-// >> log_lanes tokens, whose logits, one run of memory, go through LDS: a lane reads E of them
-// one after another (a word more every 32, so that the lanes' words are in different banks).
-template <int E>
+// >> log_lanes tokens, whose logits, one run of memory, go through LDS, and the biases: a lane
+// reads E of each one after another (four words more every 32, so that lanes 32 words apart read
+// different banks).  WIDE: all of it 16 bytes at a time.
+template <int E, bool LIST, bool WIDE>
 __global__ __launch_bounds__(256) void select_groups_kernel(const float* __restrict__ logits,
                                                             const float* __restrict__ bias, int64_t tokens,
                                                             GroupRule r, int32_t* __restrict__ top_idx,
                                                             float* __restrict__ gates) {
-  extern __shared__ float stage[];
+  extern __shared__ __attribute__((aligned(16))) float stage[];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int per_wave = 64 >> r.log_lanes;
+  const int n = r.n_experts;
   const int64_t t0 = (static_cast<int64_t>(blockIdx.x) * 4 + wave) * per_wave;
   if (t0 >= tokens) return;  // uniform per wave; no barrier follows
-  const int count = static_cast<int>(tokens - t0 < per_wave ? tokens - t0 : per_wave) * r.n_experts;
-  float* mine = stage + wave * (per_wave * r.n_experts / 32 * 33 + 33);
-  const float* src = logits + t0 * r.n_experts;
-  for (int i = lane; i < count; i += 64) mine[i + (i >> 5)] = src[i];
+  const int count = static_cast<int>(tokens - t0 < per_wave ? tokens - t0 : per_wave) * n;
+  float* mine = stage + wave * (group_stage_words(per_wave * n) + group_stage_words(n));
+  float* biases = mine + group_stage_words(per_wave * n);
+  const float* src = logits + t0 * n;
+  const auto park = [&](const float* from, float* to, int words) __attribute__((always_inline)) {
+    if constexpr (WIDE) {
+      for (int i = lane * 4; i < words; i += 256)
+        *reinterpret_cast<f32x4*>(to + i + (i >> 5) * 4) = *reinterpret_cast<const f32x4*>(from + i);
+    } else {
+      for (int i = lane; i < words; i += 64) to[i + (i >> 5) * 4] = from[i];
+    }
+  };
+  park(src, mine, count);
+  if (bias != nullptr) {
+    park(bias, biases, n);
+  } else if (r.mode == HMOE_ROUTE_SIGMOID_BIAS) {
+    for (int i = lane; i < n; i += 64) biases[i + (i >> 5) * 4] = 0.0f;
+  }
   const int64_t tok = t0 + (lane >> r.log_lanes);
   const bool store = tok < tokens;
-  const int row = store ? static_cast<int>(tok - t0) * r.n_experts : 0;
+  const int row = store ? static_cast<int>(tok - t0) * n : 0;
   // (a wave's LDS accesses run in their order)
   asm volatile("" ::: "memory");
-  const auto get = [&](int e) __attribute__((always_inline)) {
-    const int i = row + e;
-    return mine[i + (i >> 5)];
+  const auto read = [&](const float* from, int first, float (&v)[E]) __attribute__((always_inline)) {
+    if constexpr (WIDE) {
+#pragma unroll
+      for (int j = 0; j < E; j += 4) {
+        const int i = first + j;
+        const f32x4 w = *reinterpret_cast<const f32x4*>(from + i + (i >> 5) * 4);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[j + q] = w[q];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < E; ++j) v[j] = from[first + j + ((first + j) >> 5) * 4];
+    }
   };
+  const auto run = [&](int e, float (&l)[E], float (&b)[E]) __attribute__((always_inline)) {
+    read(mine, row + e, l);
+    if (r.mode == HMOE_ROUTE_SIGMOID_BIAS) read(biases, e, b);
+  };
+  const auto get = [&](int e) __attribute__((always_inline)) { return mine[row + e + ((row + e) >> 5) * 4]; };
   const int64_t tq = store ? tok : t0;
-  select_in_groups<E>(get, bias, r, store, top_idx + tq * r.top_k, gates + tq * r.top_k);
+  select_in_groups<E, LIST>(run, get, r, store, top_idx + tq * r.top_k, gates + tq * r.top_k);
 }
 
 template <int E>
@@ -993,9 +1024,18 @@ void launch_select_groups(const float* logits, const float* bias, int64_t tokens
                           hipStream_t s) {
   const GroupRule r = group_rule(n_experts, n_groups, top_groups, top_k, mode, rsf, E);
   const int per_wave = 64 >> r.log_lanes;
-  const size_t lds = static_cast<size_t>(4) * (per_wave * n_experts / 32 * 33 + 33) * sizeof(float);
-  hipLaunchKernelGGL((select_groups_kernel<E>), dim3(static_cast<unsigned>(ceil_div(tokens, 4 * per_wave))), dim3(256),
-                     lds, s, logits, bias, tokens, r, top_idx, gates);
+  const size_t lds =
+      static_cast<size_t>(4) * (group_stage_words(per_wave * n_experts) + group_stage_words(n_experts)) * sizeof(float);
+  const dim3 grid(static_cast<unsigned>(ceil_div(tokens, 4 * per_wave)));
+  const bool wide = r.size % 4 == 0 && aligned_to(logits, 16) && (bias == nullptr || aligned_to(bias, 16));
+  const auto launch = [&](auto LIST, auto WIDE) {
+    hipLaunchKernelGGL((select_groups_kernel<E, decltype(LIST)::value, decltype(WIDE)::value>), grid, dim3(256), lds, s,
+                       logits, bias, tokens, r, top_idx, gates);
+  };
+  if (top_k <= kList && wide) launch(IntC<1>(), IntC<1>());
+  else if (top_k <= kList) launch(IntC<1>(), IntC<0>());
+  else if (wide) launch(IntC<0>(), IntC<1>());
+  else launch(IntC<0>(), IntC<0>());
 }
 
 // E: as many keys a lane as leave a token eight lanes and more.
@@ -1009,8 +1049,7 @@ void select_groups(const float* logits, const float* bias, int64_t tokens, int n
   int groups = 1;
   while (groups < n_groups) groups *= 2;
   const int keys = groups >= 8 ? size : (size * groups + 7) / 8;  // for one lane
-  if (keys <= 4) run(IntC<4>());
-  else if (keys <= 8) run(IntC<8>());
+  if (keys <= 8) run(IntC<8>());
   else if (keys <= 16) run(IntC<16>());
   else run(IntC<32>());
 }
