@@ -743,6 +743,7 @@ def grouped_down_fp8_mx(h_q: torch.Tensor, h_exp: torch.Tensor, offsets: torch.T
 # start at 16 bytes, exponents at 4 (any row of such a matrix does).
 
 _U8, _TENSOR = torch.uint8, torch.Tensor
+_I8, _F32 = torch.int8, torch.float32
 
 
 def _u8(name: str, dev, t: torch.Tensor, shape: tuple):
@@ -942,10 +943,11 @@ class NormOut(NamedTuple):
 
 def _norm_operand(name: str, what: str, t: torch.Tensor, dev, shape: tuple) -> int:
     """The dtype code of a float32 or bf16 operand of that shape on the call's device."""
-    _check(t, what)
-    _same_device(name, t, dev)
-    if t.shape != shape:
-        raise ValueError(f"{name}: {what} must have shape {tuple(shape)} (got {tuple(t.shape)})")
+    if not (t.__class__ is _TENSOR and t.is_contiguous() and t.device == dev and t.shape == shape):
+        _check(t, what)
+        _same_device(name, t, dev)
+        if t.shape != shape:
+            raise ValueError(f"{name}: {what} must have shape {tuple(shape)} (got {tuple(t.shape)})")
     return _dtype_code(t)
 
 
@@ -965,24 +967,29 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor |
     shape = x.shape
     x_code = _dtype_code(x)
     w_code = _norm_operand(name, "weight", weight, dev, shape[1:])
-    out_dtype = x.dtype if out_dtype is None else out_dtype
-    if out_dtype not in _DT:
+    # (the smallest calls are as long as their allocations: empty_like is the shortest)
+    if out_dtype is None or out_dtype is x.dtype:
+        y, y_code = torch.empty_like(x), x_code
+    elif out_dtype in _DT:
+        y, y_code = torch.empty_like(x, dtype=out_dtype), _DT[out_dtype]
+    else:
         raise TypeError(f"unsupported dtype {out_dtype}; expected float32 or bfloat16")
     if quant not in _QUANT:
         raise ValueError(f"{name}: quant must be None, 'e4m3' or 'int8' (got {quant!r})")
-    r_code, total = 0, x
+    r_code, total, total_ptr, r_ptr = 0, x, None, None
     if residual is not None:
         r_code = _norm_operand(name, "residual", residual, dev, shape)
         total = torch.empty_like(residual)
-    y = x.new_empty(shape, dtype=out_dtype)
-    rstd = x.new_empty(shape[:1], dtype=torch.float32)
-    q = scale = None
+        total_ptr, r_ptr = total.data_ptr(), residual.data_ptr()
+    rows, cols = shape
+    rstd = x.new_empty((rows,), dtype=_F32)
+    q = scale = q_ptr = scale_ptr = None
     if quant is not None:
-        q = x.new_empty(shape, dtype=torch.int8 if quant == "int8" else _U8)
+        q = torch.empty_like(x, dtype=_I8 if quant == "int8" else _U8)
         scale = torch.empty_like(rstd)
-    call("hmoe_add_rms_norm", x.data_ptr(), x_code, _ptr(residual), r_code, weight.data_ptr(), w_code, float(eps),
-         shape[0], shape[1], None if residual is None else total.data_ptr(), y.data_ptr(), _DT[out_dtype],
-         rstd.data_ptr(), _ptr(q), _QUANT[quant], _ptr(scale), _stream())
+        q_ptr, scale_ptr = q.data_ptr(), scale.data_ptr()
+    call("hmoe_add_rms_norm", x.data_ptr(), x_code, r_ptr, r_code, weight.data_ptr(), w_code, eps, rows, cols,
+         total_ptr, y.data_ptr(), y_code, rstd.data_ptr(), q_ptr, _QUANT[quant], scale_ptr, _stream())
     return NormOut(y, total, rstd, q, scale)
 
 
@@ -1018,12 +1025,9 @@ def add_rms_norm_bwd(dy: torch.Tensor, total: torch.Tensor, weight: torch.Tensor
 # weight's row the reduction of one output column.  Served weights only, as for the e4m3
 # and MXFP4 experts.  Operands start at 16 bytes (any row of such a matrix does).
 
-_I8, _F32 = torch.int8, torch.float32
-
-
 def _codes(name: str, what: str, dev, t: torch.Tensor, dtype: torch.dtype, shape: tuple):
     """Checks a tensor of codes or scales: its type, contiguous, on the call's device, of
-    that size."""
+    that size.  (One expression for what is right, as in :func:`_u8`.)"""
     if (t.__class__ is _TENSOR and t.dtype is dtype and t.shape == shape and t.is_contiguous()
             and t.device == dev):
         return
@@ -1040,27 +1044,28 @@ def quantize_rows_i8(a: torch.Tensor, offsets: torch.Tensor | None = None):
     name = "quantize_rows_i8"
     dev = _current_device(name, a, 2)
     rows, cols = a.shape
-    q = a.new_empty((rows, cols), dtype=_I8)
+    q = torch.empty_like(a, dtype=_I8)
     scale = a.new_empty((rows,), dtype=_F32)
-    n = 0
+    n, off = 0, None
     if offsets is not None:
         _check_i32(name, "offsets", offsets, offsets.numel(), dev)
-        n = offsets.numel() - 1
-    call("hmoe_quantize_rows_i8", a.data_ptr(), _dtype_code(a), rows, cols, _ptr(offsets), n, q.data_ptr(),
-         scale.data_ptr(), _stream())
+        n, off = offsets.numel() - 1, offsets.data_ptr()
+    call("hmoe_quantize_rows_i8", a.data_ptr(), _dtype_code(a), rows, cols, off, n, q.data_ptr(), scale.data_ptr(),
+         _stream())
     return q, scale
 
 
 def _dequantize_rows(name: str, q: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype,
                      out_dtype: torch.dtype) -> torch.Tensor:
     dev = _current_device(name, q, 2)
-    _codes(name, "q", dev, q, dtype, q.shape)
-    _codes(name, "scale", dev, scale, _F32, q.shape[:1])
+    rows, cols = q.shape
+    if q.dtype is not dtype:
+        raise ValueError(f"{name}: q must be {dtype} (got {q.dtype})")
+    _codes(name, "scale", dev, scale, _F32, (rows,))
     if out_dtype not in _DT:
         raise TypeError(f"unsupported dtype {out_dtype}; expected float32 or bfloat16")
-    out = q.new_empty(q.shape, dtype=out_dtype)
-    call("hmoe_" + name, q.data_ptr(), scale.data_ptr(), q.shape[0], q.shape[1], out.data_ptr(), _DT[out_dtype],
-         _stream())
+    out = torch.empty_like(q, dtype=out_dtype)
+    call("hmoe_" + name, q.data_ptr(), scale.data_ptr(), rows, cols, out.data_ptr(), _DT[out_dtype], _stream())
     return out
 
 
@@ -1111,8 +1116,10 @@ def _i8_sizes(name: str, packed: torch.Tensor, scales: torch.Tensor, dev):
     """``N, rows, K`` of a packed int8 operand, its tensors checked."""
     if packed.dim() != 5:
         raise ValueError(f"{name}: a packed operand has 5 dims (got {tuple(packed.shape)})")
-    N, r, k = packed.shape[:3]
-    _codes(name, "packed codes", dev, packed, _I8, (N, r, k, 64, 16))
+    N, r, k, lanes, per_lane = packed.shape
+    if not (lanes == 64 and per_lane == 16 and packed.dtype is _I8 and packed.__class__ is _TENSOR
+            and packed.is_contiguous() and packed.device == dev):
+        _codes(name, "packed codes", dev, packed, _I8, (N, r, k, 64, 16))
     _codes(name, "packed scales", dev, scales, _F32, (N, 32 * r))
     return N, 32 * r, 32 * k
 
@@ -1124,8 +1131,9 @@ def grouped_gate_up_i8(xs_q: torch.Tensor, xs_scale: torch.Tensor, offsets: torc
     name = "grouped_gate_up_i8"
     dev = _current_device(name, xs_q, 2)
     N, F2, D = _i8_sizes(name, w_packed, w_scales, dev)
-    rows, F = xs_q.shape[0], F2 // 2
-    _codes(name, "xs_q", dev, xs_q, _I8, (rows, D))
+    (rows, cols), F = xs_q.shape, F2 // 2
+    if xs_q.dtype is not _I8 or cols != D:
+        _codes(name, "xs_q", dev, xs_q, _I8, (rows, D))
     _codes(name, "xs_scale", dev, xs_scale, _F32, (rows,))
     _check_i32(name, "offsets", offsets, N + 1, dev)
     h = xs_q.new_empty((rows, F), dtype=torch.bfloat16)
@@ -1141,8 +1149,9 @@ def grouped_gate_up_i8_gather(x_q: torch.Tensor, x_scale: torch.Tensor, plan: Pl
     name = "grouped_gate_up_i8_gather"
     dev = _current_device(name, x_q, 2)
     N, F2, D = _i8_sizes(name, w_packed, w_scales, dev)
-    T, F = x_q.shape[0], F2 // 2
-    _codes(name, "x_q", dev, x_q, _I8, (T, D))
+    (T, cols), F = x_q.shape, F2 // 2
+    if x_q.dtype is not _I8 or cols != D:
+        _codes(name, "x_q", dev, x_q, _I8, (T, D))
     _codes(name, "x_scale", dev, x_scale, _F32, (T,))
     if plan.n_experts != N or plan.slot_pos.numel() != T * plan.top_k:
         raise ValueError(f"{name}: the plan is of other tokens or experts")
@@ -1162,8 +1171,9 @@ def grouped_down_i8(h_q: torch.Tensor, h_scale: torch.Tensor, offsets: torch.Ten
     name = "grouped_down_i8"
     dev = _current_device(name, h_q, 2)
     N, D, F = _i8_sizes(name, w_packed, w_scales, dev)
-    rows = h_q.shape[0]
-    _codes(name, "h_q", dev, h_q, _I8, (rows, F))
+    rows, cols = h_q.shape
+    if h_q.dtype is not _I8 or cols != F:
+        _codes(name, "h_q", dev, h_q, _I8, (rows, F))
     _codes(name, "h_scale", dev, h_scale, _F32, (rows,))
     _check_i32(name, "offsets", offsets, N + 1, dev)
     ys = h_q.new_empty((rows, D), dtype=torch.bfloat16)
