@@ -29,7 +29,7 @@ __device__ __forceinline__ i32x16 mfma_i8(const u32x4& b, const u32x4& a, const 
 
 // Sums of 32 columns to values: `cols` are the columns' scales.  Lane L holds row L % 32 and
 // columns 8 q + 4 (L / 32) + 0..3 (q = 0..3).
-__device__ __forceinline__ f32x16 scaled(const i32x16& acc, const float* __restrict__ cols, float row, int half) {
+__device__ __forceinline__ f32x16 scaled(const i32x16& acc, const float* cols, float row, int half) {
   f32x16 y;
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
@@ -150,20 +150,25 @@ __global__ __launch_bounds__(256) void grouped_i8_rows(
 // instruction, each loaded for the next step as soon as its products are issued.  A goes
 // through LDS (buffer_load ... lds), two stages of 128 values of every row, the next
 // stage's loads issued behind the one barrier of a step: whole lines, and 16-byte chunk c of
-// row r sits at c ^ swz128(r), so that 16 lanes of a fragment read cover all banks.  The
-// last column tile may be 128 columns wide: waves 2 and 3 then load and compute the others'
+// row r sits at c ^ swz128(r), so that 16 lanes of a fragment read cover all banks.  A tile's
+// scales come with its first step into one of two regions.  The last column tile may be 128 columns wide: waves 2 and 3 then load and compute the others'
 // again and store nothing.
 constexpr int kTileThreads = 256;
 
 template <int BM, bool GATE_UP>
 struct TileCfg {
   static constexpr int kA = BM * 128;              // a stage
+  static constexpr int kScales = BM * 4 + 1024;    // a tile's row and column scales
   static constexpr int kOut = 4 * 4096;            // 4 KB a wave for the rows that are stored
-  static constexpr int kLds = 2 * kA + kOut;
+  static constexpr int kLds = 2 * (kA + kScales) + kOut;
   static constexpr int kFR = BM / 32;              // row fragments; DMA instructions a wave and step
   static constexpr int kPerCu = BM == 64 ? 3 : 2;
   static_assert(kPerCu * kLds <= 160 * 1024, "workgroups a CU");
 };
+
+__device__ __forceinline__ void dma4(__amdgpu_buffer_rsrc_t r, uint8_t* dst, uint32_t voff) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr_t)dst, 4, voff, 0, 0, 0);
+}
 
 __device__ __forceinline__ void use_here(const i32x16& v) { asm volatile("" ::"v"(v)); }
 
@@ -210,8 +215,13 @@ __global__ __launch_bounds__(kTileThreads, BM == 64 ? 3 : 2) void grouped_i8_til
   uint32_t a_voff[kFR];
   const int b_col = (kdim / 32) * 1024;  // bytes of 32 columns
   int b_wave = 0;                        // where this wave's columns begin
-  int ld_kb = 0, ld_t = first, ld_stage = 0;
-  int32_t pf_src[kFR];  // GATHER: sources of this lane's rows of the tile after, nx
+  __amdgpu_buffer_rsrc_t as_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(a_scale), 0,
+                                                                     GATHER ? gather_rows * 4 : 0, kBufferWord3);
+  __amdgpu_buffer_rsrc_t bs_rsrc = a_rsrc;
+  uint32_t as_voff = 0, bs_voff = 0;
+  const bool row_scales = wave < BM / 64;  // the waves that bring the rows' scales
+  int ld_kb = 0, ld_t = first, ld_stage = 0, ld_region = 1;
+  int32_t pf_src[kFR], pf_scale = 0;  // GATHER: sources of this lane's rows of the tile after, nx
   auto a_byte = [&](int j) __attribute__((always_inline)) {
     return static_cast<uint32_t>(((lane & 7) ^ swz128(8 * j + (lane >> 3))) * 16);
   };
@@ -221,6 +231,8 @@ __global__ __launch_bounds__(kTileThreads, BM == 64 ? 3 : 2) void grouped_i8_til
       const int r = a_row + 8 * j;
       pf_src[j] = gather_src[nx.row0 + (r < nx.rows ? r : nx.rows - 1)];
     }
+    const int r = 64 * wave + lane;
+    pf_scale = gather_src[nx.row0 + (r < nx.rows ? r : nx.rows - 1)];
   };
   // Tile ld_t becomes the one that is loaded.
   auto set_load_tile = [&]() __attribute__((always_inline)) {
@@ -230,6 +242,7 @@ __global__ __launch_bounds__(kTileThreads, BM == 64 ? 3 : 2) void grouped_i8_til
       for (int j = 0; j < kFR; ++j)
         a_voff[j] = static_cast<uint32_t>(token_of(pf_src[j], gather_k, gather_rows)) * static_cast<uint32_t>(row_bytes) +
                     a_byte(j);
+      as_voff = static_cast<uint32_t>(token_of(pf_scale, gather_k, gather_rows)) * 4u;
       if (ld_t + per_xcd < hi) nx.move(offsets, ld_t + per_xcd, n_tiles_n, by_cols, by_group);
       fetch_src();  // (on every path: a load that may not be issued is waited for at once)
     } else {
@@ -242,6 +255,9 @@ __global__ __launch_bounds__(kTileThreads, BM == 64 ? 3 : 2) void grouped_i8_til
         const int r = a_row + 8 * j;
         a_voff[j] = static_cast<uint32_t>((r < ld.rows ? r : ld.rows - 1) * row_bytes) + a_byte(j);
       }
+      as_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(a_scale + ld.row0), 0, ld.rows * 4, kBufferWord3);
+      const int r = 64 * wave + lane;
+      as_voff = static_cast<uint32_t>(r < ld.rows ? r : ld.rows - 1) * 4u;
     }
     const int64_t block = static_cast<int64_t>(ld.e) * (ncols / 32) + ld.n0 / 32;
     const int width = ncols - ld.n0 < kTileN ? ncols - ld.n0 : kTileN;
@@ -249,9 +265,18 @@ __global__ __launch_bounds__(kTileThreads, BM == 64 ? 3 : 2) void grouped_i8_til
     b_wave = part * 2 * b_col;
     b_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(B + block * b_col), 0, width * row_bytes,
                                                kBufferWord3);
+    bs_rsrc = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<float*>(b_scale + static_cast<int64_t>(ld.e) * ncols + ld.n0), 0, width * 4, kBufferWord3);
+    bs_voff = static_cast<uint32_t>(64 * part + lane) * 4u;
     ld_kb = 0;
   };
   auto issue_a = [&]() __attribute__((always_inline)) {
+    if (ld_kb == 0) {  // the tile's scales, into the region that the tile before does not read
+      ld_region ^= 1;
+      uint8_t* const to = smem + 2 * Cfg::kA + ld_region * Cfg::kScales;
+      if (row_scales) dma4(as_rsrc, to + wave * 256, as_voff);
+      dma4(bs_rsrc, to + BM * 4 + wave * 256, bs_voff);
+    }
 #pragma unroll
     for (int j = 0; j < kFR; ++j)
       dma16(a_rsrc, smem + ld_stage * Cfg::kA + (wave * kFR + j) * 1024, a_voff[j] + static_cast<uint32_t>(ld_kb * 128));
@@ -271,7 +296,7 @@ __global__ __launch_bounds__(kTileThreads, BM == 64 ? 3 : 2) void grouped_i8_til
   const int frow = lane & 31, half = lane >> 5;
   const int fsw = swz128(frow);
   i32x16 acc[kFR][2];
-  int stage = 0;
+  int stage = 0, region = 1;
   constexpr int kNewer = 8;  // loads of B in a step, behind A's
 
   // One step: 128 values of this tile, the loads of the next step behind them.
@@ -344,15 +369,14 @@ __global__ __launch_bounds__(kTileThreads, BM == 64 ? 3 : 2) void grouped_i8_til
     const __amdgpu_buffer_rsrc_t out =
         __builtin_amdgcn_make_buffer_rsrc(C + r0 * ldc, 0, cur.rows * ldc * 2, kBufferWord3);
     const bool mine = cur.n0 + wave * 64 < ncols;  // uniform per wave
+    region ^= 1;
     if (mine) {
-      const float* cs = b_scale + static_cast<int64_t>(cur.e) * ncols + cur.n0 + wave * 64;
-      uint8_t* const lds = smem + 2 * Cfg::kA + wave * 4096;
+      const float* const rs = reinterpret_cast<const float*>(smem + 2 * Cfg::kA + region * Cfg::kScales);
+      const float* const cs = rs + BM + wave * 64;
+      uint8_t* const lds = smem + 2 * (Cfg::kA + Cfg::kScales) + wave * 4096;
 #pragma unroll
       for (int i = 0; i < kFR; ++i) {
-        const int r = 32 * i + frow < cur.rows ? 32 * i + frow : cur.rows - 1;
-        int src = cur.row0 + r;
-        if (GATHER) src = token_of(gather_src[src], gather_k, gather_rows);
-        const float row_scale = a_scale[src];
+        const float row_scale = rs[32 * i + frow];
         const f32x16 y0 = scaled(acc[i][0], cs, row_scale, half), y1 = scaled(acc[i][1], cs + 32, row_scale, half);
         if constexpr (GATE_UP)
           store_y_block(swiglu16(y0, y1), out, 32 * i + frow, cur.n0 / 2 + wave * 32, ldc, half);
