@@ -159,7 +159,8 @@ template <int BM, bool GATE_UP>
 struct TileCfg {
   static constexpr int kA = BM * 128;              // a stage
   static constexpr int kScales = BM * 4 + 1024;    // a tile's row and column scales
-  static constexpr int kOut = 4 * 4096;            // 4 KB a wave for the rows that are stored
+  // h of the whole tile, or 4 KB of ys a wave, on their way out
+  static constexpr int kOut = GATE_UP ? BM * 256 : 4 * 4096;
   static constexpr int kLds = 2 * (kA + kScales) + kOut;
   static constexpr int kFR = BM / 32;              // row fragments; DMA instructions a wave and step
   static constexpr int kPerCu = BM == 64 ? 3 : 2;
@@ -370,18 +371,38 @@ __global__ __launch_bounds__(kTileThreads, BM == 64 ? 3 : 2) void grouped_i8_til
         __builtin_amdgcn_make_buffer_rsrc(C + r0 * ldc, 0, cur.rows * ldc * 2, kBufferWord3);
     const bool mine = cur.n0 + wave * 64 < ncols;  // uniform per wave
     region ^= 1;
+    const float* const rs = reinterpret_cast<const float*>(smem + 2 * Cfg::kA + region * Cfg::kScales);
+    const float* const cs = rs + BM + wave * 64;
+    uint8_t* const stage_out = smem + 2 * (Cfg::kA + Cfg::kScales);
     if (mine) {
-      const float* const rs = reinterpret_cast<const float*>(smem + 2 * Cfg::kA + region * Cfg::kScales);
-      const float* const cs = rs + BM + wave * 64;
-      uint8_t* const lds = smem + 2 * (Cfg::kA + Cfg::kScales) + wave * 4096;
 #pragma unroll
       for (int i = 0; i < kFR; ++i) {
         const float row_scale = rs[32 * i + frow];
         const f32x16 y0 = scaled(acc[i][0], cs, row_scale, half), y1 = scaled(acc[i][1], cs + 32, row_scale, half);
-        if constexpr (GATE_UP)
-          store_y_block(swiglu16(y0, y1), out, 32 * i + frow, cur.n0 / 2 + wave * 32, ldc, half);
-        else
-          store_y_blocks(y0, y1, lds, out, 32 * i, cur.n0 + wave * 64, ldc, lane);
+        if constexpr (GATE_UP) {
+          // 256 bytes of every row are put together, chunk c of row r at c ^ (r & 15)
+          u32x4 lo, hi;
+          pack_y_block(swiglu16(y0, y1), lo, hi);
+          uint8_t* const row = stage_out + (32 * i + frow) * 256;
+          *reinterpret_cast<u32x4*>(row + (((4 * wave + half) ^ (frow & 15)) * 16)) = lo;
+          *reinterpret_cast<u32x4*>(row + (((4 * wave + 2 + half) ^ (frow & 15)) * 16)) = hi;
+        } else {
+          store_y_blocks(y0, y1, stage_out + wave * 4096, out, 32 * i, cur.n0 + wave * 64, ldc, lane);
+        }
+      }
+    }
+    if constexpr (GATE_UP) {
+      fence();  // (the wait and the barrier are no memory accesses to the compiler)
+      wait_lgkm0();
+      __builtin_amdgcn_s_barrier();
+      fence();
+      const int width = ncols - cur.n0 < kTileN ? ncols - cur.n0 : kTileN;
+#pragma unroll
+      for (int m = 0; m < BM / 16; ++m) {
+        const int r = (BM / 4) * wave + 4 * m + (lane >> 4);
+        const u32x4 v = *reinterpret_cast<const u32x4*>(stage_out + r * 256 + (((lane & 15) ^ (r & 15)) * 16));
+        if ((lane & 15) * 16 < width)
+          __builtin_amdgcn_raw_buffer_store_b128(v, out, (r * ldc + cur.n0 / 2) * 2 + (lane & 15) * 16, 0, 0);
       }
     }
     fence();  // (this tile's reads of LDS stay ahead of the next step's barrier)
