@@ -430,15 +430,47 @@ bool too_many_tiles(int64_t rows_cap, int n_experts, int ncols) {
   return (ceil_div(rows_cap, 64) + n_experts) * ceil_div(ncols, kTileN) > (int64_t(1) << 30);
 }
 
+// Which kernel a product takes: the one with the least estimated time, from measured
+// rates (MI355X, us, `steps` = K / 128):
+//   rows: 3.3, and 1.15 ns for every 32 rows x 64 columns x 128 values, or 0.72 a step (split
+//     over four waves 0.19); or the experts' weights at 5.0 TB/s and, for every 64 columns, the
+//     rows at 27;
+//   64-row tiles, three a CU at a time: 4.0, and for each that a CU has 0.36 a step (0.465 for one
+//     alone) and 0.42; or the weights and 1.5;
+//   128-row tiles, two a CU: 4.2, 0.545 (0.632) and 1.65; or the weights and 1.5.
+// Measured against each other (rows, rows split, 64, 128), us:
+//   gate/up 64 experts, D 2048, F 1024, top-8: 1 token 13.4, 7.4, 12.3, 17.2; 48 tokens 41.8,
+//     41.5, 45.4, 44.3; 256 tokens 61, 52, 53.5, 45.7; 384 tokens 67, 69, 49.6, 63; 1000 tokens
+//     129, 139, 65, 60; 4000 tokens 407, 436, 194, 147; 16384 tokens 1496, 1610, 730, 500;
+//   32 experts, D 4096, F 2048, top-4: 48 tokens 88, 100, 102, 90; 300 tokens 131, 131, 107, 121;
+//   24 experts, D 1152, F 640, top-3: 100 tokens 14.2, 8.9, 10.7, 13.1; 333 tokens 15.6, 15.9,
+//     11.5, 14.6; 1500 tokens 31, 32, 14.6, 16.4;
+//   one segment, D 2048, F 1024: 200 rows 15.2, 6.8, 11.2, 16.9; 8000 rows 103, 113, 45, 39.
+// Over 182 such products the rule's choice is 1 % slower than the fastest on average, 21 % at most.
 enum Form { kRows1, kRows4, kTiles64, kTiles128 };
 
 Form choose_form(int64_t rows, int n_experts, int kdim, int ncols, int cus) {
-  const double n = live_experts(rows, n_experts), mean = rows / n;
-  const bool split = kdim >= 1024;
-  (void)ncols;
-  (void)cus;
-  if (mean <= 32 && max_row_tiles(rows, n_experts) <= 65535) return split ? kRows4 : kRows1;
-  return mean <= 256 ? kTiles64 : kTiles128;
+  const double steps = kdim / 128;
+  const double weights = live_experts(rows, n_experts) * ncols * static_cast<double>(kdim) / 5.0e6;
+  const double re_read = static_cast<double>(rows) * (ncols / 64) * kdim / 27e6;
+  const double waves = row_tiles(rows, n_experts, 32) * (ncols / 64);
+  const bool split = steps >= 2 && waves < 5.0 * cus;  // (more waves side by side fill the chip)
+  const double by_rows =
+      std::max({3.3 + waves * steps * 1.15e-3, 3.3 + steps * (split ? 0.19 : 0.72), weights + re_read + 1.0});
+  const auto by_tiles = [&](int bm, int per_cu, double start, double alone, double busy, double end) {
+    const double tiles = row_tiles(rows, n_experts, bm) * static_cast<double>(ceil_div(ncols, kTileN));
+    const double whole = std::floor(tiles / (per_cu * cus)), rest = tiles - whole * per_cu * cus;
+    const double last = rest < 1.0 ? 0.0 : std::max(1.0, std::ceil(rest / cus - 0.02));  // of a CU
+    return std::max(start + steps * (whole * per_cu * busy + (last > 0.0 ? std::max(alone, busy * last) : 0.0)) +
+                        end * (whole * per_cu + last),
+                    weights + 1.5);
+  };
+  const double by_64 = by_tiles(64, TileCfg<64, true>::kPerCu, 4.0, 0.465, 0.36, 0.42);
+  const double by_128 = by_tiles(128, TileCfg<128, true>::kPerCu, 4.2, 0.632, 0.545, 1.65);
+  // (a grid holds 65535 tiles along y)
+  if (by_rows <= std::min(by_64, by_128) && max_row_tiles(rows, n_experts) <= 65535)
+    return split ? kRows4 : kRows1;
+  return by_64 <= by_128 ? kTiles64 : kTiles128;
 }
 
 template <bool GATE_UP, bool GATHER>

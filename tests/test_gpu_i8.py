@@ -137,14 +137,19 @@ def _segments(kind, N, rng):
         return [int(c) for c in rng.integers(0, 130, N)]
     if kind == "many":
         return [int(c) for c in rng.integers(200, 700, N)]
-    counts = [0] * N                # "skewed": most rows with one expert, several without any
-    counts[N // 2], counts[-1] = 1000, 3
+    if kind == "crowd":     # (sums that the larger tiles are taken for)
+        counts = rng.multinomial(9000, rng.dirichlet([2.0] * N))
+        counts[0] = 0
+        return [int(c) for c in counts]
+    counts = [0] * N                # "skewed", "lopsided": most rows with one expert, several without any
+    counts[N // 2], counts[-1] = 14001 if kind == "lopsided" else 1000, 3
     return counts
 
 
 CASES = [("one", 1, 128, 128), ("one", 1, 2048, 256), ("few", 7, 256, 128), ("few", 9, 1152, 384), ("mid", 6, 384, 640),
          ("mid", 5, 1280, 256), ("many", 3, 256, 384), ("many", 4, 1152, 640), ("many", 8, 128, 128),
-         ("skewed", 6, 512, 256), ("skewed", 70, 128, 128), ("mid", 130, 256, 128), ("one", 1, 4096, 4096)]
+         ("skewed", 6, 512, 256), ("skewed", 70, 128, 128), ("mid", 130, 256, 128), ("one", 1, 4096, 4096),
+         ("crowd", 8, 1280, 1152), ("crowd", 40, 1152, 640), ("lopsided", 4, 896, 896), ("lopsided", 6, 128, 640)]
 
 
 @pytest.fixture(scope="module")
