@@ -232,7 +232,7 @@ extern "C" int hmoe_quantize_rows_i8(const void* a, int a_dtype, int64_t rows, i
       hipLaunchKernelGGL((quantize_rows_i8_kernel<float, kNt, kC>), grid, dim3(kThreads), 0, s,
                          static_cast<const float*>(a), rows, cols, offsets, n_experts, q, scale);
   };
-  with_row_form(rows, cols, launch);
+  with_row_form(rows, cols, 2048, launch);
   return check_launch("hmoe_quantize_rows_i8");
 }
 

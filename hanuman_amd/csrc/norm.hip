@@ -12,6 +12,8 @@
 //   dx = dr = ds + rstd (dy w - n mean_d(dy w n)),   dw = sum_t dy n.
 //
 // All of it is bound by memory: a row is read once and kept in registers.
+#include <algorithm>
+
 #include "quant_i8.h"
 #include "quant_mxfp4.h"
 #include "rows.h"
@@ -227,18 +229,29 @@ __global__ __launch_bounds__(1024) void sum_parts_kernel(const float* __restrict
   }
 }
 
-// Parts that dw is summed in: one a row, or as many as keep the memory busy.
-constexpr int kMaxParts = 1024;
+// Parts that dw is summed in: rows of 1024 values and more are a workgroup's, and 512 of them
+// keep the memory busy (16384 x 4096 in bf16: 88 us; 1024 parts 99, 384 91).  Shorter ones are
+// a wave's, and are the more at a time the shorter they are (30000 x 512: 1024 parts 70 us, 2048
+// 49; 100000 x 256: 1024 99, 2048 62, 4096 48; 200000 x 128 float32: 4096 102, 8192 107), and past
+// 1024 of four rows at least (4000 x 1024: 1024 parts 13.6 us, 2048 16.8: the parts are read again).
+constexpr int kBwdWaveCols = 1024;
+constexpr int64_t kMaxParts = 4096;
+int64_t most_parts(int64_t rows, int cols) {
+  if (cols > kBwdWaveCols || rows < kWaveRows) return 512;
+  const int64_t most = std::max(int64_t(1024), std::min((int64_t(1) << 20) / cols, ceil_div(rows, 16) * 4));
+  return most < kMaxParts ? most : kMaxParts;
+}
 struct BwdShape {
   unsigned grid;
   int parts;
 };
 BwdShape bwd_shape(int64_t rows, int cols) {
   BwdShape b{0, 0};
-  with_row_form(rows, cols, [&](auto nt, auto) {
+  with_row_form(rows, cols, kBwdWaveCols, [&](auto nt, auto) {
     constexpr int per_group = decltype(nt)::value == 64 ? 4 : 1;
+    const int64_t most = most_parts(rows, cols) / per_group;
     const int64_t g = ceil_div(rows, per_group);
-    b.grid = static_cast<unsigned>(g < kMaxParts / per_group ? g : kMaxParts / per_group);
+    b.grid = static_cast<unsigned>(g < most ? g : most);
     b.parts = static_cast<int>(b.grid) * per_group;
   });
   return b;
@@ -282,7 +295,7 @@ extern "C" int hmoe_add_rms_norm(const void* x, int x_dtype, const void* residua
   HMOE_REQUIRE_ALIGNED(what, 16, x, residual, weight, sum, y);
   HMOE_REQUIRE_ALIGNED(what, 8, q);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  with_row_form(rows, cols, [&](auto nt, auto c) {
+  with_row_form(rows, cols, 2048, [&](auto nt, auto c) {
     constexpr int kNt = decltype(nt)::value, kC = decltype(c)::value;
     constexpr int kThreads = kNt < 256 ? 256 : kNt;
     with_float_type(x_dtype, [&](auto tx) {
@@ -336,7 +349,7 @@ extern "C" int hmoe_add_rms_norm_bwd(const void* dy, int dy_dtype, const void* s
   HMOE_REQUIRE_CODE(d_weight == nullptr || need == 0 || (workspace && workspace_bytes >= need), HMOE_ERR_WORKSPACE,
                     "%s: workspace has %zu bytes, needs %zu", what, workspace ? workspace_bytes : size_t(0), need);
   float* parts = d_weight == nullptr ? nullptr : b.parts > 1 ? static_cast<float*>(workspace) : d_weight;
-  with_row_form(rows, cols, [&](auto nt, auto c) {
+  with_row_form(rows, cols, kBwdWaveCols, [&](auto nt, auto c) {
     constexpr int kNt = decltype(nt)::value, kC = decltype(c)::value;
     with_float_type(dy_dtype, [&](auto tg) {
       with_float_type(sum_dtype, [&](auto ts) {

@@ -128,7 +128,8 @@ def test_gradients(gpu, rows, cols, g_type, s_type, more):
     # n, dn and their product are rounded, then the row's sum; the last line's operations
     bound = (_terms(cols) + 4) * u * r * n.abs() * size + 6 * u * (r * (dn.abs() + (n * mean).abs()) + want.abs())
     assert ((dx.double() - want).abs() <= bound + 1.01 * HALF_STEP[s_type] * (want.abs() + bound) + 1e-40).all()
-    parts = min(rows, 1024)
+    # a part's rows one after another, a run of parts, the 32 runs, the products and n
+    parts = max(1, _lib.lib().hmoe_add_rms_norm_bwd_workspace_bytes(rows, cols) // (4 * cols))
     terms = -(-rows // parts) + 1 + -(-parts // 32) + 32 + 2
     assert ((dw.double() - (dy.double() * n).sum(0)).abs() <= terms * u * (dy.double() * n).abs().sum(0) + 1e-40).all()
     only, none = K.add_rms_norm_bwd(dy, s, w, rstd, ds, need_weight=False)
