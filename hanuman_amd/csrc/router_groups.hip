@@ -101,7 +101,10 @@ void select_groups(const float* logits, const float* bias, int64_t tokens, int n
   else run(IntC<16>());
 }
 
-int validate_groups(int n_experts, int top_k, int mode, int n_groups, int top_groups) {
+int validate_groups(int64_t tokens, int n_experts, int top_k, int mode, int n_groups, int top_groups) {
+  // (64 lanes a token at most, fewer than 2^32 threads a launch)
+  HMOE_REQUIRE(tokens < (int64_t(1) << 26), "router: tokens must be below 2^26 with groups (got %lld)",
+               (long long)tokens);
   HMOE_REQUIRE(n_groups >= 1 && n_groups <= kMaxGroups && n_experts % n_groups == 0,
                "router: n_groups must divide n_experts and be in [1, %d] (got %d, n_experts %d)", kMaxGroups, n_groups,
                n_experts);
@@ -125,7 +128,7 @@ extern "C" int hmoe_router_grouped(const void* x, int x_dtype, const void* route
                                    int32_t* top_idx, float* gates, hmoe_stream_t stream) {
   using namespace hmoe;
   if (int rc = validate_routing(tokens, n_experts, top_k, mode)) return rc;
-  if (int rc = validate_groups(n_experts, top_k, mode, n_groups, top_groups)) return rc;
+  if (int rc = validate_groups(tokens, n_experts, top_k, mode, n_groups, top_groups)) return rc;
   if (top_groups == n_groups)  // every expert is left
     return hmoe_router(x, x_dtype, router_w, w_dtype, bias, tokens, d_model, n_experts, top_k, mode,
                        routed_scaling_factor, logits, top_idx, gates, stream);
@@ -160,7 +163,7 @@ extern "C" int hmoe_router_grouped_from_logits(const float* logits, const float*
                                                int top_groups, int32_t* top_idx, float* gates, hmoe_stream_t stream) {
   using namespace hmoe;
   if (int rc = validate_routing(tokens, n_experts, top_k, mode)) return rc;
-  if (int rc = validate_groups(n_experts, top_k, mode, n_groups, top_groups)) return rc;
+  if (int rc = validate_groups(tokens, n_experts, top_k, mode, n_groups, top_groups)) return rc;
   if (top_groups == n_groups)
     return hmoe_router_from_logits(logits, bias, tokens, n_experts, top_k, mode, routed_scaling_factor, top_idx, gates,
                                    stream);

@@ -7,6 +7,7 @@ launch (``hmoe_add_rms_norm``) and is differentiable (``hmoe_add_rms_norm_bwd``)
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import kernels as K
 from .moe import Param, _aligned
@@ -73,6 +74,7 @@ class _AddRmsNorm(torch.autograd.Function):
         return y, total
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, d_y, d_total=None):
         total, w, rstd = ctx.saved_tensors
         x_type, r_type, w_type = ctx.types

@@ -94,7 +94,7 @@ int hmoe_router_from_logits(const float* logits, const float* bias, int64_t toke
  * top_groups groups with the largest scores (the lower index first where equal; a score that is
  * NaN is below all others); gates as above.  With top_groups == n_groups these are the calls
  * above.  n_groups <= 64 divides N, top_k <= top_groups * (N / n_groups), with sigmoid groups of
- * two experts at least.  hmoe_router_bwd and hmoe_router_aux take the results as they are. */
+ * two experts at least, tokens < 2^26.  hmoe_router_bwd and hmoe_router_aux take the results as they are. */
 int hmoe_router_grouped(const void* x, int x_dtype, const void* router_w, int w_dtype,
                         const float* bias, int64_t tokens, int d_model, int n_experts, int top_k,
                         int mode, float routed_scaling_factor, int n_groups, int top_groups,
@@ -490,8 +490,9 @@ int hmoe_grouped_down_mxfp4(const uint8_t* h_q, const uint8_t* h_exp, const int3
 /* ---- root-mean-square norm with the residual's addition (the reference's Block norms what
  *      it gives the layer, model/transformer.py:14-24, 82-95; no counterpart in moe.py) -------- */
 
-/* sum = rnd(x + residual) in the residual's type, rstd = (mean_d sum^2 + eps)^(-1/2) of the
- * rounded sum, y = rnd(sum * rstd * weight); float32 sums in a fixed order.  x, y, residual and
+/* sum = rnd(x + residual) in the residual's type (added in float32), rstd = (mean_d sum^2 +
+ * eps)^(-1/2) of the rounded sum, y = rnd(sum * rstd * weight); float32 sums in a fixed order (rows
+ * whose squares pass float32's range have rstd 0).  x, y, residual and
  * weight are F32 or BF16 each, [rows, cols] and [cols].  Without a residual (NULL, then sum NULL
  * too) the norm is x's.  rstd [rows] f32 (or NULL) is what the gradients need.  q (or NULL, then
  * scale NULL too) [rows, cols] and scale [rows] f32: the 8-bit codes of the rounded y, HMOE_I8 by

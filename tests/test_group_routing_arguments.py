@@ -29,6 +29,7 @@ CALLS = [
 @pytest.mark.parametrize("name,args", CALLS, ids=[c[0] for c in CALLS])
 def test_groups(name, args):
     expect(INVALID, "tokens", name, *args(-1, 64, 8, 0, 8, 4, P))
+    expect(INVALID, "2^26", name, *args(1 << 26, 64, 8, 0, 8, 4, P))
     expect(INVALID, "n_experts", name, *args(4, 257, 8, 0, 1, 1, P))
     expect(INVALID, "top_k", name, *args(4, 64, 33, 0, 8, 8, P))
     expect(INVALID, "mode", name, *args(4, 64, 8, 2, 8, 4, P))
