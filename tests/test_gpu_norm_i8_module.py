@@ -8,6 +8,7 @@ import torch
 
 import i8_reference as R
 from hanuman_amd import MoE, RMSNorm, kernels as K, workloads as W
+from hanuman_amd._lib import HmoeError
 from hanuman_amd.layer import DeviceLayer
 
 pytestmark = pytest.mark.gpu
@@ -264,6 +265,95 @@ def test_captured_and_replayed(gpu):
         assert torch.equal(eager[0], want[-1 - i][0])
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+def test_gradients_captured_and_replayed(gpu, dtype):
+    """The norm's forward and backward in a graph, of two sizes of dw's sum, against eager runs
+    between the replays; a second graph beside it has a workspace of its own."""
+    rows, graphs = (1, 700), []
+    norm = RMSNorm(D, device=gpu)
+    norm.scale.value.requires_grad_(True)
+
+    def step(x, r, dy):
+        y, total = norm.with_sum(x, r)
+        return torch.autograd.grad((y, total), (x, r, norm.scale.value), (dy, dy))
+
+    def operands(n, seed):
+        g = torch.Generator(device=gpu).manual_seed(seed)
+        x, r, dy = (torch.randn((n, D), generator=g, device=gpu).to(dtype) for _ in range(3))
+        return x.requires_grad_(True), r.requires_grad_(True), dy
+
+    for n in rows:
+        fixed = operands(n, 0)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(*fixed)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = step(*fixed)
+        graphs.append((graph, n, fixed, got))
+    for seed in (1, 2, 3):
+        want = []
+        for graph, n, fixed, _ in graphs:
+            new = operands(n, seed)
+            with torch.no_grad():
+                for a, b in zip(fixed, new):
+                    a.copy_(b)
+            graph.replay()
+            want.append(step(*new))
+        torch.cuda.synchronize()
+        for (_, _, _, got), w in zip(graphs, want):
+            for a, b in zip(got, w):
+                assert torch.equal(a, b)
+
+
+def test_one_tensor_twice_and_broadcast_ones(gpu):
+    """x as its own residual has both gradients; a row that is broadcast has its rows' sum."""
+    norm = RMSNorm(D, device=gpu)
+    g = torch.Generator(device=gpu).manual_seed(5)
+    x = torch.randn((B, S, D), generator=g, device=gpu).requires_grad_(True)
+    dy = torch.randn((B, S, D), generator=g, device=gpu)
+    y, total = norm.with_sum(x, x)
+    assert torch.equal(total, 2 * x.detach())
+    both, = torch.autograd.grad((y, total), x, (dy, dy))
+    other = x.detach().clone().requires_grad_(True)
+    y, total = norm.with_sum(x, other)
+    one, two = torch.autograd.grad((y, total), (x, other), (dy, dy))
+    assert torch.equal(one, two) and torch.equal(both, one + two)
+    row = torch.randn((1, 1, D), generator=g, device=gpu).requires_grad_(True)
+    y, total = norm.with_sum(x, row.expand(B, S, D))
+    each, summed = torch.autograd.grad((y, total), (x, row), (dy, dy))
+    assert torch.equal(summed, each.sum((0, 1), keepdim=True))
+
+
+def test_second_derivatives_are_refused(gpu):
+    norm = RMSNorm(D, device=gpu)
+    x = _tokens(gpu, 1, torch.float32).requires_grad_(True)
+    dx, = torch.autograd.grad(norm(x).square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        dx.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+def test_mxfp4_experts_of_groups(gpu, dtype):
+    """The 4-bit experts with routing by groups, whose tokens are quantised in a launch of their
+    own: the operators in a row."""
+    layer = _layer(gpu, expert_dtype="mxfp4", n_groups=4, top_groups=2)
+    x = _tokens(gpu, 1, dtype)
+    out, aux = layer(x)
+    t = x.view(-1, D)
+    _, idx, gates = K.router(t, layer.router.value, layer.bias.value, TOP, 0, 2.5, 4, 2)
+    plan = K.dispatch_plan(idx, N, t.shape[0] * TOP)
+    gu = K.pack_mxfp4_gate_up(layer.expert_w_gate.value, layer.expert_w_up.value)
+    dn = K.pack_mxfp4_down(layer.expert_w_down.value)
+    h = K.grouped_gate_up_mxfp4_gather(*K.quantize_rows_mxfp4(t), plan, *gu)
+    ys = K.grouped_down_mxfp4(*h, plan.offsets, *dn)
+    part = layer._shared_ffn_promoted(t) if dtype == torch.float32 else layer._shared_ffn(t)
+    assert torch.equal(out.view(-1, D), K.combine(ys, plan, gates, part, torch.float32))
+    assert torch.equal(aux["expert_counts"], plan.counts)
+
+
 def test_two_streams_at_once(gpu):
     layer = _layer(gpu, expert_dtype="int8", n_groups=4, top_groups=2)
     norm = RMSNorm(D, device=gpu)
@@ -282,8 +372,23 @@ def test_two_streams_at_once(gpu):
 
 
 def test_no_tokens_and_one(gpu):
+    """No tokens: the layer refuses them as without a norm (its losses are means over them), the
+    operators give empty results."""
     layer = _layer(gpu, expert_dtype="int8", n_groups=4, top_groups=2)
     norm = RMSNorm(D, device=gpu)
     x = _tokens(gpu)[:1, :1]
     out, total, aux = layer.behind_norm(norm, x, x)
     assert out.shape == (1, 1, D) and int(aux["expert_counts"].sum()) == TOP
+    none = x[:0]
+    with pytest.raises(HmoeError, match="batch"):
+        layer.behind_norm(norm, none, none)
+    y, total = norm.with_sum(none, none)
+    assert y.shape == total.shape == none.shape
+    r = norm.rows(none, none, quant="int8")
+    _, idx, _ = K.router(r.y, layer.router.value, layer.bias.value, TOP, 0, 2.5, 4, 2)
+    gu = K.pack_i8_gate_up(layer.expert_w_gate.value, layer.expert_w_up.value)
+    dn = K.pack_i8_down(layer.expert_w_down.value)
+    off = torch.zeros(N + 1, dtype=torch.int32, device=gpu)
+    h = K.grouped_gate_up_i8(r.q, r.scale, off, *gu)
+    ys = K.grouped_down_i8(*K.quantize_rows_i8(h, off), off, *dn)
+    assert idx.shape == (0, TOP) and h.shape == (0, F) and ys.shape == (0, D)

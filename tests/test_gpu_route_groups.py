@@ -141,6 +141,69 @@ def test_router(gpu, x_type, w_type, tokens, d_model, shape, mode):
     assert np.array_equal(idx.cpu().numpy(), want_idx) and np.array_equal(gates.cpu().numpy(), want_gates)
 
 
+@pytest.mark.parametrize("shape", [(96, 6, 3, 9), (256, 8, 4, 32), (34, 17, 16, 32), (64, 4, 1, 16)], ids=str)
+@pytest.mark.parametrize("mode", [SIGMOID, SOFTMAX], ids=["sigmoid", "softmax"])
+def test_router_with_more_experts_a_token(gpu, shape, mode):
+    """More than eight experts: the selection in a launch behind the logits'."""
+    n, groups, top, k = shape
+    g = torch.Generator(device=gpu).manual_seed(n)
+    x = torch.randn((130, 128), generator=g, device=gpu).bfloat16()
+    w = torch.randn((128, n), generator=g, device=gpu).bfloat16() * 128**-0.5
+    bias = 0.05 * torch.randn(n, generator=g, device=gpu) if mode == SIGMOID else None
+    logits, idx, gates = K.router(x, w, bias, k, mode, 1.5, groups, top)
+    assert torch.equal(logits, K.router(x, w, bias, 8, mode, 1.5)[0])
+    want_idx, want_gates = _select(logits.cpu().numpy(), None if bias is None else bias.cpu().numpy(), k, mode, 1.5,
+                                   groups, top)
+    assert np.array_equal(idx.cpu().numpy(), want_idx) and np.array_equal(gates.cpu().numpy(), want_gates)
+
+
+@pytest.mark.parametrize("shape", [(256, 8, 4, 8), (64, 8, 2, 12), (36, 3, 2, 7)], ids=str)
+@pytest.mark.parametrize("logits_at,bias_at", [(1, 0), (0, 1), (2, 3), (3, 0)])
+def test_logits_and_bias_inside_buffers(gpu, shape, logits_at, bias_at):
+    """Operands that start anywhere: the results of the same values at 16 bytes."""
+    n, groups, top, k = shape
+    rng = np.random.default_rng(n + logits_at)
+    logits = torch.from_numpy(rng.standard_normal((77, n)).astype(np.float32)).to(gpu)
+    bias = torch.from_numpy((0.05 * rng.standard_normal(n)).astype(np.float32)).to(gpu)
+
+    def inside(t, at):
+        buffer = torch.full((t.numel() + 8,), float("nan"), device=gpu)
+        buffer[at:at + t.numel()] = t.reshape(-1)
+        return buffer[at:at + t.numel()].view(t.shape)
+
+    want = K.router_from_logits(logits, bias, k, SIGMOID, 2.5, groups, top)
+    got = K.router_from_logits(inside(logits, logits_at), inside(bias, bias_at), k, SIGMOID, 2.5, groups, top)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("shape", [(64, 8, 3, 8), (250, 5, 2, 7), (128, 4, 2, 20)], ids=str)
+@pytest.mark.parametrize("mode", [SIGMOID, SOFTMAX], ids=["sigmoid", "softmax"])
+def test_nan_takes_experts_that_exist(gpu, shape, mode):
+    """Rows with NaN, alone or throughout, from logits and from tokens: every slot has another
+    expert, from as many groups as are taken; rows without are not touched by them."""
+    n, groups, top, k = shape
+    g = torch.Generator(device=gpu).manual_seed(n)
+    x = torch.randn((48, 64), generator=g, device=gpu)
+    w = torch.randn((64, n), generator=g, device=gpu) / 8
+    bias = 0.05 * torch.randn(n, generator=g, device=gpu) if mode == SIGMOID else None
+    clean = K.router(x, w, bias, k, mode, 1.0, groups, top)
+    bad = x.clone()
+    bad[3] = float("nan")
+    bad[17, 5] = float("inf")
+    one = clean[0].clone()
+    one[3] = float("nan")
+    one[17, n // 2:n // 2 + 3] = float("nan")
+    one[18, ::2] = -float("nan")
+    ordinary = torch.ones(48, dtype=torch.bool, device=gpu)
+    ordinary[[3, 17, 18]] = False
+    for idx, gates in (K.router(bad, w, bias, k, mode, 1.0, groups, top)[1:],
+                       K.router_from_logits(one, bias, k, mode, 1.0, groups, top)):
+        assert int(idx.min()) >= 0 and int(idx.max()) < n
+        for row in idx.cpu().tolist():
+            assert len(set(row)) == k and len({i // (n // groups) for i in row}) <= top
+        assert torch.equal(idx[ordinary], clean[1][ordinary]) and torch.equal(gates[ordinary], clean[2][ordinary])
+
+
 def test_no_tokens(gpu):
     logits, idx, gates = K.router(torch.empty((0, 64), device=gpu), torch.zeros((64, 8), device=gpu), None, 2, SOFTMAX,
                                   1.0, 4, 2)
