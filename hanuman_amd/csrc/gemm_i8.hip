@@ -50,7 +50,10 @@ __device__ __forceinline__ f32x16 swiglu16(const f32x16& g, const f32x16& u) {
 // 32 rows x 64 columns a wave, operands straight from memory into registers: with few
 // rows an expert every weight is used once or twice, and a fragment is one run of 1 KB.
 // A workgroup is four waves: side by side (SPLIT 1), or on a quarter of the reduction
-// each, joined in LDS (SPLIT 4; the sums are exact, so the order does not matter).
+// each, joined in LDS (SPLIT 4; the sums are exact, so the order does not matter).  Bound by
+// the latency of a wave's chain of loads, then by the weights' bytes: one token on 64 experts,
+// top-8, D 2048, F 1024 (34 and 17 MB of weights) 9.8 us gate/up and 6.8 down, split (13.4
+// gate/up side by side).
 template <bool GATE_UP, bool GATHER, int SPLIT>
 __global__ __launch_bounds__(256) void grouped_i8_rows(
     const int8_t* __restrict__ A, const float* __restrict__ a_scale, const int8_t* __restrict__ B,
@@ -151,8 +154,19 @@ __global__ __launch_bounds__(256) void grouped_i8_rows(
 // through LDS (buffer_load ... lds), two stages of 128 values of every row, the next
 // stage's loads issued behind the one barrier of a step: whole lines, and 16-byte chunk c of
 // row r sits at c ^ swz128(r), so that 16 lanes of a fragment read cover all banks.  A tile's
-// scales come with its first step into one of two regions.  The last column tile may be 128 columns wide: waves 2 and 3 then load and compute the others'
-// again and store nothing.
+// scales come with its first step into one of two regions (from memory in the epilogue: 529 and
+// 333 us against 506 and 269 below).  h is put together in LDS and leaves as 256 bytes of a row
+// (1000 tokens on 64 experts 72 -> 64 us).  The last column tile may be 128 columns wide: waves 2
+// and 3 then load and compute the others' again and store nothing.
+//
+// 131072 rows, D 2048, F 1024, gate/up and down: 500 and 270 us (2.2 and 2.0 POP/s; the matrix
+// cores alone, from registers, 3.6, where the package's power takes the clock to 1.8 GHz; the
+// vendor library's product of 8192^3 1.9).  They are busy in 63 % and 49 % of the cycles at 1.66
+// and 1.78 GHz, and a quarter of the lines that are asked for miss L2.  With operands of zeros
+// (2.4 GHz) 394 and 202 us; every load a hit of L2 463 and 251; without the products 383 and 202:
+// power, the loads' way and the epilogue (438 and 219 without it) share the time, none has all of
+// it.  No faster: A three stages deep (508 and 275 against 517 and 280), steps in another order for
+// each tile, row-tile groups of 1 to 32, two workgroups of 64 rows a CU, no turns.
 constexpr int kTileThreads = 256;
 
 template <int BM, bool GATE_UP>

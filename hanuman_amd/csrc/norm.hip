@@ -11,7 +11,9 @@
 //
 //   dx = dr = ds + rstd (dy w - n mean_d(dy w n)),   dw = sum_t dy n.
 //
-// All of it is bound by memory: a row is read once and kept in registers.
+// All of it is bound by memory: a row is read once and kept in registers, from the addition
+// through the norm to the codes, or from the dot product to dx and dw's part.  (As launches of
+// their own addition, norm and quantisation would read and write 1.4 times the bytes.)
 #include <algorithm>
 
 #include "quant_i8.h"
@@ -37,7 +39,11 @@ struct SumType<TX, NoResidual> {
   typedef TX type;
 };
 
-// NT threads a row, C chunks of eight values each.
+// NT threads a row, C chunks of eight values each.  All loads of a row are issued before the
+// first is used, past the caches' replacement (a row is not read again).  16384 x 2048 in bf16,
+// with a residual and e4m3 codes: 51 us for 302 MB (6.0 TB/s, more than a copy's 4.9: half of
+// the 134 MB that are read still lie in the 256 MB cache); int8 codes the same.  One row: 2.6 us,
+// a chain of one load, two reductions and a store.
 template <typename TX, typename TR, typename TY, int NT, int C>
 __global__ __launch_bounds__(NT < 256 ? 256 : NT) void add_rms_norm_kernel(
     const TX* __restrict__ x, const TR* __restrict__ residual, const void* __restrict__ weight, bool weight_bf16,
@@ -137,7 +143,9 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void add_rms_norm_kernel(
 
 // Gradients.  A workgroup (NT 256 and more) or a wave (NT 64) takes rows a stride apart and
 // keeps its columns' part of dw in registers; the parts are summed in their order by
-// sum_parts_kernel.
+// sum_parts_kernel.  16384 x 4096 in bf16: 82 us for 537 MB (6.5 TB/s; half of what is read
+// lies in the 256 MB cache), and 4.7 for the parts; 2048 x 1536 in float32: 13 and 3.8, four rows
+// one after another in each workgroup.
 template <typename TG, typename TS, int NT, int C>
 __global__ __launch_bounds__(NT < 256 ? 256 : NT) void add_rms_norm_bwd_kernel(
     const TG* __restrict__ dy, const TS* __restrict__ s, const void* __restrict__ weight, bool weight_bf16,

@@ -12,6 +12,11 @@
 // eights, merged), which also gives a group's two largest; lanes of groups that are not taken
 // empty theirs, and the token's lists are merged over its lanes.  More are taken in rounds, the
 // largest of all each time.
+//
+// Bound by vector instructions, 85 a key, of which the sigmoid is 26 (its single operations are
+// what makes the choice the same everywhere) and the lists the rest: 16384 tokens on 256 experts
+// 12 us, of which the logits' 17 MB are 3.7.  In rounds for all, with keys compared as two
+// integers, they took 30 us; with sigmoid_det's range checks and division 13.5.
 #pragma once
 
 #include <type_traits>

@@ -1,5 +1,7 @@
 // Router entries with the selection limited to groups (route_groups.h): in the router's launch
-// for up to eight experts a token, from its logits for more, and from given logits.
+// for up to eight experts a token, from its logits for more, and from given logits.  (As a launch
+// behind the logits one token on 64 experts takes 16.1 us against 14.5, 4096 on 256 82.6 against
+// 75.0; without groups the router's launch takes 16.3 and 77.1.)
 #include "router_kernels.h"
 
 namespace hmoe {
@@ -86,7 +88,8 @@ void launch_select_groups(const float* logits, const float* bias, int64_t tokens
   else launch(IntC<0>(), IntC<0>());
 }
 
-// E: as many keys a lane as leave a token eight lanes and more.
+// E: as many keys a lane as leave a token eight lanes and more (16384 tokens on 256 experts in
+// eight groups, E 8, 16 and 32: 15.8, 11.0 and 12.3 us).
 void select_groups(const float* logits, const float* bias, int64_t tokens, int n_experts, int n_groups,
                    int top_groups, int top_k, int mode, float rsf, int32_t* top_idx, float* gates, hipStream_t s) {
   const auto run = [&](auto E) {

@@ -30,7 +30,11 @@ class RMSNorm:
                      out_dtype, quant)
 
     def with_sum(self, x: torch.Tensor, residual: torch.Tensor | None = None, *, out_dtype=None):
-        """``(y, total)`` in ``x``'s shape; ``total`` is ``x`` without a residual."""
+        """``(y, total)`` in ``x``'s shape; ``total`` is ``x`` without a residual.
+
+        A graph that captures gradients takes them with ``torch.autograd.grad``, or while no
+        autograd graph of the same leaves from before the capture is alive: autograd adds into a
+        leaf's ``.grad`` on the stream of the first of them, which may not be captured."""
         w = self.scale.value
         if residual is not None and residual.shape != x.shape:
             raise ValueError(f"residual must have x's shape {tuple(x.shape)} (got {tuple(residual.shape)})")
