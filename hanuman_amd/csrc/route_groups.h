@@ -7,11 +7,10 @@
 //
 // A token has L lanes: groups g = 0 .. G padded to a power of two, LG lanes for each, E keys in
 // each lane's registers.  A key and its expert are one positive float64 that orders like the
-// pair, so that a comparison-and-exchange is a maximum and a minimum.  Up to eight experts are
-// taken from lists: each lane sorts its keys into the eight largest (a sorting network over
-// eights, merged), which also gives a group's two largest; lanes of groups that are not taken
-// empty theirs, and the token's lists are merged over its lanes.  More are taken in rounds, the
-// largest of all each time.
+// pair, so that a comparison-and-exchange is a maximum and a minimum.  Each lane sorts its keys
+// into a list of the eight, sixteen or 32 largest (top_k and more; a sorting network over eights,
+// merged), which also gives a group's two largest; lanes of groups that are not taken empty
+// theirs, and the token's lists are merged over its lanes.
 //
 // Bound by vector instructions, 85 a key, of which the sigmoid is 26 (its single operations are
 // what makes the choice the same everywhere) and the lists the rest: 16384 tokens on 256 experts
@@ -26,7 +25,7 @@
 namespace hmoe {
 
 constexpr int kMaxGroups = 64;
-constexpr int kList = 8;
+constexpr int kList = 8, kLongList = 16, kLongestList = 32;
 
 struct GroupRule {
   int n_experts, n_groups, top_groups, top_k, mode;
@@ -141,21 +140,56 @@ __device__ __forceinline__ void for_logs(int lo, int hi, F f) {
 }
 
 // Eight values in descending order, with 19 exchanges.
-__device__ __forceinline__ void sort8(double (&c)[kList]) {
+__device__ __forceinline__ void sort8(double (&c)[8]) {
   constexpr int kPairs[19][2] = {{0, 1}, {2, 3}, {4, 5}, {6, 7}, {0, 2}, {1, 3}, {4, 6}, {5, 7}, {1, 2}, {5, 6},
                                  {0, 4}, {3, 7}, {1, 5}, {2, 6}, {1, 4}, {3, 6}, {2, 4}, {3, 5}, {3, 4}};
 #pragma unroll
   for (int i = 0; i < 19; ++i) order2(c[kPairs[i][0]], c[kPairs[i][1]]);
 }
-// a: the eight largest of a and b, both descending.
-__device__ __forceinline__ void merge8(double (&a)[kList], const double (&b)[kList]) {
+// Values that rise and then fall, or the other way, in descending order.
+template <int L>
+__device__ __forceinline__ void order_bitonic(double (&a)[L]) {
 #pragma unroll
-  for (int i = 0; i < kList; ++i) a[i] = dmax(a[i], b[kList - 1 - i]);
+  for (int d = L / 2; d > 0; d /= 2)
 #pragma unroll
-  for (int d = 4; d > 0; d /= 2)
-#pragma unroll
-    for (int i = 0; i < kList; ++i)
+    for (int i = 0; i < L; ++i)
       if ((i & d) == 0) order2(a[i], a[i + d]);
+}
+// a: the L largest of a and b, both descending.
+template <int L>
+__device__ __forceinline__ void merge_lists(double (&a)[L], const double (&b)[L]) {
+#pragma unroll
+  for (int i = 0; i < L; ++i) a[i] = dmax(a[i], b[L - 1 - i]);
+  order_bitonic(a);
+}
+// list: the L largest of c, descending.
+template <int E, int L>
+__device__ __forceinline__ void sort_list(const double (&c)[E], double (&list)[L]) {
+  static_assert(E == 8 || E == 16, "keys of a lane");
+  double part[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) part[i] = c[i];
+  if constexpr (E == 8) {
+    sort8(part);
+  } else {
+    double a[8], b[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      a[i] = c[i];
+      b[i] = c[8 + i];
+    }
+    sort8(a);
+    sort8(b);
+    if constexpr (L == 8) merge_lists(a, b);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      part[i] = a[i];
+      part[15 - i] = b[i];
+    }
+    if constexpr (L > 8) order_bitonic(part);
+  }
+#pragma unroll
+  for (int i = 0; i < L; ++i) list[i] = i < E ? part[i < E ? i : 0] : kNone;
 }
 
 // How many of the token's lanes hold a larger value than this one.
@@ -185,9 +219,9 @@ __device__ __forceinline__ int count_above(double v, int log_lanes) {
 
 // Selection and gates of one token by its lanes.  run(e, l, b): the logits and (sigmoid) the
 // biases of E experts from e on, anything past the last one; get(e): the logit of one.  Every
-// lane of the wave takes part; `store` says whether the token is there.  LIST: top_k is at most
-// eight.
-template <int E, bool LIST, typename Run, typename Get>
+// lane of the wave takes part; `store` says whether the token is there.  L: the lists' length,
+// top_k and more.
+template <int E, int L, typename Run, typename Get>
 __device__ __forceinline__ void select_in_groups(Run run, Get get, const GroupRule& r, bool store,
                                                  int32_t* __restrict__ idx_row, float* __restrict__ gates_row) {
 #pragma clang fp contract(off)
@@ -199,8 +233,7 @@ __device__ __forceinline__ void select_in_groups(Run run, Get get, const GroupRu
   const int e0 = group * r.size + in0;
   const int live = group < r.n_groups ? r.size - in0 : 0;  // of this lane's keys
   const bool sigmoid = r.mode == HMOE_ROUTE_SIGMOID_BIAS;
-  constexpr int kKeys = LIST && E < kList ? kList : E;
-  double c[kKeys];
+  double c[E];
   float l[E], b[E];
   run(live > 0 ? e0 : 0, l, b);
   if (sigmoid) {
@@ -217,34 +250,11 @@ __device__ __forceinline__ void select_in_groups(Run run, Get get, const GroupRu
   }
 #pragma unroll
   for (int j = 0; j < E; ++j) c[j] = j < live ? ranked(l[j], e0 + j) : kNone;
-#pragma unroll
-  for (int j = E; j < kKeys; ++j) c[j] = kNone;
 
-  // this lane's two largest
-  double list[kList];
-  double best1 = kNone, best2 = kNone;
-  if constexpr (LIST) {
-#pragma unroll
-    for (int i = 0; i < kList; ++i) list[i] = c[i];
-    sort8(list);
-#pragma unroll
-    for (int j = kList; j < kKeys; j += kList) {
-      double more[kList];
-#pragma unroll
-      for (int i = 0; i < kList; ++i) more[i] = c[j + i];
-      sort8(more);
-      merge8(list, more);
-    }
-    best1 = list[0];
-    best2 = list[1];
-  } else {
-#pragma unroll
-    for (int j = 0; j < E; ++j) {
-      best2 = dmax(best2, dmin(best1, c[j]));
-      best1 = dmax(best1, c[j]);
-    }
-  }
-  // the group's
+  double list[L];
+  sort_list(c, list);
+  // the group's two largest
+  double best1 = list[0], best2 = list[1];
   for_logs(0, r.log_lg, [&](auto log) __attribute__((always_inline)) {
     double a1, b1, a2, b2;
     beside<decltype(log)::value>(best1, a1, b1);
@@ -261,46 +271,30 @@ __device__ __forceinline__ void select_in_groups(Run run, Get get, const GroupRu
   // (a group's lanes hold the same score)
   const bool taken = count_above(score, r.log_lanes) < r.top_groups << r.log_lg;
 
-  // slot k of the token is kept by lane k % lanes, as its (k / lanes)th
-  double mine[4] = {kNone, kNone, kNone, kNone};
-  if constexpr (LIST) {
 #pragma unroll
-    for (int i = 0; i < kList; ++i) list[i] = taken ? list[i] : kNone;
-    for_logs(0, r.log_lanes, [&](auto log) __attribute__((always_inline)) {
-      double other[kList];
+  for (int i = 0; i < L; ++i) list[i] = taken ? list[i] : kNone;
+  for_logs(0, r.log_lanes, [&](auto log) __attribute__((always_inline)) {
+    double other[L];
 #pragma unroll
-      for (int i = 0; i < kList; ++i) {
-        double a, b;
-        beside<decltype(log)::value>(list[i], a, b);
-        list[i] = a;
-        other[i] = b;
-      }
-      merge8(list, other);
-    });
-    // (a token has eight lanes at least)
-#pragma unroll
-    for (int i = 0; i < kList; ++i) mine[0] = p == i ? list[i] : mine[0];
-  } else {
-#pragma unroll
-    for (int j = 0; j < E; ++j) c[j] = taken ? c[j] : kNone;
-    for (int k = 0; k < r.top_k; ++k) {
-      double most = c[0];
-#pragma unroll
-      for (int j = 1; j < E; ++j) most = dmax(most, c[j]);
-      for_logs(0, r.log_lanes, [&](auto log) __attribute__((always_inline)) {
-        double a, b;
-        beside<decltype(log)::value>(most, a, b);
-        most = dmax(a, b);
-      });
-#pragma unroll
-      for (int j = 0; j < E; ++j) c[j] = c[j] == most ? kNone : c[j];
-      const int slot = k >> r.log_lanes;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) mine[q] = q == slot && (k & (lanes - 1)) == p ? most : mine[q];
+    for (int i = 0; i < L; ++i) {
+      double a, b;
+      beside<decltype(log)::value>(list[i], a, b);
+      list[i] = a;
+      other[i] = b;
     }
+    merge_lists(list, other);
+  });
+  // slot k of the token is kept by lane k % lanes, as its (k / lanes)th (a token has eight lanes
+  // at least)
+  constexpr int kSlots = L / 8;
+  double mine[kSlots];
+#pragma unroll
+  for (int q = 0; q < kSlots; ++q) {
+    mine[q] = kNone;
+#pragma unroll
+    for (int i = 8 * q; i < L; ++i) mine[q] = p == i - (q << r.log_lanes) ? list[i] : mine[q];
   }
   // gates, summed in the slots' order
-  constexpr int kSlots = LIST ? 1 : 4;
   int at[kSlots];
   float value[kSlots];
 #pragma unroll
@@ -316,20 +310,17 @@ __device__ __forceinline__ void select_in_groups(Run run, Get get, const GroupRu
 #pragma unroll
     for (int q = 0; q < kSlots; ++q) value[q] = exp_det(value[q] - most);
   }
-  float sum = 0.0f;
-  if constexpr (LIST) {
-    float v[kList];
+  float v[L];
 #pragma unroll
-    for (int k = 0; k < kList; ++k) v[k] = __shfl(value[0], first + k);
+  for (int k = 0; k < L; ++k) {
+    float of = value[0];
 #pragma unroll
-    for (int k = 0; k < kList; ++k) sum = k < r.top_k ? sum + v[k] : sum;
-  } else {
-    for (int k = 0; k < r.top_k; ++k) {
-      const int slot = k >> r.log_lanes;
-      const float v = slot == 0 ? value[0] : slot == 1 ? value[1] : slot == 2 ? value[2] : value[3];
-      sum = sum + __shfl(v, first + (k & (lanes - 1)));
-    }
+    for (int q = 1; q <= k / 8; ++q) of = k >> r.log_lanes == q ? value[q] : of;
+    v[k] = __shfl(of, first + (k & (lanes - 1)));
   }
+  float sum = 0.0f;
+#pragma unroll
+  for (int k = 0; k < L; ++k) sum = k < r.top_k ? sum + v[k] : sum;
 #pragma unroll
   for (int q = 0; q < kSlots; ++q) {
     const int k = (q << r.log_lanes) + p;

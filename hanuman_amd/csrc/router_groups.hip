@@ -11,7 +11,7 @@ namespace {
 // >> log_lanes tokens, whose logits, one run of memory, go through LDS, and the biases: a lane
 // reads E of each one after another (four words more every 32, so that lanes 32 words apart read
 // different banks).  WIDE: all of it 16 bytes at a time.
-template <int E, bool LIST, bool WIDE>
+template <int E, int L, bool WIDE>
 __global__ __launch_bounds__(256) void select_groups_kernel(const float* __restrict__ logits,
                                                             const float* __restrict__ bias, int64_t tokens,
                                                             GroupRule r, int32_t* __restrict__ top_idx,
@@ -65,7 +65,7 @@ __global__ __launch_bounds__(256) void select_groups_kernel(const float* __restr
   };
   const auto get = [&](int e) __attribute__((always_inline)) { return mine[row + e + ((row + e) >> 5) * 4]; };
   const int64_t tq = store ? tok : t0;
-  select_in_groups<E, LIST>(run, get, r, store, top_idx + tq * r.top_k, gates + tq * r.top_k);
+  select_in_groups<E, L>(run, get, r, store, top_idx + tq * r.top_k, gates + tq * r.top_k);
 }
 
 template <int E>
@@ -78,14 +78,17 @@ void launch_select_groups(const float* logits, const float* bias, int64_t tokens
       static_cast<size_t>(4) * (group_stage_words(per_wave * n_experts) + group_stage_words(n_experts)) * sizeof(float);
   const dim3 grid(static_cast<unsigned>(ceil_div(tokens, 4 * per_wave)));
   const bool wide = r.size % 4 == 0 && aligned_to(logits, 16) && (bias == nullptr || aligned_to(bias, 16));
-  const auto launch = [&](auto LIST, auto WIDE) {
-    hipLaunchKernelGGL((select_groups_kernel<E, decltype(LIST)::value, decltype(WIDE)::value>), grid, dim3(256), lds, s,
+  const auto launch = [&](auto L, auto WIDE) {
+    hipLaunchKernelGGL((select_groups_kernel<E, decltype(L)::value, decltype(WIDE)::value>), grid, dim3(256), lds, s,
                        logits, bias, tokens, r, top_idx, gates);
   };
-  if (top_k <= kList && wide) launch(IntC<1>(), IntC<1>());
-  else if (top_k <= kList) launch(IntC<1>(), IntC<0>());
-  else if (wide) launch(IntC<0>(), IntC<1>());
-  else launch(IntC<0>(), IntC<0>());
+  const auto with_list = [&](auto L) {
+    if (wide) launch(L, IntC<1>());
+    else launch(L, IntC<0>());
+  };
+  if (top_k <= kList) with_list(IntC<kList>());
+  else if (top_k <= kLongList) with_list(IntC<kLongList>());
+  else with_list(IntC<kLongestList>());
 }
 
 // E: as many keys a lane as leave a token eight lanes and more (16384 tokens on 256 experts in

@@ -409,7 +409,7 @@ __device__ __forceinline__ void router_select_groups(const float* lg, const floa
       }
     };
     const auto get = [&](int e) __attribute__((always_inline)) { return mine[e]; };
-    select_in_groups<E, true>(run, get, r, store, top_idx + tq * r.top_k, gates + tq * r.top_k);
+    select_in_groups<E, kList>(run, get, r, store, top_idx + tq * r.top_k, gates + tq * r.top_k);
   }
 }
 
