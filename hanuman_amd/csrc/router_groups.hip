@@ -10,11 +10,12 @@ namespace {
 // Selection and gates among the experts of the best groups from given logits.  A wave takes 64
 // >> log_lanes tokens, whose logits, one run of memory, go through LDS, and the biases: a lane
 // reads E of each one after another (four words more every 32, so that lanes 32 words apart read
-// different banks).  WIDE: all of it 16 bytes at a time.
+// different banks).  WIDE: the lanes' reads 16 bytes at a time, `wide_in`: the loads from memory.
 template <int E, int L, bool WIDE>
 __global__ __launch_bounds__(256) void select_groups_kernel(const float* __restrict__ logits,
                                                             const float* __restrict__ bias, int64_t tokens,
-                                                            GroupRule r, int32_t* __restrict__ top_idx,
+                                                            GroupRule r, bool wide_in,
+                                                            int32_t* __restrict__ top_idx,
                                                             float* __restrict__ gates) {
   extern __shared__ __attribute__((aligned(16))) float stage[];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -27,12 +28,13 @@ __global__ __launch_bounds__(256) void select_groups_kernel(const float* __restr
   float* biases = mine + group_stage_words(per_wave * n);
   const float* src = logits + t0 * n;
   const auto park = [&](const float* from, float* to, int words) __attribute__((always_inline)) {
-    if constexpr (WIDE) {
-      for (int i = lane * 4; i < words; i += 256)
+    int done = 0;
+    if (wide_in) {  // uniform
+      done = words & ~3;
+      for (int i = lane * 4; i < done; i += 256)
         *reinterpret_cast<f32x4*>(to + i + (i >> 5) * 4) = *reinterpret_cast<const f32x4*>(from + i);
-    } else {
-      for (int i = lane; i < words; i += 64) to[i + (i >> 5) * 4] = from[i];
     }
+    for (int i = done + lane; i < words; i += 64) to[i + (i >> 5) * 4] = from[i];
   };
   park(src, mine, count);
   if (bias != nullptr) {
@@ -77,13 +79,15 @@ void launch_select_groups(const float* logits, const float* bias, int64_t tokens
   const size_t lds =
       static_cast<size_t>(4) * (group_stage_words(per_wave * n_experts) + group_stage_words(n_experts)) * sizeof(float);
   const dim3 grid(static_cast<unsigned>(ceil_div(tokens, 4 * per_wave)));
-  const bool wide = r.size % 4 == 0 && aligned_to(logits, 16) && (bias == nullptr || aligned_to(bias, 16));
+  // (a wave's logits start a multiple of per_wave * n_experts words on)
+  const bool wide_in =
+      per_wave * n_experts % 4 == 0 && aligned_to(logits, 16) && (bias == nullptr || aligned_to(bias, 16));
   const auto launch = [&](auto L, auto WIDE) {
     hipLaunchKernelGGL((select_groups_kernel<E, decltype(L)::value, decltype(WIDE)::value>), grid, dim3(256), lds, s,
-                       logits, bias, tokens, r, top_idx, gates);
+                       logits, bias, tokens, r, wide_in, top_idx, gates);
   };
   const auto with_list = [&](auto L) {
-    if (wide) launch(L, IntC<1>());
+    if (r.size % 4 == 0) launch(L, IntC<1>());
     else launch(L, IntC<0>());
   };
   if (top_k <= kList) with_list(IntC<kList>());
