@@ -197,9 +197,20 @@ def lib() -> ctypes.CDLL:
     return so
 
 
+class _Entries(dict):
+    """Entry points by name, each looked up at its first call."""
+
+    def __missing__(self, name: str):
+        self[name] = fn = getattr(lib(), name)
+        return fn
+
+
+_ENTRIES = _Entries()
+
+
 def call(name: str, *args) -> None:
     """Calls a status-returning entry point and raises :class:`HmoeError` on failure."""
-    rc = getattr(lib(), name)(*args)
+    rc = _ENTRIES[name](*args)
     if rc != OK:
         msg = lib().hmoe_last_error().decode(errors="replace")
         raise HmoeError(name, rc, msg)

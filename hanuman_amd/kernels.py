@@ -17,6 +17,7 @@ from . import _lib
 from ._lib import call
 
 _DT = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
+_get_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
 def _dtype_code(t: torch.Tensor) -> int:
@@ -33,7 +34,7 @@ def _ptr(t):
 def _stream() -> int:
     # torch.cuda.current_stream().cuda_stream without the Stream object, which takes
     # 2.7 us to make: as long as a launch
-    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+    return _raw_stream(_get_device())
 
 
 def _check(t: torch.Tensor, name: str, ndim: int | None = None):
@@ -72,9 +73,9 @@ def _router_operands(x, router_w, bias, top_k: int):
         if bias.dtype != torch.float32 or bias.shape[0] != N:
             raise ValueError("bias must be float32 [n_experts]")
     dev = x.device
-    logits = torch.empty((T, N), dtype=torch.float32, device=dev)
-    top_idx = torch.empty((T, top_k), dtype=torch.int32, device=dev)
-    gates = torch.empty((T, top_k), dtype=torch.float32, device=dev)
+    logits = torch.empty(T, N, dtype=torch.float32, device=dev)
+    top_idx = torch.empty(T, top_k, dtype=torch.int32, device=dev)
+    gates = torch.empty(T, top_k, dtype=torch.float32, device=dev)
     return T, D, N, logits, top_idx, gates
 
 
@@ -166,8 +167,9 @@ def router_from_logits(logits: torch.Tensor, bias: torch.Tensor | None, top_k: i
         _check(bias, "bias", 1)
         if bias.dtype != torch.float32 or bias.shape[0] != N:
             raise ValueError("bias must be float32 [n_experts]")
-    top_idx = torch.empty((T, top_k), dtype=torch.int32, device=logits.device)
-    gates = torch.empty((T, top_k), dtype=torch.float32, device=logits.device)
+    dev = logits.device
+    top_idx = torch.empty(T, top_k, dtype=torch.int32, device=dev)
+    gates = torch.empty(T, top_k, dtype=torch.float32, device=dev)
     if top_groups is not None and top_groups != n_groups:
         dev = _current_device("router_from_logits", logits, 2)
         if bias is not None:
@@ -743,7 +745,7 @@ def grouped_down_fp8_mx(h_q: torch.Tensor, h_exp: torch.Tensor, offsets: torch.T
 # start at 16 bytes, exponents at 4 (any row of such a matrix does).
 
 _U8, _TENSOR = torch.uint8, torch.Tensor
-_I8, _F32 = torch.int8, torch.float32
+_I8, _F32, _BF16 = torch.int8, torch.float32, torch.bfloat16
 
 
 def _u8(name: str, dev, t: torch.Tensor, shape: tuple):
@@ -767,9 +769,10 @@ def _same_device(name: str, t: torch.Tensor, dev):
 def _current_device(name: str, t: torch.Tensor, ndim: int):
     """The device of a call's first tensor, which has to be the current one: the call
     goes to that one's current stream."""
-    _check(t, name, ndim)
+    if not (t.__class__ is _TENSOR and t.is_cuda and t.is_contiguous() and t.dim() == ndim):
+        _check(t, name, ndim)
     dev = t.device
-    if dev.index != torch._C._cuda_getDevice():
+    if dev.index != _get_device():
         raise ValueError(f"{name}: tensors on {dev}, but the current device is "
                          f"cuda:{torch.cuda.current_device()}")
     return dev
@@ -982,14 +985,14 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor |
         total = torch.empty_like(residual)
         total_ptr, r_ptr = total.data_ptr(), residual.data_ptr()
     rows, cols = shape
-    rstd = x.new_empty((rows,), dtype=_F32)
+    rstd = torch.empty(rows, dtype=_F32, device=dev)
     q = scale = q_ptr = scale_ptr = None
     if quant is not None:
         q = torch.empty_like(x, dtype=_I8 if quant == "int8" else _U8)
         scale = torch.empty_like(rstd)
         q_ptr, scale_ptr = q.data_ptr(), scale.data_ptr()
     call("hmoe_add_rms_norm", x.data_ptr(), x_code, r_ptr, r_code, weight.data_ptr(), w_code, eps, rows, cols,
-         total_ptr, y.data_ptr(), y_code, rstd.data_ptr(), q_ptr, _QUANT[quant], scale_ptr, _stream())
+         total_ptr, y.data_ptr(), y_code, rstd.data_ptr(), q_ptr, _QUANT[quant], scale_ptr, _raw_stream(dev.index))
     return NormOut(y, total, rstd, q, scale)
 
 
@@ -1012,9 +1015,9 @@ def add_rms_norm_bwd(dy: torch.Tensor, total: torch.Tensor, weight: torch.Tensor
     dx = torch.empty_like(total)
     dw, ws, ws_bytes = None, None, 0
     if need_weight:
-        dw = total.new_empty(shape[1:], dtype=torch.float32)
+        dw = torch.empty(shape[1], dtype=_F32, device=dev)
         ws_bytes = _lib.lib().hmoe_add_rms_norm_bwd_workspace_bytes(shape[0], shape[1])
-        ws = total.new_empty(ws_bytes, dtype=_U8)
+        ws = torch.empty(ws_bytes, dtype=_U8, device=dev)
     call("hmoe_add_rms_norm_bwd", dy.data_ptr(), g_code, total.data_ptr(), s_code, weight.data_ptr(), w_code,
          rstd.data_ptr(), _ptr(d_sum), shape[0], shape[1], dx.data_ptr(), _ptr(dw), _ptr(ws), ws_bytes, _stream())
     return dx, dw
@@ -1045,13 +1048,14 @@ def quantize_rows_i8(a: torch.Tensor, offsets: torch.Tensor | None = None):
     dev = _current_device(name, a, 2)
     rows, cols = a.shape
     q = torch.empty_like(a, dtype=_I8)
-    scale = a.new_empty((rows,), dtype=_F32)
+    scale = torch.empty(rows, dtype=_F32, device=dev)
     n, off = 0, None
     if offsets is not None:
-        _check_i32(name, "offsets", offsets, offsets.numel(), dev)
-        n, off = offsets.numel() - 1, offsets.data_ptr()
+        n = offsets.numel() - 1
+        _check_i32(name, "offsets", offsets, n + 1, dev)
+        off = offsets.data_ptr()
     call("hmoe_quantize_rows_i8", a.data_ptr(), _dtype_code(a), rows, cols, off, n, q.data_ptr(), scale.data_ptr(),
-         _stream())
+         _raw_stream(dev.index))
     return q, scale
 
 
@@ -1065,7 +1069,8 @@ def _dequantize_rows(name: str, q: torch.Tensor, scale: torch.Tensor, dtype: tor
     if out_dtype not in _DT:
         raise TypeError(f"unsupported dtype {out_dtype}; expected float32 or bfloat16")
     out = torch.empty_like(q, dtype=out_dtype)
-    call("hmoe_" + name, q.data_ptr(), scale.data_ptr(), rows, cols, out.data_ptr(), _DT[out_dtype], _stream())
+    call("hmoe_" + name, q.data_ptr(), scale.data_ptr(), rows, cols, out.data_ptr(), _DT[out_dtype],
+         _raw_stream(dev.index))
     return out
 
 
@@ -1136,9 +1141,9 @@ def grouped_gate_up_i8(xs_q: torch.Tensor, xs_scale: torch.Tensor, offsets: torc
         _codes(name, "xs_q", dev, xs_q, _I8, (rows, D))
     _codes(name, "xs_scale", dev, xs_scale, _F32, (rows,))
     _check_i32(name, "offsets", offsets, N + 1, dev)
-    h = xs_q.new_empty((rows, F), dtype=torch.bfloat16)
+    h = torch.empty(rows, F, dtype=_BF16, device=dev)
     call("hmoe_grouped_gate_up_i8", xs_q.data_ptr(), xs_scale.data_ptr(), offsets.data_ptr(), N, rows, D, F,
-         w_packed.data_ptr(), w_scales.data_ptr(), h.data_ptr(), _stream())
+         w_packed.data_ptr(), w_scales.data_ptr(), h.data_ptr(), _raw_stream(dev.index))
     return h
 
 
@@ -1153,14 +1158,15 @@ def grouped_gate_up_i8_gather(x_q: torch.Tensor, x_scale: torch.Tensor, plan: Pl
     if x_q.dtype is not _I8 or cols != D:
         _codes(name, "x_q", dev, x_q, _I8, (T, D))
     _codes(name, "x_scale", dev, x_scale, _F32, (T,))
-    if plan.n_experts != N or plan.slot_pos.numel() != T * plan.top_k:
+    offsets, perm_src, rows, top_k = plan.offsets, plan.perm_src, plan.rows_cap, plan.top_k
+    if plan.n_experts != N or plan.slot_pos.numel() != T * top_k:
         raise ValueError(f"{name}: the plan is of other tokens or experts")
-    _check_i32(name, "offsets", plan.offsets, N + 1, dev)
-    _check_i32(name, "perm_src", plan.perm_src, plan.rows_cap, dev)
-    h = x_q.new_empty((plan.rows_cap, F), dtype=torch.bfloat16)
-    call("hmoe_grouped_gate_up_i8_gather", x_q.data_ptr(), x_scale.data_ptr(), T, plan.top_k,
-         plan.perm_src.data_ptr(), plan.offsets.data_ptr(), N, plan.rows_cap, D, F, w_packed.data_ptr(),
-         w_scales.data_ptr(), h.data_ptr(), _stream())
+    _check_i32(name, "offsets", offsets, N + 1, dev)
+    _check_i32(name, "perm_src", perm_src, rows, dev)
+    h = torch.empty(rows, F, dtype=_BF16, device=dev)
+    call("hmoe_grouped_gate_up_i8_gather", x_q.data_ptr(), x_scale.data_ptr(), T, top_k, perm_src.data_ptr(),
+         offsets.data_ptr(), N, rows, D, F, w_packed.data_ptr(), w_scales.data_ptr(), h.data_ptr(),
+         _raw_stream(dev.index))
     return h
 
 
@@ -1176,9 +1182,9 @@ def grouped_down_i8(h_q: torch.Tensor, h_scale: torch.Tensor, offsets: torch.Ten
         _codes(name, "h_q", dev, h_q, _I8, (rows, F))
     _codes(name, "h_scale", dev, h_scale, _F32, (rows,))
     _check_i32(name, "offsets", offsets, N + 1, dev)
-    ys = h_q.new_empty((rows, D), dtype=torch.bfloat16)
+    ys = torch.empty(rows, D, dtype=_BF16, device=dev)
     call("hmoe_grouped_down_i8", h_q.data_ptr(), h_scale.data_ptr(), offsets.data_ptr(), N, rows, F, D,
-         w_packed.data_ptr(), w_scales.data_ptr(), ys.data_ptr(), _stream())
+         w_packed.data_ptr(), w_scales.data_ptr(), ys.data_ptr(), _raw_stream(dev.index))
     return ys
 
 
@@ -1457,7 +1463,7 @@ def router_bwd(logits: torch.Tensor | None, top_idx: torch.Tensor, gates: torch.
     T, K = top_idx.shape
     if logits is not None:
         _check(logits, "logits", 2)
-    dl = torch.empty((T, n_experts), dtype=torch.float32, device=top_idx.device)
+    dl = torch.empty(T, n_experts, dtype=torch.float32, device=top_idx.device)
     call("hmoe_router_bwd", _ptr(logits), _ptr(top_idx), _ptr(gates), _ptr(d_gates), T,
          n_experts, K, mode, routed_scaling_factor, _ptr(dl), _stream())
     return dl
