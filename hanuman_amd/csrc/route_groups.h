@@ -5,7 +5,7 @@
 // index first where equal (totalOrder).  A score that is NaN is below every other.  Gates as
 // without groups.
 //
-// A token has L lanes: groups g = 0 .. G padded to a power of two, LG lanes for each, E keys in
+// A token has 2^log_lanes lanes: groups g = 0 .. G padded to a power of two, 2^log_lg each, E keys in
 // each lane's registers.  A key and its expert are one positive float64 that orders like the
 // pair, so that a comparison-and-exchange is a maximum and a minimum.  Each lane sorts its keys
 // into a list of the eight, sixteen or 32 largest (top_k and more; a sorting network over eights,

@@ -47,7 +47,9 @@ def _select(logits, bias, k, mode, rsf, groups, top):
 # experts, groups, groups taken, experts taken
 SHAPES = [(64, 8, 4, 8), (256, 8, 4, 8), (256, 2, 1, 32), (80, 4, 2, 8), (256, 64, 3, 12), (6, 3, 2, 3), (8, 2, 1, 4),
           (255, 3, 2, 7), (130, 5, 1, 26), (16, 8, 1, 2), (160, 16, 4, 9), (4, 2, 1, 1), (128, 32, 31, 32), (96, 3, 2, 6),
-          (250, 2, 1, 5), (34, 17, 16, 32), (256, 128 // 4, 2, 16)]
+          (250, 2, 1, 5), (34, 17, 16, 32), (256, 128 // 4, 2, 16),
+          # lists of sixteen and of 32, on tokens of eight and sixteen lanes
+          (128, 8, 2, 32), (120, 8, 3, 25), (112, 8, 7, 17), (120, 8, 1, 13), (60, 4, 3, 9), (256, 16, 2, 32), (252, 7, 6, 31)]
 
 
 def _check(gpu, logits, bias, shape, mode, rsf=2.5):
@@ -141,7 +143,8 @@ def test_router(gpu, x_type, w_type, tokens, d_model, shape, mode):
     assert np.array_equal(idx.cpu().numpy(), want_idx) and np.array_equal(gates.cpu().numpy(), want_gates)
 
 
-@pytest.mark.parametrize("shape", [(96, 6, 3, 9), (256, 8, 4, 32), (34, 17, 16, 32), (64, 4, 1, 16)], ids=str)
+@pytest.mark.parametrize("shape", [(96, 6, 3, 9), (256, 8, 4, 32), (34, 17, 16, 32), (64, 4, 1, 16), (128, 8, 5, 32)],
+                         ids=str)
 @pytest.mark.parametrize("mode", [SIGMOID, SOFTMAX], ids=["sigmoid", "softmax"])
 def test_router_with_more_experts_a_token(gpu, shape, mode):
     """More than eight experts: the selection in a launch behind the logits'."""
