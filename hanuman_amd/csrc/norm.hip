@@ -141,21 +141,63 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void add_rms_norm_kernel(
   }
 }
 
+// dw of few rows, 64 columns a workgroup: dy, s and rstd are all that it needs.  Runs of rows a
+// stride apart, eight columns a thread, each summed on its own and the runs one after another.
+template <typename TG, typename TS, int THREADS>
+__device__ __forceinline__ void sum_columns(const TG* __restrict__ dy, const TS* __restrict__ s,
+                                            const float* __restrict__ rstd, int rows, int cols,
+                                            float* __restrict__ d_weight) {
+  constexpr int kRuns = THREADS / 8;
+  __shared__ float run[kRuns][65];
+  const int c0 = blockIdx.x * 64, c = (threadIdx.x & 7) * 8;
+  const int mine = threadIdx.x >> 3;
+  float dw[8] = {};
+  if (c0 + c < cols) {
+#pragma unroll 4
+    for (int row = mine; row < rows; row += kRuns) {
+      Chunk8<TG> g;
+      Chunk8<TS> v;
+      g.load(dy + static_cast<int64_t>(row) * cols + c0 + c);
+      v.load(s + static_cast<int64_t>(row) * cols + c0 + c);
+      const float rs = rstd[row];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) dw[i] = __builtin_fmaf(g.get(i), v.get(i) * rs, dw[i]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) run[mine][c + i] = dw[i];
+  __syncthreads();
+  if (threadIdx.x < 64 && c0 + static_cast<int>(threadIdx.x) < cols) {
+    float total = run[0][threadIdx.x];
+#pragma unroll 8
+    for (int k = 1; k < kRuns; ++k) total += run[k][threadIdx.x];
+    d_weight[c0 + threadIdx.x] = total;
+  }
+}
+
 // Gradients.  A workgroup (NT 256 and more) or a wave (NT 64) takes rows a stride apart and
 // keeps its columns' part of dw in registers; the parts are summed in their order by
 // sum_parts_kernel.  16384 x 4096 in bf16: 82 us for 537 MB (6.5 TB/s; half of what is read
 // lies in the 256 MB cache), and 4.7 for the parts; 2048 x 1536 in float32: 13 and 3.8, four rows
-// one after another in each workgroup.
-template <typename TG, typename TS, int NT, int C>
+// one after another in each workgroup.  FEW: the first dw_groups workgroups sum dw's columns
+// instead, beside the rows' (kFewRows).
+template <typename TG, typename TS, int NT, int C, bool FEW>
 __global__ __launch_bounds__(NT < 256 ? 256 : NT) void add_rms_norm_bwd_kernel(
     const TG* __restrict__ dy, const TS* __restrict__ s, const void* __restrict__ weight, bool weight_bf16,
     const float* __restrict__ rstd, const TS* __restrict__ d_sum, int64_t rows, int cols, TS* __restrict__ dx,
-    float* __restrict__ dw_parts) {
+    float* __restrict__ dw_parts, unsigned dw_groups) {
   constexpr int kThreads = NT < 256 ? 256 : NT;
+  if constexpr (FEW) {
+    if (blockIdx.x < dw_groups) {  // uniform
+      sum_columns<TG, TS, kThreads>(dy, s, rstd, static_cast<int>(rows), cols, dw_parts);
+      return;
+    }
+  }
   __shared__ float part[2][NT / 64];
   const int t = threadIdx.x % NT;
   const int chunks = cols / 8;
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * (kThreads / NT) + threadIdx.x / NT;
+  const int64_t first =
+      static_cast<int64_t>(blockIdx.x - (FEW ? dw_groups : 0u)) * (kThreads / NT) + threadIdx.x / NT;
   const int64_t stride = static_cast<int64_t>(gridDim.x) * (kThreads / NT);
   float dw[C][8] = {};
   float w[C][8];
@@ -206,7 +248,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void add_rms_norm_bwd_kernel(
       if (c < chunks) round_store8(dx + r0 + c * 8, d);
     }
   }
-  if (dw_parts == nullptr) return;
+  if (FEW || dw_parts == nullptr) return;
 #pragma unroll
   for (int u = 0; u < C; ++u) {
     const int c = u * NT + t;
@@ -244,6 +286,9 @@ __global__ __launch_bounds__(1024) void sum_parts_kernel(const float* __restrict
 // 1024 of four rows at least (4000 x 1024: 1024 parts 13.6 us, 2048 16.8: the parts are read again).
 constexpr int kBwdWaveCols = 1024;
 constexpr int64_t kMaxParts = 4096;
+// Up to so many rows every one would be a part: dy and s are read again instead, by workgroups of
+// the same launch, and no workspace is needed.
+constexpr int64_t kFewRows = 512;
 int64_t most_parts(int64_t rows, int cols) {
   if (cols > kBwdWaveCols || rows < kWaveRows) return 512;
   const int64_t most = std::max(int64_t(1024), std::min((int64_t(1) << 20) / cols, ceil_div(rows, 16) * 4));
@@ -263,6 +308,11 @@ BwdShape bwd_shape(int64_t rows, int cols) {
     b.parts = static_cast<int>(b.grid) * per_group;
   });
   return b;
+}
+
+bool overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y + b_bytes && y < x + a_bytes;
 }
 
 bool float_type(int dtype) { return dtype == HMOE_F32 || dtype == HMOE_BF16; }
@@ -329,7 +379,7 @@ extern "C" int hmoe_add_rms_norm(const void* x, int x_dtype, const void* residua
 extern "C" size_t hmoe_add_rms_norm_bwd_workspace_bytes(int64_t rows, int cols) {
   using namespace hmoe;
   if (rows <= 0 || cols <= 0) return 0;
-  const int parts = bwd_shape(rows, cols).parts;
+  const int parts = rows <= kFewRows ? 1 : bwd_shape(rows, cols).parts;
   return parts > 1 ? static_cast<size_t>(parts) * cols * sizeof(float) : 0;
 }
 
@@ -352,23 +402,47 @@ extern "C" int hmoe_add_rms_norm_bwd(const void* dy, int dy_dtype, const void* s
   }
   HMOE_REQUIRE(dy && sum && weight && rstd && dx, "%s: null pointer argument", what);
   HMOE_REQUIRE_ALIGNED(what, 16, dy, sum, weight, d_sum, dx, d_weight, workspace);
+  const auto run = [&](auto few, unsigned grid, unsigned dw_groups, float* dw) {
+    with_row_form(rows, cols, kBwdWaveCols, [&](auto nt, auto c) {
+      constexpr int kNt = decltype(nt)::value, kC = decltype(c)::value;
+      constexpr bool kFew = decltype(few)::value;
+      // (few rows are a workgroup's each)
+      if constexpr (!kFew || kNt > 64) {
+        with_float_type(dy_dtype, [&](auto tg) {
+          with_float_type(sum_dtype, [&](auto ts) {
+            typedef decltype(tg) TG;
+            typedef decltype(ts) TS;
+            hipLaunchKernelGGL((add_rms_norm_bwd_kernel<TG, TS, kNt, kC, kFew>), dim3(grid),
+                               dim3(kNt < 256 ? 256 : kNt), 0, st, static_cast<const TG*>(dy),
+                               static_cast<const TS*>(sum), weight, w_dtype == HMOE_BF16, rstd,
+                               static_cast<const TS*>(d_sum), rows, cols, static_cast<TS*>(dx), dw, dw_groups);
+          });
+        });
+      }
+    });
+  };
+  if (rows <= kFewRows) {
+    static_assert(kFewRows < kWaveRows, "few rows are a workgroup's each");
+    const unsigned groups = d_weight == nullptr ? 0u : static_cast<unsigned>(ceil_div(cols, 64));
+    // dx may be written over sum or dy, which dw's columns read: then one launch behind the other
+    const size_t values = static_cast<size_t>(rows) * cols, sum_size = sum_dtype == HMOE_BF16 ? 2 : 4;
+    const size_t dx_bytes = values * sum_size;
+    const bool over = overlap(dx, dx_bytes, sum, dx_bytes) ||
+                      overlap(dx, dx_bytes, dy, values * (dy_dtype == HMOE_BF16 ? 2 : 4));
+    if (over && groups > 0) {
+      run(std::true_type{}, groups, groups, d_weight);
+      run(std::true_type{}, static_cast<unsigned>(rows), 0u, nullptr);
+    } else {
+      run(std::true_type{}, groups + static_cast<unsigned>(rows), groups, d_weight);
+    }
+    return check_launch("hmoe_add_rms_norm_bwd");
+  }
   const BwdShape b = bwd_shape(rows, cols);
   const size_t need = hmoe_add_rms_norm_bwd_workspace_bytes(rows, cols);
   HMOE_REQUIRE_CODE(d_weight == nullptr || need == 0 || (workspace && workspace_bytes >= need), HMOE_ERR_WORKSPACE,
                     "%s: workspace has %zu bytes, needs %zu", what, workspace ? workspace_bytes : size_t(0), need);
   float* parts = d_weight == nullptr ? nullptr : b.parts > 1 ? static_cast<float*>(workspace) : d_weight;
-  with_row_form(rows, cols, kBwdWaveCols, [&](auto nt, auto c) {
-    constexpr int kNt = decltype(nt)::value, kC = decltype(c)::value;
-    with_float_type(dy_dtype, [&](auto tg) {
-      with_float_type(sum_dtype, [&](auto ts) {
-        typedef decltype(tg) TG;
-        typedef decltype(ts) TS;
-        hipLaunchKernelGGL((add_rms_norm_bwd_kernel<TG, TS, kNt, kC>), dim3(b.grid), dim3(kNt < 256 ? 256 : kNt), 0,
-                           st, static_cast<const TG*>(dy), static_cast<const TS*>(sum), weight, w_dtype == HMOE_BF16,
-                           rstd, static_cast<const TS*>(d_sum), rows, cols, static_cast<TS*>(dx), parts);
-      });
-    });
-  });
+  run(std::false_type{}, b.grid, 0u, parts);
   if (d_weight != nullptr && b.parts > 1)
     hipLaunchKernelGGL(sum_parts_kernel, dim3(columns), dim3(1024), 0, st, static_cast<const float*>(parts), b.parts,
                        cols, d_weight);

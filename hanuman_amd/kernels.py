@@ -1017,7 +1017,7 @@ def add_rms_norm_bwd(dy: torch.Tensor, total: torch.Tensor, weight: torch.Tensor
     if need_weight:
         dw = torch.empty(shape[1], dtype=_F32, device=dev)
         ws_bytes = _lib.lib().hmoe_add_rms_norm_bwd_workspace_bytes(shape[0], shape[1])
-        ws = torch.empty(ws_bytes, dtype=_U8, device=dev)
+        ws = torch.empty(ws_bytes, dtype=_U8, device=dev) if ws_bytes else None
     call("hmoe_add_rms_norm_bwd", dy.data_ptr(), g_code, total.data_ptr(), s_code, weight.data_ptr(), w_code,
          rstd.data_ptr(), _ptr(d_sum), shape[0], shape[1], dx.data_ptr(), _ptr(dw), _ptr(ws), ws_bytes, _stream())
     return dx, dw
