@@ -200,50 +200,73 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void add_rms_norm_bwd_kernel(
       static_cast<int64_t>(blockIdx.x - (FEW ? dw_groups : 0u)) * (kThreads / NT) + threadIdx.x / NT;
   const int64_t stride = static_cast<int64_t>(gridDim.x) * (kThreads / NT);
   float dw[C][8] = {};
-  float w[C][8];
-#pragma unroll
-  for (int u = 0; u < C; ++u) {
+  // (a thread of 1024 has 128 registers: with four chunks the weight and d_sum are read where they
+  // are used; 4000 x 32768 in bf16 316 us, held with the rest 488)
+  constexpr bool kLean = NT == 1024 && C == 4;
+  float w[kLean ? 1 : C][8];
+  const auto weight8 = [&](int u, float (&v)[8]) __attribute__((always_inline)) {
     const int c = u * NT + t;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w[u][i] = 0.0f;
-    if (c < chunks) load8(weight, c * 8, weight_bf16, w[u]);
+    for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+    if (c < chunks) load8(weight, c * 8, weight_bf16, v);
+  };
+  if constexpr (!kLean) {
+#pragma unroll
+    for (int u = 0; u < C; ++u) weight8(u, w[u]);
   }
+  const auto take_weight = [&](int u, float (&v)[8]) __attribute__((always_inline)) {
+    if constexpr (kLean) {
+      weight8(u, v);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = w[u][i];
+    }
+  };
   int parity = 0;
   for (int64_t row = first; row < rows; row += stride, parity ^= 1) {
     const int64_t r0 = row * cols;
     Chunk8<TG> g[C];
-    Chunk8<TS> sv[C], ds[C];
+    Chunk8<TS> sv[C], ds[kLean ? 1 : C];
 #pragma unroll
     for (int u = 0; u < C; ++u) {
       const int c = u * NT + t;
       g[u].zero();
       sv[u].zero();
-      ds[u].zero();
+      if (!kLean) ds[u].zero();
       if (c < chunks) {
         g[u].load_nt(dy + r0 + c * 8);
         sv[u].load_nt(s + r0 + c * 8);
-        if (d_sum != nullptr) ds[u].load_nt(d_sum + r0 + c * 8);
+        if (!kLean && d_sum != nullptr) ds[u].load_nt(d_sum + r0 + c * 8);
       }
     }
     const float rs = rstd[row];
     float dot = 0.0f;
 #pragma unroll
-    for (int u = 0; u < C; ++u)
+    for (int u = 0; u < C; ++u) {
+      float wu[8];
+      take_weight(u, wu);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float n = sv[u].get(i) * rs;
-        dot = __builtin_fmaf(g[u].get(i) * w[u][i], n, dot);
+        dot = __builtin_fmaf(g[u].get(i) * wu[i], n, dot);
         dw[u][i] = __builtin_fmaf(g[u].get(i), n, dw[u][i]);
       }
+    }
     const float mean = row_sum<NT>(dot, part[parity]) / static_cast<float>(cols);
 #pragma unroll
     for (int u = 0; u < C; ++u) {
       const int c = u * NT + t;
-      float d[8];
+      float d[8], wu[8];
+      take_weight(u, wu);
+      Chunk8<TS>& more = ds[kLean ? 0 : u];
+      if constexpr (kLean) {
+        more.zero();
+        if (c < chunks && d_sum != nullptr) more.load_nt(d_sum + r0 + c * 8);
+      }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float n = sv[u].get(i) * rs;
-        d[i] = ds[u].get(i) + rs * (g[u].get(i) * w[u][i] - n * mean);
+        d[i] = more.get(i) + rs * (g[u].get(i) * wu[i] - n * mean);
       }
       if (c < chunks) round_store8(dx + r0 + c * 8, d);
     }
@@ -286,9 +309,10 @@ __global__ __launch_bounds__(1024) void sum_parts_kernel(const float* __restrict
 // 1024 of four rows at least (4000 x 1024: 1024 parts 13.6 us, 2048 16.8: the parts are read again).
 constexpr int kBwdWaveCols = 1024;
 constexpr int64_t kMaxParts = 4096;
-// Up to so many rows every one would be a part: dy and s are read again instead, by workgroups of
-// the same launch, and no workspace is needed.
-constexpr int64_t kFewRows = 512;
+// Up to so many rows dy and s are read again instead, by workgroups of the same launch, and no
+// workspace is needed (700 x 1536: bf16 5.1 us, in parts 7.8, float32 6.7 and 8.8; 1000 rows 6.1 and
+// 8.4, 9.5 and 10.0, but 1000 x 4096 in float32 24.5 and 21).
+constexpr int64_t kFewRows = 768;
 int64_t most_parts(int64_t rows, int cols) {
   if (cols > kBwdWaveCols || rows < kWaveRows) return 512;
   const int64_t most = std::max(int64_t(1024), std::min((int64_t(1) << 20) / cols, ceil_div(rows, 16) * 4));

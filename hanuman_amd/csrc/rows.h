@@ -102,7 +102,9 @@ __device__ __forceinline__ void load8(const void* p, int64_t at, bool bf16, floa
 // How a row of `cols` values is held: NT threads and C chunks of eight values a thread, with
 // which `f` is called.  A wave a row where there are rows enough to fill the chip with waves
 // and rows are short enough (max_wave_cols): 100000 rows of 256 values are normed in 68 us by
-// waves, 142 by workgroups, 30000 of 1024 in 61 and 70, 16384 of 2048 in the same time.
+// waves, 142 by workgroups, 30000 of 1024 in 61 and 70, 16384 of 2048 in the same time.  (The norm's
+// gradients of 1000 rows of 8200 bf16 values take 27 us with two chunks a thread of 1024, 101 with
+// four, which a thread's 128 registers do not hold.)
 constexpr int kMaxRowCols = 32768;
 constexpr int64_t kWaveRows = 2048;
 template <int N>
@@ -116,6 +118,7 @@ void with_row_form(int64_t rows, int cols, int max_wave_cols, F f) {
   else if (chunks <= 256) f(Int<256>{}, Int<1>{});
   else if (chunks <= 256 * 2) f(Int<256>{}, Int<2>{});
   else if (chunks <= 256 * 4) f(Int<256>{}, Int<4>{});
+  else if (chunks <= 1024 * 2) f(Int<1024>{}, Int<2>{});
   else f(Int<1024>{}, Int<4>{});
 }
 

@@ -507,7 +507,7 @@ int hmoe_add_rms_norm(const void* x, int x_dtype, const void* residual, int resi
  *   dx [rows, cols] = d_sum + rstd * (dy * weight - n * mean_d(dy * weight * n)), in sum's type:
  *      the gradient of x and of the residual;
  *   d_weight [cols] f32 (NULL: not wanted) = sum over the rows of dy * n, in at most 4096 parts,
- *      each summed row by row; then 32 runs of parts, then the runs.  Up to 512 rows: in 32 or 128
+ *      each summed row by row; then 32 runs of parts, then the runs.  Up to 768 rows: in 32 or 128
  *      runs of rows, then the runs, and no workspace.
  * sum, d_sum and dx have one type, dy and weight their own (F32 or BF16).  Zero rows write a zero
  * d_weight.  workspace >= hmoe_add_rms_norm_bwd_workspace_bytes where d_weight is wanted.  dx may

@@ -106,7 +106,8 @@ def test_no_rows(gpu):
 
 
 @pytest.mark.parametrize("rows,cols", [(1, 8), (3, 24), (40, 256), (5, 1032), (700, 2048), (33, 4104), (6, 8200),
-                                       (3, 32768), (2050, 40), (5000, 1056), (2049, 2048), (9000, 64), (4001, 2056)])
+                                       (3, 32768), (2050, 40), (5000, 1056), (2049, 2048), (9000, 64), (4001, 2056),
+                                       (768, 264), (769, 264), (777, 8200), (780, 16392), (40, 16384)])
 @pytest.mark.parametrize("g_type,s_type,more", [(BF16, BF16, True), (F32, F32, True), (BF16, F32, False),
                                                 (F32, BF16, True), (BF16, BF16, False)])
 def test_gradients(gpu, rows, cols, g_type, s_type, more):

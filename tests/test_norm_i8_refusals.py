@@ -48,12 +48,12 @@ def test_norm():
 
 def test_norm_bwd():
     name = "hmoe_add_rms_norm_bwd"
-    need = _lib.lib().hmoe_add_rms_norm_bwd_workspace_bytes(600, 64)
+    need = _lib.lib().hmoe_add_rms_norm_bwd_workspace_bytes(800, 64)
     assert need == 512 * 64 * 4
-    for few in (0, 1, 512):
+    for few in (0, 1, 768):
         assert _lib.lib().hmoe_add_rms_norm_bwd_workspace_bytes(few, 64) == 0
 
-    def args(dy=P, dd=BF16, s=P, sd=BF16, w=P, wd=F32, rstd=P, ds=P, rows=600, cols=64, dx=P, dw=P, ws=P, size=need):
+    def args(dy=P, dd=BF16, s=P, sd=BF16, w=P, wd=F32, rstd=P, ds=P, rows=800, cols=64, dx=P, dw=P, ws=P, size=need):
         return dy, dd, s, sd, w, wd, rstd, ds, rows, cols, dx, dw, ws, size, S
 
     expect(INVALID, "rows", name, *args(rows=-1))
