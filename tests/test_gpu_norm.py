@@ -194,6 +194,23 @@ def test_results_over_operands(gpu):
         assert torch.equal(ops[over], dx)
 
 
+@pytest.mark.parametrize("rows,cols", [(1, 264), (37, 520), (768, 1032), (900, 520), (30, 8200), (3000, 256)])
+def test_gradients_over_operands(gpu, rows, cols):
+    """dx over its operands with the weight's gradient wanted, which reads two of them."""
+    s, dy, ds = (_rows(gpu, rows, cols, BF16, i) for i in (2, 3, 4))
+    w = torch.ones(cols, device=gpu)
+    rstd = torch.rand(rows, device=gpu) + 0.5
+    dx, dw = K.add_rms_norm_bwd(dy, s, w, rstd, ds)
+    need = _lib.lib().hmoe_add_rms_norm_bwd_workspace_bytes(rows, cols)
+    for over in range(3):
+        ops = [dy.clone(), s.clone(), ds.clone()]
+        got, ws = torch.empty_like(dw), torch.empty(need, dtype=torch.uint8, device=gpu)
+        _lib.call("hmoe_add_rms_norm_bwd", ops[0].data_ptr(), _lib.BF16, ops[1].data_ptr(), _lib.BF16, w.data_ptr(),
+                  _lib.F32, rstd.data_ptr(), ops[2].data_ptr(), rows, cols, ops[over].data_ptr(), got.data_ptr(),
+                  ws.data_ptr() if need else None, need, torch.cuda.current_stream().cuda_stream)
+        assert torch.equal(ops[over], dx) and torch.equal(got, dw)
+
+
 def test_more_rows_than_a_grid(gpu):
     """Rows past 2^22 are taken in a second round of the workgroups; offsets pass 2^31 bytes."""
     rows, cols = (1 << 22) + 5, 264
