@@ -34,7 +34,8 @@ __global__ __launch_bounds__(256) void select_groups_kernel(const float* __restr
       for (int i = lane * 4; i < done; i += 256)
         *reinterpret_cast<f32x4*>(to + i + (i >> 5) * 4) = *reinterpret_cast<const f32x4*>(from + i);
     }
-    for (int i = done + lane; i < words; i += 64) to[i + (i >> 5) * 4] = from[i];
+    if (done < words)  // uniform
+      for (int i = done + lane; i < words; i += 64) to[i + (i >> 5) * 4] = from[i];
   };
   park(src, mine, count);
   if (bias != nullptr) {
