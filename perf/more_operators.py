@@ -205,10 +205,9 @@ def _codes8(v, to):
     """8-bit codes (as the values of their type, in float32) of float32 rows and the rows' scales."""
     most = LARGEST[to]
     amax = v.abs().amax(-1)
-    zero, top = amax == 0, torch.full_like(amax, most)
-    # (not by a number: that is a product with its reciprocal)
-    scale = torch.where(zero, torch.ones_like(amax), _divide32(amax, top))
-    inverse = torch.where(zero, torch.ones_like(amax), _divide32(top, amax))
+    zero = amax == 0
+    scale = torch.where(zero, torch.ones_like(amax), amax / most)
+    inverse = torch.where(zero, torch.ones_like(amax), most / amax)
     code = (v * inverse.unsqueeze(-1)).clamp(-most, most)
     return torch.round(code) if to == "int8" else code.to(torch.float8_e4m3fn).float(), scale
 
