@@ -121,17 +121,16 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void add_rms_norm_kernel(
         if (c < chunks) *reinterpret_cast<uint2*>(q + r0 + c * 8) = i8_codes8(v[u], s);
       }
     } else {
-      // (the rule of quantize_rows_fp8: a NaN is not looked at for the largest)
       float most = 0.0f;
 #pragma unroll
       for (int u = 0; u < C; ++u)
         if (u * NT + t < chunks)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(v[u][i]));
-      // (not negative and no NaN: they order like their bits)
-      const float amax = __int_as_float(row_max<NT>(__float_as_int(most), max_part[parity]));
-      const float inv = amax > 0.0f ? kE4m3Max / amax : 1.0f;
-      if (t == 0) scale[row] = amax > 0.0f ? amax / kE4m3Max : 1.0f;
+          for (int i = 0; i < 8; ++i) most = amax_nan(most, v[u][i]);
+      const int32_t bits = row_max<NT>(__float_as_int(most) & 0x7fffffff, max_part[parity]);
+      float s, inv;
+      e4m3_scales(__int_as_float(bits), s, inv);
+      if (t == 0) scale[row] = s;
 #pragma unroll
       for (int u = 0; u < C; ++u) {
         const int c = u * NT + t;

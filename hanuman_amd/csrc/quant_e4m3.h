@@ -44,13 +44,32 @@ struct Chunk8<float> {
 // Per-row rule: amax = max |v| over the row, codes e4m3(clamp(v * (448/amax),
 // +-448)) rounded to nearest even by v_cvt_pk_fp8_f32, dequantisation scale
 // amax/448 (both divisions correctly rounded); an all-zero row gets scale 1.
+// Where 448/amax passes float32's range (amax below 2^-119) the factor is 2^127
+// and the scale 2^-127: values stay below 228 and their steps are as fine as
+// e4m3's down to 2^-133.  A row with a value that is not finite has scale NaN,
+// and codes of -448 in every place: it reads back as NaN, and so does every
+// product with it.
 constexpr float kE4m3Max = 448.0f;
 
-// Scale and its inverse from the lane-partial amax (reduced over the wave).
-__device__ __forceinline__ void scales_from_amax(float amax, float& s, float& inv) {
-  amax = wave_max_f32(amax);
+// The larger of m and |v|; NaN where one of them is (one instruction for two values).
+__device__ __forceinline__ float amax_nan(float m, float v) {
+  return __builtin_elementwise_maximum(m, __builtin_fabsf(v));
+}
+
+__device__ __forceinline__ void e4m3_scales(float amax, float& s, float& inv) {
   s = amax > 0.0f ? amax / kE4m3Max : 1.0f;
   inv = amax > 0.0f ? kE4m3Max / amax : 1.0f;
+  if (inv > __FLT_MAX__) {
+    s = 0x1p-127f;
+    inv = 0x1p127f;
+  }
+  if (!(amax <= __FLT_MAX__)) s = inv = __builtin_nanf("");
+}
+
+// The same from the lane-partial amax (reduced over the wave; without their sign
+// numbers order like their bits, a NaN on top).
+__device__ __forceinline__ void scales_from_amax(float amax, float& s, float& inv) {
+  e4m3_scales(__int_as_float(wave_max_i32(__float_as_int(amax) & 0x7fffffff)), s, inv);
 }
 
 template <typename TI>
@@ -62,7 +81,7 @@ __device__ __forceinline__ void wave_row_scales(const TI* __restrict__ row, int 
     Chunk8<TI> v;
     v.load(row + static_cast<int64_t>(c) * 8);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(v.get(i)));
+    for (int i = 0; i < 8; ++i) amax = amax_nan(amax, v.get(i));
   }
   scales_from_amax(amax, s, inv);
 }
@@ -82,7 +101,7 @@ __device__ __forceinline__ void load_row_regs(const TI* __restrict__ row, int ch
     v[u].zero();
     if (c < chunks) v[u].load_nt(row + static_cast<int64_t>(c) * 8);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(v[u].get(i)));
+    for (int i = 0; i < 8; ++i) amax = amax_nan(amax, v[u].get(i));
   }
   scales_from_amax(amax, s, inv);
 }

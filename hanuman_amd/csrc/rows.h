@@ -14,11 +14,6 @@ template <int CTRL, int ROW_MASK = 0xF>
 __device__ __forceinline__ float dpp_fadd(float v) {
   return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, ROW_MASK, 0xF, false));
 }
-template <int CTRL, int ROW_MASK = 0xF>
-__device__ __forceinline__ int32_t dpp_imax(int32_t v) {
-  const int32_t t = __builtin_amdgcn_update_dpp(v, v, CTRL, ROW_MASK, 0xF, false);
-  return t > v ? t : v;
-}
 // Wave-wide, returned in every lane; the moves are those of wave_max_f32.
 __device__ __forceinline__ float wave_sum_f32(float v) {
   v = dpp_fadd<0xB1>(v);
@@ -27,15 +22,6 @@ __device__ __forceinline__ float wave_sum_f32(float v) {
   v = dpp_fadd<0x140>(v);
   v = dpp_fadd<0x142, 0xA>(v);
   v = dpp_fadd<0x143, 0xC>(v);
-  return lane_bcast(v, 63);
-}
-__device__ __forceinline__ int32_t wave_max_i32(int32_t v) {
-  v = dpp_imax<0xB1>(v);
-  v = dpp_imax<0x4E>(v);
-  v = dpp_imax<0x141>(v);
-  v = dpp_imax<0x140>(v);
-  v = dpp_imax<0x142, 0xA>(v);
-  v = dpp_imax<0x143, 0xC>(v);
   return lane_bcast(v, 63);
 }
 

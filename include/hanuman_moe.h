@@ -149,7 +149,10 @@ int hmoe_permute_rows(const void* x, int x_dtype, int64_t tokens, int d_model,
 /* xs_q[slot_pos[t*K+k]] = e4m3 codes of x[t] for kept slots, xs_scale[...] =
  * that token's scale.  Per row: amax = max|x|, codes
  * e4m3(clamp(x * (448/amax), +-448)) (round to nearest even), scale amax/448;
- * an all-zero row gets scale 1.  x [T,D] (F32/BF16), xs_q [rows_cap, D]
+ * an all-zero row gets scale 1.  Where 448/amax passes float32's range (amax
+ * below 2^-119) the factor is 2^127 and the scale 2^-127.  A row with a value
+ * that is not finite has scale NaN (and codes of -448): what is made of it is
+ * NaN.  x [T,D] (F32/BF16), xs_q [rows_cap, D]
  * uint8, xs_scale [rows_cap] f32.  D % 8 == 0. */
 int hmoe_permute_rows_fp8(const void* x, int x_dtype, int64_t tokens, int d_model,
                           int top_k, const int32_t* slot_pos, uint8_t* xs_q,

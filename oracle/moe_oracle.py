@@ -415,25 +415,37 @@ def expert_ffn(xs, offsets, wg, wu, wd, precision: str = "fp32") -> np.ndarray:
 def _e4m3_scales(amax):
     """Dequantisation scale ``amax/448`` and quantisation multiplier
     ``448/amax`` (both correctly rounded float32 divisions); an all-zero group
-    gets 1 and 1."""
+    gets 1 and 1, one whose multiplier would overflow ``2**-127`` and ``2**127``,
+    one with a value that is not finite NaN and NaN."""
     amax = np.asarray(amax, dtype=F32)
     pos = amax > 0
-    safe = np.where(pos, amax, F32(1.0)).astype(F32)
+    safe = np.where(pos & np.isfinite(amax), amax, F32(1.0)).astype(F32)
     s = np.where(pos, (safe / F32(448.0)).astype(F32), F32(1.0)).astype(F32)
-    inv = np.where(pos, (F32(448.0) / safe).astype(F32), F32(1.0)).astype(F32)
-    return s, inv
+    with np.errstate(over="ignore"):
+        inv = np.where(pos, (F32(448.0) / safe).astype(F32), F32(1.0)).astype(F32)
+    s = np.where(np.isinf(inv), F32(2.0**-127), s)
+    inv = np.where(np.isinf(inv), F32(2.0**127), inv)
+    finite = np.isfinite(amax)
+    return np.where(finite, s, F32(np.nan)), np.where(finite, inv, F32(np.nan))
+
+
+def _e4m3_scaled(a, inv):
+    """Codes of ``a * inv``, of -448 where ``inv`` is NaN."""
+    with np.errstate(invalid="ignore"):
+        v = (a * inv).astype(F32)
+    return e4m3_encode(np.where(np.isnan(inv), F32(-448.0), v))
 
 
 def quantize_rows_e4m3(a):
     """Per-row e4m3 quantisation (the fp8 workload rule for activations):
     ``amax`` = max |a| over the row, ``q = e4m3(clamp(a * (448/amax), +-448))``
     (one float32 multiply, round-to-nearest-even, saturating), dequantisation
-    scale ``s = amax/448``.  Returns (codes uint8, scales float32)."""
+    scale ``s = amax/448`` (tiny rows and ones that are not finite:
+    :func:`_e4m3_scales`).  Returns (codes uint8, scales float32)."""
     a = np.asarray(a, dtype=F32)
     amax = np.max(np.abs(a), axis=-1)
     s, inv = _e4m3_scales(amax)
-    q = e4m3_encode((a * inv[..., None]).astype(F32))
-    return q, s
+    return _e4m3_scaled(a, inv[..., None]), s
 
 
 def quantize_cols_e4m3(w):
@@ -443,8 +455,7 @@ def quantize_cols_e4m3(w):
     w = np.asarray(w, dtype=F32)
     amax = np.max(np.abs(w), axis=-2)
     s, inv = _e4m3_scales(amax)
-    q = e4m3_encode((w * inv[..., None, :]).astype(F32))
-    return q, s
+    return _e4m3_scaled(w, inv[..., None, :]), s
 
 
 E4M3_BLOCK = 32          # columns per power-of-two scale block of h
