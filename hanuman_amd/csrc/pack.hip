@@ -8,7 +8,7 @@
 // gate columns and 32 up columns of the same h columns, so one 32x32 MFMA
 // output block of gate and the next one of up hold matching h elements in the
 // same lanes and the SwiGLU runs in registers.
-#include "hmoe_common.h"
+#include "quant_e4m3.h"
 
 namespace hmoe {
 namespace {
@@ -153,9 +153,8 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(const TW* __restrict__ s
 }
 
 // ----------------------------------------------------------- e4m3 packing --
-// Per-output-channel e4m3 codes (same rule as the activations: codes
-// e4m3(clamp(w * (448/amax), +-448)), scale amax/448, amax over the reduction
-// dimension of the column).  Three passes: column amax into `scales` (packed
+// Per-output-channel e4m3 codes (the rule of the activations, quant_e4m3.h,
+// amax over the reduction dimension of the column).  Three passes: column amax into `scales` (packed
 // order), the transpose-quantise, then amax -> amax/448 in place.
 
 // amax over rows_r of column c of src[e] (rows_r x cols_c), written to
@@ -171,12 +170,12 @@ __global__ __launch_bounds__(256) void colmax_kernel(const TW* __restrict__ src,
   float m = 0.0f;
   if (c < cols_c) {
     const TW* col = src + static_cast<int64_t>(e) * rows_r * cols_c + c;
-    for (int r = ty; r < rows_r; r += 4) m = fmaxf(m, fabsf(load_w(col, static_cast<int64_t>(r) * cols_c)));
+    for (int r = ty; r < rows_r; r += 4) m = amax_nan(m, load_w(col, static_cast<int64_t>(r) * cols_c));
   }
   part[ty][tx] = m;
   __syncthreads();
   if (ty == 0 && c < cols_c) {
-    m = fmaxf(fmaxf(part[0][tx], part[1][tx]), fmaxf(part[2][tx], part[3][tx]));
+    m = amax_nan(amax_nan(part[0][tx], part[1][tx]), amax_nan(part[2][tx], part[3][tx]));
     // Packed row of column c: gate/up interleave 32 columns of each per 64 rows.
     const int p = GATE_UP ? (c >> 5) * 64 + up_half * 32 + (c & 31) : c;
     out[static_cast<int64_t>(e) * out_stride + p] = m;
@@ -223,7 +222,8 @@ __global__ __launch_bounds__(256) void pack_fp8_kernel(const TW* __restrict__ sr
     const int r = r0 + tx;
     if (p < dst_rows && r < rows_r) {
       const float m = amax[static_cast<int64_t>(e) * dst_rows + p];
-      const float inv = m > 0.0f ? 448.0f / m : 1.0f;
+      float s, inv;
+      e4m3_scales(m, s, inv);
       dst[(static_cast<int64_t>(e) * dst_rows + p) * rows_r + r] = e4m3_code(tile[tx][pp] * inv);
     }
   }
@@ -231,7 +231,10 @@ __global__ __launch_bounds__(256) void pack_fp8_kernel(const TW* __restrict__ sr
 
 __global__ __launch_bounds__(256) void amax_to_scale_kernel(float* __restrict__ v, int64_t n) {
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (i < n) v[i] = v[i] > 0.0f ? v[i] / 448.0f : 1.0f;
+  if (i >= n) return;
+  float s, inv;
+  e4m3_scales(v[i], s, inv);
+  v[i] = s;
 }
 
 }  // namespace

@@ -82,3 +82,33 @@ def test_of_the_norm(gpu, rows, cols, dtype):
         w = torch.full((cols,), most / 16, device=gpu)
         out = K.add_rms_norm(a, w, None, 1e-6, quant="e4m3")
         _same(out.q, out.scale, out.y)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_columns_of_the_masters(gpu, dtype):
+    """Output columns that are not ordinary, of the gate, the up and the down master."""
+    k, cols, n = 96, 64, 2
+    bad, tiny = [1, 33, 40], {2: 1e-36, 34: 2.0**-126, 5: 3e-39}
+
+    def master(seed):
+        w = 0.02 * torch.randn((n, k, cols), generator=torch.Generator().manual_seed(seed))
+        w[0, 3, 1], w[0, k - 1, 33], w[0, 0, 40] = float("nan"), float("inf"), -float("inf")
+        w[1, :, 0] = 0.0
+        for col, most in tiny.items():
+            w[1, :, col] = (w[1, :, col].double() / w[1, :, col].abs().max() * most).float()
+        return w.to(dtype).to(gpu)
+
+    def rule(w):
+        q, s = O.quantize_cols_e4m3(w.float().cpu().numpy())
+        assert np.array_equal(np.isnan(s[0]), np.isin(np.arange(cols), bad)) and not np.isnan(s[1]).any()
+        return np.swapaxes(q, 1, 2), s
+
+    wg, wu = master(1), master(2)
+    packed, scale = (t.cpu().numpy() for t in K.pack_fp8_gate_up(wg, wu))
+    for up, w in enumerate((wg, wu)):
+        at = [(c // 32) * 64 + 32 * up + c % 32 for c in range(cols)]
+        q, s = rule(w)
+        assert np.array_equal(scale[:, at], s, equal_nan=True) and np.array_equal(packed[:, at], q)
+    packed, scale = (t.cpu().numpy() for t in K.pack_fp8_down(wg))
+    q, s = rule(wg)
+    assert np.array_equal(scale, s, equal_nan=True) and np.array_equal(packed, q)
