@@ -39,7 +39,7 @@
 #include <algorithm>
 #include <cmath>
 
-#include "hmoe_common.h"
+#include "quant_e4m3.h"
 
 namespace hmoe {
 namespace {
@@ -64,6 +64,18 @@ typedef float f32x2_t __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t pack_bf16x2_rne(float lo, float hi) {
   f32x2_t v = {lo, hi};
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2_t));
+}
+
+// The exponent of a block of h whose 32 columns lanes L and L + 32 hold, from each lane's
+// largest |h| (amax_nan): the smallest e with max <= 448 * 2^e, at least -127, and 128, which is
+// stored as E8M0's NaN, where a value is not finite.
+__device__ __forceinline__ int h_block_exponent(float amax) {
+  const uint32_t bits = __float_as_uint(amax) & 0x7fffffffu;
+  const auto pair = __builtin_amdgcn_permlane32_swap(bits, bits, false, false);
+  const uint32_t most = pair[0] > pair[1] ? pair[0] : pair[1];
+  int ex = static_cast<int>(most >> 23) - 135 + ((most & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+  ex = ex > -127 ? ex : -127;
+  return most >= 0x7f800000u ? 128 : ex;
 }
 
 // silu(g) = g / (1 + e^-g) with the hardware reciprocal (v_rcp_f32, 1 ulp)
@@ -838,14 +850,10 @@ __global__ __launch_bounds__(kW8Threads) void grouped_gemm_w8_fp8(
                                    acc[i][1][q * 4 + k + 1] * sa * su[k + 1]));
             hv[q * 4 + k] = __uint_as_float(pk << 16);
             hv[q * 4 + k + 1] = __uint_as_float(pk & 0xffff0000u);
-            amax = fmaxf(amax, fmaxf(fabsf(hv[q * 4 + k]), fabsf(hv[q * 4 + k + 1])));
+            amax = amax_nan(amax_nan(amax, hv[q * 4 + k]), hv[q * 4 + k + 1]);
           }
         }
-        const uint32_t abits = __float_as_uint(amax);
-        const auto pa = __builtin_amdgcn_permlane32_swap(abits, abits, false, false);
-        const uint32_t bmax = __float_as_uint(fmaxf(__uint_as_float(pa[0]), __uint_as_float(pa[1])));
-        int ex = static_cast<int>(bmax >> 23) - 135 + ((bmax & 0x7FFFFFu) > 0x600000u ? 1 : 0);
-        ex = ex > -127 ? ex : -127;
+        const int ex = h_block_exponent(amax);
         const float inv = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
         uint32_t d[4];
 #pragma unroll
@@ -1608,13 +1616,9 @@ __global__ __launch_bounds__(kThreads) void grouped_gemm_few(
                                               swiglu_bf16_points(acc[i][0][k + 1], acc[i][1][k + 1]));
           hv[k] = __uint_as_float(pk << 16);
           hv[k + 1] = __uint_as_float(pk & 0xffff0000u);
-          amax = fmaxf(amax, fmaxf(fabsf(hv[k]), fabsf(hv[k + 1])));
+          amax = amax_nan(amax_nan(amax, hv[k]), hv[k + 1]);
         }
-        const uint32_t abits = __float_as_uint(amax);
-        const auto pa = __builtin_amdgcn_permlane32_swap(abits, abits, false, false);
-        const uint32_t bmax = __float_as_uint(fmaxf(__uint_as_float(pa[0]), __uint_as_float(pa[1])));
-        int ex = static_cast<int>(bmax >> 23) - 135 + ((bmax & 0x7FFFFFu) > 0x600000u ? 1 : 0);
-        ex = ex > -127 ? ex : -127;
+        const int ex = h_block_exponent(amax);
         const float inv = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
         uint32_t d[4];
 #pragma unroll

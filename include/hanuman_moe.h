@@ -329,7 +329,9 @@ int hmoe_grouped_down_fp8(const uint8_t* h_q, const float* h_scale, const int32_
  * power-of-two scale 2^e, e the smallest integer with max|h| <= 448 * 2^e
  * over the block (at least -127), and the codes are e4m3(h * 2^-e) rounded
  * to nearest even: h_q [rows_cap, F] uint8 and h_exp [rows_cap, F / 32]
- * uint8 biased exponents e + 127 (E8M0).  Rows past offsets[N] are not
+ * uint8 biased exponents e + 127 (E8M0).  A block with a value that is not
+ * finite has exponent 255, E8M0's NaN, and codes that say nothing: what the
+ * down GEMM makes of its row is NaN.  Rows past offsets[N] are not
  * written.  The down GEMM feeds h_exp to the MFMA's per-32-value operand
  * scales and dequantises the accumulators by the column scales only.
  * Shape rules as for the _fp8 entries. */

@@ -463,7 +463,8 @@ E4M3_BLOCK = 32          # columns per power-of-two scale block of h
 
 def block_exponent_e8m0(amax) -> np.ndarray:
     """Smallest integer ``e`` with ``amax <= 448 * 2**e``, at least -127 (the
-    bottom of the E8M0 scale range; an all-zero block gets -127).
+    bottom of the E8M0 scale range; an all-zero block gets -127); 128, which
+    biased is E8M0's NaN, where ``amax`` is not finite.
 
     From the float32 fields of ``amax = 1.m * 2**(E-127)``: ``amax * 2**-e =
     1.m * 2**(8-c)`` for ``e = E - 135 + c``, which is at most 448 exactly when
@@ -473,7 +474,7 @@ def block_exponent_e8m0(amax) -> np.ndarray:
     bits = np.asarray(amax, dtype=F32).view(np.uint32).astype(np.int64)
     E = (bits >> 23) & 0xFF
     e = E - 135 + ((bits & 0x7FFFFF) > 0x600000)
-    return np.maximum(e, -127)
+    return np.where(E == 255, 128, np.maximum(e, -127))
 
 
 def quantize_blocks_e4m3(a, block: int = E4M3_BLOCK):
@@ -482,7 +483,8 @@ def quantize_blocks_e4m3(a, block: int = E4M3_BLOCK):
     ``e = block_exponent_e8m0(max |a| over the block)``, and the codes are
     ``e4m3(a * 2**-e)`` (an exact scaling, then round-to-nearest-even; the
     scaled magnitudes are at most 448 by the choice of ``e``, so nothing
-    saturates).  Returns (codes uint8 [..., C], biased exponents uint8
+    saturates; a block that is not finite has the exponent 255 and codes that
+    say nothing).  Returns (codes uint8 [..., C], biased exponents uint8
     [..., C/block] = ``e + 127``, the E8M0 encoding of ``2**e``)."""
     a = np.asarray(a, dtype=F32)
     C = a.shape[-1]
@@ -491,12 +493,14 @@ def quantize_blocks_e4m3(a, block: int = E4M3_BLOCK):
     blk = a.reshape(a.shape[:-1] + (C // block, block))
     e = block_exponent_e8m0(np.max(np.abs(blk), axis=-1))
     scaled = (blk.astype(F64) * np.ldexp(1.0, -e)[..., None]).astype(F32)
+    scaled[e == 128] = 0.0
     return e4m3_encode(scaled).reshape(a.shape), (e + 127).astype(np.uint8)
 
 
 def dequantize_blocks_e4m3(q, e8, block: int = E4M3_BLOCK) -> np.ndarray:
-    """float64 values of block-scaled codes: ``decode(q) * 2**(e8 - 127)``."""
-    scale = np.ldexp(1.0, np.asarray(e8, np.int64) - 127)
+    """float64 values of block-scaled codes: ``decode(q) * 2**(e8 - 127)``, NaN
+    where the exponent is 255."""
+    scale = np.where(np.asarray(e8) == 255, np.nan, np.ldexp(1.0, np.asarray(e8, np.int64) - 127))
     return e4m3_decode(q).astype(F64) * np.repeat(scale, block, axis=-1)
 
 

@@ -50,3 +50,13 @@ def test_columns_are_rows_of_the_transpose():
     q, s = O.quantize_cols_e4m3(a.T)
     qr, sr = O.quantize_rows_e4m3(a)
     assert np.array_equal(q, qr.T) and np.array_equal(s, sr, equal_nan=True)
+
+
+def test_blocks_that_are_not_finite_read_back_as_nan():
+    a = _rows()[:, :32].repeat(2, axis=1)
+    a[1, 32:] = 1.0                     # NaN in the first block only
+    q, e = O.quantize_blocks_e4m3(a)
+    bad = ~np.isfinite(a.reshape(12, 2, 32)).all(2)
+    assert np.array_equal(e == 255, bad) and bad[1].tolist() == [True, False]
+    back = O.dequantize_blocks_e4m3(q, e).reshape(12, 2, 32)
+    assert np.isnan(back[bad]).all() and np.isfinite(back[~bad]).all()

@@ -112,3 +112,39 @@ def test_columns_of_the_masters(gpu, dtype):
     packed, scale = (t.cpu().numpy() for t in K.pack_fp8_down(wg))
     q, s = rule(wg)
     assert np.array_equal(scale, s, equal_nan=True) and np.array_equal(packed, q)
+
+
+# few rows an expert, and tiles of 256
+@pytest.mark.parametrize("tokens,n,top_k", [(24, 16, 2), (3000, 4, 2)], ids=["few", "tiles"])
+def test_block_scaled_h(gpu, tokens, n, top_k):
+    """Tokens that are not finite, and ones whose h overflows in some columns, through the
+    products: exponents 255 where h is not finite, NaN in those tokens' results only."""
+    d, f = 256, 256
+    g = torch.Generator(device=gpu).manual_seed(tokens)
+    x = torch.randn((tokens, d), generator=g, device=gpu).to(BF16)
+    clean = x.clone()
+    x[2, 7], x[11, 0], x[19, 255] = float("nan"), float("inf"), -float("inf")
+    x[5] = x[5] * 2.0**65               # g and u about 0.3 * 2^65: one h in 30 passes 2^128
+    wg, wu, wd = (0.02 * torch.randn(s, generator=g, device=gpu) for s in ((n, d, f), (n, d, f), (n, f, d)))
+    gu, gu_s = K.pack_fp8_gate_up(wg, wu)
+    dn, dn_s = K.pack_fp8_down(wd)
+    idx = torch.stack([torch.randperm(n, generator=torch.Generator().manual_seed(t))[:top_k] for t in range(tokens)])
+    plan = K.dispatch_plan(idx.to(torch.int32).to(gpu), n, tokens * top_k)
+    token = plan.perm_src.long() // top_k
+
+    def run(t):
+        t_q, t_s = K.quantize_rows_fp8(t)
+        h = K.grouped_gate_up_fp8_gather(t_q, t_s, plan, gu, gu_s)
+        h_q, h_exp = K.grouped_gate_up_fp8_gather_qh(t_q, t_s, plan, gu, gu_s)
+        return h, h_exp, K.grouped_down_fp8_mx(h_q, h_exp, plan.offsets, dn, dn_s)
+
+    h, h_exp, ys = run(x)
+    lost = ~torch.isfinite(h).view(-1, f // 32, 32).all(2)
+    assert torch.equal(h_exp == 255, lost)
+    assert lost[(token == 2) | (token == 11) | (token == 19)].all()
+    over = lost[token == 5]
+    assert over.any() and not over.all()
+    assert torch.equal(torch.isnan(ys).all(1), lost.any(1)) and torch.equal(torch.isnan(ys).any(1), lost.any(1))
+    same = ~((token == 2) | (token == 11) | (token == 19) | (token == 5))
+    _, _, want = run(clean)
+    assert torch.equal(ys[same], want[same])
