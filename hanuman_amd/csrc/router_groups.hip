@@ -113,8 +113,9 @@ void select_groups(const float* logits, const float* bias, int64_t tokens, int n
 }
 
 int validate_groups(int64_t tokens, int n_experts, int top_k, int mode, int n_groups, int top_groups) {
-  // (64 lanes a token at most, fewer than 2^32 threads a launch)
-  HMOE_REQUIRE(tokens < (int64_t(1) << 26), "router: tokens must be below 2^26 with groups (got %lld)",
+  // (a launch has fewer than 2^32 threads: 64 a token for the selection, in workgroups of four
+  // tokens and more, and for the logits of more than 240 experts, in workgroups of sixteen)
+  HMOE_REQUIRE(tokens <= (int64_t(1) << 26) - 16, "router: tokens must be at most 2^26 - 16 with groups (got %lld)",
                (long long)tokens);
   HMOE_REQUIRE(n_groups >= 1 && n_groups <= kMaxGroups && n_experts % n_groups == 0,
                "router: n_groups must divide n_experts and be in [1, %d] (got %d, n_experts %d)", kMaxGroups, n_groups,

@@ -94,7 +94,8 @@ int hmoe_router_from_logits(const float* logits, const float* bias, int64_t toke
  * top_groups groups with the largest scores (the lower index first where equal; a score that is
  * NaN is below all others); gates as above.  With top_groups == n_groups these are the calls
  * above.  n_groups <= 64 divides N, top_k <= top_groups * (N / n_groups), with sigmoid groups of
- * two experts at least, tokens < 2^26.  hmoe_router_bwd and hmoe_router_aux take the results as they are. */
+ * two experts at least, tokens <= 2^26 - 16.  hmoe_router_bwd and hmoe_router_aux take the results
+ * as they are. */
 int hmoe_router_grouped(const void* x, int x_dtype, const void* router_w, int w_dtype,
                         const float* bias, int64_t tokens, int d_model, int n_experts, int top_k,
                         int mode, float routed_scaling_factor, int n_groups, int top_groups,

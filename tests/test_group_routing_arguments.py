@@ -86,3 +86,17 @@ def test_norm_on_the_cpu():
         norm(torch.zeros((2, 64)))
     with pytest.raises(ValueError, match="shape"):
         norm.with_sum(torch.zeros((2, 64)), torch.zeros((3, 64)))
+
+
+@pytest.mark.parametrize("name,args", CALLS, ids=[c[0] for c in CALLS])
+def test_the_most_tokens(name, args):
+    """A launch has fewer than 2^32 threads: 64 for each token with 33 groups and more (four
+    tokens a workgroup), and in the router's own launch with more than 240 experts (sixteen)."""
+    most = (1 << 26) - 16
+    for experts, k in ((66, 2), (256, 8), (256, 12)):
+        groups = 33 if experts == 66 else 64
+        expect(INVALID, "2^26", name, *args(most + 1, experts, k, 0, groups, 8, P))
+        expect(INVALID, "2^26", name, *args((1 << 26) - 3, experts, k, 0, groups, 8, P))
+        expect(INVALID, "null", name, *args(most, experts, k, 0, groups, 8, None))
+    for per_block, threads in ((4, 256), (16, 1024)):
+        assert -(-most // per_block) * threads < 1 << 32
