@@ -95,6 +95,26 @@ XLA_FFI_DEFINE_HANDLER_SYMBOL(HmoeRouter, RouterImpl,
                                   .Ret<ffi::Buffer<ffi::S32>>()
                                   .Ret<ffi::Buffer<ffi::F32>>());
 
+static ffi::Error BadSizes(const char* what) {
+  return ffi::Error(ffi::ErrorCode::kInvalidArgument, std::string(what) + ": operands and results do not fit together");
+}
+template <typename X, typename Y>
+static bool SameRows(const X& x, const Y& y) {  // both [R, C]
+  return x.dimensions().size() == 2 && y.dimensions().size() == 2 && Rows(x) == Rows(y) && Cols(x) == Cols(y);
+}
+// logits [T, N], bias [N] or of no elements (softmax reads none) -> top_idx and gates [T, K].
+template <typename L, typename B, typename I, typename G>
+static bool SelectionFits(const L& logits, const B& bias, int64_t mode, const I& top_idx, const G& gates) {
+  return logits.dimensions().size() == 2 && top_idx.dimensions().size() == 2 && Rows(top_idx) == Rows(logits) &&
+         SameRows(top_idx, gates) &&
+         (mode != HMOE_ROUTE_SIGMOID_BIAS || bias.element_count() == 0 ||
+          static_cast<int64_t>(bias.element_count()) == Cols(logits));
+}
+template <typename B>
+static const float* BiasOrNull(B& bias) {
+  return bias.element_count() > 0 ? bias.typed_data() : nullptr;
+}
+
 // The same with the experts taken from the best groups.
 static ffi::Error RouterGroupedImpl(hipStream_t stream, ffi::AnyBuffer x, ffi::AnyBuffer w,
                                     ffi::Buffer<ffi::F32> bias, int64_t mode, float rsf, int64_t n_groups,
@@ -103,7 +123,11 @@ static ffi::Error RouterGroupedImpl(hipStream_t stream, ffi::AnyBuffer x, ffi::A
   const int xd = DtypeCode(x.element_type()), wd = DtypeCode(w.element_type());
   if (xd < 0) return BadDtype("hmoe_router_grouped x");
   if (wd < 0) return BadDtype("hmoe_router_grouped router_w");
-  return Status(hmoe_router_grouped(x.untyped_data(), xd, w.untyped_data(), wd, bias.typed_data(), Rows(x),
+  if (x.dimensions().size() != 2 || w.dimensions().size() != 2 || Rows(w) != Cols(x) ||
+      logits->dimensions().size() != 2 || Rows(*logits) != Rows(x) || Cols(*logits) != Cols(w) ||
+      !SelectionFits(*logits, bias, mode, *top_idx, *gates))
+    return BadSizes("hmoe_router_grouped");
+  return Status(hmoe_router_grouped(x.untyped_data(), xd, w.untyped_data(), wd, BiasOrNull(bias), Rows(x),
                                     static_cast<int>(Cols(x)), static_cast<int>(Cols(w)),
                                     static_cast<int>(Cols(*top_idx)), static_cast<int>(mode), rsf,
                                     static_cast<int>(n_groups), static_cast<int>(top_groups), logits->typed_data(),
@@ -129,8 +153,9 @@ static ffi::Error RouterGroupedFromLogitsImpl(hipStream_t stream, ffi::Buffer<ff
                                               int64_t n_groups, int64_t top_groups,
                                               ffi::ResultBuffer<ffi::S32> top_idx,
                                               ffi::ResultBuffer<ffi::F32> gates) {
+  if (!SelectionFits(logits, bias, mode, *top_idx, *gates)) return BadSizes("hmoe_router_grouped_from_logits");
   return Status(hmoe_router_grouped_from_logits(
-      logits.typed_data(), bias.typed_data(), Rows(logits), static_cast<int>(Cols(logits)),
+      logits.typed_data(), BiasOrNull(bias), Rows(logits), static_cast<int>(Cols(logits)),
       static_cast<int>(Cols(*top_idx)), static_cast<int>(mode), rsf, static_cast<int>(n_groups),
       static_cast<int>(top_groups), top_idx->typed_data(), gates->typed_data(), S(stream)));
 }
@@ -848,13 +873,6 @@ XLA_FFI_DEFINE_HANDLER_SYMBOL(HmoeGroupedDownMxfp4, GroupedDownMxfp4Impl,
                                   .Ret<ffi::Buffer<ffi::BF16>>());
 
 // ---- root-mean-square norm with the residual's addition; int8 experts --------------
-static ffi::Error BadSizes(const char* what) {
-  return ffi::Error(ffi::ErrorCode::kInvalidArgument, std::string(what) + ": operands and results do not fit together");
-}
-template <typename X, typename Y>
-static bool SameRows(const X& x, const Y& y) {  // both [R, C]
-  return x.dimensions().size() == 2 && y.dimensions().size() == 2 && Rows(x) == Rows(y) && Cols(x) == Cols(y);
-}
 // Codes [N, rows / 32, K / 32, 64, 16] and scales [N, rows] of an int8 operand.
 template <typename Q, typename Sc>
 static bool I8Operand(const Q& q, const Sc& scales) {
