@@ -17,6 +17,7 @@ import weakref
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from . import kernels as K
@@ -170,6 +171,15 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     """``t`` where calls that load 16 bytes at a time can read it: a tensor that starts inside a buffer (a
     flat one of parameters, say) is copied unless it starts at 16 bytes."""
     return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _refuse_tangents(name: str, *tensors) -> None:
+    """Refuses forward-mode derivatives: the library's results would carry none, without a
+    word.  (Outside ``torch.autograd.forward_ad`` this is one comparison.)"""
+    if forward_ad._current_level < 0 or not torch._C._is_fwd_grad_enabled():
+        return
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{name} has no forward-mode derivatives; backward() and autograd.grad are built")
 
 
 class MoE:
@@ -421,7 +431,8 @@ class MoE:
         of the whole module (:func:`hanuman_amd.backward.moe_backward`):
         ``out``, ``router_z_loss``, ``balance_loss`` and ``mean_entropy``
         are differentiable, ``expert_counts`` is not (``train.py:191-200``
-        differentiates the same outputs)."""
+        differentiates the same outputs).  Forward-mode derivatives are refused."""
+        _refuse_tangents("MoE", x, *self._params())
         if torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in self._params())):
             if self.expert_dtype is not None:
                 raise NotImplementedError(f"{self.expert_dtype} experts have no backward: call under "
@@ -447,9 +458,10 @@ class MoE:
         :class:`hanuman_amd.RMSNorm`.  Returns ``(out [B,S,D] float32, total [B,S,D], aux)``;
         the block's output is ``total + out``.  The addition, the norm and, for int8 experts,
         the tokens' codes are one launch.  Under autograd it is ``norm`` and the layer as
-        two nodes."""
+        two nodes; forward-mode derivatives are refused."""
         if x.dim() != 3:
             raise ValueError(f"x must be [B, S, d_model] (got {tuple(x.shape)})")
+        _refuse_tangents("behind_norm", x, residual, norm.scale.value, *self._params())
         tracked = (x, norm.scale.value, *self._params()) if residual is None else (
             x, residual, norm.scale.value, *self._params())
         if torch.is_grad_enabled() and any(t.requires_grad for t in tracked):

@@ -10,7 +10,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import kernels as K
-from .moe import Param, _aligned
+from .moe import Param, _aligned, _refuse_tangents
 
 
 class RMSNorm:
@@ -34,8 +34,10 @@ class RMSNorm:
 
         A graph that captures gradients takes them with ``torch.autograd.grad``, or while no
         autograd graph of the same leaves from before the capture is alive: autograd adds into a
-        leaf's ``.grad`` on the stream of the first of them, which may not be captured."""
+        leaf's ``.grad`` on the stream of the first of them, which may not be captured.
+        Second and forward-mode derivatives are refused."""
         w = self.scale.value
+        _refuse_tangents("RMSNorm", x, residual, w)
         if residual is not None and residual.shape != x.shape:
             raise ValueError(f"residual must have x's shape {tuple(x.shape)} (got {tuple(residual.shape)})")
         tracked = x.requires_grad or w.requires_grad or (residual is not None and residual.requires_grad)
