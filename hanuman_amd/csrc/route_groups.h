@@ -2,8 +2,9 @@
 // score is its largest key (softmax; a key is a logit) or the float32 sum of its two largest
 // (sigmoid; a key is the score plus the bias).  The top_groups groups with the largest scores
 // keep their experts, the top_k of these with the largest keys are taken, in both the lower
-// index first where equal (totalOrder).  A score that is NaN is below every other.  Gates as
-// without groups.
+// index first where equal (totalOrder).  A sum that is NaN is below every score, since the sign of
+// an arithmetic's NaN says nothing; a logit that is NaN keeps its place in totalOrder, as without
+// groups.  Gates as without groups.
 //
 // A token has 2^log_lanes lanes: groups g = 0 .. G padded to a power of two, 2^log_lg each, E keys in
 // each lane's registers.  A key and its expert are one positive float64 that orders like the

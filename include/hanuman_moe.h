@@ -91,8 +91,10 @@ int hmoe_router_from_logits(const float* logits, const float* bias, int64_t toke
  * n_group that nothing reads).  The experts are n_groups groups of N / n_groups one after another.
  * A key is the logit (HMOE_ROUTE_SOFTMAX) or sigmoid + bias; a group's score is its largest key, or
  * with sigmoid the float32 sum of its two largest.  The experts are taken, by their keys, from the
- * top_groups groups with the largest scores (the lower index first where equal; a score that is
- * NaN is below all others); gates as above.  With top_groups == n_groups these are the calls
+ * top_groups groups with the largest scores, keys and scores in IEEE totalOrder, the lower index
+ * first where equal.  A sum that is NaN is below every score; a logit that is NaN has its own
+ * place (above infinity, or below minus infinity with its sign set) and its group with it.  Gates as
+ * above.  With top_groups == n_groups these are the calls
  * above.  n_groups <= 64 divides N, top_k <= top_groups * (N / n_groups), with sigmoid groups of
  * two experts at least, tokens <= 2^26 - 16.  hmoe_router_bwd and hmoe_router_aux take the results
  * as they are. */

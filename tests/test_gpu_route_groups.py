@@ -256,3 +256,21 @@ def test_rows_beside_the_results_are_left(gpu):
     _lib.call("hmoe_router_grouped_from_logits", logits.data_ptr(), None, t, n, k, SOFTMAX, 1.0, 8, 2, idx.data_ptr(),
               gates.data_ptr(), torch.cuda.current_stream().cuda_stream)
     assert (idx[t:] == 77).all() and (gates[t:] == 7.0).all() and (idx[:t] < n).all()
+
+
+def test_where_nan_is(gpu):
+    """Softmax: a NaN's group comes first, one of NaNs with the sign set last; sigmoid: a group
+    whose sum is NaN comes last."""
+    logits = np.tile(np.linspace(0.0, 1.0, 16, dtype=np.float32), (4, 1))
+    nan, minus = np.array([0x7FC00000, 0xFFFFFFFF], dtype=np.uint32).view(np.float32)
+    logits[1, 2] = logits[2, 9] = nan
+    logits[3, 12:] = minus
+    dev = torch.from_numpy(logits).to(gpu)
+    idx, gates = K.router_from_logits(dev, None, 4, SOFTMAX, 1.0, 4, 1)
+    groups = (idx // 4).cpu().numpy()
+    assert (groups == np.array([3, 0, 2, 2])[:, None]).all()
+    assert idx[1, 0] == 2 and idx[2, 0] == 9
+    assert torch.isnan(gates[1:3]).all() and torch.isfinite(gates[[0, 3]]).all()
+    idx, _ = K.router_from_logits(dev, None, 12, SIGMOID, 1.0, 4, 3)
+    left_out = [(set(range(4)) - set((idx[t] // 4).tolist())).pop() for t in range(4)]
+    assert left_out[0] == 0 and left_out[3] == 3
