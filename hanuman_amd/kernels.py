@@ -105,7 +105,8 @@ def router(x: torch.Tensor, router_w: torch.Tensor, bias: torch.Tensor | None, t
              _ptr(bias), T, D, N, top_k, mode, float(routed_scaling_factor), n_groups, top_groups,
              _ptr(logits), _ptr(top_idx), _ptr(gates), _stream())
         return logits, top_idx, gates
-    _whole_groups("router", router_w.shape[-1], n_groups)
+    if n_groups != 1:
+        _whole_groups("router", router_w.shape[-1], n_groups)
     T, D, N, logits, top_idx, gates = _router_operands(x, router_w, bias, top_k)
     call("hmoe_router", _ptr(x), _dtype_code(x), _ptr(router_w), _dtype_code(router_w),
          _ptr(bias), T, D, N, top_k, mode, float(routed_scaling_factor), _ptr(logits),

@@ -100,3 +100,11 @@ def test_the_most_tokens(name, args):
         expect(INVALID, "null", name, *args(most, experts, k, 0, groups, 8, None))
     for per_block, threads in ((4, 256), (16, 1024)):
         assert -(-most // per_block) * threads < 1 << 32
+
+
+def test_operands_are_checked_in_their_order():
+    """Without groups a call is checked as it was before it took any: x first, then the weight."""
+    x = torch.zeros((4, 64))
+    for w in (None, [1.0], torch.zeros(())):
+        with pytest.raises(ValueError, match="x must be on a GPU"):
+            K.router(x, w, None, 2)
