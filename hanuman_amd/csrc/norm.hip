@@ -199,8 +199,10 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void add_rms_norm_bwd_kernel(
       static_cast<int64_t>(blockIdx.x - (FEW ? dw_groups : 0u)) * (kThreads / NT) + threadIdx.x / NT;
   const int64_t stride = static_cast<int64_t>(gridDim.x) * (kThreads / NT);
   float dw[C][8] = {};
-  // (a thread of 1024 has 128 registers: with four chunks the weight and d_sum are read where they
-  // are used; 4000 x 32768 in bf16 316 us, held with the rest 488)
+  // (a thread of 1024 has 128 registers: with four chunks, rows past 16384 values, the weight and
+  // d_sum are read where they are used; 4000 x 32768 in bf16 312 us, held with the rest 488.  What is
+  // left still passes 128 by 31 to 53 registers, and the loop spills: 1.46 times the bytes' time at a
+  // copy's rate.  Two chunks, rows of 8193 to 16384 values, spill nothing.)
   constexpr bool kLean = NT == 1024 && C == 4;
   float w[kLean ? 1 : C][8];
   const auto weight8 = [&](int u, float (&v)[8]) __attribute__((always_inline)) {
@@ -309,8 +311,10 @@ __global__ __launch_bounds__(1024) void sum_parts_kernel(const float* __restrict
 constexpr int kBwdWaveCols = 1024;
 constexpr int64_t kMaxParts = 4096;
 // Up to so many rows dy and s are read again instead, by workgroups of the same launch, and no
-// workspace is needed (700 x 1536: bf16 5.1 us, in parts 7.8, float32 6.7 and 8.8; 1000 rows 6.1 and
-// 8.4, 9.5 and 10.0, but 1000 x 4096 in float32 24.5 and 21).
+// workspace is needed.  768 rows so and in parts, us: bf16 of 1536 columns 5.3 and 8.1, 4096 8.1 and
+// 13.3, 8192 16 and 21, 32768 61 and 94; float32 8.1 and 9.2, 21.6 and 18.4, 28 and 31, 121 and 153.
+// (1000 rows: 1536 columns of bf16 6.1 and 8.4, of float32 9.5 and 10.0, 4096 of float32 24.5 and 21.
+// What the launch reads again grows with the rows, what the parts move does not.)
 constexpr int64_t kFewRows = 768;
 int64_t most_parts(int64_t rows, int cols) {
   if (cols > kBwdWaveCols || rows < kWaveRows) return 512;

@@ -500,13 +500,13 @@ int hmoe_grouped_down_mxfp4(const uint8_t* h_q, const uint8_t* h_exp, const int3
 
 /* sum = rnd(x + residual) in the residual's type (added in float32), rstd = (mean_d sum^2 +
  * eps)^(-1/2) of the rounded sum, y = rnd(sum * rstd * weight); float32 sums in a fixed order (rows
- * whose squares pass float32's range have rstd 0).  x, y, residual and
- * weight are F32 or BF16 each, [rows, cols] and [cols].  Without a residual (NULL, then sum NULL
+ * whose squares pass float32's range have rstd 0; with eps 0, rows whose squares all round to zero
+ * have an infinite one).  x, y, residual and weight are F32 or BF16 each, [rows, cols] and [cols].  Without a residual (NULL, then sum NULL
  * too) the norm is x's.  rstd [rows] f32 (or NULL) is what the gradients need.  q (or NULL, then
  * scale NULL too) [rows, cols] and scale [rows] f32: the 8-bit codes of the rounded y, HMOE_I8 by
  * the rule of hmoe_quantize_rows_i8 or HMOE_FP8_E4M3 by that of hmoe_quantize_rows_fp8 (the same
  * bits as those calls on y).  cols % 8 == 0, up to 32768; matrices 16-byte aligned, q 8-byte.
- * sum may be x or residual where the types agree, y may be x: a row is read before it is written. */
+ * sum may be x or residual, y may be x, where the types agree: a row is read before it is written. */
 int hmoe_add_rms_norm(const void* x, int x_dtype, const void* residual, int residual_dtype,
                       const void* weight, int w_dtype, float eps, int64_t rows, int cols, void* sum,
                       void* y, int y_dtype, float* rstd, void* q, int q_type, float* scale,
