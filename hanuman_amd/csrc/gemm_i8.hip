@@ -161,9 +161,9 @@ __global__ __launch_bounds__(256) void grouped_i8_rows(
 //
 // 131072 rows, D 2048, F 1024, gate/up and down: 500 and 270 us (2.2 and 2.0 POP/s; the matrix
 // cores alone, from registers, 3.6, where the package's power takes the clock to 1.8 GHz; the
-// vendor library's product of 8192^3 1.9).  They are busy in 63 % and 49 % of the cycles at 1.66
-// and 1.78 GHz, and a quarter of the lines that are asked for miss L2.  With operands of zeros
-// (2.4 GHz) 394 and 202 us; every load a hit of L2 463 and 251; without the products 383 and 202:
+// vendor library's product of 16384 x 8192 x 8192 1.9).  They are busy in 63 % and 49 % of the
+// cycles at 1.66 and 1.78 GHz, and a quarter of the lines that are asked for miss L2.  With operands
+// of zeros (2.4 GHz) 394 and 202 us; every load a hit of L2 463 and 251; without the products 383 and 202:
 // power, the loads' way and the epilogue (438 and 219 without it) share the time, none has all of
 // it.  No faster: A three stages deep (508 and 275 against 517 and 280), steps in another order for
 // each tile, row-tile groups of 1 to 32, two workgroups of 64 rows a CU, no turns.

@@ -15,9 +15,9 @@
 //
 // Bound by vector instructions, 85 a key, of which the sigmoid is 26 (its single operations are
 // what makes the choice the same everywhere) and the lists the rest: 16384 tokens on 256 experts
-// 12 us, of which the logits' 17 MB are 3.7.  In rounds, the largest of all taken each time, with
-// keys compared as two integers, they took 30 us; with sigmoid_det's range checks and division
-// 13.5.  Twelve experts a token 14 us (in rounds on these keys 21), 32 21 us (39); one token 4.8, 6.2
+// 11.3 us (captured again and again; 12.3 traced from Python), of which the logits' 17 MB are
+// 3.7.  In rounds, the largest of all taken each time, with keys compared as two integers, they
+// took 30 us; with sigmoid_det's range checks and division 13.5.  Twelve experts a token 14 us (in rounds on these keys 21), 32 21 us (39); one token 4.8, 6.2
 // and 9.1 us (9.9 and 18.7 in rounds).
 #pragma once
 
